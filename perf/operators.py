@@ -3,8 +3,8 @@ held in 4 bits.
 
 Four operators share one format. A group of 32 numbers is held as 32 E2M1 codes (bit 3 the sign, bits 0..2 the
 magnitude 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte b that stands for 2^(b - 127): the smallest power of two s
-with max|x| <= 7 s, b in [1, 254] (fp16 numbers: at most 140); codes round to the nearest, ties to the even code,
-above 6 to 6. A group with a NaN or an infinity in it has b = 255 and reads as NaN.
+with max|x| <= 7 s, b in [1, 252] (fp16 numbers: at most 140, so that every value is finite); codes round to the
+nearest, ties to the even code, above 6 to 6. A group with a NaN or an infinity in it has b = 255 and reads as NaN.
 
   append  K and V rows (views of a step's q|k|v rows) quantised into a cache at (slot, position), then read back: the
           writer and the reader of the cache, as a prompt's prefix is stored and exported
@@ -149,7 +149,7 @@ def _rows(case, seed, g):
 def _cache(case, slots, cap, g):
     """A filled cache: quantised keys and values, a slot at a time."""
     kv, dim = case["kv"], case["dim"]
-    top = 140 if case["dtype"] == "fp16" else 254
+    top = 140 if case["dtype"] == "fp16" else 252
     c = _empty_cache(case, slots, cap)
     strong = torch.exp(0.7 * _normal(g, kv, 1, dim))
     for s in range(slots):
@@ -174,7 +174,7 @@ def _weight(case, g):
     np_, kp = -(-n // 16) * 16, -(-k // 128) * 128
     w = torch.zeros(np_, kp, device=DEV)
     w[:n, :k] = _normal(g, n, k) * (k ** -0.5)
-    codes, scales = _quantise(w, 254)
+    codes, scales = _quantise(w, 252)
     steps = kp // 128
     codes = _bytes(codes).view(np_ // 16, 16, steps, 4, 16).permute(0, 2, 3, 1, 4).reshape(np_ // 16, steps, 64, 16)
     full = torch.zeros(np_, -(-steps // 4), 4, 4, dtype=torch.uint8, device=DEV)  # row, four steps, step, group
@@ -259,7 +259,7 @@ def _dim_major(v, vs):
 
 
 def _plain_append(s):
-    c, dim, top = s.cache, s.case["dim"], 140 if s.case["dtype"] == "fp16" else 254
+    c, dim, top = s.cache, s.case["dim"], 140 if s.case["dtype"] == "fp16" else 252
     p = s.pos.long()
     codes, scales = _quantise(s.k, top)
     c.k[s.slots, :, p] = _bytes(codes)
@@ -430,7 +430,7 @@ def exact(case, seed):
     s = prepare(case, seed)
     op, dim = case["op"], case.get("dim")
     if op == "append":
-        top = 140 if case["dtype"] == "fp16" else 254
+        top = 140 if case["dtype"] == "fp16" else 252
         return _round64(s.k, top), _round64(s.v, top)
     if op == "read":
         ks, vs = [], []
