@@ -507,6 +507,73 @@ size_t m3x_backbone_run_layer_bytes(void);
  * add+norms, gate|up, SwiGLU, down), its final norm (:229-232) and the length update (:233). */
 int m3x_backbone_run(const M3xBackboneRun* args, void* stream);
 
+/* ---- 4-bit cache and weights ------------------------------------------------------------------------------------
+ * One format: a group of 32 numbers is 32 E2M1 codes (bit 3 the sign, bits 0..2 the magnitude 0, .5, 1, 1.5, 2, 3, 4,
+ * 6) and a scale byte b for s = 2^(b - 127), the smallest power of two with max|x| <= 7 s (1 <= b <= 252; fp16 numbers
+ * <= 140); codes to nearest, ties to the even code, 6 above 5 s, so |x - value| <= s (fp16 numbers above 57344 and
+ * bf16 numbers above 7 * 2^125 lose up to 2 s). A group holding a NaN or an infinity is stored with b = 255 and reads
+ * as NaN. No counterpart in the reference, whose caches and weights are 16-bit (serve/fast_backbone.py:146-150).
+ *
+ * The cache (per layer; cap % 32 == 0, head_dim D in {64, 128}; all four 16-byte aligned and contiguous), bytes:
+ *   k4  [slots][kv_heads][cap][D / 2]               byte j: dims 2j (low half), 2j + 1
+ *   ks4 [slots][kv_heads][cap][D / 32]              scale bytes
+ *   v4  [slots][kv_heads][cap / 4][16][4][D / 32]   four positions together; chunk c: dims c D/16 .. (c + 1) D/16 - 1
+ *   vs4 [slots][kv_heads][cap / 4][D / 32][4]       scale bytes
+ * A row whose slot is outside [0, nslots) or whose position is outside [0, cap) is outside the cache. */
+
+/* K and V rows [rows, kv_heads, D] (row and head strides % 8 == 0) quantised to position pos[r] of slot slots[r]; a
+ * row outside the cache is not written. Rows of one call at the same place leave either row's bytes there. */
+int m3x_kv4_append(const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h, void* k4, void* ks4,
+                   void* v4, void* vs4, const int64_t* slots, const int32_t* pos, int rows, int nslots, int kv_heads,
+                   int head_dim, int cap, int dtype, void* stream);
+
+/* m3x_qk_norm_rope_cache over the 4-bit cache: q_out and the rotated bf16 keys have its bits, and keys and values are
+ * quantised as m3x_kv4_append does (the RoPE row of a position outside the tables is the nearest one's). bf16. */
+int m3x_qk_norm_rope_kv4(const void* qkv, long s_qkv, void* q_out, long s_qo_b, long s_qo_h, void* k4, void* ks4,
+                         void* v4, void* vs4, const int64_t* slots, const int32_t* pos, const void* cos,
+                         const void* sin, long s_cos, const void* wq, const void* wk, float eps, int rows, int heads,
+                         int nslots, int kv_heads, int head_dim, int cap, void* stream);
+
+/* k[r], v[r] ([kv_heads, D] 16-bit, strides % 8 == 0) = the numbers at position pos[r] of slot slots[r], zeros for a
+ * row outside the cache. Exact where the type holds the number (bf16 always, fp16 for a cache written from fp16). */
+int m3x_kv4_read(const void* k4, const void* ks4, const void* v4, const void* vs4, const int64_t* slots,
+                 const int32_t* pos, void* k, long sk_r, long sk_h, void* v, long sv_r, long sv_h, int rows, int nslots,
+                 int kv_heads, int head_dim, int cap, int dtype, void* stream);
+
+/* Bytes of workspace m3x_kv4_attn needs (0 when max_ctx <= chunk). */
+size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, int chunk);
+
+/* out[r, h] = softmax(scale q[r, h] . K^T) V over positions 0 .. pos[r] of slot slots[r], kv head h / (heads /
+ * kv_heads); q and out [rows, heads, D] 16-bit (strides % 8 == 0, 16-byte aligned). pos[r] < 0 or a slot outside the
+ * cache: zeros. max_ctx >= pos[r] + 1 for every row (keys past it are not attended), <= cap; chunk = keys per split,
+ * a multiple of 128. What a row does not see has no part in its result, whatever it holds. Rows next to each other in
+ * the call, of one slot at consecutive positions (a prompt's), share one pass over the keys; a row's bits do not
+ * depend on that, and not on the other rows. Fixed summation order. */
+int m3x_kv4_attn(const void* q, long sq_b, long sq_h, const void* k4, const void* ks4, const void* v4, const void* vs4,
+                 void* out, long so_b, long so_h, const int64_t* slots, const int32_t* pos, float scale, int rows,
+                 int heads, int nslots, int kv_heads, int head_dim, int cap, int max_ctx, int chunk, void* workspace,
+                 size_t ws_bytes, int dtype, void* stream);
+
+/* A weight [N, K] (K % 32 == 0) in 4 bits, groups along K: N in tiles of 16 rows (zero rows behind N), K in steps of
+ * 128 (zeros behind K).
+ *   codes  [tiles][steps][64][16]           lane l: row l % 16 of the tile, inputs 32 (l / 16) .. + 31 of the step
+ *   scales [tiles][ceil(steps / 4)][64][4]  the lane's scale byte of four consecutive steps
+ * m3x_packed_weight4_bytes: size of the codes (scales = 0) or of the scales; -1 if K % 32. m3x_pack_weight4: from
+ * bf16, fp16 or fp32 rows (ldw % 8 == 0, 16-byte aligned), once at load time. */
+long m3x_packed_weight4_bytes(int N, int K, int scales);
+int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes, void* scales, int dtype, void* stream);
+
+/* y[M, N] = x[M, K] . W^T with W from m3x_pack_weight4; bf16 / fp16 rows (ldx % 8 == 0, x 16-byte aligned), fp32
+ * products and sums, one rounding. The 4-bit form of m3x_linear for few rows (any M; weights are read once per 64
+ * rows). Deterministic, one launch, no workspace. */
+int m3x_linear4(const void* x, long ldx, const void* codes, const void* scales, void* y, long ldy, int M, int N, int K,
+                int dtype, void* stream);
+
+/* y[M, I] = silu(x . Wg^T) * (x . Wu^T) (M3X_ACT_SWIGLU) or gelu(x . Wg^T) (M3X_ACT_GELU, erf form; u_* unused), the
+ * 4-bit form of m3x_linear_act; the activation in fp32, one rounding at the end. */
+int m3x_linear4_act(const void* x, long ldx, const void* g_codes, const void* g_scales, const void* u_codes,
+                    const void* u_scales, void* y, long ldy, int M, int I, int K, int kind, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

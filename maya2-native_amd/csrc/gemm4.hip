@@ -1,0 +1,240 @@
+// Products of few rows with 4-bit weights and a scale per 32 inputs (format: m3x_fp4.h): y = act(x . W^T).
+//
+// Packed weight [N, K]: N in tiles of 16 rows (zero rows behind N), K in steps of 128 (zeros behind K). A step's codes
+// are 1 KB: lane l's 16 bytes hold row l % 16, inputs 32 (l / 16) .. + 31, i.e. one group; its scale bytes of four
+// consecutive steps are one word, so a wave reads contiguous kilobytes and a lane applies one scale to all it holds.
+//   codes  [tiles][steps][64][16]      scales [tiles][ceil(steps / 4)][64][4]
+//
+// Bound: the weights' bytes, 17 / 32 of a byte each, and below some megabytes the launch and one memory round trip. A
+// lane's words become 16-bit MFMA operands in registers (16 conversions a KB) and meet the rows of x, the product's
+// columns, as read from memory: per step and 16 rows of x four MFMA 16x16x32, the lane's inputs 8 i .. 8 i + 7 in the
+// i-th. The waves of a workgroup share the steps out and their sums meet in LDS, added in wave order (deterministic).
+// Products and sums are fp32; the one rounding is the store's.
+#include "m3x_fp4.h"
+
+namespace {
+struct Lin4 {
+  const uint16_t* x;
+  long ldx;
+  const uint8_t* w[2];
+  const uint8_t* s[2];
+  uint16_t* y;
+  long ldy;
+  int M, N, K, steps, tiles;
+};
+enum { L4_NONE, L4_SWIGLU, L4_GELU };
+}  // namespace
+
+// TW output tiles and 16 MT rows of x per workgroup of NW waves
+template <int DT, int TW, int MT, int NW, int ACT>
+__global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
+  constexpr int P = ACT == L4_SWIGLU ? 2 : 1;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int li = lane & 15, lg = lane >> 4;
+  const int tile0 = blockIdx.x * TW;
+  const int m0 = blockIdx.y * (16 * MT);
+  const int quads = (a.steps + 3) >> 2;
+  const int per = (a.steps + NW - 1) / NW;
+  const int s0 = wave * per, s1 = min(s0 + per, a.steps);
+
+  f32x4_t acc[TW * P][MT];
+#pragma unroll
+  for (int t = 0; t < TW * P; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[t][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (int s = s0; s < s1; ++s) {
+    fp4_u4 cw[TW * P];
+    uint32_t sw[TW * P];
+#pragma unroll
+    for (int t = 0; t < TW * P; ++t) {
+      const long tile = min(tile0 + t / P, a.tiles - 1);  // a tile past the last repeats it and is not stored
+      cw[t] = __builtin_nontemporal_load(
+          reinterpret_cast<const fp4_u4*>(a.w[t % P] + ((tile * a.steps + s) * 64 + lane) * 16));
+      sw[t] = *reinterpret_cast<const uint32_t*>(a.s[t % P] + ((tile * quads + (s >> 2)) * 64 + lane) * 4);
+    }
+    u16x8 xv[MT][4];
+    const int k = 128 * s + 32 * lg;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = m0 + 16 * m + li;
+      if (r < a.M && k < a.K) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xv[m][i] = ld16(a.x + (long)r * a.ldx + k + 8 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xv[m][i] = zero_v8<DT>();
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TW * P; ++t) {
+      const float sc = fp4_scale((sw[t] >> (8 * (s & 3))) & 255u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u16x8 wv = fp4_eight<DT>(cw[t][i], sc);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[t][m] = mfma16x16x32<DT>(wv, xv[m][i], acc[t][m]);
+      }
+    }
+  }
+
+  __shared__ f32x4_t red[NW][TW * P * MT][64];
+#pragma unroll
+  for (int t = 0; t < TW * P; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) red[wave][t * MT + m][lane] = acc[t][m];
+  __syncthreads();
+  for (int f = wave; f < TW * MT; f += NW) {
+    const int t = f / MT, m = f % MT;
+    f32x4_t v[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      v[p] = red[0][(t * P + p) * MT + m][lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) v[p] += red[w][(t * P + p) * MT + m][lane];
+    }
+    const int row = m0 + 16 * m + li;
+    const int n = 16 * (tile0 + t) + 4 * lg;
+    if (row >= a.M || n >= a.N) continue;
+    uint16_t o[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float y = v[0][r];
+      if constexpr (ACT == L4_SWIGLU) y = silu16(y) * v[P - 1][r];
+      if constexpr (ACT == L4_GELU) y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
+      o[r] = E<DT>::from_f(y);
+    }
+    uint16_t* yp = a.y + (long)row * a.ldy + n;
+    if (n + 4 <= a.N && (((uintptr_t)yp) & 7) == 0) {
+      *reinterpret_cast<uint2*>(yp) = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.N) yp[r] = o[r];
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(64) void pack_weight4_kernel(const Elt<DT>* __restrict__ w, long ldw, int N, int K,
+                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                          int steps) {
+  const int lane = threadIdx.x;
+  const int s = blockIdx.x;
+  const long tile = blockIdx.y;
+  const int row = 16 * (int)tile + (lane & 15), k = 128 * s + 32 * (lane >> 4);
+  float x[32];
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 32; e += 8) {
+    const V8<DT> v = row < N && k < K ? ldv<DT>(w + (long)row * ldw + k + e) : zero_v8<DT>();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[e + i] = E<DT>::to_f(v.v[i]);
+      m = max(m, __float_as_uint(x[e + i]) & 0x7FFFFFFFu);
+    }
+  }
+  uint32_t byte = 255;
+  fp4_u4 c = {0, 0, 0, 0};
+  if (m < 0x7F800000u) {
+    byte = fp4_scale_byte(__uint_as_float(m), fp4_top_of<DT>());
+    const float sc = fp4_scale(byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t r = 0;
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[8 * i], x[8 * i + 1], sc, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[8 * i + 2], x[8 * i + 3], sc, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[8 * i + 4], x[8 * i + 5], sc, 2);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x[8 * i + 6], x[8 * i + 7], sc, 3);
+      c[i] = r;
+    }
+  }
+  *reinterpret_cast<fp4_u4*>(codes + ((tile * steps + s) * 64 + lane) * 16) = c;
+  uint8_t* sp = scales + ((tile * ((steps + 3) >> 2) + (s >> 2)) * 64 + lane) * 4;
+  sp[s & 3] = (uint8_t)byte;
+  if (s == steps - 1)
+    for (int i = (s & 3) + 1; i < 4; ++i) sp[i] = 1;  // steps that are not there
+}
+
+M3X_API long m3x_packed_weight4_bytes(int N, int K, int scales) {
+  if (N <= 0 || K <= 0 || K % 32) return -1;
+  const long tiles = (N + 15L) / 16, steps = (K + 127L) / 128;
+  return scales ? tiles * ((steps + 3) / 4) * 256 : tiles * steps * 1024;
+}
+
+M3X_API int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes, void* scales, int dtype,
+                             void* stream) {
+  if (N <= 0 || K <= 0 || K % 32 || ldw & 7) return M3X_EINVAL;
+  if (!w || !codes || !scales) return M3X_ENULL;
+  if (!m3x_aligned16(w) || !m3x_aligned16(codes) || !m3x_aligned16(scales)) return M3X_EINVAL;
+  const int steps = m3x_ceil_div(K, 128), tiles = m3x_ceil_div(N, 16);
+  hipStream_t st = (hipStream_t)stream;
+  const int ny = tiles < 65535 ? tiles : 65535;
+  if (tiles > 65535) return M3X_EINVAL;
+  const dim3 grid(steps, ny);
+  if (dtype == M3X_BF16)
+    hipLaunchKernelGGL(pack_weight4_kernel<M3X_BF16>, grid, dim3(64), 0, st, (const uint16_t*)w, ldw, N, K,
+                       (uint8_t*)codes, (uint8_t*)scales, steps);
+  else if (dtype == M3X_F16)
+    hipLaunchKernelGGL(pack_weight4_kernel<M3X_F16>, grid, dim3(64), 0, st, (const uint16_t*)w, ldw, N, K,
+                       (uint8_t*)codes, (uint8_t*)scales, steps);
+  else if (dtype == M3X_F32)
+    hipLaunchKernelGGL(pack_weight4_kernel<M3X_F32>, grid, dim3(64), 0, st, (const float*)w, ldw, N, K,
+                       (uint8_t*)codes, (uint8_t*)scales, steps);
+  else
+    return M3X_EUNSUPPORTED;
+  M3X_CHECK_LAUNCH();
+  return M3X_OK;
+}
+
+namespace {
+template <int DT, int TW, int MT, int NW, int ACT> void launch4(const Lin4& a, hipStream_t st) {
+  hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT>), dim3(m3x_ceil_div(a.tiles, TW), m3x_ceil_div(a.M, 16 * MT)),
+                     dim3(64 * NW), 0, st, a);
+}
+template <int DT, int ACT> void plan4(const Lin4& a, hipStream_t st) {
+  if (a.M <= 16) launch4<DT, 1, 1, 8, ACT>(a, st);
+  else if (a.M <= 32) launch4<DT, 1, 2, 8, ACT>(a, st);
+  else launch4<DT, 1, 4, 8, ACT>(a, st);
+}
+int linear4_any(const void* x, long ldx, const void* wg, const void* sg, const void* wu, const void* su, void* y,
+                long ldy, int M, int N, int K, int act, int dtype, void* stream) {
+  if (M < 0 || N <= 0 || K <= 0 || K % 32) return M3X_EINVAL;
+  if (dtype != M3X_BF16 && dtype != M3X_F16) return M3X_EUNSUPPORTED;
+  if (act != L4_NONE && act != L4_SWIGLU && act != L4_GELU) return M3X_EUNSUPPORTED;
+  if (M == 0) return M3X_OK;
+  if (!x || !wg || !sg || !y || (act == L4_SWIGLU && (!wu || !su))) return M3X_ENULL;
+  if ((ldx & 7) || !m3x_aligned16(x) || !m3x_aligned16(wg) || !m3x_aligned16(sg) || ((uintptr_t)y & 1)) return M3X_EINVAL;
+  if (act == L4_SWIGLU && (!m3x_aligned16(wu) || !m3x_aligned16(su))) return M3X_EINVAL;
+  if (M > 65535 * 16) return M3X_EINVAL;
+  const Lin4 a = {(const uint16_t*)x, ldx, {(const uint8_t*)wg, (const uint8_t*)wu},
+                  {(const uint8_t*)sg, (const uint8_t*)su}, (uint16_t*)y, ldy, M, N, K, m3x_ceil_div(K, 128),
+                  m3x_ceil_div(N, 16)};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == M3X_BF16) {
+    if (act == L4_NONE) plan4<M3X_BF16, L4_NONE>(a, st);
+    else if (act == L4_SWIGLU) plan4<M3X_BF16, L4_SWIGLU>(a, st);
+    else plan4<M3X_BF16, L4_GELU>(a, st);
+  } else {
+    if (act == L4_NONE) plan4<M3X_F16, L4_NONE>(a, st);
+    else if (act == L4_SWIGLU) plan4<M3X_F16, L4_SWIGLU>(a, st);
+    else plan4<M3X_F16, L4_GELU>(a, st);
+  }
+  M3X_CHECK_LAUNCH();
+  return M3X_OK;
+}
+}  // namespace
+
+M3X_API int m3x_linear4(const void* x, long ldx, const void* codes, const void* scales, void* y, long ldy, int M, int N,
+                        int K, int dtype, void* stream) {
+  return linear4_any(x, ldx, codes, scales, nullptr, nullptr, y, ldy, M, N, K, L4_NONE, dtype, stream);
+}
+
+M3X_API int m3x_linear4_act(const void* x, long ldx, const void* g_codes, const void* g_scales, const void* u_codes,
+                            const void* u_scales, void* y, long ldy, int M, int I, int K, int kind, int dtype,
+                            void* stream) {
+  if (kind != 0 && kind != 1) return M3X_EUNSUPPORTED;  // M3X_ACT_SWIGLU, M3X_ACT_GELU
+  return linear4_any(x, ldx, g_codes, g_scales, u_codes, u_scales, y, ldy, M, I, K, kind == 0 ? L4_SWIGLU : L4_GELU,
+                     dtype, stream);
+}

@@ -583,6 +583,277 @@ def backbone_run(args: BackboneRunArgs):
     check(lib().m3x_backbone_run(ctypes.byref(args), _stream()), "backbone_run")
 
 
+# ---------------------------------------------------------------- 4-bit cache and weights
+def _one_device(*ts):
+    """The device that all the given tensors (None skipped) are on."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("m3x kernels take device tensors")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev
+
+
+def _call_on(dev, name, *args):
+    """Entry point m3x_<name> on the tensors' device and its current stream, whichever device is current."""
+    fn = getattr(lib(), "m3x_" + name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, name)
+
+
+class Kv4Cache:
+    """A layer's KV cache in 4 bits (format and layout: include/m3x.h): uint8 tensors
+    k [slots, kv_heads, cap, head_dim / 2], ks [slots, kv_heads, cap, head_dim / 32],
+    v [slots, kv_heads, cap / 4, 16, 4, head_dim / 32], vs [slots, kv_heads, cap / 4, head_dim / 32, 4].
+    head_dim 64 or 128, cap a multiple of 32."""
+    __slots__ = ("k", "ks", "v", "vs", "slots", "kv_heads", "cap", "head_dim", "device")
+
+    def __init__(self, k, ks, v, vs):
+        if k.dim() != 4:
+            raise ValueError(f"Kv4Cache: k must be [slots, kv_heads, cap, head_dim / 2], got {tuple(k.shape)}")
+        S, KV, cap, half = k.shape
+        D = 2 * half
+        if D not in (64, 128) or cap % 32 or min(S, KV, cap) < 1:
+            raise ValueError(f"Kv4Cache: head_dim {D} must be 64 or 128 and cap {cap} a multiple of 32")
+        for t, shape, name in ((k, (S, KV, cap, D // 2), "k"), (ks, (S, KV, cap, D // 32), "ks"),
+                               (v, (S, KV, cap // 4, 16, 4, D // 32), "v"), (vs, (S, KV, cap // 4, D // 32, 4), "vs")):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"Kv4Cache: {name} must be contiguous uint8 {shape}, got {t.dtype} {tuple(t.shape)}")
+            if t.device != k.device or t.data_ptr() % 16:
+                raise ValueError(f"Kv4Cache: {name} must be 16-byte aligned on {k.device}")
+        self.k, self.ks, self.v, self.vs = k, ks, v, vs
+        self.slots, self.kv_heads, self.cap, self.head_dim, self.device = S, KV, cap, D, k.device
+
+    @classmethod
+    def empty(cls, slots, kv_heads, cap, head_dim, device):
+        """A new cache (all zeros)."""
+        if head_dim not in (64, 128):
+            raise ValueError(f"Kv4Cache: head_dim {head_dim} must be 64 or 128")
+
+        def z(*shape):
+            return torch.zeros(*shape, dtype=torch.uint8, device=device)
+        D = head_dim
+        return cls(z(slots, kv_heads, cap, D // 2), z(slots, kv_heads, cap, D // 32),
+                   z(slots, kv_heads, cap // 4, 16, 4, D // 32), z(slots, kv_heads, cap // 4, D // 32, 4))
+
+    def memory_bytes(self):
+        return sum(t.numel() for t in (self.k, self.ks, self.v, self.vs))
+
+    def _ptrs(self):
+        return self.k.data_ptr(), self.ks.data_ptr(), self.v.data_ptr(), self.vs.data_ptr()
+
+
+def _kv4_rows(name, cache, slots, pos):
+    if not isinstance(cache, Kv4Cache):
+        raise TypeError(f"{name}: the cache must be an ops.Kv4Cache")
+    if slots.dtype != torch.long or pos.dtype != torch.int32:
+        raise ValueError(f"{name}: slots must be int64 and pos int32, got {slots.dtype}, {pos.dtype}")
+    if slots.dim() != 1 or pos.shape != slots.shape or not slots.is_contiguous() or not pos.is_contiguous():
+        raise ValueError(f"{name}: slots and pos must be contiguous [rows], got {tuple(slots.shape)}, {tuple(pos.shape)}")
+    return slots.shape[0]
+
+
+def _kv4_heads(name, what, t, rows, heads, D, dtype=None):
+    if t.dim() != 3 or tuple(t.shape) != (rows, heads, D) or (t.numel() and t.stride(2) != 1):
+        raise ValueError(f"{name}: {what} must be [{rows}, {heads}, {D}] with a contiguous last dimension, "
+                         f"got {tuple(t.shape)}")
+    if t.dtype not in _DT or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name}: {what} must be {'bfloat16 or float16' if dtype is None else dtype}, got {t.dtype}")
+    if t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: {what} needs 16-byte aligned rows (strides {t.stride()})")
+
+
+def kv4_append(k, v, cache, slots, pos):
+    """K and V rows [rows, kv_heads, head_dim] (bf16 or fp16, any row and head strides) quantised to position pos[r]
+    (int32) of slot slots[r] (int64). A row whose slot or position is outside the cache is not written."""
+    rows = _kv4_rows("kv4_append", cache, slots, pos)
+    _kv4_heads("kv4_append", "k", k, rows, cache.kv_heads, cache.head_dim)
+    _kv4_heads("kv4_append", "v", v, rows, cache.kv_heads, cache.head_dim, k.dtype)
+    dev = _one_device(k, v, cache.k, slots, pos)
+    _call_on(dev, "kv4_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+             *cache._ptrs(), slots.data_ptr(), pos.data_ptr(), rows, cache.slots, cache.kv_heads, cache.head_dim,
+             cache.cap, _DT[k.dtype])
+
+
+def qk_norm_rope_kv4(qkv, q_out, cache, slots, pos, cos, sin, wq, wk, eps, heads):
+    """qk_norm_rope_cache over a Kv4Cache: q_out's bits are its, and the rotated keys (bf16) and the values are
+    quantised as kv4_append does. bf16; cos, sin [>= cache.cap, head_dim]."""
+    rows = _kv4_rows("qk_norm_rope_kv4", cache, slots, pos)
+    D, KV = cache.head_dim, cache.kv_heads
+    _rows2d(qkv, "qkv")
+    if tuple(qkv.shape) != (rows, (heads + 2 * KV) * D):
+        raise ValueError(f"qk_norm_rope_kv4: qkv must be [{rows}, {(heads + 2 * KV) * D}], got {tuple(qkv.shape)}")
+    _kv4_heads("qk_norm_rope_kv4", "q_out", q_out, rows, heads, D, torch.bfloat16)
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t.dim() != 2 or t.shape[0] < cache.cap or t.shape[1] != D or t.stride(1) != 1:
+            raise ValueError(f"qk_norm_rope_kv4: {name} must be [>= {cache.cap}, {D}], got {tuple(t.shape)}")
+    if cos.stride(0) != sin.stride(0):
+        raise ValueError("qk_norm_rope_kv4: cos and sin share one row stride")
+    if wq.numel() != D or wk.numel() != D or not wq.is_contiguous() or not wk.is_contiguous():
+        raise ValueError(f"qk_norm_rope_kv4: wq and wk have {D} elements")
+    if any(t.dtype != torch.bfloat16 for t in (qkv, cos, sin, wq, wk)):
+        raise ValueError("qk_norm_rope_kv4: bf16 only")
+    dev = _one_device(qkv, q_out, cache.k, slots, pos, cos, sin, wq, wk)
+    _call_on(dev, "qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0),
+             q_out.stride(1), *cache._ptrs(), slots.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+             cos.stride(0), wq.data_ptr(), wk.data_ptr(), float(eps), rows, heads, cache.slots, KV, D, cache.cap)
+
+
+def kv4_read(cache, slots, pos, k, v):
+    """k, v [rows, kv_heads, head_dim] (bf16 or fp16, any row and head strides) = the numbers at position pos[r] of
+    slot slots[r]; zeros for a row outside the cache."""
+    rows = _kv4_rows("kv4_read", cache, slots, pos)
+    _kv4_heads("kv4_read", "k", k, rows, cache.kv_heads, cache.head_dim)
+    _kv4_heads("kv4_read", "v", v, rows, cache.kv_heads, cache.head_dim, k.dtype)
+    dev = _one_device(k, v, cache.k, slots, pos)
+    _call_on(dev, "kv4_read", *cache._ptrs(), slots.data_ptr(), pos.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
+             v.data_ptr(), v.stride(0), v.stride(1), rows, cache.slots, cache.kv_heads, cache.head_dim, cache.cap,
+             _DT[k.dtype])
+
+
+def kv4_attn_chunk(rows, heads, kv_heads, max_ctx) -> int:
+    """Keys per split of kv4_attn for `rows` rows of up to max_ctx keys."""
+    want = rows * kv_heads * max_ctx / 1024.0
+    c = 128
+    while c < want and c < 8192:
+        c *= 2
+    return c
+
+
+def kv4_attn_workspace(rows, heads, head_dim, max_ctx, chunk) -> int:
+    """Bytes of workspace for kv4_attn (0: none)."""
+    return int(lib().m3x_kv4_attn_workspace(rows, heads, head_dim, max_ctx, chunk))
+
+
+def kv4_attn(q, cache, out, slots, pos, scale, max_ctx, chunk, workspace):
+    """out[r, h] = softmax(scale q[r, h] . K^T) V over positions 0 .. pos[r] of slot slots[r]; q, out
+    [rows, heads, head_dim] (bf16 or fp16, any row and head strides). A row with pos[r] < 0 or a slot outside the
+    cache gets zeros. max_ctx: at least every pos[r] + 1; chunk: keys per split (kv4_attn_chunk); workspace: a tensor of
+    kv4_attn_workspace bytes, or None when that is 0. Rows of one slot at consecutive positions (a prompt's) that
+    stand next to each other share one pass over the keys."""
+    rows = _kv4_rows("kv4_attn", cache, slots, pos)
+    heads = q.shape[1] if q.dim() == 3 else 0
+    _kv4_heads("kv4_attn", "q", q, rows, heads, cache.head_dim)
+    _kv4_heads("kv4_attn", "out", out, rows, heads, cache.head_dim, q.dtype)
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"kv4_attn: {heads} query heads over {cache.kv_heads} kv heads")
+    if not 1 <= max_ctx <= cache.cap or chunk < 128 or chunk % 128:
+        raise ValueError(f"kv4_attn: max_ctx {max_ctx} must be in [1, {cache.cap}] and chunk {chunk} a multiple of 128")
+    dev = _one_device(q, out, cache.k, slots, pos, workspace)
+    ws, ws_bytes = 0, 0
+    if workspace is not None:
+        if not workspace.is_contiguous() or workspace.data_ptr() % 16:
+            raise ValueError("kv4_attn: the workspace must be contiguous and 16-byte aligned")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if max_ctx > chunk and ws_bytes < kv4_attn_workspace(rows, heads, cache.head_dim, max_ctx, chunk):
+        raise ValueError(f"kv4_attn: a workspace of {kv4_attn_workspace(rows, heads, cache.head_dim, max_ctx, chunk)} "
+                         f"bytes is needed, got {ws_bytes}")
+    _call_on(dev, "kv4_attn", q.data_ptr(), q.stride(0), q.stride(1), *cache._ptrs(), out.data_ptr(), out.stride(0),
+             out.stride(1), slots.data_ptr(), pos.data_ptr(), float(scale), rows, heads, cache.slots, cache.kv_heads,
+             cache.head_dim, cache.cap, int(max_ctx), int(chunk), ws, ws_bytes, _DT[q.dtype])
+
+
+class PackedWeight4:
+    """An [N, K] weight in 4 bits (format and layout: include/m3x.h): uint8 codes [tiles, steps, 64, 16] and scales
+    [tiles, ceil(steps / 4), 64, 4], tiles of 16 rows and steps of 128 inputs."""
+    __slots__ = ("codes", "scales", "N", "K")
+
+    def __init__(self, codes, scales, N, K):
+        if N < 1 or K < 32 or K % 32:
+            raise ValueError(f"PackedWeight4: K={K} must be a multiple of 32")
+        tiles, steps = -(-N // 16), -(-K // 128)
+        for t, shape, name in ((codes, (tiles, steps, 64, 16), "codes"), (scales, (tiles, -(-steps // 4), 64, 4), "scales")):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"PackedWeight4: {name} must be contiguous, aligned uint8 {shape}, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        self.codes, self.scales, self.N, self.K = codes, scales, N, K
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def rows(self, start, stop):
+        """Rows [start, stop) as their own packed weight (start % 16 == 0); shares storage. A stop inside a tile leaves
+        the tile's other rows in place, unused."""
+        if start % 16 or not 0 <= start < stop <= self.N:
+            raise ValueError(f"rows({start}, {stop}) of a packed [{self.N}, {self.K}] weight")
+        a, b = start // 16, -(-stop // 16)
+        return PackedWeight4(self.codes[a:b], self.scales[a:b], stop - start, self.K)
+
+    def memory_bytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def pack_weight4(w):
+    """w [N, K] (bf16, fp16 or fp32; row stride % 8 == 0, K % 32 == 0) in 4 bits; one launch on the current stream."""
+    _rows2d(w, "w")
+    N, K = w.shape
+    if N < 1 or K < 32 or K % 32:
+        raise ValueError(f"pack_weight4: K={K} must be a multiple of 32")
+    if w.stride(0) % 8 or w.data_ptr() % 16:
+        raise ValueError(f"pack_weight4: w needs 16-byte aligned rows (stride {w.stride(0)})")
+    dt, dev = _dt3(w), _one_device(w)
+    tiles, steps = -(-N // 16), -(-K // 128)
+    codes = torch.empty(tiles, steps, 64, 16, dtype=torch.uint8, device=dev)
+    scales = torch.empty(tiles, -(-steps // 4), 64, 4, dtype=torch.uint8, device=dev)
+    _call_on(dev, "pack_weight4", w.data_ptr(), w.stride(0), N, K, codes.data_ptr(), scales.data_ptr(), dt)
+    return PackedWeight4(codes, scales, N, K)
+
+
+def _lin4_args(name, x, w, y):
+    if not isinstance(w, PackedWeight4):
+        raise TypeError(f"{name}: the weight must be packed with ops.pack_weight4")
+    if x.dim() != 2 or x.shape[1] != w.K or x.dtype not in _DT:
+        raise ValueError(f"{name}: x must be bfloat16 or float16 [rows, {w.K}], got {x.dtype} {tuple(x.shape)}")
+    M = x.shape[0]
+    if M and (x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16):
+        raise ValueError(f"{name}: x needs 16-byte aligned rows (strides {x.stride()})")
+    if y is None:
+        y = torch.empty(M, w.N, dtype=x.dtype, device=x.device)
+    elif tuple(y.shape) != (M, w.N) or y.dtype != x.dtype or (y.numel() and y.stride(1) != 1):
+        raise ValueError(f"{name}: y must be {x.dtype} {(M, w.N)} with a contiguous last dimension, got {y.dtype} "
+                         f"{tuple(y.shape)}")
+    return M, y
+
+
+def linear4(x, w, y=None):
+    """y = x @ W.T for rows x [M, K] (bf16 or fp16) and a weight packed by pack_weight4; the 4-bit form of `linear`
+    for few rows. Returns y [M, N] (new unless given)."""
+    M, y = _lin4_args("linear4", x, w, y)
+    dev = _one_device(x, w.codes, w.scales, y)
+    _call_on(dev, "linear4", x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), y.data_ptr(),
+             y.stride(0), M, w.N, w.K, _DT[x.dtype])
+    return y
+
+
+def linear4_act(x, w_gate, w_up, kind, y=None):
+    """SWIGLU: y = silu(x @ Wg.T) * (x @ Wu.T); GELU: y = gelu(x @ Wg.T) (w_up None); the 4-bit form of `linear_act`,
+    rounded once."""
+    M, y = _lin4_args("linear4_act", x, w_gate, y)
+    if kind not in (ACT_SWIGLU, ACT_GELU):
+        raise ValueError("linear4_act: kind must be ACT_SWIGLU or ACT_GELU")
+    u = (0, 0)
+    if kind == ACT_SWIGLU:
+        if not isinstance(w_up, PackedWeight4) or (w_up.N, w_up.K) != (w_gate.N, w_gate.K):
+            raise ValueError("linear4_act: w_up must be a packed weight of w_gate's shape")
+        u = (w_up.codes.data_ptr(), w_up.scales.data_ptr())
+    dev = _one_device(x, w_gate.codes, w_gate.scales, None if w_up is None else w_up.codes,
+                      None if w_up is None else w_up.scales, y)
+    _call_on(dev, "linear4_act", x.data_ptr(), x.stride(0), w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), *u,
+             y.data_ptr(), y.stride(0), M, w_gate.N, w_gate.K, kind, _DT[x.dtype])
+    return y
+
+
 # ---------------------------------------------------------------- Mimi decode (serve/fast_codec.py)
 def rvq_decode(codes, tables, out):
     """out[b] = [table_0[codes[b, 0]] | sum over q >= 1 of table_q[codes[b, q]]]; tables [nq, n_codes, dim]."""
