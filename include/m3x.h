@@ -519,26 +519,32 @@ int m3x_backbone_run(const M3xBackboneRun* args, void* stream);
  *   ks4 [slots][kv_heads][cap][D / 32]              scale bytes
  *   v4  [slots][kv_heads][cap / 4][16][4][D / 32]   four positions together; chunk c: dims c D/16 .. (c + 1) D/16 - 1
  *   vs4 [slots][kv_heads][cap / 4][D / 32][4]       scale bytes
- * A row whose slot is outside [0, nslots) or whose position is outside [0, cap) is outside the cache. */
+ * A row whose slot is outside [0, slots) or whose position is outside [0, cap) is outside the cache. */
+typedef struct M3xKv4 {
+  void* k;  /* k4 */
+  void* ks; /* ks4 */
+  void* v;  /* v4 */
+  void* vs; /* vs4 */
+  int slots, kv_heads, head_dim, cap;
+} M3xKv4;
+
+/* The struct is on the host and read during the call. */
 
 /* K and V rows [rows, kv_heads, D] (row and head strides % 8 == 0) quantised to position pos[r] of slot slots[r]; a
  * row outside the cache is not written. Rows of one call at the same place leave either row's bytes there. */
-int m3x_kv4_append(const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h, void* k4, void* ks4,
-                   void* v4, void* vs4, const int64_t* slots, const int32_t* pos, int rows, int nslots, int kv_heads,
-                   int head_dim, int cap, int dtype, void* stream);
+int m3x_kv4_append(const M3xKv4* cache, const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h,
+                   const int64_t* slots, const int32_t* pos, int rows, int dtype, void* stream);
 
 /* m3x_qk_norm_rope_cache over the 4-bit cache: q_out and the rotated bf16 keys have its bits, and keys and values are
  * quantised as m3x_kv4_append does (the RoPE row of a position outside the tables is the nearest one's). bf16. */
-int m3x_qk_norm_rope_kv4(const void* qkv, long s_qkv, void* q_out, long s_qo_b, long s_qo_h, void* k4, void* ks4,
-                         void* v4, void* vs4, const int64_t* slots, const int32_t* pos, const void* cos,
-                         const void* sin, long s_cos, const void* wq, const void* wk, float eps, int rows, int heads,
-                         int nslots, int kv_heads, int head_dim, int cap, void* stream);
+int m3x_qk_norm_rope_kv4(const M3xKv4* cache, const void* qkv, long s_qkv, void* q_out, long s_qo_b, long s_qo_h,
+                         const int64_t* slots, const int32_t* pos, const void* cos, const void* sin, long s_cos,
+                         const void* wq, const void* wk, float eps, int rows, int heads, void* stream);
 
 /* k[r], v[r] ([kv_heads, D] 16-bit, strides % 8 == 0) = the numbers at position pos[r] of slot slots[r], zeros for a
  * row outside the cache. Exact where the type holds the number (bf16 always, fp16 for a cache written from fp16). */
-int m3x_kv4_read(const void* k4, const void* ks4, const void* v4, const void* vs4, const int64_t* slots,
-                 const int32_t* pos, void* k, long sk_r, long sk_h, void* v, long sv_r, long sv_h, int rows, int nslots,
-                 int kv_heads, int head_dim, int cap, int dtype, void* stream);
+int m3x_kv4_read(const M3xKv4* cache, const int64_t* slots, const int32_t* pos, void* k, long sk_r, long sk_h, void* v,
+                 long sv_r, long sv_h, int rows, int dtype, void* stream);
 
 /* Bytes of workspace m3x_kv4_attn needs (0 when max_ctx <= chunk). */
 size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, int chunk);
@@ -546,13 +552,12 @@ size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, in
 /* out[r, h] = softmax(scale q[r, h] . K^T) V over positions 0 .. pos[r] of slot slots[r], kv head h / (heads /
  * kv_heads); q and out [rows, heads, D] 16-bit (strides % 8 == 0, 16-byte aligned). pos[r] < 0 or a slot outside the
  * cache: zeros. max_ctx >= pos[r] + 1 for every row (keys past it are not attended), <= cap; chunk = keys per split,
- * a multiple of 128. What a row does not see has no part in its result, whatever it holds. Rows next to each other in
+ * a multiple of 128; at most 2^20 rows and 65535 splits. What a row does not see has no part in its result, whatever it holds. Rows next to each other in
  * the call, of one slot at consecutive positions (a prompt's), share one pass over the keys; a row's bits do not
  * depend on that, and not on the other rows. Fixed summation order. */
-int m3x_kv4_attn(const void* q, long sq_b, long sq_h, const void* k4, const void* ks4, const void* v4, const void* vs4,
-                 void* out, long so_b, long so_h, const int64_t* slots, const int32_t* pos, float scale, int rows,
-                 int heads, int nslots, int kv_heads, int head_dim, int cap, int max_ctx, int chunk, void* workspace,
-                 size_t ws_bytes, int dtype, void* stream);
+int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
+                 const int64_t* slots, const int32_t* pos, float scale, int rows, int heads, int max_ctx, int chunk,
+                 void* workspace, size_t ws_bytes, int dtype, void* stream);
 
 /* A weight [N, K] (K % 32 == 0) in 4 bits, groups along K: N in tiles of 16 rows (zero rows behind N), K in steps of
  * 128 (zeros behind K).

@@ -44,74 +44,87 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[t][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  for (int s = s0; s < s1; ++s) {
+  struct Step {
     fp4_u4 cw[TW * P];
     uint32_t sw[TW * P];
+    u16x8 x[MT][4];
+  };
+  auto load = [&](Step& q, int s) {
 #pragma unroll
     for (int t = 0; t < TW * P; ++t) {
       const long tile = min(tile0 + t / P, a.tiles - 1);  // a tile past the last repeats it and is not stored
-      cw[t] = __builtin_nontemporal_load(
+      q.cw[t] = __builtin_nontemporal_load(
           reinterpret_cast<const fp4_u4*>(a.w[t % P] + ((tile * a.steps + s) * 64 + lane) * 16));
-      sw[t] = *reinterpret_cast<const uint32_t*>(a.s[t % P] + ((tile * quads + (s >> 2)) * 64 + lane) * 4);
+      q.sw[t] = *reinterpret_cast<const uint32_t*>(a.s[t % P] + ((tile * quads + (s >> 2)) * 64 + lane) * 4);
     }
-    u16x8 xv[MT][4];
     const int k = 128 * s + 32 * lg;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r = m0 + 16 * m + li;
       if (r < a.M && k < a.K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[m][i] = ld16(a.x + (long)r * a.ldx + k + 8 * i);
+        for (int i = 0; i < 4; ++i) q.x[m][i] = ld16(a.x + (long)r * a.ldx + k + 8 * i);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[m][i] = zero_v8<DT>();
+        for (int i = 0; i < 4; ++i) q.x[m][i] = zero_v8<DT>();
       }
     }
+  };
+  auto multiply = [&](const Step& q, int s) {
 #pragma unroll
     for (int t = 0; t < TW * P; ++t) {
-      const float sc = fp4_scale((sw[t] >> (8 * (s & 3))) & 255u);
+      const float sc = fp4_scale((q.sw[t] >> (8 * (s & 3))) & 255u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u16x8 wv = fp4_eight<DT>(cw[t][i], sc);
+        const u16x8 wv = fp4_eight<DT>(q.cw[t][i], sc);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[t][m] = mfma16x16x32<DT>(wv, xv[m][i], acc[t][m]);
+        for (int m = 0; m < MT; ++m) acc[t][m] = mfma16x16x32<DT>(wv, q.x[m][i], acc[t][m]);
       }
     }
+  };
+  for (int s = s0; s < s1; ++s) {
+    Step q;
+    load(q, s);
+    multiply(q, s);
   }
 
-  __shared__ f32x4_t red[NW][TW * P * MT][64];
+  // as many output tiles at a time as 64 KB hold the waves' sums of
+  constexpr int RT = NW * P * MT * TW <= 64 ? TW : 64 / (NW * P * MT);
+  __shared__ f32x4_t red[NW][RT * P * MT][64];
 #pragma unroll
-  for (int t = 0; t < TW * P; ++t)
+  for (int t0 = 0; t0 < TW; t0 += RT) {
+    if (t0) __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MT; ++m) red[wave][t * MT + m][lane] = acc[t][m];
-  __syncthreads();
-  for (int f = wave; f < TW * MT; f += NW) {
-    const int t = f / MT, m = f % MT;
-    f32x4_t v[P];
+    for (int i = 0; i < RT * P * MT; ++i) red[wave][i][lane] = acc[t0 * P + i / MT][i % MT];
+    __syncthreads();
+    for (int f = wave; f < RT * MT; f += NW) {
+      const int t = f / MT, m = f % MT;
+      f32x4_t v[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      v[p] = red[0][(t * P + p) * MT + m][lane];
+      for (int p = 0; p < P; ++p) {
+        v[p] = red[0][(t * P + p) * MT + m][lane];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) v[p] += red[w][(t * P + p) * MT + m][lane];
-    }
-    const int row = m0 + 16 * m + li;
-    const int n = 16 * (tile0 + t) + 4 * lg;
-    if (row >= a.M || n >= a.N) continue;
-    uint16_t o[4];
+        for (int w = 1; w < NW; ++w) v[p] += red[w][(t * P + p) * MT + m][lane];
+      }
+      const int row = m0 + 16 * m + li;
+      const int n = 16 * (tile0 + t0 + t) + 4 * lg;
+      if (row >= a.M || n >= a.N) continue;
+      uint16_t o[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float y = v[0][r];
-      if constexpr (ACT == L4_SWIGLU) y = silu16(y) * v[P - 1][r];
-      if constexpr (ACT == L4_GELU) y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
-      o[r] = E<DT>::from_f(y);
-    }
-    uint16_t* yp = a.y + (long)row * a.ldy + n;
-    if (n + 4 <= a.N && (((uintptr_t)yp) & 7) == 0) {
-      *reinterpret_cast<uint2*>(yp) = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
-    } else {
+      for (int r = 0; r < 4; ++r) {
+        float y = v[0][r];
+        if constexpr (ACT == L4_SWIGLU) y = silu16(y) * v[P - 1][r];
+        if constexpr (ACT == L4_GELU) y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
+        o[r] = E<DT>::from_f(y);
+      }
+      uint16_t* yp = a.y + (long)row * a.ldy + n;
+      if (n + 4 <= a.N && (((uintptr_t)yp) & 7) == 0) {
+        *reinterpret_cast<uint2*>(yp) = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < a.N) yp[r] = o[r];
+        for (int r = 0; r < 4; ++r)
+          if (n + r < a.N) yp[r] = o[r];
+      }
     }
   }
 }
@@ -194,9 +207,25 @@ template <int DT, int TW, int MT, int NW, int ACT> void launch4(const Lin4& a, h
                      dim3(64 * NW), 0, st, a);
 }
 template <int DT, int ACT> void plan4(const Lin4& a, hipStream_t st) {
-  if (a.M <= 16) launch4<DT, 1, 1, 8, ACT>(a, st);
-  else if (a.M <= 32) launch4<DT, 1, 2, 8, ACT>(a, st);
-  else launch4<DT, 1, 4, 8, ACT>(a, st);
+  // x meets every group of weight tiles anew, from L2 and in 16-byte pieces of 64-byte lines, so a workgroup takes as
+  // many tiles, then rows, as leave each of the 256 CUs one. Measured on MI355X (graph-timed, us; TW x MT x NW, the
+  // rule's first): N 16384, K 8192: 9 rows 4x1x16 16.0, 2x1x8 17.4, 1x1x8 25.0; 32 rows 4x2x8 24, 4x1x8 32, 1x1x8 66;
+  // 64 rows 8x2x8 33, 4x4x4 37, 4x1x8 56, 1x1x8 128. N 4096, K 4096: 16 rows 1x1x8 6.7, 2x1x8 7.4, 4x1x8 9.1; 32 rows
+  // 2x1x8 7.6, 1x1x8 10.9; 64 rows 4x1x8 9.6, 1x1x8 18.7. N 4096, K 1024, one row: 1x1x8 2.8, 2x1x8 3.0, 4x1x8 3.6.
+  const int blocks = m3x_ceil_div(a.M, 16);
+  const long share = (long)a.tiles * blocks / 256;
+  if (share < 2) launch4<DT, 1, 1, 8, ACT>(a, st);
+  else if (share < 4) launch4<DT, 2, 1, 8, ACT>(a, st);
+  else if (blocks == 1 || share < 8) {
+    if constexpr (ACT == L4_SWIGLU) {
+      if (blocks == 1) launch4<DT, 4, 1, 8, ACT>(a, st);  // 16384 x 8192 twice, 16 rows: 32.5, 2x1x8 33.6
+      else launch4<DT, 2, 2, 8, ACT>(a, st);              // 8192 x 4096 twice, 32 rows: 15.0, 4x1x8 16.8
+    } else {
+      launch4<DT, 4, 1, 16, ACT>(a, st);
+    }
+  } else if (blocks == 2 || share < 16) launch4<DT, 4, 2, 8, ACT>(a, st);
+  else if constexpr (ACT == L4_SWIGLU) launch4<DT, 4, 4, 4, ACT>(a, st);  // 16384 x 8192 twice, 64 rows: 51, 4x2x8 70
+  else launch4<DT, 8, 2, 8, ACT>(a, st);
 }
 int linear4_any(const void* x, long ldx, const void* wg, const void* sg, const void* wu, const void* su, void* y,
                 long ldy, int M, int N, int K, int act, int dtype, void* stream) {
@@ -207,7 +236,7 @@ int linear4_any(const void* x, long ldx, const void* wg, const void* sg, const v
   if (!x || !wg || !sg || !y || (act == L4_SWIGLU && (!wu || !su))) return M3X_ENULL;
   if ((ldx & 7) || !m3x_aligned16(x) || !m3x_aligned16(wg) || !m3x_aligned16(sg) || ((uintptr_t)y & 1)) return M3X_EINVAL;
   if (act == L4_SWIGLU && (!m3x_aligned16(wu) || !m3x_aligned16(su))) return M3X_EINVAL;
-  if (M > 65535 * 16) return M3X_EINVAL;
+  if (M > 65535 * 16 || N > (1 << 26)) return M3X_EINVAL;  // launches of fewer than 2^32 threads
   const Lin4 a = {(const uint16_t*)x, ldx, {(const uint8_t*)wg, (const uint8_t*)wu},
                   {(const uint8_t*)sg, (const uint8_t*)su}, (uint16_t*)y, ldy, M, N, K, m3x_ceil_div(K, 128),
                   m3x_ceil_div(N, 16)};

@@ -9,8 +9,27 @@
 //                               16-byte load (8 at D = 64), and 16 positions are one contiguous load of a wave, so V
 //                               needs no transpose through LDS; a position's write stays whole words.
 //   vs  [cap / 4][D / 32][4]    the four positions' bytes of a group are one word
+#include <algorithm>
+#include <type_traits>
+
 #include "m3x_norm.h"
 #include "m3x_fp4.h"
+
+#ifndef KV4_OCC
+#define KV4_OCC 3
+#endif
+#ifndef KV4_NW
+#define KV4_NW 4
+#endif
+
+// mirror of M3xKv4 (include/m3x.h)
+struct M3xKv4 {
+  void* k;
+  void* ks;
+  void* v;
+  void* vs;
+  int slots, kv_heads, head_dim, cap;
+};
 
 namespace {
 struct Kv4 {
@@ -148,7 +167,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 // A workgroup takes one (block of rows, kv head, split of the keys). The score product has the keys as its rows and
 // 16 columns: the G query heads of up to 16 / G rows that stand next to each other in the call, of one slot at
 // consecutive positions (a prompt's), found from slots and pos by the workgroup itself; the block's later rows' own
-// workgroups leave at once. A single token is a block of one row. Each of the 4 waves takes every 4th 32-key tile:
+// workgroups leave at once. A single token is a block of one row. Each of the NW waves takes every NW-th 32-key tile:
 //   S^T = K . Q^T   per 16 keys D / 32 MFMA 16x16x32: a lane's words of K become 16-bit operands in registers
 //   softmax         running maximum and sum in fp32, exp2; a lane keeps its own column's, its keys' partial sum
 //   O^T += V^T . P  D / 16 MFMA per 32 keys: S^T's accumulator is the P operand as it stands, and V's words, which
@@ -157,14 +176,15 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 // between the loads and the output is exact or fp32.
 namespace {
 template <int NI> struct Words { uint32_t w[NI]; };
-template <int NI> __device__ __forceinline__ Words<NI> kv4_load(const uint8_t* p) {
+// `base` is the same in every lane, so the load takes a scalar address and a 32-bit lane offset
+template <int NI> __device__ __forceinline__ Words<NI> kv4_load(const uint8_t* base, uint32_t off) {
   Words<NI> r;
   if constexpr (NI == 4) {
-    const fp4_u4 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u4*>(p));
+    const fp4_u4 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u4*>(base + off));
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.w[i] = x[i];
   } else {
-    const fp4_u2 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u2*>(p));
+    const fp4_u2 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u2*>(base + off));
     r.w[0] = x[0];
     r.w[1] = x[1];
   }
@@ -179,18 +199,29 @@ struct Kv4Attn {
   const int64_t* slots;
   const int32_t* pos;
   float scale_log2;
-  int rows, heads, G, hblocks, chunk, max_ctx, max_splits;
+  int rows, heads, G, hblocks, qb, R, nblk, chunk, max_ctx, max_splits;
+  uint32_t over_Gc;  // x * over_Gc >> 8 = x / min(G, 16) for x < 16
   float* part;  // [rows * heads][max_splits][D] then [rows * heads][max_splits][2] (maximum, sum)
 };
 
-// the A operand of dim tile T: element e is the number of dim T of the lane's chunk at key e
-template <int DT, int D, int T>
-__device__ __forceinline__ void kv4_vop(const Words<D / 32> (&v)[2], const float (&sc)[8], u16x8& lo, u16x8& hi) {
+// four outputs O / L (one quotient: its rounding and the products' are fp32's)
+template <int DT> __device__ __forceinline__ void kv4_store_out(uint16_t* p, const f32x4_t& O, float L) {
+  const float r = 1.f / L;
+  *reinterpret_cast<uint2*>(p) = make_uint2(E<DT>::from_f(O[0] * r) | (uint32_t)E<DT>::from_f(O[1] * r) << 16,
+                                            E<DT>::from_f(O[2] * r) | (uint32_t)E<DT>::from_f(O[3] * r) << 16);
+}
+
+// the A operands of dim tiles 2 B and 2 B + 1 over 32 keys (two 16-key groups' words v0, v1 and scale words s0, s1):
+// element e is the number of dim 2 B (+ 1) of the lane's chunk at key e
+template <int DT, int D, int B>
+__device__ __forceinline__ void kv4_vop(const Words<D / 32>& v0, const Words<D / 32>& v1, uint32_t s0, uint32_t s1,
+                                        u16x8& lo, u16x8& hi) {
   uint32_t a[8];
-#define KV4_PAIR(E)                                                                                             \
-  if constexpr (D == 128) a[E] = fp4_pair<DT, T>(v[E / 4].w[E & 3], sc[E]);                                    \
-  else a[E] = fp4_pair<DT, 2 * (E & 1) + T>(v[E / 4].w[(E & 3) >> 1], sc[E]);
-  KV4_PAIR(0) KV4_PAIR(1) KV4_PAIR(2) KV4_PAIR(3) KV4_PAIR(4) KV4_PAIR(5) KV4_PAIR(6) KV4_PAIR(7)
+#define KV4_PAIR(E, V, S)                                                                              \
+  if constexpr (D == 128) a[E] = fp4_pair<DT, B>(V.w[E & 3], fp4_scale_of<E & 3>(S));                 \
+  else a[E] = fp4_pair<DT, 2 * (E & 1) + B>(V.w[(E & 3) >> 1], fp4_scale_of<E & 3>(S));
+  KV4_PAIR(0, v0, s0) KV4_PAIR(1, v0, s0) KV4_PAIR(2, v0, s0) KV4_PAIR(3, v0, s0)
+  KV4_PAIR(4, v1, s1) KV4_PAIR(5, v1, s1) KV4_PAIR(6, v1, s1) KV4_PAIR(7, v1, s1)
 #undef KV4_PAIR
   fp4_u4 l, h;
 #pragma unroll
@@ -202,78 +233,38 @@ __device__ __forceinline__ void kv4_vop(const Words<D / 32> (&v)[2], const float
   hi = __builtin_bit_cast(u16x8, h);
 }
 
-template <int DT, int D, int B = 0>
-__device__ __forceinline__ void kv4_pv(const Words<D / 32> (&v)[2], const float (&sc)[8], const u16x8& pop,
-                                       f32x4_t (&acc)[D / 16]) {
-  u16x8 lo, hi;
-  kv4_vop<DT, D, B>(v, sc, lo, hi);
-  acc[2 * B] = mfma16x16x32<DT>(lo, pop, acc[2 * B]);
-  acc[2 * B + 1] = mfma16x16x32<DT>(hi, pop, acc[2 * B + 1]);
-  if constexpr (B + 1 < D / 32) kv4_pv<DT, D, B + 1>(v, sc, pop, acc);
+template <int DT, int D, int NG, int B = 0>
+__device__ __forceinline__ void kv4_pv(const Words<D / 32> (&v)[NG], const uint32_t (&vs)[NG],
+                                       const u16x8 (&pop)[NG / 2], f32x4_t (&acc)[D / 16]) {
+#pragma unroll
+  for (int h = 0; h < NG / 2; ++h) {
+    u16x8 lo, hi;
+    kv4_vop<DT, D, B>(v[2 * h], v[2 * h + 1], vs[2 * h], vs[2 * h + 1], lo, hi);
+    acc[2 * B] = mfma16x16x32<DT>(lo, pop[h], acc[2 * B]);
+    acc[2 * B + 1] = mfma16x16x32<DT>(hi, pop[h], acc[2 * B + 1]);
+  }
+  if constexpr (B + 1 < D / 32) kv4_pv<DT, D, NG, B + 1>(v, vs, pop, acc);
 }
 
-// the same where a key that a row of the block does not see may be no number: for each row in turn the keys past its
-// limit (lim0 + j, at most lim; key0 = the lane's first key) are cleared, and its columns take the result
-template <int DT, int D, int B = 0>
-__device__ __forceinline__ void kv4_pv_rows(const Words<D / 32> (&v)[2], const float (&sc)[8], const u16x8& pop,
-                                            f32x4_t (&acc)[D / 16], int n, int jq, int key0, int lim0, int lim) {
-  u16x8 lo, hi;
-  kv4_vop<DT, D, B>(v, sc, lo, hi);
-  for (int j = 0; j < n; ++j) {
-    const int klim = min(lim, lim0 + j);
-    u16x8 l, h;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool off = key0 + 16 * (e >> 2) + (e & 3) > klim;
-      l.v[e] = off ? 0 : lo.v[e];
-      h.v[e] = off ? 0 : hi.v[e];
-    }
-    const f32x4_t x = mfma16x16x32<DT>(l, pop, acc[2 * B]), y = mfma16x16x32<DT>(h, pop, acc[2 * B + 1]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      acc[2 * B][r] = jq == j ? x[r] : acc[2 * B][r];
-      acc[2 * B + 1][r] = jq == j ? y[r] : acc[2 * B + 1][r];
-    }
-  }
-  if constexpr (B + 1 < D / 32) kv4_pv_rows<DT, D, B + 1>(v, sc, pop, acc, n, jq, key0, lim0, lim);
-}
 }  // namespace
 
-template <int DT, int D>
-__global__ __launch_bounds__(256, 3) void kv4_attn_kernel(Kv4 c, Kv4Attn a) {
+// one block: rows row .. row + n - 1 of slot `slot`, the first at position p0
+template <int D, int NW> struct Kv4Lds {
+  __align__(16) float o[NW][16][D + 4];
+  float m[NW][16], l[NW][16];
+};
+template <int DT, int D, int NW>
+__device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int row, int n, long slot, int p0, int kh,
+                                             int h0, int Gc, int split, int wave, int lane, Kv4Lds<D, NW>& lds) {
   constexpr int NI = D / 32;   // words a lane holds of 16 keys; score steps
   constexpr int ND = D / 16;   // dim tiles
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  constexpr int KT = 32, NG = KT / 16;  // keys of a tile, and its 16-key groups
   const int li = lane & 15, lg = lane >> 4;
-  const int row = blockIdx.x;
-  const int kh = blockIdx.y / a.hblocks;
-  const int h0 = (blockIdx.y % a.hblocks) * 16;  // first query head of the block within the kv head's G
-  const int Gc = min(a.G - h0, 16);
-  const int split = blockIdx.z;
-
-  // the block: rows row .. row + n - 1
-  const int qb = a.hblocks > 1 ? 1 : 16 / Gc;
-  const int ri = row - 1 + lane;
-  const int rc = min(max(ri, 0), a.rows - 1);
-  const long slot_i = a.slots[rc];
-  const int pos_i = a.pos[rc];
-  // the exchanges stand before the conditions: a lane that a condition leaves out gives its neighbour no value
-  const long slot_b = __shfl_up(slot_i, 1, 64);
-  const int pos_b = __shfl_up(pos_i, 1, 64);
-  const bool follows = lane > 0 && lane <= qb && ri < a.rows && ri % qb != 0 && slot_b == slot_i && pos_i > 0 &&
-                       pos_b == pos_i - 1;
-  const uint64_t chain = __ballot(follows);  // bit i: row - 1 + i continues the row before it
-  if (chain & 2u) return;
-  const int n = 1 + __builtin_ctzll(~(chain >> 2));
-  const long slot = __shfl(slot_i, 1, 64);
-  const int p0 = __builtin_amdgcn_readfirstlane(__shfl(pos_i, 1, 64));
   const int plim = min(c.cap, a.max_ctx) - 1;  // the host keeps pos below both; every access stays inside whatever pos holds
-  const bool inside = __builtin_amdgcn_readfirstlane(slot >= 0 && slot < c.slots && p0 >= 0);
-  if (!inside) {  // no key: zeros
+  if (slot < 0 || slot >= c.slots || p0 < 0) {  // no key: zeros
     if (split == 0)
       for (int j = 0; j < n; ++j)
-        for (int i = threadIdx.x; i < Gc * D; i += 256)
+        for (int i = threadIdx.x; i < Gc * D; i += 64 * NW)
           a.out[(long)(row + j) * a.so_b + (long)(kh * a.G + h0 + i / D) * a.so_h + i % D] = 0;
     return;
   }
@@ -282,159 +273,221 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_kernel(Kv4 c, Kv4Attn a) {
   if (kstart > plast) return;
   const int kend = min(kstart + a.chunk, plast + 1);
 
-  const int jq = li / Gc;  // the column's row within the block
-  const int hq = li - jq * Gc;
-  const bool live = jq < n;
+  const int jq = li * a.over_Gc >> 8;  // the column's row within the block
+  const int hq = li - jq * min(a.G, 16);
+  const bool live = jq < n && hq < Gc;
   const int pq = live ? min(p0 + jq, plim) : -1;  // the column sees keys <= pq
-  u16x8 qop[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    if (live) {
-      qop[i] = ld16(a.q + (long)(row + jq) * a.sq_b + (long)(kh * a.G + h0 + hq) * a.sq_h + (D / 4) * lg + 8 * i);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qop[i].v[e] = 0;
-    }
-  }
-
   const long base = (slot * c.kv_heads + kh) * (long)c.cap;
-  const uint8_t* kb = c.k + base * (D / 2) + li * (D / 2) + lg * (D / 8);
-  const uint8_t* ksb = c.ks + base * NI + li * NI + (D == 128 ? lg : lg >> 1);
-  const uint8_t* vb = c.v + base * (D / 2) + lg * (2 * D) + li * (D / 8);
-  const uint8_t* vsb = c.vs + base * NI + lg * (4 * NI) + (D == 128 ? li >> 2 : li >> 3) * 4;
-  Words<NI> kw[2], vw[2];
-  uint32_t ks[2], vs[2];
-  auto load_k = [&](int k0) {
+  // scale bytes come as whole words (a byte's widening would be waited for where it is loaded): the key's four at
+  // D = 128, two keys' two each at D = 64; ks_rot brings the lane's byte to the exponent's place
+  const uint32_t k_at = li * (D / 2) + lg * (D / 8), ks_at = (li * NI) & ~3;
+  const int ks_rot = (23 - 8 * (D == 128 ? lg : 2 * (li & 1) + (lg >> 1))) & 31;
+  const uint32_t v_at = lg * (2 * D) + li * (D / 8), vs_at = lg * (4 * NI) + (D == 128 ? li >> 2 : li >> 3) * 4;
+  // a column past the block's rows computes with the first row's queries and is dropped
+  u16x8 qop[NI];
+  const uint16_t* qp = a.q + (long)(row + (live ? jq : 0)) * a.sq_b + (long)(kh * a.G + h0 + (live ? hq : 0)) * a.sq_h;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      kw[g] = kv4_load<NI>(kb + (long)(k0 + 16 * g) * (D / 2));
-      ks[g] = ksb[(long)(k0 + 16 * g) * NI];
-    }
+  for (int i = 0; i < NI; ++i) qop[i] = ld16(qp + (D / 4) * lg + 8 * i);
+  // Two tiles' words in turn: a tile's keys are loaded two tiles ahead, behind the products of the keys they replace, its
+  // values likewise. The pointers stand at the tile to be loaded next and are the same in every lane: a load takes them
+  // as its scalar address, beside the lane's 32-bit offset. Loads are never conditional (one whose registers are
+  // merged behind a branch is waited for there): past the wave's last tile they repeat it. cap % 32 == 0: a tile that
+  // begins inside the slot ends inside it.
+  struct Buf {
+    Words<NI> kw[NG], vw[NG];
+    uint32_t ks[NG], vs[NG];
   };
-  auto load_v = [&](int k0) {
+  int k0 = kstart + KT * wave;
+  const long tile0 = base + min(k0, (kend - 1) & ~(KT - 1));
+  const uint8_t* kp = c.k + tile0 * (D / 2);
+  const uint8_t* ksp = c.ks + tile0 * NI;
+  const uint8_t* vp = c.v + tile0 * (D / 2);
+  const uint8_t* vsp = c.vs + tile0 * NI;
+  int kn = k0, vn = k0;
+  auto load_k = [&](Buf& t) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      vw[g] = kv4_load<NI>(vb + (long)(k0 + 16 * g) * (D / 2));
-      vs[g] = *reinterpret_cast<const uint32_t*>(vsb + (long)(k0 + 16 * g) * NI);
+    for (int g = 0; g < NG; ++g) {
+      t.kw[g] = kv4_load<NI>(kp + g * (8 * D), k_at);
+      t.ks[g] = *reinterpret_cast<const uint32_t*>(ksp + g * (16 * NI) + ks_at);
     }
+    kn += KT * NW;
+    const int step = kn < kend ? KT * NW : 0;
+    kp += step * (D / 2);
+    ksp += step * NI;
   };
+  auto load_v = [&](Buf& t) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      t.vw[g] = kv4_load<NI>(vp + g * (8 * D), v_at);
+      t.vs[g] = *reinterpret_cast<const uint32_t*>(vsp + g * (16 * NI) + vs_at);
+    }
+    vn += KT * NW;
+    const int step = vn < kend ? KT * NW : 0;
+    vp += step * (D / 2);
+    vsp += step * NI;
+  };
+  Buf b0, b1;
+  __builtin_amdgcn_sched_barrier(0);  // the queries' loads stay first: the loop waits for them with the first keys
+  load_k(b0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(b0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_k(b1);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(b1);
+  __builtin_amdgcn_sched_barrier(0);
 
   float m_run = -INFINITY, l_run = 0.f;
   f32x4_t acc[ND];
 #pragma unroll
   for (int T = 0; T < ND; ++T) acc[T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  // a tile's keys are loaded while the tile before is weighted, its values while its keys are multiplied
-  // (cap % 32 == 0: a tile that begins inside the slot ends inside it)
-  int k0 = kstart + 32 * wave;
-  if (k0 < kend) {
-    load_k(k0);
-    load_v(k0);
-  }
-  for (; k0 < kend; k0 += 128) {
-    float sv[8];
+  const int full = min(p0 + 1, kend);  // keys below it are seen by every row of the block
+  auto tile = [&](Buf& t, int k0) {
+    const bool edge = k0 + KT > full;  // the tile is masked by column
+    float sv[4 * NG];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < NG; ++g) {
       f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-      const float sc = fp4_scale(ks[g]);
+      const float sc = __uint_as_float(__builtin_rotateleft32(t.ks[g], ks_rot));
 #pragma unroll
-      for (int i = 0; i < NI; ++i) s = mfma16x16x32<DT>(fp4_eight<DT>(kw[g].w[i], sc), qop[i], s);
+      for (int i = 0; i < NI; ++i) s = mfma16x16x32<DT>(fp4_eight<DT>(t.kw[g].w[i], sc), qop[i], s);
 #pragma unroll
       for (int r = 0; r < 4; ++r) sv[4 * g + r] = s[r] * a.scale_log2;
     }
-    const bool more = k0 + 128 < kend;
-    if (more) load_k(k0 + 128);
-    // the tile reaches past what the block's first row sees: mask by column
-    const bool edge = k0 + 31 > min(p0, plim);
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(t);
+    __builtin_amdgcn_sched_barrier(0);
+    int lane_o = lane;
     if (edge) {
+      asm volatile("" : "+v"(lane_o));  // what the masks need is made here, not kept over the loop
+      const int lg = lane_o >> 4;
       const int klim = min(kend - 1, pq);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 4 * NG; ++e)
         if (k0 + 16 * (e >> 2) + 4 * lg + (e & 3) > klim) sv[e] = -INFINITY;
     }
     float mx = sv[0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sv[e]);
+    for (int e = 1; e < 4 * NG; ++e) mx = fmaxf(mx, sv[e]);
     mx = fmaxf(m_run, xor32_max(xor16_max(mx)));
     const float mu = mx == -INFINITY ? 0.f : mx;  // no key seen yet: every weight is exp2(-inf) = 0
-    const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
+    if (__ballot(mx > m_run)) {  // a column's maximum grew
+      asm volatile("");  // keeps the products behind the branch
+      const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
+      l_run *= alpha;
+#pragma unroll
+      for (int T = 0; T < ND; ++T) acc[T] *= alpha;
+    }
     m_run = mx;
     // fp16 weights stand 2^15 higher (up to 32768), as do their sums: below 2^-14 fp16 loses relative precision, and
     // many keys of small weight would lose their part
     const float mp = mu - (DT == M3X_F16 ? 15.f : 0.f);
-    u16x8 pop;
+    u16x8 pop[NG / 2];
     float ps = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4 * NG; ++e) {
       const float p = __builtin_amdgcn_exp2f(sv[e] - mp);
       ps += p;
-      pop.v[e] = E<DT>::from_f(p);
+      pop[e / 8].v[e % 8] = E<DT>::from_f(p);
     }
-    l_run = l_run * alpha + ps;
-#pragma unroll
-    for (int T = 0; T < ND; ++T) acc[T] *= alpha;
-    float sc[8];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      sc[4 * g] = fp4_scale_of<0>(vs[g]);
-      sc[4 * g + 1] = fp4_scale_of<1>(vs[g]);
-      sc[4 * g + 2] = fp4_scale_of<2>(vs[g]);
-      sc[4 * g + 3] = fp4_scale_of<3>(vs[g]);
-    }
-    // 0 * V is 0 only for finite V: where a masked key may hold anything (stale or a later row's NaN), each row of the
-    // block takes the product with the keys it does not see cleared
-    bool bad = false;
+    l_run += ps;
+    // 0 * V is 0 only for finite V. Keys of an edge tile whose scale is past every written number's (stale bytes, or a
+    // NaN that a later row of the block may see) stand apart: cleared here, added below to the columns that see them.
+    uint32_t odd = 0;  // bit e: the lane's key e, in any of its groups
     if (edge) {
-      bool b = false;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b |= sc[e] > fp4_scale(fp4_top_of<DT>());
-      bad = __ballot(b) != 0;
+      for (int e = 0; e < 4 * NG; ++e) odd |= (t.vs[e / 4] >> (8 * (e & 3)) & 255u) > fp4_top_of<DT>() ? 1u << e : 0u;
+      if (__ballot(odd != 0)) {
+        odd |= __builtin_amdgcn_mov_dpp(odd, 0x128, 0xF, 0xF, false);  // row_ror 8, 4, 2, 1: over the lane's row of 16
+        odd |= __builtin_amdgcn_mov_dpp(odd, 0x124, 0xF, 0xF, false);
+        odd |= __builtin_amdgcn_mov_dpp(odd, 0x122, 0xF, 0xF, false);
+        odd |= __builtin_amdgcn_mov_dpp(odd, 0x121, 0xF, 0xF, false);
+#pragma unroll
+        for (int e = 0; e < 4 * NG; ++e)
+          if (odd >> e & 1u) {
+            t.vs[e / 4] &= ~(255u << (8 * (e & 3)));  // the smallest scale, of zeros
+            if constexpr (D == 128) t.vw[e / 4].w[e & 3] = 0;
+            else t.vw[e / 4].w[(e & 3) >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+          }
+      }
     }
-    if (!bad) kv4_pv<DT, D>(vw, sc, pop, acc);
-    else kv4_pv_rows<DT, D>(vw, sc, pop, acc, n, jq, k0 + 4 * lg, p0, kend - 1);
-    if (more) load_v(k0 + 128);
+    kv4_pv<DT, D, NG>(t.vw, t.vs, pop, acc);
+    if (edge) {
+      const int li = lane_o & 15, lg = lane_o >> 4;
+      if (__ballot(odd != 0)) {
+      for (int q = 0; q < 4; ++q)
+      for (uint32_t left = __builtin_amdgcn_readlane(odd, 16 * q); left; left &= left - 1) {
+        const int at = __builtin_ctz(left), key = k0 + 16 * (at >> 2) + 4 * q + (at & 3);
+        uint16_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4 * NG; ++e)
+          if (e == at) mine = pop[e / 8].v[e % 8];
+        const float p = E<DT>::to_f((uint16_t)__shfl((int)mine, 16 * q + li, 64));
+        if (key > min(kend - 1, pq)) continue;
+        const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
+        const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int ch = 4 * lg + r;
+          const float s1 = fp4_scale(sp[4 * (ch * ND >> 5)]);
+          uint32_t w;
+          if constexpr (D == 128) w = *reinterpret_cast<const uint32_t*>(wp + ch * (4 * NI));
+          else w = *reinterpret_cast<const uint16_t*>(wp + ch * (4 * NI));
+          const u16x8 x = fp4_eight<DT>(w, s1);
+#pragma unroll
+          for (int T = 0; T < ND; ++T) acc[T][r] += p * E<DT>::to_f(x.v[T]);
+        }
+      }
+      // all loads of this path have arrived (vmcnt 0), so that behind it the tiles' own are counted as on the other
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      }
+    }
+    load_v(t);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (; k0 + KT * NW < kend; k0 += 2 * KT * NW) {
+    tile(b0, k0);
+    tile(b1, k0 + KT * NW);
   }
+  if (k0 < kend) tile(b0, k0);
   l_run = xor32_sum(xor16_sum(l_run));
 
   // merge the waves: lane (column, lg) holds dims ND (4 lg + r) + T
-  __shared__ __align__(16) float lo[4][16][D + 4];
-  __shared__ float lm[4][16], ll[4][16];
   if (live) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int T = 0; T < ND; T += 4) {
         const f32x4_t x = {acc[T][r], acc[T + 1][r], acc[T + 2][r], acc[T + 3][r]};
-        *reinterpret_cast<f32x4_t*>(&lo[wave][li][ND * (4 * lg + r) + T]) = x;
+        *reinterpret_cast<f32x4_t*>(&lds.o[wave][li][ND * (4 * lg + r) + T]) = x;
       }
   }
   if (lg == 0) {
-    lm[wave][li] = m_run;
-    ll[wave][li] = l_run;
+    lds.m[wave][li] = m_run;
+    lds.l[wave][li] = l_run;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n * Gc * (D / 4); i += 256) {
+  for (int i = threadIdx.x; i < n * Gc * (D / 4); i += 64 * NW) {
     const int col = i / (D / 4), d = (i % (D / 4)) * 4;
-    const int j = col / Gc, h = col - j * Gc;
+    const int j = col * a.over_Gc >> 8, h = col - j * min(a.G, 16);
     const int pj = min(p0 + j, plim);
     if (kstart > pj) continue;  // the row has no keys in this split
-    float M = fmaxf(fmaxf(lm[0][col], lm[1][col]), fmaxf(lm[2][col], lm[3][col]));
+    float M = lds.m[0][col];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, lds.m[w][col]);
     const float mu = M == -INFINITY ? 0.f : M;
     float L = 0.f;
     f32x4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(lm[w][col] - mu);
-      L += ll[w][col] * f;
-      O += *reinterpret_cast<const f32x4_t*>(&lo[w][col][d]) * f;
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds.m[w][col] - mu);
+      L += lds.l[w][col] * f;
+      O += *reinterpret_cast<const f32x4_t*>(&lds.o[w][col][d]) * f;
     }
     const long rh = (long)(row + j) * a.heads + kh * a.G + h0 + h;
     if (pj < a.chunk) {
-      uint32_t o[2];
-      o[0] = E<DT>::from_f(O[0] / L) | (uint32_t)E<DT>::from_f(O[1] / L) << 16;
-      o[1] = E<DT>::from_f(O[2] / L) | (uint32_t)E<DT>::from_f(O[3] / L) << 16;
-      *reinterpret_cast<uint2*>(a.out + (long)(row + j) * a.so_b + (long)(kh * a.G + h0 + h) * a.so_h + d) =
-          make_uint2(o[0], o[1]);
+      kv4_store_out<DT>(a.out + (long)(row + j) * a.so_b + (long)(kh * a.G + h0 + h) * a.so_h + d, O, L);
     } else {
       const long at = rh * a.max_splits + split;
       *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = O;
@@ -444,6 +497,46 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_kernel(Kv4 c, Kv4Attn a) {
         ml[1] = L;
       }
     }
+  }
+  __syncthreads();  // the next block's sums take the same place
+}
+
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4Attn a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  int kh = blockIdx.y, h0 = 0;  // h0: first query head of the block within the kv head's G
+  if (a.hblocks > 1) {
+    kh = blockIdx.y / a.hblocks;
+    h0 = (blockIdx.y - kh * a.hblocks) * 16;
+  }
+  const int Gc = min(a.G - h0, 16);
+  const int split = blockIdx.z;
+  __shared__ Kv4Lds<D, NW> lds;
+
+  // The workgroup's candidates: R rows of an aligned group of qb. All first parts of groups come before all second
+  // ones in launch order, so that a prompt's live workgroups, which its groups' first parts are, spread over the XCDs.
+  int part = 0, group = blockIdx.x;
+  for (; group >= a.nblk; group -= a.nblk) ++part;
+  const int first = group * a.qb;
+  const int ri = first - 1 + lane;
+  const int rc = min(max(ri, 0), a.rows - 1);
+  const long slot_i = a.slots[rc];
+  const int pos_i = a.pos[rc];
+  // the exchanges stand before the conditions: a lane that a condition leaves out gives its neighbour no value
+  const long slot_b = __shfl_up(slot_i, 1, 64);
+  const int pos_b = __shfl_up(pos_i, 1, 64);
+  const bool follows = lane > 1 && lane <= a.qb && ri < a.rows && slot_b == slot_i && pos_i > 0 && pos_b == pos_i - 1;
+  const uint64_t chain = __ballot(follows);  // bit i: row first - 1 + i continues the row before it
+  const int last = min(min((part + 1) * a.R, a.qb), a.rows - first);
+  for (int cand = part * a.R; cand < last; ++cand) {
+    if (chain >> (cand + 1) & 1u) continue;  // in the block of a row before it
+    int l = lane;
+    asm volatile("" : "+v"(l));  // the block's addresses are made anew: kept over the loop they would spill
+    kv4_attn_row<DT, D, NW>(c, a, first + cand, 1 + __builtin_ctzll(~(chain >> (cand + 2))),
+                            (long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)slot_i, cand + 1) |
+                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(slot_i >> 32), cand + 1) << 32),
+                            __builtin_amdgcn_readlane(pos_i, cand + 1), kh, h0, Gc, split, wave, l, lds);
   }
 }
 
@@ -493,23 +586,24 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4 c, Kv4Attn a) {
     L += sl[i] * f;
     O += *reinterpret_cast<const f32x4_t*>(&so[i][d]) * f;
   }
-  const uint32_t o0 = E<DT>::from_f(O[0] / L) | (uint32_t)E<DT>::from_f(O[1] / L) << 16;
-  const uint32_t o1 = E<DT>::from_f(O[2] / L) | (uint32_t)E<DT>::from_f(O[3] / L) << 16;
-  *reinterpret_cast<uint2*>(a.out + (long)row * a.so_b + (long)head * a.so_h + d) = make_uint2(o0, o1);
+  kv4_store_out<DT>(a.out + (long)row * a.so_b + (long)head * a.so_h + d, O, L);
 }
 
 // ---------------------------------------------------------------------------------------------------------
 namespace {
-int kv4_check(const void* k, const void* ks, const void* v, const void* vs, int slots, int kv_heads, int head_dim,
-              int cap) {
-  if (slots <= 0 || kv_heads <= 0 || cap <= 0) return M3X_EINVAL;
-  if (!k || !ks || !v || !vs) return M3X_ENULL;
-  if (head_dim != 64 && head_dim != 128) return M3X_EUNSUPPORTED;
-  if (cap % 32 || !m3x_aligned16(k) || !m3x_aligned16(v) || !m3x_aligned16(ks) || !m3x_aligned16(vs)) return M3X_EINVAL;
+// the kernels' view of a caller's cache, or a status
+int kv4_take(const M3xKv4* p, Kv4& c) {
+  if (!p) return M3X_ENULL;
+  if (p->slots <= 0 || p->kv_heads <= 0 || p->cap <= 0) return M3X_EINVAL;
+  if (!p->k || !p->ks || !p->v || !p->vs) return M3X_ENULL;
+  if (p->head_dim != 64 && p->head_dim != 128) return M3X_EUNSUPPORTED;
+  if (p->cap % 32 || !m3x_aligned16(p->k) || !m3x_aligned16(p->v) || !m3x_aligned16(p->ks) || !m3x_aligned16(p->vs))
+    return M3X_EINVAL;
+  c = Kv4{(uint8_t*)p->k, (uint8_t*)p->ks, (uint8_t*)p->v, (uint8_t*)p->vs, p->slots, p->kv_heads, p->cap};
   return M3X_OK;
 }
-// items of D / 8 threads that a grid of 256-thread workgroups can hold
-bool kv4_fits(long items) { return items <= (1L << 31); }
+// whether D / 8 threads for each of `items` fit a launch (fewer than 2^32 threads)
+bool kv4_fits(long items, int head_dim) { return items * (head_dim / 8) < (1L << 32) - 256; }
 }  // namespace
 
 #define KV4_DISPATCH(KERNEL, GRID, ...)                                                                          \
@@ -524,44 +618,41 @@ bool kv4_fits(long items) { return items <= (1L << 31); }
       hipLaunchKernelGGL((KERNEL<M3X_F16, 64>), GRID, dim3(256), 0, (hipStream_t)stream, __VA_ARGS__);           \
   } while (0)
 
-M3X_API int m3x_kv4_append(const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h, void* k4, void* ks4,
-                           void* v4, void* vs4, const int64_t* slots, const int32_t* pos, int rows, int nslots,
-                           int kv_heads, int head_dim, int cap, int dtype, void* stream) {
+M3X_API int m3x_kv4_append(const M3xKv4* cache, const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h,
+                           const int64_t* slots, const int32_t* pos, int rows, int dtype, void* stream) {
+  Kv4 c;
+  if (const int st = kv4_take(cache, c)) return st;
   if (rows < 0) return M3X_EINVAL;
-  if (const int st = kv4_check(k4, ks4, v4, vs4, nslots, kv_heads, head_dim, cap)) return st;
   if (dtype != M3X_BF16 && dtype != M3X_F16) return M3X_EUNSUPPORTED;
   if (rows == 0) return M3X_OK;
   if (!k || !v || !slots || !pos) return M3X_ENULL;
   if (((sk_r | sk_h | sv_r | sv_h) & 7) || !m3x_aligned16(k) || !m3x_aligned16(v)) return M3X_EINVAL;
-  const long items = (long)rows * kv_heads;
-  if (!kv4_fits(items)) return M3X_EINVAL;
-  const Kv4 c = {(uint8_t*)k4, (uint8_t*)ks4, (uint8_t*)v4, (uint8_t*)vs4, nslots, kv_heads, cap};
+  const int head_dim = cache->head_dim;
+  const long items = (long)rows * c.kv_heads;
+  if (!kv4_fits(items, head_dim)) return M3X_EINVAL;
   KV4_DISPATCH(kv4_append_kernel, dim3(m3x_ceil_div(items, 2048 / head_dim)), (const uint16_t*)k, sk_r, sk_h,
                (const uint16_t*)v, sv_r, sv_h, c, slots, pos, rows);
   M3X_CHECK_LAUNCH();
   return M3X_OK;
 }
 
-M3X_API int m3x_qk_norm_rope_kv4(const void* qkv, long s_qkv, void* q_out, long s_qo_b, long s_qo_h, void* k4, void* ks4,
-                                 void* v4, void* vs4, const int64_t* slots, const int32_t* pos, const void* cos,
-                                 const void* sin, long s_cos, const void* wq, const void* wk, float eps, int rows,
-                                 int heads, int nslots, int kv_heads, int head_dim, int cap, void* stream) {
+M3X_API int m3x_qk_norm_rope_kv4(const M3xKv4* cache, const void* qkv, long s_qkv, void* q_out, long s_qo_b, long s_qo_h,
+                                 const int64_t* slots, const int32_t* pos, const void* cos, const void* sin, long s_cos,
+                                 const void* wq, const void* wk, float eps, int rows, int heads, void* stream) {
+  Kv4 c;
+  if (const int st = kv4_take(cache, c)) return st;
   if (rows < 0 || heads <= 0) return M3X_EINVAL;
-  if (const int st = kv4_check(k4, ks4, v4, vs4, nslots, kv_heads, head_dim, cap)) return st;
   if (rows == 0) return M3X_OK;
   if (!qkv || !q_out || !slots || !pos || !cos || !sin || !wq || !wk) return M3X_ENULL;
   if ((s_qkv | s_qo_b | s_qo_h | s_cos) & 7) return M3X_EINVAL;
   if (!m3x_aligned16(qkv) || !m3x_aligned16(q_out) || !m3x_aligned16(cos) || !m3x_aligned16(sin) ||
       !m3x_aligned16(wq) || !m3x_aligned16(wk))
     return M3X_EINVAL;
-  const long items = (long)rows * (heads + kv_heads);
-  if (!kv4_fits(items)) return M3X_EINVAL;
-  const Kv4 c = {(uint8_t*)k4, (uint8_t*)ks4, (uint8_t*)v4, (uint8_t*)vs4, nslots, kv_heads, cap};
+  const int head_dim = cache->head_dim;
+  const long items = (long)rows * ((long)heads + c.kv_heads);
+  if (!kv4_fits(items, head_dim)) return M3X_EINVAL;
   const dim3 grid(m3x_ceil_div(items, 2048 / head_dim));
-#define KV4_QKN(DD)                                                                                                   \
-  hipLaunchKernelGGL((qk_norm_rope_kv4_kernel<DD>), grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t*)qkv,     \
-                     s_qkv, (uint16_t*)q_out, s_qo_b, s_qo_h, c, slots, pos, (const uint16_t*)cos,                     \
-                     (const uint16_t*)sin, s_cos, (const uint16_t*)wq, (const uint16_t*)wk, eps, rows, heads)
+#define KV4_QKN(DD)                                                                                                  hipLaunchKernelGGL((qk_norm_rope_kv4_kernel<DD>), grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t*)qkv,                      s_qkv, (uint16_t*)q_out, s_qo_b, s_qo_h, c, slots, pos, (const uint16_t*)cos,                                       (const uint16_t*)sin, s_cos, (const uint16_t*)wq, (const uint16_t*)wk, eps, rows, heads)
   if (head_dim == 128) KV4_QKN(128);
   else KV4_QKN(64);
 #undef KV4_QKN
@@ -569,18 +660,18 @@ M3X_API int m3x_qk_norm_rope_kv4(const void* qkv, long s_qkv, void* q_out, long 
   return M3X_OK;
 }
 
-M3X_API int m3x_kv4_read(const void* k4, const void* ks4, const void* v4, const void* vs4, const int64_t* slots,
-                         const int32_t* pos, void* k, long sk_r, long sk_h, void* v, long sv_r, long sv_h, int rows,
-                         int nslots, int kv_heads, int head_dim, int cap, int dtype, void* stream) {
+M3X_API int m3x_kv4_read(const M3xKv4* cache, const int64_t* slots, const int32_t* pos, void* k, long sk_r, long sk_h,
+                         void* v, long sv_r, long sv_h, int rows, int dtype, void* stream) {
+  Kv4 c;
+  if (const int st = kv4_take(cache, c)) return st;
   if (rows < 0) return M3X_EINVAL;
-  if (const int st = kv4_check(k4, ks4, v4, vs4, nslots, kv_heads, head_dim, cap)) return st;
   if (dtype != M3X_BF16 && dtype != M3X_F16) return M3X_EUNSUPPORTED;
   if (rows == 0) return M3X_OK;
   if (!k || !v || !slots || !pos) return M3X_ENULL;
   if (((sk_r | sk_h | sv_r | sv_h) & 7) || !m3x_aligned16(k) || !m3x_aligned16(v)) return M3X_EINVAL;
-  const long items = (long)rows * kv_heads;
-  if (!kv4_fits(items)) return M3X_EINVAL;
-  const Kv4 c = {(uint8_t*)k4, (uint8_t*)ks4, (uint8_t*)v4, (uint8_t*)vs4, nslots, kv_heads, cap};
+  const int head_dim = cache->head_dim;
+  const long items = (long)rows * c.kv_heads;
+  if (!kv4_fits(items, head_dim)) return M3X_EINVAL;
   KV4_DISPATCH(kv4_read_kernel, dim3(m3x_ceil_div(items, 2048 / head_dim)), c, slots, pos, (uint16_t*)k, sk_r, sk_h,
                (uint16_t*)v, sv_r, sv_h, rows);
   M3X_CHECK_LAUNCH();
@@ -593,31 +684,47 @@ M3X_API size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max
   return splits > 1 ? (size_t)rows * heads * splits * (head_dim + 2) * sizeof(float) : 0;
 }
 
-M3X_API int m3x_kv4_attn(const void* q, long sq_b, long sq_h, const void* k4, const void* ks4, const void* v4,
-                         const void* vs4, void* out, long so_b, long so_h, const int64_t* slots, const int32_t* pos,
-                         float scale, int rows, int heads, int nslots, int kv_heads, int head_dim, int cap, int max_ctx,
+namespace {
+template <int DT, int D> void kv4_launch(const Kv4& c, const Kv4Attn& a, hipStream_t st) {
+  const dim3 grid(a.nblk * m3x_ceil_div(std::min(a.qb, a.rows), a.R), c.kv_heads * a.hblocks, a.max_splits);
+  hipLaunchKernelGGL((kv4_attn_kernel<DT, D, KV4_NW>), grid, dim3(64 * KV4_NW), 0, st, c, a);
+  if (a.max_splits > 1) hipLaunchKernelGGL((kv4_combine_kernel<DT, D>), dim3(a.rows, a.heads), dim3(256), 0, st, c, a);
+}
+}  // namespace
+
+M3X_API int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
+                         const int64_t* slots, const int32_t* pos, float scale, int rows, int heads, int max_ctx,
                          int chunk, void* workspace, size_t ws_bytes, int dtype, void* stream) {
+  Kv4 c;
+  if (const int st = kv4_take(cache, c)) return st;
   if (rows < 0 || heads <= 0 || max_ctx <= 0) return M3X_EINVAL;
-  if (const int st = kv4_check(k4, ks4, v4, vs4, nslots, kv_heads, head_dim, cap)) return st;
   if (dtype != M3X_BF16 && dtype != M3X_F16) return M3X_EUNSUPPORTED;
-  if (heads % kv_heads) return M3X_EUNSUPPORTED;
-  if (chunk <= 0 || chunk % 128 || max_ctx > cap) return M3X_EINVAL;
+  if (heads % c.kv_heads) return M3X_EUNSUPPORTED;
+  if (chunk <= 0 || chunk % 128 || max_ctx > c.cap) return M3X_EINVAL;
   if (rows == 0) return M3X_OK;
   if (!q || !out || !slots || !pos) return M3X_ENULL;
   if (((sq_b | sq_h | so_b | so_h) & 7) || !m3x_aligned16(q) || !m3x_aligned16(out)) return M3X_EINVAL;
   const int splits = m3x_ceil_div(max_ctx, chunk);
-  const int G = heads / kv_heads, hb = m3x_ceil_div(G, 16);
-  if ((long)kv_heads * hb > 65535 || heads > 65535 || splits > 65535) return M3X_EINVAL;
+  const int G = heads / c.kv_heads, hb = m3x_ceil_div(G, 16);
+  if (rows > (1 << 20) || (long)c.kv_heads * hb > 65535 || heads > 65535 || splits > 65535) return M3X_EINVAL;
+  const int head_dim = cache->head_dim;
   if (splits > 1) {
     if (!workspace) return M3X_ENULL;
     if (ws_bytes < m3x_kv4_attn_workspace(rows, heads, head_dim, max_ctx, chunk)) return M3X_EWORKSPACE;
     if (!m3x_aligned16(workspace)) return M3X_EINVAL;
   }
-  const Kv4 c = {(uint8_t*)k4, (uint8_t*)ks4, (uint8_t*)v4, (uint8_t*)vs4, nslots, kv_heads, cap};
+  const int Gc = std::min(G, 16), qb = hb > 1 ? 1 : 16 / G;
+  int R = 1;
+  while (R < qb && (long)rows * c.kv_heads * hb * splits >= 4096L * R) R *= 2;
+  R = R < qb ? R : qb;
   const Kv4Attn a = {(const uint16_t*)q, sq_b, sq_h, (uint16_t*)out, so_b, so_h, slots, pos,
-                     scale * 1.44269504088896341f, rows, heads, G, hb, chunk, max_ctx, splits, (float*)workspace};
-  KV4_DISPATCH(kv4_attn_kernel, dim3(rows, kv_heads * hb, splits), c, a);
-  if (splits > 1) KV4_DISPATCH(kv4_combine_kernel, dim3(rows, heads), c, a);
+                     scale * 1.44269504088896341f, rows, heads, G, hb, qb, R, m3x_ceil_div(rows, qb), chunk, max_ctx, splits,
+                     (uint32_t)((256 + Gc - 1) / Gc), (float*)workspace};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == M3X_BF16 && head_dim == 128) kv4_launch<M3X_BF16, 128>(c, a, st);
+  else if (dtype == M3X_BF16) kv4_launch<M3X_BF16, 64>(c, a, st);
+  else if (head_dim == 128) kv4_launch<M3X_F16, 128>(c, a, st);
+  else kv4_launch<M3X_F16, 64>(c, a, st);
   M3X_CHECK_LAUNCH();
   return M3X_OK;
 }

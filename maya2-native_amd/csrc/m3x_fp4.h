@@ -30,12 +30,13 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(float amax, uint32_t top) {
   return (uint32_t)min(max(b, 1), (int)top);
 }
 
-// 2^(b - 127) as a float (the conversions read its exponent field only; b = 255 is the infinity's, and gives NaN)
+// 2^(b - 127) as the conversions take it: the exponent field counts, sign and mantissa do not (checked on MI355X for
+// random words), so what stands beside the byte may stay. b = 255 gives NaN.
 __device__ __forceinline__ float fp4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 // the same from byte I of a word
 template <int I> __device__ __forceinline__ float fp4_scale_of(uint32_t w) {
-  if constexpr (I == 3) return __uint_as_float((w >> 1) & 0x7F800000u);
-  else return __uint_as_float((w << (23 - 8 * I)) & 0x7F800000u);
+  if constexpr (I == 3) return __uint_as_float(w >> 1);
+  else return __uint_as_float(w << (23 - 8 * I));
 }
 
 // the two numbers of byte SEL of w, packed 16-bit (low code first)

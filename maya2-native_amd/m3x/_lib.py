@@ -81,13 +81,11 @@ SIGNATURES = {
     "m3x_advance_tokens": (_I, [_P, _P, _I, _I, _I, _P]),
     "m3x_conv_gemm": (_I, [_P, _L, _P, _P, _P, _L, _P, _L, _I, _I, _I, _I, _P, _L, _P, _I, _I, _I, _I, _I, _P]),
     "m3x_resid_ln": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _L, _F, _I, _I, _I, _P]),
-    "m3x_kv4_append": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
-    "m3x_qk_norm_rope_kv4": (_I, [_P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P, _P, _F, _I, _I, _I, _I,
-                                  _I, _I, _P]),
-    "m3x_kv4_read": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _I, _P]),
+    "m3x_kv4_append": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _P]),
+    "m3x_qk_norm_rope_kv4": (_I, [_P, _P, _L, _P, _L, _L, _P, _P, _P, _P, _L, _P, _P, _F, _I, _I, _P]),
+    "m3x_kv4_read": (_I, [_P, _P, _P, _P, _L, _L, _P, _L, _L, _I, _I, _P]),
     "m3x_kv4_attn_workspace": (_Z, [_I, _I, _I, _I, _I]),
-    "m3x_kv4_attn": (_I, [_P, _L, _L, _P, _P, _P, _P, _P, _L, _L, _P, _P, _F, _I, _I, _I, _I, _I, _I, _I, _I, _P, _Z,
-                          _I, _P]),
+    "m3x_kv4_attn": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _P, _F, _I, _I, _I, _I, _P, _Z, _I, _P]),
     "m3x_packed_weight4_bytes": (_L, [_I, _I, _I]),
     "m3x_pack_weight4": (_I, [_P, _L, _I, _I, _P, _P, _I, _P]),
     "m3x_linear4": (_I, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _P]),

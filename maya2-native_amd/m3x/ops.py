@@ -584,39 +584,33 @@ def backbone_run(args: BackboneRunArgs):
 
 
 # ---------------------------------------------------------------- 4-bit cache and weights
-def _one_device(*ts):
-    """The device that all the given tensors (None skipped) are on."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("m3x kernels take device tensors")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return dev
+_raw_stream = torch._C._cuda_getCurrentRawStream  # a device's current stream as torch.cuda.current_stream, ~2 us cheaper
 
 
-def _call_on(dev, name, *args):
-    """Entry point m3x_<name> on the tensors' device and its current stream, whichever device is current."""
-    fn = getattr(lib(), "m3x_" + name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+def _launch(dev, fn, *args):
+    """A launching entry point on device `dev` (an index) and its current stream, whichever device is current."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(dev))
     if rc:
-        check(rc, name)
+        check(rc, fn.__name__)
+
+
+class Kv4CacheArgs(ctypes.Structure):
+    """Mirror of M3xKv4 (include/m3x.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "ks", "v", "vs")] + [
+        (n, ctypes.c_int) for n in ("slots", "kv_heads", "head_dim", "cap")]
 
 
 class Kv4Cache:
     """A layer's KV cache in 4 bits (format and layout: include/m3x.h): uint8 tensors
     k [slots, kv_heads, cap, head_dim / 2], ks [slots, kv_heads, cap, head_dim / 32],
     v [slots, kv_heads, cap / 4, 16, 4, head_dim / 32], vs [slots, kv_heads, cap / 4, head_dim / 32, 4].
-    head_dim 64 or 128, cap a multiple of 32."""
-    __slots__ = ("k", "ks", "v", "vs", "slots", "kv_heads", "cap", "head_dim", "device")
+    head_dim 64 or 128, cap a multiple of 32. The tensors are the handle's for its life: their storage is not resized
+    or replaced."""
+    __slots__ = ("k", "ks", "v", "vs", "slots", "kv_heads", "cap", "head_dim", "device", "_index", "_args", "_ref")
 
     def __init__(self, k, ks, v, vs):
         if k.dim() != 4:
@@ -633,6 +627,9 @@ class Kv4Cache:
                 raise ValueError(f"Kv4Cache: {name} must be 16-byte aligned on {k.device}")
         self.k, self.ks, self.v, self.vs = k, ks, v, vs
         self.slots, self.kv_heads, self.cap, self.head_dim, self.device = S, KV, cap, D, k.device
+        self._index = k.get_device()
+        self._args = Kv4CacheArgs(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), S, KV, D, cap)
+        self._ref = ctypes.addressof(self._args)
 
     @classmethod
     def empty(cls, slots, kv_heads, cap, head_dim, device):
@@ -649,76 +646,84 @@ class Kv4Cache:
     def memory_bytes(self):
         return sum(t.numel() for t in (self.k, self.ks, self.v, self.vs))
 
-    def _ptrs(self):
-        return self.k.data_ptr(), self.ks.data_ptr(), self.v.data_ptr(), self.vs.data_ptr()
-
 
 def _kv4_rows(name, cache, slots, pos):
+    """(rows, slots pointer, pos pointer) of a call's rows."""
     if not isinstance(cache, Kv4Cache):
         raise TypeError(f"{name}: the cache must be an ops.Kv4Cache")
-    if slots.dtype != torch.long or pos.dtype != torch.int32:
+    if slots.dtype != torch.int64 or pos.dtype != torch.int32:
         raise ValueError(f"{name}: slots must be int64 and pos int32, got {slots.dtype}, {pos.dtype}")
-    if slots.dim() != 1 or pos.shape != slots.shape or not slots.is_contiguous() or not pos.is_contiguous():
-        raise ValueError(f"{name}: slots and pos must be contiguous [rows], got {tuple(slots.shape)}, {tuple(pos.shape)}")
-    return slots.shape[0]
+    shape = slots.shape
+    if len(shape) != 1 or pos.shape != shape or not slots.is_contiguous() or not pos.is_contiguous():
+        raise ValueError(f"{name}: slots and pos must be contiguous [rows], got {tuple(shape)}, {tuple(pos.shape)}")
+    if slots.get_device() != cache._index or pos.get_device() != cache._index:
+        raise ValueError(f"{name}: slots on {slots.device}, pos on {pos.device}, the cache on {cache.device}")
+    return shape[0], slots.data_ptr(), pos.data_ptr()
 
 
-def _kv4_heads(name, what, t, rows, heads, D, dtype=None):
-    if t.dim() != 3 or tuple(t.shape) != (rows, heads, D) or (t.numel() and t.stride(2) != 1):
-        raise ValueError(f"{name}: {what} must be [{rows}, {heads}, {D}] with a contiguous last dimension, "
-                         f"got {tuple(t.shape)}")
-    if t.dtype not in _DT or (dtype is not None and t.dtype != dtype):
+def _kv4_heads(name, what, t, cache, rows, heads, dtype=None):
+    """(pointer, row stride, head stride) of rows [rows, heads, head_dim]."""
+    if t.shape != (rows, heads, cache.head_dim):
+        raise ValueError(f"{name}: {what} must be {(rows, heads, cache.head_dim)}, got {tuple(t.shape)}")
+    if t.dtype not in _DT if dtype is None else t.dtype != dtype:
         raise ValueError(f"{name}: {what} must be {'bfloat16 or float16' if dtype is None else dtype}, got {t.dtype}")
-    if t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: {what} needs 16-byte aligned rows (strides {t.stride()})")
+    if t.get_device() != cache._index:
+        raise ValueError(f"{name}: {what} on {t.device}, the cache on {cache.device}")
+    sr, sh, sd = t.stride()
+    ptr = t.data_ptr()
+    if (sr | sh | ptr >> 1) & 7 or (sd != 1 and rows):
+        raise ValueError(f"{name}: {what} needs a contiguous last dimension and 16-byte aligned rows (strides {t.stride()})")
+    return ptr, sr, sh
+
+
+def _on_gpu(name, cache):
+    if cache._index < 0:
+        raise ValueError(f"{name}: m3x kernels take device tensors")
 
 
 def kv4_append(k, v, cache, slots, pos):
     """K and V rows [rows, kv_heads, head_dim] (bf16 or fp16, any row and head strides) quantised to position pos[r]
     (int32) of slot slots[r] (int64). A row whose slot or position is outside the cache is not written."""
-    rows = _kv4_rows("kv4_append", cache, slots, pos)
-    _kv4_heads("kv4_append", "k", k, rows, cache.kv_heads, cache.head_dim)
-    _kv4_heads("kv4_append", "v", v, rows, cache.kv_heads, cache.head_dim, k.dtype)
-    dev = _one_device(k, v, cache.k, slots, pos)
-    _call_on(dev, "kv4_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-             *cache._ptrs(), slots.data_ptr(), pos.data_ptr(), rows, cache.slots, cache.kv_heads, cache.head_dim,
-             cache.cap, _DT[k.dtype])
+    rows, sp, pp = _kv4_rows("kv4_append", cache, slots, pos)
+    ka = _kv4_heads("kv4_append", "k", k, cache, rows, cache.kv_heads)
+    va = _kv4_heads("kv4_append", "v", v, cache, rows, cache.kv_heads, k.dtype)
+    _on_gpu("kv4_append", cache)
+    _launch(cache._index, lib().m3x_kv4_append, cache._ref, *ka, *va, sp, pp, rows, _DT[k.dtype])
 
 
 def qk_norm_rope_kv4(qkv, q_out, cache, slots, pos, cos, sin, wq, wk, eps, heads):
     """qk_norm_rope_cache over a Kv4Cache: q_out's bits are its, and the rotated keys (bf16) and the values are
     quantised as kv4_append does. bf16; cos, sin [>= cache.cap, head_dim]."""
-    rows = _kv4_rows("qk_norm_rope_kv4", cache, slots, pos)
+    name = "qk_norm_rope_kv4"
+    rows, sp, pp = _kv4_rows(name, cache, slots, pos)
     D, KV = cache.head_dim, cache.kv_heads
     _rows2d(qkv, "qkv")
-    if tuple(qkv.shape) != (rows, (heads + 2 * KV) * D):
-        raise ValueError(f"qk_norm_rope_kv4: qkv must be [{rows}, {(heads + 2 * KV) * D}], got {tuple(qkv.shape)}")
-    _kv4_heads("qk_norm_rope_kv4", "q_out", q_out, rows, heads, D, torch.bfloat16)
-    for t, name in ((cos, "cos"), (sin, "sin")):
+    if qkv.shape != (rows, (heads + 2 * KV) * D):
+        raise ValueError(f"{name}: qkv must be [{rows}, {(heads + 2 * KV) * D}], got {tuple(qkv.shape)}")
+    qa = _kv4_heads(name, "q_out", q_out, cache, rows, heads, torch.bfloat16)
+    for t, what in ((cos, "cos"), (sin, "sin")):
         if t.dim() != 2 or t.shape[0] < cache.cap or t.shape[1] != D or t.stride(1) != 1:
-            raise ValueError(f"qk_norm_rope_kv4: {name} must be [>= {cache.cap}, {D}], got {tuple(t.shape)}")
+            raise ValueError(f"{name}: {what} must be [>= {cache.cap}, {D}], got {tuple(t.shape)}")
     if cos.stride(0) != sin.stride(0):
-        raise ValueError("qk_norm_rope_kv4: cos and sin share one row stride")
+        raise ValueError(f"{name}: cos and sin share one row stride")
     if wq.numel() != D or wk.numel() != D or not wq.is_contiguous() or not wk.is_contiguous():
-        raise ValueError(f"qk_norm_rope_kv4: wq and wk have {D} elements")
-    if any(t.dtype != torch.bfloat16 for t in (qkv, cos, sin, wq, wk)):
-        raise ValueError("qk_norm_rope_kv4: bf16 only")
-    dev = _one_device(qkv, q_out, cache.k, slots, pos, cos, sin, wq, wk)
-    _call_on(dev, "qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0),
-             q_out.stride(1), *cache._ptrs(), slots.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-             cos.stride(0), wq.data_ptr(), wk.data_ptr(), float(eps), rows, heads, cache.slots, KV, D, cache.cap)
+        raise ValueError(f"{name}: wq and wk have {D} elements")
+    for t in (qkv, cos, sin, wq, wk):
+        if t.dtype != torch.bfloat16 or t.get_device() != cache._index:
+            raise ValueError(f"{name}: bfloat16 tensors on {cache.device}, got {t.dtype} on {t.device}")
+    _on_gpu(name, cache)
+    _launch(cache._index, lib().m3x_qk_norm_rope_kv4, cache._ref, qkv.data_ptr(), qkv.stride(0), *qa, sp, pp,
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0), wq.data_ptr(), wk.data_ptr(), float(eps), rows, heads)
 
 
 def kv4_read(cache, slots, pos, k, v):
     """k, v [rows, kv_heads, head_dim] (bf16 or fp16, any row and head strides) = the numbers at position pos[r] of
     slot slots[r]; zeros for a row outside the cache."""
-    rows = _kv4_rows("kv4_read", cache, slots, pos)
-    _kv4_heads("kv4_read", "k", k, rows, cache.kv_heads, cache.head_dim)
-    _kv4_heads("kv4_read", "v", v, rows, cache.kv_heads, cache.head_dim, k.dtype)
-    dev = _one_device(k, v, cache.k, slots, pos)
-    _call_on(dev, "kv4_read", *cache._ptrs(), slots.data_ptr(), pos.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
-             v.data_ptr(), v.stride(0), v.stride(1), rows, cache.slots, cache.kv_heads, cache.head_dim, cache.cap,
-             _DT[k.dtype])
+    rows, sp, pp = _kv4_rows("kv4_read", cache, slots, pos)
+    ka = _kv4_heads("kv4_read", "k", k, cache, rows, cache.kv_heads)
+    va = _kv4_heads("kv4_read", "v", v, cache, rows, cache.kv_heads, k.dtype)
+    _on_gpu("kv4_read", cache)
+    _launch(cache._index, lib().m3x_kv4_read, cache._ref, sp, pp, *ka, *va, rows, _DT[k.dtype])
 
 
 def kv4_attn_chunk(rows, heads, kv_heads, max_ctx) -> int:
@@ -741,26 +746,26 @@ def kv4_attn(q, cache, out, slots, pos, scale, max_ctx, chunk, workspace):
     cache gets zeros. max_ctx: at least every pos[r] + 1; chunk: keys per split (kv4_attn_chunk); workspace: a tensor of
     kv4_attn_workspace bytes, or None when that is 0. Rows of one slot at consecutive positions (a prompt's) that
     stand next to each other share one pass over the keys."""
-    rows = _kv4_rows("kv4_attn", cache, slots, pos)
+    rows, sp, pp = _kv4_rows("kv4_attn", cache, slots, pos)
     heads = q.shape[1] if q.dim() == 3 else 0
-    _kv4_heads("kv4_attn", "q", q, rows, heads, cache.head_dim)
-    _kv4_heads("kv4_attn", "out", out, rows, heads, cache.head_dim, q.dtype)
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"kv4_attn: {heads} query heads over {cache.kv_heads} kv heads")
+    qa = _kv4_heads("kv4_attn", "q", q, cache, rows, heads)
+    oa = _kv4_heads("kv4_attn", "out", out, cache, rows, heads, q.dtype)
     if not 1 <= max_ctx <= cache.cap or chunk < 128 or chunk % 128:
         raise ValueError(f"kv4_attn: max_ctx {max_ctx} must be in [1, {cache.cap}] and chunk {chunk} a multiple of 128")
-    dev = _one_device(q, out, cache.k, slots, pos, workspace)
     ws, ws_bytes = 0, 0
-    if workspace is not None:
-        if not workspace.is_contiguous() or workspace.data_ptr() % 16:
-            raise ValueError("kv4_attn: the workspace must be contiguous and 16-byte aligned")
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    if max_ctx > chunk and ws_bytes < kv4_attn_workspace(rows, heads, cache.head_dim, max_ctx, chunk):
-        raise ValueError(f"kv4_attn: a workspace of {kv4_attn_workspace(rows, heads, cache.head_dim, max_ctx, chunk)} "
-                         f"bytes is needed, got {ws_bytes}")
-    _call_on(dev, "kv4_attn", q.data_ptr(), q.stride(0), q.stride(1), *cache._ptrs(), out.data_ptr(), out.stride(0),
-             out.stride(1), slots.data_ptr(), pos.data_ptr(), float(scale), rows, heads, cache.slots, cache.kv_heads,
-             cache.head_dim, cache.cap, int(max_ctx), int(chunk), ws, ws_bytes, _DT[q.dtype])
+    if max_ctx > chunk:
+        need = kv4_attn_workspace(rows, heads, cache.head_dim, max_ctx, chunk)
+        if workspace is not None:
+            ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if ws_bytes < need:
+            raise ValueError(f"kv4_attn: a workspace of {need} bytes is needed, got {ws_bytes}")
+        if ws_bytes and (not workspace.is_contiguous() or ws % 16 or workspace.get_device() != cache._index):
+            raise ValueError(f"kv4_attn: the workspace must be contiguous, 16-byte aligned and on {cache.device}")
+    _on_gpu("kv4_attn", cache)
+    _launch(cache._index, lib().m3x_kv4_attn, cache._ref, *qa, *oa, sp, pp, scale, rows, heads, max_ctx, chunk, ws,
+            ws_bytes, _DT[q.dtype])
 
 
 class PackedWeight4:
@@ -776,6 +781,8 @@ class PackedWeight4:
             if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"PackedWeight4: {name} must be contiguous, aligned uint8 {shape}, got {t.dtype} "
                                  f"{tuple(t.shape)}")
+        if codes.device != scales.device:
+            raise ValueError(f"PackedWeight4: codes on {codes.device}, scales on {scales.device}")
         self.codes, self.scales, self.N, self.K = codes, scales, N, K
 
     @property
@@ -802,55 +809,66 @@ def pack_weight4(w):
         raise ValueError(f"pack_weight4: K={K} must be a multiple of 32")
     if w.stride(0) % 8 or w.data_ptr() % 16:
         raise ValueError(f"pack_weight4: w needs 16-byte aligned rows (stride {w.stride(0)})")
-    dt, dev = _dt3(w), _one_device(w)
+    dt = _dt3(w)
+    _dev(w)
     tiles, steps = -(-N // 16), -(-K // 128)
-    codes = torch.empty(tiles, steps, 64, 16, dtype=torch.uint8, device=dev)
-    scales = torch.empty(tiles, -(-steps // 4), 64, 4, dtype=torch.uint8, device=dev)
-    _call_on(dev, "pack_weight4", w.data_ptr(), w.stride(0), N, K, codes.data_ptr(), scales.data_ptr(), dt)
+    codes = torch.empty(tiles, steps, 64, 16, dtype=torch.uint8, device=w.device)
+    scales = torch.empty(tiles, -(-steps // 4), 64, 4, dtype=torch.uint8, device=w.device)
+    _launch(w.get_device(), lib().m3x_pack_weight4, w.data_ptr(), w.stride(0), N, K, codes.data_ptr(),
+            scales.data_ptr(), dt)
     return PackedWeight4(codes, scales, N, K)
 
 
 def _lin4_args(name, x, w, y):
+    """(y, device index, x's pointer and row stride, y's pointer and row stride, rows)."""
     if not isinstance(w, PackedWeight4):
         raise TypeError(f"{name}: the weight must be packed with ops.pack_weight4")
-    if x.dim() != 2 or x.shape[1] != w.K or x.dtype not in _DT:
-        raise ValueError(f"{name}: x must be bfloat16 or float16 [rows, {w.K}], got {x.dtype} {tuple(x.shape)}")
-    M = x.shape[0]
-    if M and (x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16):
-        raise ValueError(f"{name}: x needs 16-byte aligned rows (strides {x.stride()})")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != w.K or x.dtype not in _DT:
+        raise ValueError(f"{name}: x must be bfloat16 or float16 [rows, {w.K}], got {x.dtype} {tuple(shape)}")
+    M = shape[0]
+    sr, sk = x.stride()
+    xp = x.data_ptr()
+    if (sr | xp >> 1) & 7 or (sk != 1 and M):
+        raise ValueError(f"{name}: x needs a contiguous last dimension and 16-byte aligned rows (strides {x.stride()})")
     if y is None:
-        y = torch.empty(M, w.N, dtype=x.dtype, device=x.device)
-    elif tuple(y.shape) != (M, w.N) or y.dtype != x.dtype or (y.numel() and y.stride(1) != 1):
-        raise ValueError(f"{name}: y must be {x.dtype} {(M, w.N)} with a contiguous last dimension, got {y.dtype} "
-                         f"{tuple(y.shape)}")
-    return M, y
+        y = x.new_empty((M, w.N))
+        ldy = w.N
+    else:
+        if y.shape != (M, w.N) or y.dtype != x.dtype or (M and w.N > 1 and y.stride(1) != 1):
+            raise ValueError(f"{name}: y must be {x.dtype} {(M, w.N)} with a contiguous last dimension, got {y.dtype} "
+                             f"{tuple(y.shape)}")
+        ldy = y.stride(0)
+    dev = x.get_device()
+    if dev < 0:
+        raise ValueError(f"{name}: m3x kernels take device tensors")
+    if w.codes.get_device() != dev or y.get_device() != dev:
+        raise ValueError(f"{name}: x on {x.device}, the weight on {w.device}, y on {y.device}")
+    return y, dev, xp, sr, y.data_ptr(), ldy, M
 
 
 def linear4(x, w, y=None):
     """y = x @ W.T for rows x [M, K] (bf16 or fp16) and a weight packed by pack_weight4; the 4-bit form of `linear`
     for few rows. Returns y [M, N] (new unless given)."""
-    M, y = _lin4_args("linear4", x, w, y)
-    dev = _one_device(x, w.codes, w.scales, y)
-    _call_on(dev, "linear4", x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), y.data_ptr(),
-             y.stride(0), M, w.N, w.K, _DT[x.dtype])
+    y, dev, xp, ldx, yp, ldy, M = _lin4_args("linear4", x, w, y)
+    _launch(dev, lib().m3x_linear4, xp, ldx, w.codes.data_ptr(), w.scales.data_ptr(), yp, ldy, M, w.N, w.K, _DT[x.dtype])
     return y
 
 
 def linear4_act(x, w_gate, w_up, kind, y=None):
     """SWIGLU: y = silu(x @ Wg.T) * (x @ Wu.T); GELU: y = gelu(x @ Wg.T) (w_up None); the 4-bit form of `linear_act`,
     rounded once."""
-    M, y = _lin4_args("linear4_act", x, w_gate, y)
     if kind not in (ACT_SWIGLU, ACT_GELU):
         raise ValueError("linear4_act: kind must be ACT_SWIGLU or ACT_GELU")
     u = (0, 0)
     if kind == ACT_SWIGLU:
-        if not isinstance(w_up, PackedWeight4) or (w_up.N, w_up.K) != (w_gate.N, w_gate.K):
-            raise ValueError("linear4_act: w_up must be a packed weight of w_gate's shape")
+        if not isinstance(w_up, PackedWeight4) or not isinstance(w_gate, PackedWeight4) or \
+                (w_up.N, w_up.K) != (w_gate.N, w_gate.K) or w_up.device != w_gate.device:
+            raise ValueError("linear4_act: w_up must be a packed weight of w_gate's shape, on its device")
         u = (w_up.codes.data_ptr(), w_up.scales.data_ptr())
-    dev = _one_device(x, w_gate.codes, w_gate.scales, None if w_up is None else w_up.codes,
-                      None if w_up is None else w_up.scales, y)
-    _call_on(dev, "linear4_act", x.data_ptr(), x.stride(0), w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), *u,
-             y.data_ptr(), y.stride(0), M, w_gate.N, w_gate.K, kind, _DT[x.dtype])
+    y, dev, xp, ldx, yp, ldy, M = _lin4_args("linear4_act", x, w_gate, y)
+    _launch(dev, lib().m3x_linear4_act, xp, ldx, w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), *u, yp, ldy, M,
+            w_gate.N, w_gate.K, kind, _DT[x.dtype])
     return y
 
 

@@ -51,6 +51,8 @@ def test_rows_refused():
             ops.kv4_append(ok, ok, c, s, p)
     with pytest.raises(ValueError, match="device"):
         ops.kv4_append(ok, ok, c, slots, pos)
+    with pytest.raises(ValueError, match="device"):
+        ops.kv4_read(c, slots, pos, ok, ok)
     with pytest.raises(TypeError):
         ops.kv4_append(ok, ok, (c.k, c.v), slots, pos)
 
@@ -112,18 +114,42 @@ def test_weights_refused():
         ops.linear4_act(x, p, p, ops.ACT_NONE)
 
 
+def _kv4(kw):
+    """The cache argument of a call whose keyword arguments may change its fields."""
+    from m3x.ops import Kv4CacheArgs
+    a = dict(k4=4096, ks4=4096, v4=4096, vs4=4096, nslots=1, kv_heads=2, head_dim=128, cap=64)
+    a.update({n: kw.pop(n) for n in list(kw) if n in a})
+    return Kv4CacheArgs(*a.values())
+
+
 def _append(L, **kw):
-    a = dict(k=P, sk_r=256, sk_h=128, v=P, sv_r=256, sv_h=128, k4=P, ks4=P, v4=P, vs4=P, slots=P, pos=P, rows=1, nslots=1,
-             kv_heads=2, head_dim=128, cap=64, dtype=0)
+    c = _kv4(kw)
+    a = dict(k=P, sk_r=256, sk_h=128, v=P, sv_r=256, sv_h=128, slots=P, pos=P, rows=1, dtype=0)
     assert set(kw) <= set(a)
-    return L.m3x_kv4_append(*{**a, **kw}.values(), None)
+    return L.m3x_kv4_append(ctypes.addressof(c), *{**a, **kw}.values(), None)
 
 
 def _attn(L, **kw):
-    a = dict(q=P, sq_b=512, sq_h=128, k4=P, ks4=P, v4=P, vs4=P, out=P, so_b=512, so_h=128, slots=P, pos=P, scale=1.0, rows=1,
-             heads=4, nslots=1, kv_heads=2, head_dim=128, cap=64, max_ctx=64, chunk=128, workspace=None, ws_bytes=0, dtype=0)
+    c = _kv4(kw)
+    a = dict(q=P, sq_b=512, sq_h=128, out=P, so_b=512, so_h=128, slots=P, pos=P, scale=1.0, rows=1, heads=4, max_ctx=64,
+             chunk=128, workspace=None, ws_bytes=0, dtype=0)
     assert set(kw) <= set(a)
-    return L.m3x_kv4_attn(*{**a, **kw}.values(), None)
+    return L.m3x_kv4_attn(ctypes.addressof(c), *{**a, **kw}.values(), None)
+
+
+def _read(L, **kw):
+    c = _kv4(kw)
+    a = dict(slots=P, pos=P, k=P, sk_r=256, sk_h=128, v=P, sv_r=256, sv_h=128, rows=1, dtype=0)
+    assert set(kw) <= set(a)
+    return L.m3x_kv4_read(ctypes.addressof(c), *{**a, **kw}.values(), None)
+
+
+def _rope(L, **kw):
+    c = _kv4(kw)
+    a = dict(qkv=P, s_qkv=1024, q_out=P, s_qo_b=512, s_qo_h=128, slots=P, pos=P, cos=P, sin=P, s_cos=128, wq=P, wk=P,
+             eps=1e-6, rows=1, heads=4)
+    assert set(kw) <= set(a)
+    return L.m3x_qk_norm_rope_kv4(ctypes.addressof(c), *{**a, **kw}.values(), None)
 
 
 def _linear(L, **kw):
@@ -139,18 +165,22 @@ ODD = ctypes.c_void_p(4098)
     (_append, dict(rows=0), 0), (_append, dict(rows=-1), -1), (_append, dict(head_dim=96), -5), (_append, dict(cap=40), -1),
     (_append, dict(nslots=0), -1), (_append, dict(kv_heads=0), -1), (_append, dict(dtype=2), -5),
     (_append, dict(k=None), -2), (_append, dict(vs4=None), -2), (_append, dict(slots=None), -2), (_append, dict(sk_r=12), -1),
-    (_append, dict(sv_h=4), -1), (_append, dict(v=ODD), -1), (_append, dict(k4=ODD), -1),
-    (_append, dict(rows=2 ** 31 - 1, kv_heads=64), -1),
+    (_append, dict(sv_h=4), -1), (_append, dict(v=ODD), -1), (_append, dict(k4=4098), -1),
+    (_append, dict(rows=2 ** 31 - 1, kv_heads=64), -1), (_append, dict(rows=1 << 25, kv_heads=8), -1),
+    (_read, dict(rows=0), 0), (_read, dict(rows=-1), -1), (_read, dict(cap=40), -1), (_read, dict(k4=None), -2),
+    (_read, dict(v=None), -2), (_read, dict(k=ODD), -1), (_read, dict(sv_r=3), -1), (_read, dict(dtype=2), -5),
+    (_rope, dict(rows=0), 0), (_rope, dict(rows=-1), -1), (_rope, dict(heads=0), -1), (_rope, dict(head_dim=32), -5),
+    (_rope, dict(cos=None), -2), (_rope, dict(wk=ODD), -1), (_rope, dict(s_cos=4), -1), (_rope, dict(ks4=4104), -1),
     (_attn, dict(rows=0), 0), (_attn, dict(rows=-1), -1), (_attn, dict(heads=0), -1), (_attn, dict(heads=5), -5),
     (_attn, dict(head_dim=256), -5), (_attn, dict(dtype=2), -5), (_attn, dict(max_ctx=65), -1), (_attn, dict(max_ctx=0), -1),
     (_attn, dict(chunk=64), -1), (_attn, dict(chunk=0), -1), (_attn, dict(out=None), -2), (_attn, dict(pos=None), -2),
     (_attn, dict(sq_h=100), -1), (_attn, dict(out=ODD), -1), (_attn, dict(cap=256, max_ctx=256), -2),
     (_attn, dict(cap=256, max_ctx=256, workspace=P, ws_bytes=100), -3),
     (_attn, dict(cap=256, max_ctx=256, workspace=ODD, ws_bytes=1 << 20), -1),
-    (_attn, dict(heads=131072, kv_heads=2), -1), (_attn, dict(cap=1 << 25, max_ctx=1 << 25, workspace=P, ws_bytes=1 << 40), -1),
+    (_attn, dict(heads=131072, kv_heads=2), -1), (_attn, dict(rows=(1 << 20) + 1), -1), (_attn, dict(cap=1 << 25, max_ctx=1 << 25, workspace=P, ws_bytes=1 << 40), -1),
     (_linear, dict(M=0), 0), (_linear, dict(M=-1), -1), (_linear, dict(N=0), -1), (_linear, dict(K=48), -1),
     (_linear, dict(ldx=60), -1), (_linear, dict(x=ODD), -1), (_linear, dict(codes=None), -2), (_linear, dict(y=None), -2),
-    (_linear, dict(dtype=2), -5), (_linear, dict(M=2 ** 31 - 1), -1)])
+    (_linear, dict(dtype=2), -5), (_linear, dict(M=2 ** 31 - 1), -1), (_linear, dict(N=1 << 27), -1)])
 def test_status(call, kw, status):
     from m3x._lib import lib
     assert call(lib(), **kw) == status
@@ -161,6 +191,7 @@ def test_weight_sizes():
     L = lib()
     assert L.m3x_packed_weight4_bytes(20, 672, 0) == 2 * 6 * 1024 and L.m3x_packed_weight4_bytes(20, 672, 1) == 2 * 2 * 256
     assert L.m3x_packed_weight4_bytes(20, 48, 0) == -1 and L.m3x_packed_weight4_bytes(0, 32, 0) == -1
+    assert L.m3x_kv4_append(None, P, 256, 128, P, 256, 128, P, P, 1, 0, None) == -2
     assert L.m3x_linear4_act(P, 64, P, P, None, None, P, 20, 1, 20, 64, 0, 0, None) == -2
     assert L.m3x_linear4_act(P, 64, P, P, P, P, P, 20, 1, 20, 64, -1, 0, None) == -5
     assert L.m3x_pack_weight4(P, 64, 20, 48, P, P, 0, None) == -1 and L.m3x_pack_weight4(P, 64, 20, 64, P, P, 3, None) == -5
