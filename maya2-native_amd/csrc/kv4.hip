@@ -540,51 +540,69 @@ __global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4At
   }
 }
 
-// Joins the splits of a row's keys, in order within each of 1024 / D groups of splits, then the groups in order. One
-// workgroup per (row, head).
-template <int DT, int D>
+// Joins the splits of a row's keys: NG groups of D / 4 threads a (row, head), each every NG-th split in order, then the
+// groups in order (the same order whatever the launch). Bound by the launch and two memory round trips; the first
+// splits are loaded beside the row's position, before it is known which of them there are.
+template <int DT, int D, int NG>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4 c, Kv4Attn a) {
-  constexpr int TD = D / 4, NG = 256 / TD;
-  const int row = blockIdx.x, head = blockIdx.y;
+  constexpr int TD = D / 4, HB = 256 / (TD * NG), U = 4;
+  const int row = blockIdx.x;
+  const int g = threadIdx.x / TD % NG, d = (threadIdx.x % TD) * 4, hb = threadIdx.x / (TD * NG);
+  const int head = min((int)(blockIdx.y * HB + hb), a.heads - 1);  // a group past the last head repeats it
   const long slot = a.slots[row];
-  const int p = min(a.pos[row], min(c.cap, a.max_ctx) - 1);
-  if (slot < 0 || slot >= c.slots || p < a.chunk) return;  // no key, or one split: the attention wrote the row
-  const int ns = p / a.chunk + 1;
+  const int pos = a.pos[row];
   const long at = ((long)row * a.heads + head) * a.max_splits;
   const float* ml = a.part + (long)a.rows * a.heads * a.max_splits * D + at * 2;
   const float* po = a.part + at * D;
-  const int g = threadIdx.x / TD, d = (threadIdx.x % TD) * 4;
+  float2 x[U];
+  f32x4_t o[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int s = min(s0 + i * NG, a.max_splits - 1);
+      x[i] = *reinterpret_cast<const float2*>(ml + 2 * s);
+      o[i] = *reinterpret_cast<const f32x4_t*>(po + (long)s * D + d);
+    }
+  };
+  load(g);
+  const int p = min(pos, min(c.cap, a.max_ctx) - 1);
+  if (slot < 0 || slot >= c.slots || p < a.chunk) return;  // no key, or one split: the attention wrote the row
+  const int ns = p / a.chunk + 1;
   float M = -INFINITY, L = 0.f;
   f32x4_t O = {0.f, 0.f, 0.f, 0.f};
-  for (int s = g; s < ns; s += NG) {
-    const float m = ml[2 * s], l = ml[2 * s + 1];
-    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(po + (long)s * D + d);
-    const float mx = fmaxf(M, m), mu = mx == -INFINITY ? 0.f : mx;
-    const float f0 = __builtin_amdgcn_exp2f(M - mu), f1 = __builtin_amdgcn_exp2f(m - mu);
-    L = L * f0 + l * f1;
-    O = O * f0 + o * f1;
-    M = mx;
+  for (int s0 = g; s0 < ns; s0 += U * NG) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (s0 + i * NG < ns) {
+        const float mx = fmaxf(M, x[i].x), mu = mx == -INFINITY ? 0.f : mx;
+        const float f0 = __builtin_amdgcn_exp2f(M - mu), f1 = __builtin_amdgcn_exp2f(x[i].x - mu);
+        L = L * f0 + x[i].y * f1;
+        O = O * f0 + o[i] * f1;
+        M = mx;
+      }
+    }
+    if (s0 + U * NG < ns) load(s0 + U * NG);
   }
-  __shared__ __align__(16) float so[NG][D];
-  __shared__ float sm[NG], sl[NG];
-  *reinterpret_cast<f32x4_t*>(&so[g][d]) = O;
+  __shared__ __align__(16) float so[HB][NG][D];
+  __shared__ float sm[HB][NG], sl[HB][NG];
+  *reinterpret_cast<f32x4_t*>(&so[hb][g][d]) = O;
   if (d == 0) {
-    sm[g] = M;
-    sl[g] = L;
+    sm[hb][g] = M;
+    sl[hb][g] = L;
   }
   __syncthreads();
-  if (threadIdx.x >= TD) return;
-  M = sm[0];
+  if (g || blockIdx.y * HB + hb >= a.heads) return;
+  M = sm[hb][0];
 #pragma unroll
-  for (int i = 1; i < NG; ++i) M = fmaxf(M, sm[i]);
+  for (int i = 1; i < NG; ++i) M = fmaxf(M, sm[hb][i]);
   const float mu = M == -INFINITY ? 0.f : M;
   L = 0.f;
   O = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    const float f = __builtin_amdgcn_exp2f(sm[i] - mu);
-    L += sl[i] * f;
-    O += *reinterpret_cast<const f32x4_t*>(&so[i][d]) * f;
+    const float f = __builtin_amdgcn_exp2f(sm[hb][i] - mu);
+    L += sl[hb][i] * f;
+    O += *reinterpret_cast<const f32x4_t*>(&so[hb][i][d]) * f;
   }
   kv4_store_out<DT>(a.out + (long)row * a.so_b + (long)head * a.so_h + d, O, L);
 }
@@ -688,7 +706,10 @@ namespace {
 template <int DT, int D> void kv4_launch(const Kv4& c, const Kv4Attn& a, hipStream_t st) {
   const dim3 grid(a.nblk * m3x_ceil_div(std::min(a.qb, a.rows), a.R), c.kv_heads * a.hblocks, a.max_splits);
   hipLaunchKernelGGL((kv4_attn_kernel<DT, D, KV4_NW>), grid, dim3(64 * KV4_NW), 0, st, c, a);
-  if (a.max_splits > 1) hipLaunchKernelGGL((kv4_combine_kernel<DT, D>), dim3(a.rows, a.heads), dim3(256), 0, st, c, a);
+  if (a.max_splits > 4)
+    hipLaunchKernelGGL((kv4_combine_kernel<DT, D, 8>), dim3(a.rows, m3x_ceil_div(a.heads, 128 / D)), dim3(256), 0, st, c, a);
+  else if (a.max_splits > 1)
+    hipLaunchKernelGGL((kv4_combine_kernel<DT, D, 1>), dim3(a.rows, m3x_ceil_div(a.heads, 1024 / D)), dim3(256), 0, st, c, a);
 }
 }  // namespace
 

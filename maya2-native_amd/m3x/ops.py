@@ -726,13 +726,19 @@ def kv4_read(cache, slots, pos, k, v):
     _launch(cache._index, lib().m3x_kv4_read, cache._ref, sp, pp, *ka, *va, rows, _DT[k.dtype])
 
 
-def kv4_attn_chunk(rows, heads, kv_heads, max_ctx) -> int:
-    """Keys per split of kv4_attn for `rows` rows of up to max_ctx keys."""
-    want = rows * kv_heads * max_ctx / 1024.0
-    c = 128
-    while c < want and c < 8192:
-        c *= 2
-    return c
+def kv4_attn_chunk(rows, heads, kv_heads, max_ctx, head_dim=128) -> int:
+    """Keys per split of kv4_attn for `rows` rows of up to max_ctx keys: a workgroup (a row, a kv head, a split) per CU
+    at head_dim 128, two at 64 (whose arithmetic is the larger share), and at least 128 keys each; up to 512 keys whole
+    (no join of splits behind).
+
+    Measured on MI355X (graph-timed, us, 16/8 heads of 128, combine included): one row at 2048 keys 7.2 (128 keys a
+    split; 256: 7.5, 1024: 10.4), at 32000 12.7 (1024; 256: 18.5, 4096: 23.9); 4 rows at 32000 27.9 (4096; 1024: 31.2,
+    16384: 75); 32 rows at 2048 14.9 whole (512: 20.5); 224 rows at 2048 79 whole (1024: 91); one row at 300 5.2 whole
+    (128: 6.9). 32/4 heads of 64: 16 rows at 32000 30 (4096; 8192: 36, 512: 42)."""
+    if max_ctx <= 512:
+        return 512
+    blocks = rows * kv_heads * -(-heads // (16 * kv_heads))
+    return 128 * max(1, -(-blocks * max_ctx // (128 * (256 if head_dim == 128 else 512))))
 
 
 def kv4_attn_workspace(rows, heads, head_dim, max_ctx, chunk) -> int:
