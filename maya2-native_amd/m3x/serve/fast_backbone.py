@@ -27,6 +27,12 @@ How a step runs here:
     projection also gets a copy in MFMA fragment order (ops.pack_weight).
 `attention`, `fuse_proj`, `fuse_rope` and `fused_norm` are accepted for construction-site compatibility; there is
 one kernel path.
+
+`kv_bits=4` (no counterpart in the reference) holds the cache in 4 bits (ops.Kv4Cache, one per layer in `kv4`; `k` and
+`v` are then empty): 136 bytes a position and kv head instead of 512. A step writes it with qk_norm_rope_kv4 and attends
+with kv4_attn, which finds a prompt's rows by itself, so decode, mixed and spread-out steps share one graph a bucket;
+one-row steps take the same launches. What is installed is quantised, what is exported is the numbers held, and an
+exported prefix installs as exactly itself.
 """
 from __future__ import annotations
 
@@ -102,12 +108,15 @@ class _StepGraph:
 class StaticBackbone:
     def __init__(self, backbone, max_slots, capacity=1536,
                  batch_buckets=(1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96), ctx_buckets=(512, 768, 1024, 1536),
-                 attention='gather', fused_norm=False, use_graphs=True, fuse_proj=False, fuse_rope=False):
+                 attention='gather', fused_norm=False, use_graphs=True, fuse_proj=False, fuse_rope=False, kv_bits=16):
+        if kv_bits not in (16, 4):
+            raise ValueError(f'kv_bits must be 16 or 4, got {kv_bits}')
         if attention not in ('gather', 'triton'):
             raise ValueError('attention must be gather or triton')
         lib()  # the kernels are the only path: fail here if the library is missing
         self.attention, self.fused_norm, self.use_graphs = attention, fused_norm, use_graphs
         self.fuse_proj = self.fuse_rope = True
+        self.kv_bits = kv_bits
         with torch.inference_mode():
             self._read_model(backbone)
             self.max_slots, self.capacity, self.dummy = int(max_slots), int(capacity), int(max_slots)
@@ -187,8 +196,10 @@ class StaticBackbone:
         # `capacity` positions, as the reference's tensors are
         self._extent = -(-self.capacity // TILE) * TILE
         full = (self.max_slots + 1, self.kv_heads, self._extent, self.head_dim)
-        self._kfull = [torch.zeros(full, dtype=self.dtype, device=self.device) for _ in self.layers]
-        self._vfull = [torch.zeros(full, dtype=self.dtype, device=self.device) for _ in self.layers]
+        self.kv4 = [ops.Kv4Cache.empty(*full, self.device) for _ in self.layers] if self.kv_bits == 4 else []
+        wide = self.layers if self.kv_bits == 16 else ()
+        self._kfull = [torch.zeros(full, dtype=self.dtype, device=self.device) for _ in wide]
+        self._vfull = [torch.zeros(full, dtype=self.dtype, device=self.device) for _ in wide]
         self.k = [t[:, :, :self.capacity] for t in self._kfull]
         self.v = [t[:, :, :self.capacity] for t in self._vfull]
         self.lengths = torch.zeros(self.max_slots + 1, dtype=torch.long, device=self.device)
@@ -202,11 +213,25 @@ class StaticBackbone:
         self.lengths[slot] = n
         self.lengths_cpu[slot] = n
 
+    def _positions_of(self, slot, length):
+        """(slots, positions) of a slot's first `length` positions, as the 4-bit cache's rows."""
+        return (torch.full((length,), int(slot), dtype=torch.long, device=self.device),
+                torch.arange(length, dtype=torch.int32, device=self.device))
+
     def _install(self, slot, length, pairs):
         """Copy the first `length` positions of per-layer (keys, values) [kv_heads, >= length, head_dim]."""
         check_slots([slot], self.max_slots)
         if length > self.capacity:
             raise ValueError(f'length {length} exceeds capacity {self.capacity}')
+        if self.kv_bits == 4:
+            if length:
+                at = self._positions_of(slot, length)
+                for c, (keys, values) in zip(self.kv4, pairs):
+                    rows = [t[:, :length].to(self.device, self.dtype).transpose(0, 1).contiguous()
+                            for t in (keys, values)]
+                    ops.kv4_append(*rows, c, *at)
+            self._set_length(slot, length)
+            return
         for i, (keys, values) in enumerate(pairs):
             self.k[i][slot, :, :length].copy_(keys[:, :length])
             self.v[i][slot, :, :length].copy_(values[:, :length])
@@ -237,6 +262,14 @@ class StaticBackbone:
         n = self.lengths_cpu[slot] if length is None else int(length)
         if not 0 <= n <= self.lengths_cpu[slot]:
             raise ValueError(f'length {n} outside the slot\'s {self.lengths_cpu[slot]} cached positions')
+        if self.kv_bits == 4:
+            at, out = self._positions_of(slot, n), []
+            for c in self.kv4:
+                k, v = (torch.empty(1, self.kv_heads, n, self.head_dim, dtype=self.dtype, device=self.device)
+                        for _ in 'kv')
+                ops.kv4_read(c, *at, k[0].transpose(0, 1), v[0].transpose(0, 1))
+                out.append((k, v))
+            return out
         return [(self.k[i][slot:slot + 1, :, :n].clone(), self.v[i][slot:slot + 1, :, :n].clone())
                 for i in range(len(self.layers))]
 
@@ -277,8 +310,13 @@ class StaticBackbone:
         # the 16-column tile statistics the residual projections leave for the next norm
         b.part = torch.empty(ops.tile_stats_elems(rows, hid), dtype=torch.float32, device=dev)
         b.q = torch.empty(rows, H, D, dtype=dt, device=dev)
-        b.chunk = item_chunk(rows) if b.decode_items else attn_chunk(rows, KV, ctx)
         b.items = None
+        if self.kv_bits == 4:
+            b.chunk = ops.kv4_attn_chunk(rows, H, KV, ctx, D)
+            b.attn_ws = torch.empty(max(ops.kv4_attn_workspace(rows, H, D, ctx, b.chunk), 16) // 4, dtype=torch.float32,
+                                    device=dev)
+            return b
+        b.chunk = item_chunk(rows) if b.decode_items else attn_chunk(rows, KV, ctx)
         if mixed or b.decode_items:
             # work items (ops.attn_items): until a step stages its own, every row is its own item
             b.item_bins = ops.attn_item_bins(rows, KV, ctx, b.chunk)
@@ -295,8 +333,8 @@ class StaticBackbone:
         """Whether a step of `rows` rows runs as one persistent kernel: one row (the one-seat frame), the
         Qwen3-0.6B geometry the kernel implements (hidden 1024 with the folded norms, 16 q / 8 kv heads of 128,
         SwiGLU 3072, bf16), a per-slot extent of at most 4096 positions, one workgroup per CU on a 256-CU part."""
-        return (self.persistent and rows == 1 and self.fused_norms and self.dtype == torch.bfloat16
-                and self.heads == 16 and self.kv_heads == 8
+        return (self.persistent and rows == 1 and self.kv_bits == 16
+                and self.fused_norms and self.dtype == torch.bfloat16 and self.heads == 16 and self.kv_heads == 8
                 and self.head_dim == 128 and self.inter == 3072 and self._extent <= 4096 and self._nwg == 256)
 
     def _run_args(self, b):
@@ -339,6 +377,19 @@ class StaticBackbone:
         self._run_sync[2].zero_()
         self._watch.evt = None
 
+    def _attend4(self, b, i, x_norm):
+        """q|k|v of layer i (x_norm: the first layer's normed input, else the residual with its norm to come), the
+        4-bit cache write and the attention over it."""
+        attn = self.layers[i].self_attn
+        if x_norm is not None or not self.fused_norms:
+            ops.linear(b.y if x_norm is None else x_norm, self.pqkv[i], b.qkv)
+        else:
+            ops.linear_normed(b.h, b.part, self.eps, ops.NORM_RMS, self.pqkv[i], y=b.qkv)
+        ops.qk_norm_rope_kv4(b.qkv, b.q, self.kv4[i], b.slots, b.pos, self.cos, self.sin, attn.q_norm.weight,
+                             attn.k_norm.weight, self.eps, self.heads)
+        ops.kv4_attn(b.q, self.kv4[i], b.o.view(b.rows, self.heads, self.head_dim), b.slots, b.pos, self.scaling, b.ctx,
+                     b.chunk, b.attn_ws)
+
     def forward(self, b):
         """One decode step over the rows of buffer set `b` (positions from lengths[slots] + offset); returns b.out."""
         H, KV, D, eps = self.heads, self.kv_heads, self.head_dim, self.eps
@@ -351,21 +402,27 @@ class StaticBackbone:
         fused = self.fused_norms
         rms = ops.NORM_RMS
         for i, layer in enumerate(self.layers):
-            attn, kc, vc = layer.self_attn, self._kfull[i], self._vfull[i]
+            attn = layer.self_attn
             w_in, w_post = layer.input_layernorm.weight, layer.post_attention_layernorm.weight
-            qk = (b.qkv, b.q, kc, vc, b.slots, b.pos, self.cos, self.sin, attn.q_norm.weight, attn.k_norm.weight,
-                  eps, H, KV)
             if i == 0:
                 ops.add_rms(b.x, None, w_in, eps, y=b.y)
-                ops.linear_qk_rope(b.y, self.pqkv[i], *qk)
-            elif fused:  # the norm of the residual the previous down projection left, folded into the projection
-                ops.linear_qk_rope(b.h, self.pqkv[i], *qk, part=b.part, eps_in=eps)
-            else:
+            elif not fused:
                 ops.add_rms(b.h, b.pend, w_in, eps, h_out=b.h, y=b.y)
-                ops.linear(b.y, self.pqkv[i], b.qkv)
-                ops.qk_norm_rope_cache(*qk)
-            ops.decode_attn(b.q, kc, vc, o3, b.slots, b.pos, self.scaling, b.ctx, b.chunk, b.attn_ws, H, KV,
-                            items=b.items)
+            if self.kv_bits == 4:
+                self._attend4(b, i, b.y if i == 0 else None)
+            else:
+                kc, vc = self._kfull[i], self._vfull[i]
+                qk = (b.qkv, b.q, kc, vc, b.slots, b.pos, self.cos, self.sin, attn.q_norm.weight, attn.k_norm.weight,
+                      eps, H, KV)
+                if i == 0:
+                    ops.linear_qk_rope(b.y, self.pqkv[i], *qk)
+                elif fused:  # the norm of the residual the previous down projection left, folded into the projection
+                    ops.linear_qk_rope(b.h, self.pqkv[i], *qk, part=b.part, eps_in=eps)
+                else:
+                    ops.linear(b.y, self.pqkv[i], b.qkv)
+                    ops.qk_norm_rope_cache(*qk)
+                ops.decode_attn(b.q, kc, vc, o3, b.slots, b.pos, self.scaling, b.ctx, b.chunk, b.attn_ws, H, KV,
+                                items=b.items)
             if fused:
                 ops.linear_resid(b.o, self.po[i], b.x if i == 0 else b.h, b.h, b.part, rms)
                 ops.linear_normed(b.h, b.part, eps, rms, self.pgate[i], self.pup[i], ops.ACT_SWIGLU, y=b.act)
@@ -385,6 +442,8 @@ class StaticBackbone:
     # ---------------------------------------------------------------- graphs
     @torch.inference_mode()
     def _graph(self, rows, ctx, mixed=False, items=False):
+        if self.kv_bits == 4:
+            mixed = items = False  # one launch attends every kind of step
         key = (rows, ctx, 'mixed') if mixed else ((rows, ctx, 'items') if items else (rows, ctx))
         g = self.graphs.get(key)
         if g is not None:
@@ -418,7 +477,7 @@ class StaticBackbone:
     def _spread(self, rows, runs):
         """Whether a decode step of `rows` rows (runs as _rows_of gives them) takes the item launch: its longest
         context more than ITEM_SKEW times the mean."""
-        if rows < ITEM_MIN_ROWS or self._persistent_ok(rows):
+        if rows < ITEM_MIN_ROWS or self.kv_bits == 4 or self._persistent_ok(rows):
             return False
         ctxs = np.asarray(runs, dtype=np.int64).reshape(-1, 3)[:, 2] + 1
         return int(ctxs.max()) > ITEM_SKEW * (int(ctxs.sum()) / len(ctxs))
@@ -468,7 +527,7 @@ class StaticBackbone:
         # a decode step keyed by its seats restages nothing when they repeat
         b.table.stage(dict(slot=row_slot, real=np.ones(n, dtype=np.int64), offset=row_off),
                       key=None if prefills else ('decode', tuple(slots)))
-        if prefills or spread:
+        if (prefills or spread) and self.kv_bits == 16:
             # a decode step's list stays valid while every row keeps its number of splits (the kernels take each
             # split's keys and a row's split count from the positions at run time): it is rebuilt only when a row
             # crosses a split boundary or the seats change
@@ -534,4 +593,5 @@ class StaticBackbone:
         return out[:B].clone(), [out[e].clone() for e in ends]
 
     def memory_bytes(self):
-        return sum(t.numel() * t.element_size() for t in self._kfull + self._vfull)
+        return sum(t.numel() * t.element_size() for t in self._kfull + self._vfull) \
+            + sum(c.memory_bytes() for c in self.kv4)
