@@ -203,7 +203,8 @@ struct Kv4Attn {
   long so_b, so_h;
   const int64_t* slots;
   const int32_t* pos;
-  float scale_log2;
+  float scale_log2;   // |scale| log2(e), not 0
+  uint32_t q_flip;    // the sign bits of two query elements where scale < 0
   int rows, heads, G, hblocks, qb, R, nblk, chunk, max_ctx, max_splits;
   uint32_t over_Gc;  // x * over_Gc >> 8 = x / min(G, 16) for x < 16
   float* part;  // [rows * heads][max_splits][D] then [rows * heads][max_splits][2] (maximum, sum)
@@ -240,13 +241,14 @@ __device__ __forceinline__ void kv4_vop(const Words<D / 32>& v0, const Words<D /
 
 template <int DT, int D, int NG, int B = 0>
 __device__ __forceinline__ void kv4_pv(const Words<D / 32> (&v)[NG], const uint32_t (&vs)[NG],
-                                       const u16x8 (&pop)[NG / 2], f32x4_t (&acc)[D / 16]) {
+                                       const fp4_u4 (&pop)[NG / 2], f32x4_t (&acc)[D / 16]) {
 #pragma unroll
   for (int h = 0; h < NG / 2; ++h) {
     u16x8 lo, hi;
     kv4_vop<DT, D, B>(v[2 * h], v[2 * h + 1], vs[2 * h], vs[2 * h + 1], lo, hi);
-    acc[2 * B] = mfma16x16x32<DT>(lo, pop[h], acc[2 * B]);
-    acc[2 * B + 1] = mfma16x16x32<DT>(hi, pop[h], acc[2 * B + 1]);
+    const u16x8 p = __builtin_bit_cast(u16x8, pop[h]);
+    acc[2 * B] = mfma16x16x32<DT>(lo, p, acc[2 * B]);
+    acc[2 * B + 1] = mfma16x16x32<DT>(hi, p, acc[2 * B + 1]);
   }
   if constexpr (B + 1 < D / 32) kv4_pv<DT, D, NG, B + 1>(v, vs, pop, acc);
 }
@@ -341,6 +343,8 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
   __builtin_amdgcn_sched_barrier(0);
   load_v(b1);
   __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) qop[i] = __builtin_bit_cast(u16x8, __builtin_bit_cast(fp4_u4, qop[i]) ^ a.q_flip);
 
   float m_run = -INFINITY, l_run = 0.f;
   f32x4_t acc[ND];
@@ -358,7 +362,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
 #pragma unroll
       for (int i = 0; i < NI; ++i) s = mfma16x16x32<DT>(fp4_eight<DT>(t.kw[g].w[i], sc), qop[i], s);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sv[4 * g + r] = s[r] * a.scale_log2;
+      for (int r = 0; r < 4; ++r) sv[4 * g + r] = s[r];
     }
     __builtin_amdgcn_sched_barrier(0);
     load_k(t);
@@ -379,7 +383,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     const float mu = mx == -INFINITY ? 0.f : mx;  // no key seen yet: every weight is exp2(-inf) = 0
     if (__ballot(mx > m_run)) {  // a column's maximum grew
       asm volatile("");  // keeps the products behind the branch
-      const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
+      const float alpha = __builtin_amdgcn_exp2f((m_run - mu) * a.scale_log2);
       l_run *= alpha;
 #pragma unroll
       for (int T = 0; T < ND; ++T) acc[T] *= alpha;
@@ -387,14 +391,16 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     m_run = mx;
     // fp16 weights stand 2^15 higher (up to 32768), as do their sums: below 2^-14 fp16 loses relative precision, and
     // many keys of small weight would lose their part
-    const float mp = mu - (DT == M3X_F16 ? 15.f : 0.f);
-    u16x8 pop[NG / 2];
+    const float mp = mu * a.scale_log2 - (DT == M3X_F16 ? 15.f : 0.f);
+    fp4_u4 pop[NG / 2];
     float ps = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4 * NG; ++e) {
-      const float p = __builtin_amdgcn_exp2f(sv[e] - mp);
-      ps += p;
-      pop[e / 8].v[e % 8] = E<DT>::from_f(p);
+    for (int e = 0; e < 4 * NG; e += 2) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -mp));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], a.scale_log2, -mp));
+      ps += x;
+      ps += y;
+      pop[e / 8][e % 8 / 2] = fp4_pack<DT>(x, y);
     }
     l_run += ps;
     // 0 * V is 0 only for finite V. Keys of an edge tile whose scale is past every written number's (stale bytes, or a
@@ -424,11 +430,11 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
       for (int q = 0; q < 4; ++q)
       for (uint32_t left = __builtin_amdgcn_readlane(odd, 16 * q); left; left &= left - 1) {
         const int at = __builtin_ctz(left), key = k0 + 16 * (at >> 2) + 4 * q + (at & 3);
-        uint16_t mine = 0;
+        uint32_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < 4 * NG; ++e)
-          if (e == at) mine = pop[e / 8].v[e % 8];
-        const float p = E<DT>::to_f((uint16_t)__shfl((int)mine, 16 * q + li, 64));
+        for (int e = 0; e < 4 * NG; e += 2)
+          if (e == (at & ~1)) mine = pop[e / 8][e % 8 / 2];
+        const float p = E<DT>::to_f((uint16_t)(__shfl((int)mine, 16 * q + li, 64) >> (16 * (at & 1))));
         if (key > min(kend - 1, pq)) continue;
         const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
         const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
@@ -469,7 +475,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
       }
   }
   if (lg == 0) {
-    lds.m[wave][li] = m_run;
+    lds.m[wave][li] = m_run * a.scale_log2;
     lds.l[wave][li] = l_run;
   }
   __syncthreads();
@@ -743,8 +749,12 @@ M3X_API int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_
   int R = 1;
   while (R < qb && (long)rows * c.kv_heads * hb * splits >= 4096L * R) R *= 2;
   R = R < qb ? R : qb;
+  // a weight is exp2 of one fused multiply-add of the raw score: its factor must not be negative (the running maximum is
+  // the raw scores') or 0 (0 * -inf of a masked key); one this small leaves every weight of finite scores at 1
+  float weight = fabsf(scale) * 1.44269504088896341f;
+  if (weight < 0x1p-100f) weight = 0x1p-100f;
   const Kv4Attn a = {(const uint16_t*)q, sq_b, sq_h, (uint16_t*)out, so_b, so_h, slots, pos,
-                     scale * 1.44269504088896341f, rows, heads, G, hb, qb, R, m3x_ceil_div(rows, qb), chunk, max_ctx, splits,
+                     weight, scale < 0.f ? 0x80008000u : 0u, rows, heads, G, hb, qb, R, m3x_ceil_div(rows, qb), chunk, max_ctx, splits,
                      (uint32_t)((256 + Gc - 1) / Gc), (float*)workspace};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == M3X_BF16 && head_dim == 128) kv4_launch<M3X_BF16, 128>(c, a, st);

@@ -46,6 +46,12 @@ template <int DT, int SEL> __device__ __forceinline__ uint32_t fp4_pair(uint32_t
   else
     return __builtin_bit_cast(uint32_t, (fp4_bf2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
 }
+// a | b << 16 as 16-bit numbers (to nearest even), one instruction
+template <int DT> __device__ __forceinline__ uint32_t fp4_pack(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == M3X_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), fp4_h2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), fp4_bf2));
+}
 // the eight numbers of w in order
 template <int DT> __device__ __forceinline__ u16x8 fp4_eight(uint32_t w, float scale) {
   const fp4_u4 r = {fp4_pair<DT, 0>(w, scale), fp4_pair<DT, 1>(w, scale), fp4_pair<DT, 2>(w, scale),
