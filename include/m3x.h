@@ -512,14 +512,15 @@ int m3x_backbone_run(const M3xBackboneRun* args, void* stream);
  * 6) and a scale byte b for s = 2^(b - 127), the smallest power of two with max|x| <= 7 s (1 <= b <= 252; fp16 numbers
  * <= 140); codes to nearest, ties to the even code, 6 above 5 s, so |x - value| <= s (fp16 numbers above 57344 and
  * bf16 numbers above 7 * 2^125 lose up to 2 s). A group holding a NaN or an infinity is stored with b = 255 and reads
- * as NaN. No counterpart in the reference, whose caches and weights are 16-bit (serve/fast_backbone.py:146-150).
+ * as NaN. A call takes the numbers in its 16-bit type, rounded to nearest where the type is not the one they came from
+ * (fp16 holds them all for 104 <= b <= 140). No counterpart in the reference, whose caches and weights are 16-bit (serve/fast_backbone.py:146-150).
  *
  * The cache (per layer; cap % 32 == 0, head_dim D in {64, 128}; all four 16-byte aligned and contiguous), bytes:
  *   k4  [slots][kv_heads][cap][D / 2]               byte j: dims 2j (low half), 2j + 1
  *   ks4 [slots][kv_heads][cap][D / 32]              scale bytes
  *   v4  [slots][kv_heads][cap / 4][16][4][D / 32]   four positions together; chunk c: dims c D/16 .. (c + 1) D/16 - 1
  *   vs4 [slots][kv_heads][cap / 4][D / 32][4]       scale bytes
- * A row whose slot is outside [0, slots) or whose position is outside [0, cap) is outside the cache. */
+ * cap <= 2^30. A row whose slot is outside [0, slots) or whose position is outside [0, cap) is outside the cache. */
 typedef struct M3xKv4 {
   void* k;  /* k4 */
   void* ks; /* ks4 */
@@ -531,7 +532,8 @@ typedef struct M3xKv4 {
 /* The struct is on the host and read during the call. */
 
 /* K and V rows [rows, kv_heads, D] (row and head strides % 8 == 0) quantised to position pos[r] of slot slots[r]; a
- * row outside the cache is not written. Rows of one call at the same place leave either row's bytes there. */
+ * row outside the cache is not written. Rows of one call are to be at different places: at one place they leave a
+ * mixture of their codes and scales. */
 int m3x_kv4_append(const M3xKv4* cache, const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h,
                    const int64_t* slots, const int32_t* pos, int rows, int dtype, void* stream);
 
@@ -552,9 +554,10 @@ size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, in
 /* out[r, h] = softmax(scale q[r, h] . K^T) V over positions 0 .. pos[r] of slot slots[r], kv head h / (heads /
  * kv_heads); q and out [rows, heads, D] 16-bit (strides % 8 == 0, 16-byte aligned). pos[r] < 0 or a slot outside the
  * cache: zeros. max_ctx >= pos[r] + 1 for every row (keys past it are not attended), <= cap; chunk = keys per split,
- * a multiple of 128; at most 2^20 rows and 65535 splits. What a row does not see has no part in its result, whatever it holds. Rows next to each other in
- * the call, of one slot at consecutive positions (a prompt's), share one pass over the keys; a row's bits do not
- * depend on that, and not on the other rows. Fixed summation order. */
+ * a multiple of 128; at most 2^20 rows and 65535 splits. What a row does not see has no part in its result, whatever it
+ * holds. Rows next to each other in the call, of one slot at consecutive positions (a prompt's), share one pass over the
+ * keys; a row's bits do not depend on that, and not on the other rows. Fixed summation order. Two calls that may run at
+ * the same time need a workspace each. */
 int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
                  const int64_t* slots, const int32_t* pos, float scale, int rows, int heads, int max_ctx, int chunk,
                  void* workspace, size_t ws_bytes, int dtype, void* stream);
@@ -569,8 +572,8 @@ long m3x_packed_weight4_bytes(int N, int K, int scales);
 int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes, void* scales, int dtype, void* stream);
 
 /* y[M, N] = x[M, K] . W^T with W from m3x_pack_weight4; bf16 / fp16 rows (ldx % 8 == 0, x 16-byte aligned), fp32
- * products and sums, one rounding. The 4-bit form of m3x_linear for few rows (any M; weights are read once per 64
- * rows). Deterministic, one launch, no workspace. */
+ * products and sums, one rounding. The 4-bit form of m3x_linear for few rows (M <= 1048560, N <= 2^26; the weights are
+ * read once per 16 to 64 rows). Deterministic, one launch, no workspace. */
 int m3x_linear4(const void* x, long ldx, const void* codes, const void* scales, void* y, long ldy, int M, int N, int K,
                 int dtype, void* stream);
 

@@ -617,8 +617,8 @@ class Kv4Cache:
             raise ValueError(f"Kv4Cache: k must be [slots, kv_heads, cap, head_dim / 2], got {tuple(k.shape)}")
         S, KV, cap, half = k.shape
         D = 2 * half
-        if D not in (64, 128) or cap % 32 or min(S, KV, cap) < 1:
-            raise ValueError(f"Kv4Cache: head_dim {D} must be 64 or 128 and cap {cap} a multiple of 32")
+        if D not in (64, 128) or cap % 32 or cap > 1 << 30 or min(S, KV, cap) < 1:
+            raise ValueError(f"Kv4Cache: head_dim {D} must be 64 or 128 and cap {cap} a multiple of 32 up to 2^30")
         for t, shape, name in ((k, (S, KV, cap, D // 2), "k"), (ks, (S, KV, cap, D // 32), "ks"),
                                (v, (S, KV, cap // 4, 16, 4, D // 32), "v"), (vs, (S, KV, cap // 4, D // 32, 4), "vs")):
             if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
@@ -683,7 +683,8 @@ def _on_gpu(name, cache):
 
 def kv4_append(k, v, cache, slots, pos):
     """K and V rows [rows, kv_heads, head_dim] (bf16 or fp16, any row and head strides) quantised to position pos[r]
-    (int32) of slot slots[r] (int64). A row whose slot or position is outside the cache is not written."""
+    (int32) of slot slots[r] (int64). A row whose slot or position is outside the cache is not written; rows at one
+    place leave a mixture there."""
     rows, sp, pp = _kv4_rows("kv4_append", cache, slots, pos)
     ka = _kv4_heads("kv4_append", "k", k, cache, rows, cache.kv_heads)
     va = _kv4_heads("kv4_append", "v", v, cache, rows, cache.kv_heads, k.dtype)
@@ -750,8 +751,8 @@ def kv4_attn(q, cache, out, slots, pos, scale, max_ctx, chunk, workspace):
     """out[r, h] = softmax(scale q[r, h] . K^T) V over positions 0 .. pos[r] of slot slots[r]; q, out
     [rows, heads, head_dim] (bf16 or fp16, any row and head strides). A row with pos[r] < 0 or a slot outside the
     cache gets zeros. max_ctx: at least every pos[r] + 1; chunk: keys per split (kv4_attn_chunk); workspace: a tensor of
-    kv4_attn_workspace bytes, or None when that is 0. Rows of one slot at consecutive positions (a prompt's) that
-    stand next to each other share one pass over the keys."""
+    kv4_attn_workspace bytes, or None when that is 0 (calls that may run at the same time need one each). Rows of one
+    slot at consecutive positions (a prompt's) that stand next to each other share one pass over the keys."""
     rows, sp, pp = _kv4_rows("kv4_attn", cache, slots, pos)
     heads = q.shape[1] if q.dim() == 3 else 0
     if heads == 0 or heads % cache.kv_heads:

@@ -166,6 +166,7 @@ ODD = ctypes.c_void_p(4098)
     (_append, dict(nslots=0), -1), (_append, dict(kv_heads=0), -1), (_append, dict(dtype=2), -5),
     (_append, dict(k=None), -2), (_append, dict(vs4=None), -2), (_append, dict(slots=None), -2), (_append, dict(sk_r=12), -1),
     (_append, dict(sv_h=4), -1), (_append, dict(v=ODD), -1), (_append, dict(k4=4098), -1),
+    (_append, dict(cap=(1 << 30) + 32), -1), (_attn, dict(cap=(1 << 30) + 32), -1),
     (_append, dict(rows=2 ** 31 - 1, kv_heads=64), -1), (_append, dict(rows=1 << 25, kv_heads=8), -1),
     (_read, dict(rows=0), 0), (_read, dict(rows=-1), -1), (_read, dict(cap=40), -1), (_read, dict(k4=None), -2),
     (_read, dict(v=None), -2), (_read, dict(k=ODD), -1), (_read, dict(sv_r=3), -1), (_read, dict(dtype=2), -5),

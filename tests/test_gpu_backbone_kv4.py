@@ -168,3 +168,29 @@ def test_refusals(gpu):
         sb.export_prefix(1, 2)
     with pytest.raises(ValueError):
         sb.prefill(5, torch.zeros(CAP + 1, 1024, dtype=torch.bfloat16, device=gpu))
+
+
+def test_other_geometry(gpu):
+    """Eight query heads of 64 over two kv heads at a width without folded norms: decode, prefill and a graph's replay."""
+    from m3x.serve.fast_backbone import StaticBackbone
+    geo = dict(layers=2, hidden=512, heads=8, kv_heads=2, head_dim=64, inter=768, seed=31, affine=synth.AFFINE)
+    bb_c = synth.qwen3_backbone(device="cpu", **geo)
+    sb = StaticBackbone(synth.qwen3_backbone(device=gpu, **geo), 3, capacity=200, batch_buckets=(2, 32),
+                        ctx_buckets=(200,), kv_bits=4)
+    assert not sb.fused_norms and sb.kv4[0].cap == 224
+    cos, sin = O.rope_tables(64, 1e6, 224, torch.bfloat16)
+    new = lambda dt: [Q4(torch.zeros(4, 2, 200, 64, dtype=dt)) for _ in range(2)]  # noqa: E731
+    st = (sb, bb_c, new(torch.bfloat16), new(torch.bfloat16), torch.zeros(4, dtype=torch.long), cos, sin,
+          dict(bb=convert(bb_c, torch.float32), kc=new(torch.float32), vc=new(torch.float32),
+               lengths=torch.zeros(4, dtype=torch.long), cos=cos.float(), sin=sin.float()))
+    g = torch.Generator().manual_seed(32)
+    p = (torch.randn(30, 512, generator=g) * 0.5).to(torch.bfloat16)
+    got = sb.prefill(1, p.to(gpu))
+    ref, truth = _both(st, [1] * 30, p, torch.arange(30))
+    ok, info = floor_check(got[None], ref[-1:], truth[-1:])
+    assert ok, info
+    for _ in range(3):
+        x = torch.randn(2, 512, generator=g).to(torch.bfloat16)
+        ok, info = floor_check(sb.step([1, 2], x.to(gpu)), *_both(st, [1, 2], x))
+        assert ok, info
+    assert sb.lengths_cpu[:3] == [0, 33, 3]

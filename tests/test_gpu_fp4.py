@@ -305,6 +305,35 @@ def test_attn_extreme_scores(gpu):
         assert torch.isnan(got[4, 1]).all() and torch.isfinite(got[4, 0]).all()
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128)])
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.2, 1e-30, -1e-40, 2.0, -2.0])
+def test_attn_scales(gpu, dtype, D, scale):
+    """Any finite scale: 0 (every weight the same), negative, one below the smallest normal number, large."""
+    c = _filled(gpu, 2, 2, 288, D, dtype, 3)
+    pos, slots = torch.tensor([0, 31, 40, 41, 42, 287]), torch.tensor([1, 0, 1, 1, 1, 0])
+    q = torch.randn(len(pos), 4, D, generator=_g(4)).to(dtype).to(gpu)
+    for chunk in (128, 384):
+        _check(_attend(q, c, slots.to(gpu), pos.int().to(gpu), scale, 288, chunk), q, c, slots, pos, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_read_every_scale(gpu, dtype):
+    """Each code at each scale byte reads as its number rounded to the type, whichever type it was written from."""
+    from m3x import ops
+    c = ops.Kv4Cache.empty(1, 1, 256, 64, gpu)
+    code = torch.arange(64) % 16
+    kb = (code[0::2] | code[1::2] << 4).to(torch.uint8)
+    c.k.copy_(kb.expand(1, 1, 256, 32))
+    c.ks.copy_(torch.arange(256).to(torch.uint8)[None, None, :, None].expand(1, 1, 256, 2))
+    k = torch.empty(256, 1, 64, dtype=dtype, device=gpu)
+    ops.kv4_read(c, torch.zeros(256, dtype=torch.long, device=gpu), torch.arange(256, dtype=torch.int32, device=gpu), k,
+                 torch.empty_like(k))
+    mag = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+    want = torch.cat([mag, -mag])[code] * 2.0 ** (torch.arange(256, dtype=torch.float64)[:, None] - 127)
+    want = want.float().to(dtype)  # exact in fp32, one rounding to the type
+    assert torch.equal(k[:255, 0].cpu(), want[:255]) and k[255].isnan().all()
+
+
 def test_attn_long_split(gpu):
     """A long context in many splits (offsets of its last slot past 2^31 are in test_attn_far_slot)."""
     dtype, D = torch.bfloat16, 64
