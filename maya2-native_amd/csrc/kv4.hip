@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 // consecutive positions (a prompt's), found from slots and pos by the workgroup itself; the block's later rows' own
 // workgroups leave at once. A single token is a block of one row. Each of the NW waves takes every NW-th 32-key tile:
 //   S^T = K . Q^T   per 16 keys D / 32 MFMA 16x16x32: a lane's words of K become 16-bit operands in registers
-//   softmax         running reference and sum in fp32, exp2; a lane keeps its own column's, its keys' partial sum
+//   softmax         running maximum and sum in fp32, exp2; a lane keeps its own column's, its keys' partial sum
 //   O^T += V^T . P  D / 16 MFMA per 32 keys: S^T's accumulator is the P operand as it stands, and V's words, which
 //                   hold two dims of a key each, are paired over keys by byte permutes
 // P is rounded to the 16-bit type (at most half a step, relative 2^-8 bf16 / 2^-11 fp16, per key); everything else
@@ -212,7 +212,7 @@ struct Kv4Attn {
   uint32_t q_flip;    // the sign bits of two query elements where scale < 0
   int rows, heads, G, hblocks, qb, R, chunk, max_ctx, max_splits;
   uint32_t over_Gc;  // x * over_Gc >> 8 = x / min(G, 16) for x < 16
-  float* part;  // [rows * heads][max_splits][D] then [rows * heads][max_splits][2] (reference, sum)
+  float* part;  // [rows * heads][max_splits][D] then [rows * heads][max_splits][2] (maximum, sum)
 };
 
 // four outputs O / L (one quotient: its rounding and the products' are fp32's)
@@ -351,10 +351,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
 #pragma unroll
   for (int i = 0; i < NI; ++i) qop[i] = __builtin_bit_cast(u16x8, __builtin_bit_cast(fp4_u4, qop[i]) ^ a.q_flip);
 
-  // Weights reach 2^(REF_GAP + W_TOP). fp16's stand 2^11 higher, as do their sums, and stay below 2^15: below 2^-14 it
-  // loses relative precision, and many keys of small weight would lose their part.
-  constexpr float REF_GAP = DT == M3X_F16 ? 4.f : 8.f, W_TOP = DT == M3X_F16 ? 11.f : 0.f;
-  float m_ref = -INFINITY, shift = -W_TOP, l_run = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
   f32x4_t acc[ND];
 #pragma unroll
   for (int T = 0; T < ND; ++T) acc[T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -387,26 +384,25 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     float mx = sv[0];
 #pragma unroll
     for (int e = 1; e < 4 * NG; ++e) mx = fmaxf(mx, sv[e]);
-    mx = xor32_max(xor16_max(mx));
-    // The weights' reference is a maximum seen, renewed only when a score passes it by REF_GAP: with 16 columns nearly
-    // every tile of a short context would have one that grew. A column's own scores alone decide (its bits do not
-    // depend on the others').
-    const bool renew = (mx - m_ref) * a.scale_log2 > REF_GAP;  // -inf - -inf: no key seen yet, every weight is 0
-    if (__ballot(renew)) {
+    mx = fmaxf(m_run, xor32_max(xor16_max(mx)));
+    const float mu = mx == -INFINITY ? 0.f : mx;  // no key seen yet: every weight is exp2(-inf) = 0
+    if (__ballot(mx > m_run)) {  // a column's maximum grew
       asm volatile("");  // keeps the products behind the branch
-      const float alpha = renew ? __builtin_amdgcn_exp2f((m_ref - mx) * a.scale_log2) : 1.f;
+      const float alpha = __builtin_amdgcn_exp2f((m_run - mu) * a.scale_log2);
       l_run *= alpha;
 #pragma unroll
       for (int T = 0; T < ND; ++T) acc[T] *= alpha;
-      m_ref = renew ? mx : m_ref;
-      shift = renew ? mx * a.scale_log2 - W_TOP : shift;
     }
+    m_run = mx;
+    // fp16 weights stand 2^15 higher (up to 32768), as do their sums: below 2^-14 fp16 loses relative precision, and
+    // many keys of small weight would lose their part
+    const float mp = mu * a.scale_log2 - (DT == M3X_F16 ? 15.f : 0.f);
     fp4_u4 pop[NG / 2];
     float ps = 0.f;
 #pragma unroll
     for (int e = 0; e < 4 * NG; e += 2) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -shift));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], a.scale_log2, -shift));
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -mp));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], a.scale_log2, -mp));
       ps += x;
       ps += y;
       pop[e / 8][e % 8 / 2] = fp4_pack<DT>(x, y);
@@ -484,7 +480,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
       }
   }
   if (lg == 0) {
-    lds.m[wave][li] = m_ref * a.scale_log2;
+    lds.m[wave][li] = m_run * a.scale_log2;
     lds.l[wave][li] = l_run;
   }
   __syncthreads();
