@@ -176,14 +176,17 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 //   softmax         running maximum and sum in fp32, exp2; a lane keeps its own column's, its keys' partial sum
 //   O^T += V^T . P  D / 16 MFMA per 32 keys: S^T's accumulator is the P operand as it stands, and V's words, which
 //                   hold two dims of a key each, are paired over keys by byte permutes
-// P is rounded to the 16-bit type (at most half a step, relative 2^-8 bf16 / 2^-11 fp16, per key); everything else
-// between the loads and the output is exact or fp32.
+// P is rounded to the 16-bit type (at most half a step, relative 2^-8 bf16 / 2^-11 fp16, per key), and its sum is the
+// rounded weights'; everything else between the loads and the output is exact or fp32. A weight's reference is the
+// maximum itself: one renewed only when a score passes it by 2^8 saves 3 to 5 % where the arithmetic bounds, but then
+// the largest weight is rounded too, and the error against 64 bits rises by a sixth.
 //
 // Bound, measured on MI355X with 16/8 heads of 128: the cache's bytes where rows fill the GPU (224 rows of 2048 keys
-// 79 us, 499 MB at 6.3 TB/s; its loads without the arithmetic 78, the arithmetic without the loads 58, VALU busy 48 %).
-// With two waves a SIMD or fewer a tile's own chain of steps, about 1 us (2 rows of 120000 keys, 32/4 heads of 64: 17.6
-// us of 65 MB and 3.9 for the join). Short contexts: a block's start and its merge (1600 prompt rows over up to 500 keys
-// 26 us). One row of 2048 keys: 4.8 us and 3.5 for the join.
+// 79 us, 499 MB at 6.3 TB/s; its loads without the arithmetic 78, the arithmetic without the loads 58, VALU busy 46 %).
+// Few rows: the start, the merge and the join beside the bytes (2 rows of 120000 keys, 32/4 heads of 64: 17.1 us of 65 MB
+// and 3.8 for the join; one row of 2048 keys 4.8 and 3.5). A prompt over a long context: a tile's own chain of steps, about
+// 1 us at two waves a SIMD (512 rows over 4000 keys 36 us); over a short one a block's start and merge (1600 rows over up
+// to 500 keys 26 us).
 namespace {
 template <int NI> struct Words { uint32_t w[NI]; };
 // `base` is the same in every lane, so the load takes a scalar address and a 32-bit lane offset
@@ -398,16 +401,13 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     // many keys of small weight would lose their part
     const float mp = mu * a.scale_log2 - (DT == M3X_F16 ? 15.f : 0.f);
     fp4_u4 pop[NG / 2];
-    float ps = 0.f;
 #pragma unroll
     for (int e = 0; e < 4 * NG; e += 2) {
       const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -mp));
       const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], a.scale_log2, -mp));
-      ps += x;
-      ps += y;
       pop[e / 8][e % 8 / 2] = fp4_pack<DT>(x, y);
+      l_run = fp4_add2<DT>(pop[e / 8][e % 8 / 2], l_run);
     }
-    l_run += ps;
     // 0 * V is 0 only for finite V. Keys of an edge tile whose scale is past every written number's (stale bytes, or a
     // NaN that a later row of the block may see) stand apart: cleared here, added below to the columns that see them.
     uint32_t odd = 0;  // bit e: the lane's key e, in any of its groups

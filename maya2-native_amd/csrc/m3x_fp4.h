@@ -52,6 +52,15 @@ template <int DT> __device__ __forceinline__ uint32_t fp4_pack(float a, float b)
   if constexpr (DT == M3X_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), fp4_h2));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), fp4_bf2));
 }
+// acc + both 16-bit numbers of w (none negative), in fp32, one instruction. Measured: within 3.4 x 2^-24 of the sum,
+// fp16's subnormal numbers kept (262144 random pairs).
+template <int DT> __device__ __forceinline__ float fp4_add2(uint32_t w, float acc) {
+  if constexpr (DT == M3X_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(fp4_h2, w), __builtin_bit_cast(fp4_h2, 0x3C003C00u), acc, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(fp4_bf2, w), __builtin_bit_cast(fp4_bf2, 0x3F803F80u), acc,
+                                           false);
+}
 // the eight numbers of w in order
 template <int DT> __device__ __forceinline__ u16x8 fp4_eight(uint32_t w, float scale) {
   const fp4_u4 r = {fp4_pair<DT, 0>(w, scale), fp4_pair<DT, 1>(w, scale), fp4_pair<DT, 2>(w, scale),

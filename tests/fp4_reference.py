@@ -106,9 +106,13 @@ def attention(q, K, V, pos, scale):
 
 
 def attention_bound(out, mag, ds, dtype, keys):
-    """How far a kernel's output may be off: the weights rounded to the 16-bit type (half a step each, against fp32
-    weights in the sum that divides), the scores' fp32 rounding in numerator and denominator, the fp32 sums over the
-    keys, and the store's half step."""
+    """How far a kernel's output may be off: the weights rounded to the 16-bit type, the scores' fp32 rounding in
+    numerator and denominator, the fp32 sums over the keys, and the store's half step.
+
+    The rounded weights p (1 + d), |d| <= h, stand in numerator and denominator: sum p (1 + d) v / sum p (1 + d) - out =
+    sum p d (v - out) / sum p (1 + d), at most h / (1 - h) (sum p |v| + |out|) for weights that sum to 1. Either sum is
+    off by at most 2^-24 a key and term (the denominator's takes two keys at a time, within 3.4 * 2^-24)."""
     h = torch.finfo(dtype).eps / 2
-    return h * mag + 2 * ds * mag + (2 * keys + 16) * 2.0 ** -24 * mag + h * np.abs(out) + 1e-30 + \
+    sums = (2 * keys + 16) * 2.0 ** -24
+    return h / (1 - h) * (mag + np.abs(out)) + 2 * ds * mag + sums * mag + h * np.abs(out) + 1e-30 + \
         (2.0 ** -25 if dtype == torch.float16 else 0)  # half a step of fp16's smallest numbers
