@@ -10,7 +10,7 @@
 // columns, as read from memory: per step and 16 rows of x four MFMA 16x16x32, the lane's inputs 8 i .. 8 i + 7 in the
 // i-th. The waves of a workgroup share the steps out and their sums meet in LDS, added in wave order (deterministic).
 // Products and sums are fp32; the one rounding is the store's. Measured on MI355X: 9 rows through 16384 x 8192 (71.3 MB
-// of weights) 15.6 us, 4.6 TB/s; one row through 4096 x 1024 3.1 us; 64 rows through 2816 x 1024 twice, gated, 6.1 us.
+// of weights) 15.6 us, 4.6 TB/s; one row through 4096 x 1024 3.1 us; 64 rows through 2816 x 1024 twice, gated, 5.9 us.
 #include "m3x_fp4.h"
 
 namespace {
@@ -26,8 +26,13 @@ struct Lin4 {
 enum { L4_NONE, L4_SWIGLU, L4_GELU };
 }  // namespace
 
-// TW output tiles and 16 MT rows of x per workgroup of NW waves
-template <int DT, int TW, int MT, int NW, int ACT>
+// TW output tiles and 16 MT rows of x per workgroup of NW waves.
+//
+// A lane's operand of x is 64 bytes of one row. Read as such (TURN false), each lane's 16 bytes are an access of their own
+// to the vector L1, which from some rows on costs more than the weights do. With TURN a load takes four rows' 256
+// contiguous bytes, and the wave turns them over in 4 KB of LDS of its own (places swapped by the row, so that neither
+// side meets in a bank).
+template <int DT, int TW, int MT, int NW, int ACT, bool TURN>
 __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
   constexpr int P = ACT == L4_SWIGLU ? 2 : 1;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -45,11 +50,18 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[t][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+  // as many output tiles at a time as 64 KB hold the waves' sums of
+  constexpr int RT = NW * P * MT * TW <= 64 ? TW : 64 / (NW * P * MT);
+  constexpr int SUMS = NW * RT * P * MT * 64, STAGE = TURN ? NW * MT * 256 : 0;  // 16-byte places
+  __shared__ fp4_u4 lds[SUMS > STAGE ? SUMS : STAGE];
+  fp4_u4* const stage = lds + wave * (MT * 256);
+
   struct Step {
     fp4_u4 cw[TW * P];
     uint32_t sw[TW * P];
-    u16x8 x[MT][4];
+    fp4_u4 x[MT][4];
   };
+  const int xr = TURN ? lane >> 4 : li, xp = TURN ? lane & 15 : 4 * lg;  // what the lane loads: row, 16-byte piece
   auto load = [&](Step& q, int s) {
 #pragma unroll
     for (int t = 0; t < TW * P; ++t) {
@@ -58,20 +70,43 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
           reinterpret_cast<const fp4_u4*>(a.w[t % P] + ((tile * a.steps + s) * 64 + lane) * 16));
       q.sw[t] = *reinterpret_cast<const uint32_t*>(a.s[t % P] + ((tile * quads + (s >> 2)) * 64 + lane) * 4);
     }
-    const int k = 128 * s + 32 * lg;
+    const int k = 128 * s + 8 * xp;
+    const fp4_u4 zero = {0, 0, 0, 0};
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int r = m0 + 16 * m + li;
-      if (r < a.M && k < a.K) {
+      if constexpr (TURN) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q.x[m][i] = ld16(a.x + (long)r * a.ldx + k + 8 * i);
+        for (int i = 0; i < 4; ++i) {
+          const int r = m0 + 16 * m + 4 * i + xr;
+          q.x[m][i] = r < a.M && k < a.K ? __builtin_bit_cast(fp4_u4, ld16(a.x + (long)r * a.ldx + k)) : zero;
+        }
       } else {
+        const int r = m0 + 16 * m + xr;
+        if (r < a.M && k < a.K) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q.x[m][i] = zero_v8<DT>();
+          for (int i = 0; i < 4; ++i) q.x[m][i] = __builtin_bit_cast(fp4_u4, ld16(a.x + (long)r * a.ldx + k + 8 * i));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q.x[m][i] = zero;
+        }
       }
     }
   };
-  auto multiply = [&](const Step& q, int s) {
+  auto multiply = [&](Step& q, int s) {
+    if constexpr (TURN) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();  // the step before has been read
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) stage[256 * m + 16 * (4 * i + xr) + (xp ^ (4 * i + xr))] = q.x[m][i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.x[m][i] = stage[256 * m + 16 * li + ((4 * lg + i) ^ li)];
+    }
 #pragma unroll
     for (int t = 0; t < TW * P; ++t) {
       const float sc = fp4_scale((q.sw[t] >> (8 * (s & 3))) & 255u);
@@ -79,7 +114,7 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
       for (int i = 0; i < 4; ++i) {
         const u16x8 wv = fp4_eight<DT>(q.cw[t][i], sc);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[t][m] = mfma16x16x32<DT>(wv, q.x[m][i], acc[t][m]);
+        for (int m = 0; m < MT; ++m) acc[t][m] = mfma16x16x32<DT>(wv, __builtin_bit_cast(u16x8, q.x[m][i]), acc[t][m]);
       }
     }
   };
@@ -89,12 +124,11 @@ __global__ __launch_bounds__(64 * NW) void linear4_kernel(Lin4 a) {
     multiply(q, s);
   }
 
-  // as many output tiles at a time as 64 KB hold the waves' sums of
-  constexpr int RT = NW * P * MT * TW <= 64 ? TW : 64 / (NW * P * MT);
-  __shared__ f32x4_t red[NW][RT * P * MT][64];
+  typedef f32x4_t Sums[RT * P * MT][64];
+  Sums* const red = reinterpret_cast<Sums*>(lds);
 #pragma unroll
   for (int t0 = 0; t0 < TW; t0 += RT) {
-    if (t0) __syncthreads();
+    if (TURN || t0) __syncthreads();  // the waves' x, or the tiles before, have been read
 #pragma unroll
     for (int i = 0; i < RT * P * MT; ++i) red[wave][i][lane] = acc[t0 * P + i / MT][i % MT];
     __syncthreads();
@@ -185,9 +219,8 @@ M3X_API int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes,
   if (!m3x_aligned16(w) || !m3x_aligned16(codes) || !m3x_aligned16(scales)) return M3X_EINVAL;
   const int steps = m3x_ceil_div(K, 128), tiles = m3x_ceil_div(N, 16);
   hipStream_t st = (hipStream_t)stream;
-  const int ny = tiles < 65535 ? tiles : 65535;
   if (tiles > 65535) return M3X_EINVAL;
-  const dim3 grid(steps, ny);
+  const dim3 grid(steps, tiles);
   if (dtype == M3X_BF16)
     hipLaunchKernelGGL(pack_weight4_kernel<M3X_BF16>, grid, dim3(64), 0, st, (const uint16_t*)w, ldw, N, K,
                        (uint8_t*)codes, (uint8_t*)scales, steps);
@@ -204,30 +237,46 @@ M3X_API int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes,
 }
 
 namespace {
+// x turned over in LDS or not, measured on MI355X (us; not, turned): N 1024, K 8192 (1x1x8) 9 rows 8.4, 9.0, 12 rows 9.3,
+// 9.2, 16 rows 10.6, 9.6; N 5000, K 8192 (2x1x8) 1 row 10.3, 10.5, 5 rows 11.0, 10.8, 8 rows 13.9, 11.0, 16 rows 19.7,
+// 14.2; N 16384, K 8192 (4x1x16) 9 rows 16.0, 16.5, 16 rows 18.4, 17.3; 64 rows (8x2x8) 32.1, 28.7; N 11008, K 4096, 128 rows
+// gated (4x4x4, where it takes 304 of a wave's registers) 49, 57.
 template <int DT, int TW, int MT, int NW, int ACT> void launch4(const Lin4& a, hipStream_t st) {
-  hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT>), dim3(m3x_ceil_div(a.tiles, TW), m3x_ceil_div(a.M, 16 * MT)),
-                     dim3(64 * NW), 0, st, a);
+  const dim3 grid(m3x_ceil_div(a.tiles, TW), m3x_ceil_div(a.M, 16 * MT)), block(64 * NW);
+  if constexpr (MT == 1) {
+    if (a.M > (TW == 2 ? 4 : 12)) hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, false>), grid, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, MT == 2>), grid, block, 0, st, a);
+  }
 }
 template <int DT, int ACT> void plan4(const Lin4& a, hipStream_t st) {
-  // x meets every group of weight tiles anew, from L2 and in 16-byte pieces of 64-byte lines, so a workgroup takes as
-  // many tiles, then rows, as leave each of the 256 CUs one. Measured on MI355X (graph-timed, us; TW x MT x NW, the
-  // rule's first): N 16384, K 8192: 9 rows 4x1x16 16.0, 2x1x8 17.4, 1x1x8 25.0; 32 rows 4x2x8 24, 4x1x8 32, 1x1x8 66;
-  // 64 rows 8x2x8 33, 4x4x4 37, 4x1x8 56, 1x1x8 128. N 4096, K 4096: 16 rows 1x1x8 6.7, 2x1x8 7.4, 4x1x8 9.1; 32 rows
-  // 2x1x8 7.6, 1x1x8 10.9; 64 rows 4x1x8 9.6, 1x1x8 18.7. N 4096, K 1024, one row: 1x1x8 2.8, 2x1x8 3.0, 4x1x8 3.6.
+  // Weight tiles times 16-row blocks are dealt out over 256 CUs: a workgroup takes as many as leave every CU about one, so
+  // that x, which every group of tiles reads anew, is read the fewest times. Past 16 a CU, and for few steps of K, where a
+  // large group's start and sums weigh more, smaller groups run in several rounds. Measured on MI355X (us; TW x MT x NW, the
+  // rule's first):
+  //   plain, K 8192  N 16384: 16 rows 4x1x16 17.3, 2x1x8 18.7, 1x1x8 25; 32 rows 4x2x8 21.5, 8x2x8 28, 4x1x16 30; 64 rows
+  //                  8x2x8 28.8, 4x2x8 35; 256 rows 8x2x8 111, 4x2x8 123. N 5000: 16 rows 2x1x8 11.6, 1x1x8 14.0
+  //   plain, K 4096  N 11008: 16 rows 4x1x16 9.8, 2x1x8 11.5; 32 rows 4x2x8 13.0, 4x1x16 17; 256 rows 4x2x8 48, 8x2x8 54
+  //   plain, K 1024  N 4096: 16 rows 1x1x8 3.5; 64 rows 2x1x8 4.8, 4x1x16 5.2; 128 rows 2x1x8 5.4, 4x2x8 5.6, 8x2x8 7.9; 256
+  //                  rows 4x2x8 7.0, 8x2x8 8.1
+  //   gated, K 8192  N 16384: 16 rows 2x1x8 27.3, 4x1x8 28.7; 32 rows 4x2x8 33.7, 2x2x8 34.9; 64 rows 4x4x4 46, 4x2x8 65
+  //   gated, K 1024  N 4096: 64 rows 2x2x8 5.8, 4x2x8 7.6; 128 rows 2x2x8 6.9, 4x2x8 7.8; 256 rows 2x2x8 11.2, 4x4x4 12.0
   const int blocks = m3x_ceil_div(a.M, 16);
-  const long share = (long)a.tiles * blocks / 256;
-  if (share < 2) launch4<DT, 1, 1, 8, ACT>(a, st);
-  else if (share < 4) launch4<DT, 2, 1, 8, ACT>(a, st);
-  else if (blocks == 1 || share < 8) {
-    if constexpr (ACT == L4_SWIGLU) {
-      if (blocks == 1) launch4<DT, 4, 1, 8, ACT>(a, st);  // 16384 x 8192 twice, 16 rows: 32.5, 2x1x8 33.6
-      else launch4<DT, 2, 2, 8, ACT>(a, st);              // 8192 x 4096 twice, 32 rows: 15.0, 4x1x8 16.8
-    } else {
-      launch4<DT, 4, 1, 16, ACT>(a, st);
-    }
-  } else if (blocks == 2 || share < 16) launch4<DT, 4, 2, 8, ACT>(a, st);
-  else if constexpr (ACT == L4_SWIGLU) launch4<DT, 4, 4, 4, ACT>(a, st);  // 16384 x 8192 twice, 64 rows: 51, 4x2x8 70
-  else launch4<DT, 8, 2, 8, ACT>(a, st);
+  const long units = (long)a.tiles * blocks;
+  if (units <= 256) return launch4<DT, 1, 1, 8, ACT>(a, st);
+  if constexpr (ACT == L4_SWIGLU) {
+    if (units <= 512 || blocks == 1) launch4<DT, 2, 1, 8, ACT>(a, st);
+    else if (units <= (a.steps <= 8 ? 4096 : 1024) || (units > 2048 && units <= 4096 && a.steps <= 16))
+      launch4<DT, 2, 2, 8, ACT>(a, st);
+    else if (units <= 2048) launch4<DT, 4, 2, 8, ACT>(a, st);
+    else launch4<DT, 4, 4, 4, ACT>(a, st);
+  } else {
+    if (units <= (a.steps <= 8 ? 2048 : 512)) launch4<DT, 2, 1, 8, ACT>(a, st);
+    else if (blocks == 1 || (units <= 1024 && a.steps > 8)) launch4<DT, 4, 1, 16, ACT>(a, st);
+    else if (units <= 2048 || a.steps <= 8 || (units > 4096 && a.steps < 64)) launch4<DT, 4, 2, 8, ACT>(a, st);
+    else launch4<DT, 8, 2, 8, ACT>(a, st);
+  }
 }
 int linear4_any(const void* x, long ldx, const void* wg, const void* sg, const void* wu, const void* su, void* y,
                 long ldy, int M, int N, int K, int act, int dtype, void* stream) {

@@ -166,3 +166,66 @@ def test_rows_at_one_place(gpu):
         now[1, :, 17] = old[1, :, 17]
     c.v[1, :, 4, :, 1], c.vs[1, :, 4, :, 1] = before[2][1, :, 4, :, 1], before[3][1, :, 4, :, 1]
     assert all(torch.equal(a, b) for a, b in zip((c.k, c.ks, c.v, c.vs), before))
+
+
+def _product(x, w):
+    """(sums, bound of K products summed in fp32 in any order), float64."""
+    return x @ w.T, (x.shape[1] + 8) * 2.0 ** -24 * (np.abs(x) @ np.abs(w).T)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(4, 4200, 160), (7, 4200, 160), (9, 8300, 1056), (14, 8300, 1056), (3, 33000, 96),
+                                   (40, 6000, 1056), (200, 3000, 160), (530, 2000, 1056), (130, 3700, 1184),
+                                   (224, 4800, 8192)])
+def test_linear4_groups(gpu, dtype, M, N, K):
+    """Every grouping of tiles and rows a product is dealt out in, with rows, columns and inputs that end inside one,
+    and numbers beside x that are not finite."""
+    from m3x import ops
+    g = _g(M + N + K)
+    wide = torch.full((M + 1, K + 16), float("nan"), dtype=dtype)
+    wide[:M, 8:8 + K] = torch.randn(M, K, generator=g).to(dtype)
+    x = wide.to(gpu)[:M, 8:8 + K]
+    p = ops.pack_weight4((torch.randn(N, K, generator=g) * K ** -0.5).to(dtype).to(gpu))
+    y, off = _product(_f64(x), R.weight_values(p.codes, p.scales, N, K))
+    h, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype == torch.float16 else 0
+    big = torch.full((M + 1, N + 3), 3.0, dtype=dtype, device=gpu)
+    for out in (None, big[:M, 1:1 + N]):
+        got = _f64(ops.linear4(x, p, out))
+        assert (np.abs(got - y) <= off + h * (np.abs(y) + off) + tiny).all()
+    assert (big[M] == 3).all() and (big[:, :1] == 3).all() and (big[:, 1 + N:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(4, 4200, 160), (7, 4200, 160), (40, 3000, 160), (130, 3700, 1184), (40, 6000, 1056),
+                                   (70, 14000, 2080)])
+def test_linear4_act_groups(gpu, dtype, M, N, K):
+    """The same of silu(g) u: the slope is at most 1.13, so a product's error passes at most 1.13 times; the activation
+    is within 2^-20 of its value."""
+    from m3x import ops
+    g = _g(M + N + K + 1)
+    x = (torch.randn(M, K, generator=g) * 2).to(dtype).to(gpu)
+    pg, pu = (ops.pack_weight4((torch.randn(N, K, generator=g) * K ** -0.5).to(dtype).to(gpu)) for _ in "gu")
+    a, da = _product(_f64(x), R.weight_values(pg.codes, pg.scales, N, K))
+    b, db = _product(_f64(x), R.weight_values(pu.codes, pu.scales, N, K))
+    act = a / (1 + np.exp(-a))
+    y = act * b
+    off = 1.13 * da * (np.abs(b) + db) + np.abs(act) * db + 2.0 ** -20 * np.abs(y)
+    h, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype == torch.float16 else 0
+    got = _f64(ops.linear4_act(x, pg, pu, ops.ACT_SWIGLU))
+    assert (np.abs(got - y) <= off + h * (np.abs(y) + off) + tiny).all()
+
+
+def test_rows_of_x_stay_apart(gpu):
+    """An infinity in one row of x changes that row alone, also where K ends inside a step, whatever the grouping."""
+    from m3x import ops
+    for M, N, K in ((6, 4200, 160), (16, 100, 96), (40, 6000, 1056), (130, 3700, 1184)):
+        x = torch.randn(M, K, generator=_g(M)).bfloat16().to(gpu)
+        p = ops.pack_weight4(torch.randn(N, K, generator=_g(N)).bfloat16().to(gpu))
+        clean = ops.linear4(x, p)
+        x[M - 2, K - 1] = float("inf")
+        got = ops.linear4(x, p)
+        rest = [r for r in range(M) if r != M - 2]
+        w = R.weight_values(p.codes, p.scales, N, K)[:, K - 1]
+        assert torch.equal(got[rest], clean[rest])
+        want = torch.from_numpy(np.where(w == 0, np.nan, np.copysign(np.inf, w))).bfloat16().to(gpu)
+        assert torch.equal(torch.nan_to_num(got[M - 2], nan=7.0), torch.nan_to_num(want, nan=7.0))
