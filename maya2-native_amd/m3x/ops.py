@@ -585,11 +585,12 @@ def backbone_run(args: BackboneRunArgs):
 
 # ---------------------------------------------------------------- 4-bit cache and weights
 _raw_stream = torch._C._cuda_getCurrentRawStream  # a device's current stream as torch.cuda.current_stream, ~2 us cheaper
+_current_device = torch._C._cuda_getDevice  # as torch.cuda.current_device of an initialised process, ~0.2 us cheaper
 
 
 def _launch(dev, fn, *args):
     """A launching entry point on device `dev` (an index) and its current stream, whichever device is current."""
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
