@@ -432,31 +432,31 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     if (edge) {
       const int li = lane_o & 15, lg = lane_o >> 4;
       if (__ballot(odd != 0)) {
-      for (int q = 0; q < 4; ++q)
-      for (uint32_t left = __builtin_amdgcn_readlane(odd, 16 * q); left; left &= left - 1) {
-        const int at = __builtin_ctz(left), key = k0 + 16 * (at >> 2) + 4 * q + (at & 3);
-        uint32_t mine = 0;
+        for (int q = 0; q < 4; ++q)
+          for (uint32_t left = __builtin_amdgcn_readlane(odd, 16 * q); left; left &= left - 1) {
+            const int at = __builtin_ctz(left), key = k0 + 16 * (at >> 2) + 4 * q + (at & 3);
+            uint32_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < 4 * NG; e += 2)
-          if (e == (at & ~1)) mine = pop[e / 8][e % 8 / 2];
-        const float p = E<DT>::to_f((uint16_t)(__shfl((int)mine, 16 * q + li, 64) >> (16 * (at & 1))));
-        if (key > min(kend - 1, pq)) continue;
-        const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
-        const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
+            for (int e = 0; e < 4 * NG; e += 2)
+              if (e == (at & ~1)) mine = pop[e / 8][e % 8 / 2];
+            const float p = E<DT>::to_f((uint16_t)(__shfl((int)mine, 16 * q + li, 64) >> (16 * (at & 1))));
+            if (key > min(kend - 1, pq)) continue;
+            const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
+            const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int ch = 4 * lg + r;
-          const float s1 = fp4_scale(sp[4 * (ch * ND >> 5)]);
-          uint32_t w;
-          if constexpr (D == 128) w = *reinterpret_cast<const uint32_t*>(wp + ch * (4 * NI));
-          else w = *reinterpret_cast<const uint16_t*>(wp + ch * (4 * NI));
-          const u16x8 x = fp4_eight<DT>(w, s1);
+            for (int r = 0; r < 4; ++r) {
+              const int ch = 4 * lg + r;
+              const float s1 = fp4_scale(sp[4 * (ch * ND >> 5)]);
+              uint32_t w;
+              if constexpr (D == 128) w = *reinterpret_cast<const uint32_t*>(wp + ch * (4 * NI));
+              else w = *reinterpret_cast<const uint16_t*>(wp + ch * (4 * NI));
+              const u16x8 x = fp4_eight<DT>(w, s1);
 #pragma unroll
-          for (int T = 0; T < ND; ++T) acc[T][r] += p * E<DT>::to_f(x.v[T]);
-        }
-      }
-      // all loads of this path have arrived (vmcnt 0), so that behind it the tiles' own are counted as on the other
-      __builtin_amdgcn_s_waitcnt(0x0F70);
+              for (int T = 0; T < ND; ++T) acc[T][r] += p * E<DT>::to_f(x.v[T]);
+            }
+          }
+        // all loads of this path have arrived (vmcnt 0), so that behind it the tiles' own are counted as on the other
+        __builtin_amdgcn_s_waitcnt(0x0F70);
       }
     }
     load_v(t);
@@ -725,7 +725,8 @@ M3X_API size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max
 
 namespace {
 template <int DT, int D> void kv4_launch(const Kv4& c, const Kv4Attn& a, hipStream_t st) {
-  const dim3 grid(m3x_ceil_div(a.rows, a.qb), c.kv_heads * a.hblocks, a.max_splits * m3x_ceil_div(std::min(a.qb, a.rows), a.R));
+  const int parts = m3x_ceil_div(std::min(a.qb, a.rows), a.R);
+  const dim3 grid(m3x_ceil_div(a.rows, a.qb), c.kv_heads * a.hblocks, a.max_splits * parts);
   hipLaunchKernelGGL((kv4_attn_kernel<DT, D, KV4_NW>), grid, dim3(64 * KV4_NW), 0, st, c, a);
   if (a.max_splits > 4)
     hipLaunchKernelGGL((kv4_combine_kernel<DT, D, 8>), dim3(a.rows, m3x_ceil_div(a.heads, 128 / D)), dim3(256), 0, st, c, a);

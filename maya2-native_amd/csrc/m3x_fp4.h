@@ -20,7 +20,6 @@ typedef _Float16 fp4_h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t fp4_u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t fp4_u4 __attribute__((ext_vector_type(4)));
 
-static inline int fp4_top(int dtype) { return dtype == M3X_F16 ? 140 : 252; }
 template <int DT> __device__ __forceinline__ constexpr uint32_t fp4_top_of() { return DT == M3X_F16 ? 140u : 252u; }
 
 // scale byte of a group whose largest magnitude is `amax` (finite): 1.m x 2^(E - 127) <= 7 x 2^(b - 127) means
