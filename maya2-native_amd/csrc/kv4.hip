@@ -27,7 +27,7 @@ struct M3xKv4 {
 namespace {
 // Attention's workgroups: 4 waves, 3 of a SIMD's at once (up to 168 registers). Measured at 224 rows of 2048 keys, heads
 // 16/8 of 128 (us): 79; 8 waves 92, 2 waves 93; 4 waves a SIMD (128 registers) spill, 94 to 113.
-constexpr int KV4_NW = 4, KV4_OCC = 3;
+constexpr int KV4_NW = 4, KV4_OCC = 4;
 
 struct Kv4 {
   uint8_t* k;
@@ -263,23 +263,42 @@ __device__ __forceinline__ void kv4_pv(const Words<D / 32> (&v)[NG], const uint3
 
 }  // namespace
 
-// one block: rows row .. row + n - 1 of slot `slot`, the first at position p0
 template <int D, int NW> struct Kv4Lds {
   __align__(16) float o[NW][16][D + 4];
   float m[NW][16], l[NW][16];
+  long slot[64];
+  int pos[64];
 };
+// the lane's number, made anew: kept over the loop over the keys it, and what comes from it, would spill
+__device__ __forceinline__ int kv4_lane() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
+// a column of a block of n rows, the first at position p0: query head hq of row jq, which sees the keys up to pq
+struct Kv4Col {
+  int jq, hq, pq;
+  bool live;
+  __device__ __forceinline__ Kv4Col(const Kv4Attn& a, int li, int n, int Gc, int p0, int plim) {
+    jq = li * a.over_Gc >> 8;
+    hq = li - jq * min(a.G, 16);
+    live = jq < n && hq < Gc;
+    pq = live ? min(p0 + jq, plim) : -1;
+  }
+};
+// one block: rows row .. row + n - 1 of slot `slot`, the first at position p0
 template <int DT, int D, int NW>
 __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int row, int n, long slot, int p0, int kh,
-                                             int h0, int Gc, int split, int wave, int lane, Kv4Lds<D, NW>& lds) {
+                                             int h0, int Gc, int split, int wave, Kv4Lds<D, NW>& lds) {
   constexpr int NI = D / 32;   // words a lane holds of 16 keys; score steps
   constexpr int ND = D / 16;   // dim tiles
   constexpr int KT = 32, NG = KT / 16;  // keys of a tile, and its 16-key groups
-  const int li = lane & 15, lg = lane >> 4;
-  const int plim = min(c.cap, a.max_ctx) - 1;  // the host keeps pos below both; every access stays inside whatever pos holds
+  const int lane = kv4_lane(), li = lane & 15, lg = lane >> 4;
+  const int plim = min(c.cap, a.max_ctx) - 1;  // the caller keeps pos below both; accesses stay inside whatever pos holds
   if (slot < 0 || slot >= c.slots || p0 < 0) {  // no key: zeros
     if (split == 0)
       for (int j = 0; j < n; ++j)
-        for (int i = threadIdx.x; i < Gc * D; i += 64 * NW)
+        for (int i = 64 * wave + lane; i < Gc * D; i += 64 * NW)
           a.out[(long)(row + j) * a.so_b + (long)(kh * a.G + h0 + i / D) * a.so_h + i % D] = 0;
     return;
   }
@@ -288,10 +307,6 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
   if (kstart > plast) return;
   const int kend = min(kstart + a.chunk, plast + 1);
 
-  const int jq = li * a.over_Gc >> 8;  // the column's row within the block
-  const int hq = li - jq * min(a.G, 16);
-  const bool live = jq < n && hq < Gc;
-  const int pq = live ? min(p0 + jq, plim) : -1;  // the column sees keys <= pq
   const long base = (slot * c.kv_heads + kh) * (long)c.cap;
   // scale bytes come as whole words (a byte's widening would be waited for where it is loaded): the key's four at
   // D = 128, two keys' two each at D = 64; ks_rot brings the lane's byte to the exponent's place
@@ -300,7 +315,9 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
   const uint32_t v_at = lg * (2 * D) + li * (D / 8), vs_at = lg * (4 * NI) + (D == 128 ? li >> 2 : li >> 3) * 4;
   // a column past the block's rows computes with the first row's queries and is dropped
   u16x8 qop[NI];
-  const uint16_t* qp = a.q + (long)(row + (live ? jq : 0)) * a.sq_b + (long)(kh * a.G + h0 + (live ? hq : 0)) * a.sq_h;
+  const Kv4Col col(a, li, n, Gc, p0, plim);
+  const uint16_t* qp =
+      a.q + (long)(row + (col.live ? col.jq : 0)) * a.sq_b + (long)(kh * a.G + h0 + (col.live ? col.hq : 0)) * a.sq_h;
 #pragma unroll
   for (int i = 0; i < NI; ++i) qop[i] = ld16(qp + (D / 4) * lg + 8 * i);
   // Two tiles' words in turn: a tile's keys are loaded two tiles ahead, behind the products of the keys they replace, its
@@ -375,11 +392,9 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     __builtin_amdgcn_sched_barrier(0);
     load_k(t);
     __builtin_amdgcn_sched_barrier(0);
-    int lane_o = lane;
     if (edge) {
-      asm volatile("" : "+v"(lane_o));  // what the masks need is made here, not kept over the loop
-      const int lg = lane_o >> 4;
-      const int klim = min(kend - 1, pq);
+      const int lane = kv4_lane(), lg = lane >> 4;
+      const int klim = min(kend - 1, Kv4Col(a, lane & 15, n, Gc, p0, plim).pq);
 #pragma unroll
       for (int e = 0; e < 4 * NG; ++e)
         if (k0 + 16 * (e >> 2) + 4 * lg + (e & 3) > klim) sv[e] = -INFINITY;
@@ -430,8 +445,9 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     }
     kv4_pv<DT, D, NG>(t.vw, t.vs, pop, acc);
     if (edge) {
-      const int li = lane_o & 15, lg = lane_o >> 4;
       if (__ballot(odd != 0)) {
+        const int lane = kv4_lane(), li = lane & 15, lg = lane >> 4;
+        const int klim = min(kend - 1, Kv4Col(a, li, n, Gc, p0, plim).pq);
         for (int q = 0; q < 4; ++q)
           for (uint32_t left = __builtin_amdgcn_readlane(odd, 16 * q); left; left &= left - 1) {
             const int at = __builtin_ctz(left), key = k0 + 16 * (at >> 2) + 4 * q + (at & 3);
@@ -440,7 +456,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
             for (int e = 0; e < 4 * NG; e += 2)
               if (e == (at & ~1)) mine = pop[e / 8][e % 8 / 2];
             const float p = E<DT>::to_f((uint16_t)(__shfl((int)mine, 16 * q + li, 64) >> (16 * (at & 1))));
-            if (key > min(kend - 1, pq)) continue;
+            if (key > klim) continue;
             const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
             const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
 #pragma unroll
@@ -470,21 +486,25 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
   l_run = xor32_sum(xor16_sum(l_run));
 
   // merge the waves: lane (column, lg) holds dims ND (4 lg + r) + T
-  if (live) {
+  const int tid = 64 * wave + kv4_lane();
+  {
+    const int li = tid & 15, lg = tid >> 4 & 3;
+    if (Kv4Col(a, li, n, Gc, p0, plim).live) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int T = 0; T < ND; T += 4) {
-        const f32x4_t x = {acc[T][r], acc[T + 1][r], acc[T + 2][r], acc[T + 3][r]};
-        *reinterpret_cast<f32x4_t*>(&lds.o[wave][li][ND * (4 * lg + r) + T]) = x;
-      }
-  }
-  if (lg == 0) {
-    lds.m[wave][li] = m_run * a.scale_log2;
-    lds.l[wave][li] = l_run;
+        for (int T = 0; T < ND; T += 4) {
+          const f32x4_t x = {acc[T][r], acc[T + 1][r], acc[T + 2][r], acc[T + 3][r]};
+          *reinterpret_cast<f32x4_t*>(&lds.o[wave][li][ND * (4 * lg + r) + T]) = x;
+        }
+    }
+    if (lg == 0) {
+      lds.m[wave][li] = m_run * a.scale_log2;
+      lds.l[wave][li] = l_run;
+    }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n * Gc * (D / 4); i += 64 * NW) {
+  for (int i = tid; i < n * Gc * (D / 4); i += 64 * NW) {
     const int col = i / (D / 4), d = (i % (D / 4)) * 4;
     const int j = col * a.over_Gc >> 8, h = col - j * min(a.G, 16);
     const int pj = min(p0 + j, plim);
@@ -545,15 +565,18 @@ __global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4At
   const int pos_b = __shfl_up(pos_i, 1, 64);
   const bool follows = lane > 1 && lane <= a.qb && ri < a.rows && slot_b == slot_i && pos_i > 0 && pos_b == pos_i - 1;
   const uint64_t chain = __ballot(follows);  // bit i: row first - 1 + i continues the row before it
+  lds.slot[lane] = slot_i;  // every wave writes the same, and reads behind its own writes
+  lds.pos[lane] = pos_i;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   const int last = min(min((part + 1) * a.R, a.qb), a.rows - first);
   for (int cand = part * a.R; cand < last; ++cand) {
     if (chain >> (cand + 1) & 1u) continue;  // in the block of a row before it
-    int l = lane;
-    asm volatile("" : "+v"(l));  // the block's addresses are made anew: kept over the loop they would spill
+    const long slot = lds.slot[cand + 1];
     kv4_attn_row<DT, D, NW>(c, a, first + cand, 1 + __builtin_ctzll(~(chain >> (cand + 2))),
-                            (long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)slot_i, cand + 1) |
-                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(slot_i >> 32), cand + 1) << 32),
-                            __builtin_amdgcn_readlane(pos_i, cand + 1), kh, h0, Gc, split, wave, l, lds);
+                            (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)slot) |
+                                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(slot >> 32)) << 32),
+                            __builtin_amdgcn_readfirstlane(lds.pos[cand + 1]), kh, h0, Gc, split, wave, lds);
   }
 }
 
