@@ -189,15 +189,23 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 // to 500 keys 26 us).
 namespace {
 template <int NI> struct Words { uint32_t w[NI]; };
-// `base` is the same in every lane, so the load takes a scalar address and a 32-bit lane offset
-template <int NI> __device__ __forceinline__ Words<NI> kv4_load(const uint8_t* base, uint32_t off) {
+// A tile of the cache at `base`, the same in every lane; where `live` is false its loads give zeros and access nothing:
+// the loads ahead past a wave's last tile would read a tile again (1600 rows of 500 keys: 181 -> 151 us, 224 of 2048 80.5
+// -> 77).
+typedef __amdgpu_buffer_rsrc_t Kv4Ref;
+__device__ __forceinline__ Kv4Ref kv4_ref(const uint8_t* base, bool live, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, live ? bytes : 0, 0x00020000);
+}
+// 4 NI bytes at a lane's offset; nt: non-temporal
+template <int NI, bool NT> __device__ __forceinline__ Words<NI> kv4_load(Kv4Ref ref, uint32_t off) {
+  constexpr int AUX = NT ? 2 : 0;
   Words<NI> r;
   if constexpr (NI == 4) {
-    const fp4_u4 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u4*>(base + off));
+    const fp4_u4 x = __builtin_amdgcn_raw_buffer_load_b128(ref, off, 0, AUX);
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.w[i] = x[i];
   } else {
-    const fp4_u2 x = __builtin_nontemporal_load(reinterpret_cast<const fp4_u2*>(base + off));
+    const fp4_u2 x = __builtin_amdgcn_raw_buffer_load_b64(ref, off, 0, AUX);
     r.w[0] = x[0];
     r.w[1] = x[1];
   }
@@ -287,7 +295,7 @@ struct Kv4Col {
   }
 };
 // one block: rows row .. row + n - 1 of slot `slot`, the first at position p0
-template <int DT, int D, int NW>
+template <int DT, int D, int NW, bool NT>
 __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int row, int n, long slot, int p0, int kh,
                                              int h0, int Gc, int split, int wave, Kv4Lds<D, NW>& lds) {
   constexpr int NI = D / 32;   // words a lane holds of 16 keys; score steps
@@ -298,7 +306,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
   if (slot < 0 || slot >= c.slots || p0 < 0) {  // no key: zeros
     if (split == 0)
       for (int j = 0; j < n; ++j)
-        for (int i = 64 * wave + lane; i < Gc * D; i += 64 * NW)
+        for (int i = 64 * wave + kv4_lane(); i < Gc * D; i += 64 * NW)
           a.out[(long)(row + j) * a.so_b + (long)(kh * a.G + h0 + i / D) * a.so_h + i % D] = 0;
     return;
   }
@@ -330,33 +338,33 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     uint32_t ks[NG], vs[NG];
   };
   int k0 = kstart + KT * wave;
-  const long tile0 = base + min(k0, (kend - 1) & ~(KT - 1));
+  const long tile0 = base + k0;
   const uint8_t* kp = c.k + tile0 * (D / 2);
   const uint8_t* ksp = c.ks + tile0 * NI;
   const uint8_t* vp = c.v + tile0 * (D / 2);
   const uint8_t* vsp = c.vs + tile0 * NI;
   int kn = k0, vn = k0;
   auto load_k = [&](Buf& t) {
+    const Kv4Ref kr = kv4_ref(kp, kn < kend, KT * D / 2), sr = kv4_ref(ksp, kn < kend, KT * NI);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      t.kw[g] = kv4_load<NI>(kp + g * (8 * D), k_at);
-      t.ks[g] = *reinterpret_cast<const uint32_t*>(ksp + g * (16 * NI) + ks_at);
+      t.kw[g] = kv4_load<NI, NT>(kr, k_at + g * (8 * D));
+      t.ks[g] = __builtin_amdgcn_raw_buffer_load_b32(sr, ks_at + g * (16 * NI), 0, 0);
     }
     kn += KT * NW;
-    const int step = kn < kend ? KT * NW : 0;
-    kp += step * (D / 2);
-    ksp += step * NI;
+    kp += KT * NW * (D / 2);
+    ksp += KT * NW * NI;
   };
   auto load_v = [&](Buf& t) {
+    const Kv4Ref vr = kv4_ref(vp, vn < kend, KT * D / 2), sr = kv4_ref(vsp, vn < kend, KT * NI);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      t.vw[g] = kv4_load<NI>(vp + g * (8 * D), v_at);
-      t.vs[g] = *reinterpret_cast<const uint32_t*>(vsp + g * (16 * NI) + vs_at);
+      t.vw[g] = kv4_load<NI, NT>(vr, v_at + g * (8 * D));
+      t.vs[g] = __builtin_amdgcn_raw_buffer_load_b32(sr, vs_at + g * (16 * NI), 0, 0);
     }
     vn += KT * NW;
-    const int step = vn < kend ? KT * NW : 0;
-    vp += step * (D / 2);
-    vsp += step * NI;
+    vp += KT * NW * (D / 2);
+    vsp += KT * NW * NI;
   };
   Buf b0, b1;
   __builtin_amdgcn_sched_barrier(0);  // the queries' loads stay first: the loop waits for them with the first keys
@@ -455,7 +463,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
 #pragma unroll
             for (int e = 0; e < 4 * NG; e += 2)
               if (e == (at & ~1)) mine = pop[e / 8][e % 8 / 2];
-            const float p = E<DT>::to_f((uint16_t)(__shfl((int)mine, 16 * q + li, 64) >> (16 * (at & 1))));
+            const float p = E<DT>::to_f((uint16_t)(__builtin_amdgcn_ds_bpermute(4 * (16 * q + li), (int)mine) >> (16 * (at & 1))));
             if (key > klim) continue;
             const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
             const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
@@ -573,10 +581,14 @@ __global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4At
   for (int cand = part * a.R; cand < last; ++cand) {
     if (chain >> (cand + 1) & 1u) continue;  // in the block of a row before it
     const long slot = lds.slot[cand + 1];
-    kv4_attn_row<DT, D, NW>(c, a, first + cand, 1 + __builtin_ctzll(~(chain >> (cand + 2))),
-                            (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)slot) |
-                                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(slot >> 32)) << 32),
-                            __builtin_amdgcn_readfirstlane(lds.pos[cand + 1]), kh, h0, Gc, split, wave, lds);
+    const int n = 1 + __builtin_ctzll(~(chain >> (cand + 2)));
+    const long slot_u = (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)slot) |
+                               (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(slot >> 32)) << 32);
+    const int p0 = __builtin_amdgcn_readfirstlane(lds.pos[cand + 1]);
+    // A single row's keys are a stream of their own (non-temporal loads: 224 rows of 2048 keys 77 us, 88 without); a
+    // prompt's are read by its next blocks as well (16 x 512 rows over 512 keys: 67 us, 78 with).
+    if (n > 1) kv4_attn_row<DT, D, NW, false>(c, a, first + cand, n, slot_u, p0, kh, h0, Gc, split, wave, lds);
+    else kv4_attn_row<DT, D, NW, true>(c, a, first + cand, 1, slot_u, p0, kh, h0, Gc, split, wave, lds);
   }
 }
 
