@@ -25,8 +25,8 @@ struct M3xKv4 {
 };
 
 namespace {
-// Attention's workgroups: 4 waves, 3 of a SIMD's at once (up to 168 registers). Measured at 224 rows of 2048 keys, heads
-// 16/8 of 128 (us): 79; 8 waves 92, 2 waves 93; 4 waves a SIMD (128 registers) spill, 94 to 113.
+// Attention's workgroups: 4 waves, 4 on a SIMD (128 registers; no spill, 18 spilled registers cost 30 %). Measured at 224
+// rows of 2048 keys, heads 16/8 of 128, with 3 a SIMD (us): 79; 8 waves 92, 2 waves 93.
 constexpr int KV4_NW = 4, KV4_OCC = 4;
 
 struct Kv4 {
@@ -182,11 +182,11 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 // the largest weight is rounded too, and the error against 64 bits rises by a sixth.
 //
 // Bound, measured on MI355X with 16/8 heads of 128: the cache's bytes where rows fill the GPU (224 rows of 2048 keys
-// 79 us, 499 MB at 6.3 TB/s; its loads without the arithmetic 78, the arithmetic without the loads 58, VALU busy 46 %).
-// Few rows: the start, the merge and the join beside the bytes (2 rows of 120000 keys, 32/4 heads of 64: 17.1 us of 65 MB
+// 77 us, 499 MB at 6.5 TB/s; of 4000 keys 143, 6.8 TB/s; the arithmetic without the loads 58, VALU busy 45 %).
+// Few rows: the start, the merge and the join beside the bytes (2 rows of 120000 keys, 32/4 heads of 64: 16.9 us of 65 MB
 // and 3.8 for the join; one row of 2048 keys 4.8 and 3.5). A prompt over a long context: a tile's own chain of steps, about
-// 1 us at two waves a SIMD (512 rows over 4000 keys 36 us); over a short one a block's start and merge (1600 rows over up
-// to 500 keys 26 us).
+// 1 us at two waves a SIMD (512 rows over 4000 keys 34 us); over a short one a block's start and merge (1600 rows over up
+// to 500 keys 21 us).
 namespace {
 template <int NI> struct Words { uint32_t w[NI]; };
 // A tile of the cache at `base`, the same in every lane; where `live` is false its loads give zeros and access nothing:
@@ -330,9 +330,9 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
   for (int i = 0; i < NI; ++i) qop[i] = ld16(qp + (D / 4) * lg + 8 * i);
   // Two tiles' words in turn: a tile's keys are loaded two tiles ahead, behind the products of the keys they replace, its
   // values likewise. The pointers stand at the tile to be loaded next and are the same in every lane: a load takes them
-  // as its scalar address, beside the lane's 32-bit offset. Loads are never conditional (one whose registers are
-  // merged behind a branch is waited for there): past the wave's last tile they repeat it. cap % 32 == 0: a tile that
-  // begins inside the slot ends inside it.
+  // as its scalar address, beside the lane's 32-bit offset. Loads are never conditional (one whose registers are merged
+  // behind a branch is waited for there): past the wave's last tile they are of no bytes. cap % 32 == 0: a tile that begins
+  // inside the slot ends inside it.
   struct Buf {
     Words<NI> kw[NG], vw[NG];
     uint32_t ks[NG], vs[NG];

@@ -730,16 +730,17 @@ def kv4_read(cache, slots, pos, k, v):
 
 def kv4_attn_chunk(rows, heads, kv_heads, max_ctx, head_dim=128) -> int:
     """Keys per split of kv4_attn for `rows` rows of up to max_ctx keys: a workgroup (a row, a kv head, a split) per CU
-    at head_dim 128, two at 64 (whose arithmetic is the larger share), and at least 128 keys each; up to 512 keys whole
+    at head_dim 128, two at 64 (whose arithmetic is the larger share), and at least 128 keys each; up to 1024 keys whole
     (no join of splits behind). Rows known to be a prompt's count as one per 16 // (heads // kv_heads), the rows that
     share a pass: 64 of them at 4000 keys 14 us instead of 23.
 
-    Measured on MI355X (graph-timed, us, 16/8 heads of 128, combine included): one row at 2048 keys 7.2 (128 keys a
-    split; 256: 7.5, 1024: 10.4), at 32000 12.7 (1024; 256: 18.5, 4096: 23.9); 4 rows at 32000 27.9 (4096; 1024: 31.2,
-    16384: 75); 32 rows at 2048 14.9 whole (512: 20.5); 224 rows at 2048 79 whole (1024: 91); one row at 300 5.2 whole
-    (128: 6.9). 32/4 heads of 64: 16 rows at 32000 30 (4096; 8192: 36, 512: 42)."""
-    if max_ctx <= 512:
-        return 512
+    Measured on MI355X (graph-timed, us, 16/8 heads of 128, combine included): one row at 1024 keys 7.8 whole (128 keys
+    a split: 7.3), 32 rows 8.8 (512: 12.1); one row at 2048 7.7 (128; 512: 8.7, 2048: 11.6), 32 rows 13.5 whole (1024:
+    17.3); one row at 32000 12.0 (1024; 256: 15.9, 4096: 21.8), 4 rows 27.0 (4096; 1024: 28.5, 8192: 37.1); 224 rows at
+    2048 77 whole. 32/4 heads of 64: 2 rows at 120000 18.8 (2048; 1024: 22.7, 8192: 31.0), 16 rows at 32000 29.3 (4096;
+    512: 37.9)."""
+    if max_ctx <= 1024:
+        return 1024
     blocks = rows * kv_heads * -(-heads // (16 * kv_heads))
     return 128 * max(1, -(-blocks * max_ctx // (128 * (256 if head_dim == 128 else 512))))
 
