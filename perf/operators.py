@@ -349,7 +349,7 @@ def _own_append(s):
 def _own_attn(s):
     ops = _ops()
     if "ws" not in s.kept:  # a program keeps its workspace
-        s.kept["chunk"] = ops.kv4_attn_chunk(s.pos.numel(), s.case["heads"], s.case["kv"], s.ctx)
+        s.kept["chunk"] = ops.kv4_attn_chunk(s.pos.numel(), s.case["heads"], s.case["kv"], s.ctx, s.case["dim"])
         need = ops.kv4_attn_workspace(s.pos.numel(), s.case["heads"], s.case["dim"], s.ctx, s.kept["chunk"])
         s.kept["ws"] = torch.empty(need // 4, dtype=torch.float32, device=DEV)
     out = torch.empty_like(s.q)
