@@ -554,10 +554,11 @@ size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, in
 /* out[r, h] = softmax(scale q[r, h] . K^T) V over positions 0 .. pos[r] of slot slots[r], kv head h / (heads /
  * kv_heads); q and out [rows, heads, D] 16-bit (strides % 8 == 0, 16-byte aligned). pos[r] < 0 or a slot outside the
  * cache: zeros. max_ctx >= pos[r] + 1 for every row (keys past it are not attended), <= cap; chunk = keys per split,
- * a multiple of 128; at most 2^20 rows and 4095 splits. What a row does not see has no part in its result, whatever it
- * holds. Rows next to each other in the call, of one slot at consecutive positions (a prompt's), share one pass over the
- * keys; a row's bits do not depend on that, and not on the other rows. Fixed summation order. Two calls that may run at
- * the same time need a workspace each. */
+ * a multiple of 128; at most 2^20 rows and 4095 splits; |scale| <= 2^127. A score q . K is an fp32 sum, and a weight's
+ * exponent its exact difference from the largest times the scale. What a row does not see has no part in its result,
+ * whatever it holds. Rows next to each other in the call, of one slot at consecutive positions (a prompt's), share one
+ * pass over the keys; a row's bits do not depend on that, and not on the other rows. Fixed summation order. Two calls
+ * that may run at the same time need a workspace each. */
 int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
                  const int64_t* slots, const int32_t* pos, float scale, int rows, int heads, int max_ctx, int chunk,
                  void* workspace, size_t ws_bytes, int dtype, void* stream);

@@ -223,7 +223,7 @@ struct Kv4Attn {
   uint32_t q_flip;    // the sign bits of two query elements where scale < 0
   int rows, heads, G, hblocks, qb, R, chunk, max_ctx, max_splits;
   uint32_t over_Gc;  // x * over_Gc >> 8 = x / min(G, 16) for x < 16
-  float* part;  // [rows * heads][max_splits][D] then [rows * heads][max_splits][2] (maximum, sum)
+  float* part;  // [rows * heads][max_splits][D] then [rows * heads][max_splits][2] (largest raw score, sum)
 };
 
 // four outputs O / L (one quotient: its rounding and the products' are fp32's)
@@ -420,14 +420,15 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
       for (int T = 0; T < ND; ++T) acc[T] *= alpha;
     }
     m_run = mx;
-    // fp16 weights stand 2^15 higher (up to 32768), as do their sums: below 2^-14 fp16 loses relative precision, and
-    // many keys of small weight would lose their part
-    const float mp = mu * a.scale_log2 - (DT == M3X_F16 ? 15.f : 0.f);
+    // A weight's exponent is the difference of the raw scores, which is exact near the maximum, times the factor: the
+    // largest weight is one power of two whatever the scores' size. fp16 weights stand 2^15 higher (up to 32768), as do
+    // their sums: below 2^-14 fp16 loses relative precision, and many keys of small weight would lose their part.
+    constexpr float up = DT == M3X_F16 ? 15.f : 0.f;
     fp4_u4 pop[NG / 2];
 #pragma unroll
     for (int e = 0; e < 4 * NG; e += 2) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], a.scale_log2, -mp));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1], a.scale_log2, -mp));
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e] - mu, a.scale_log2, up));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e + 1] - mu, a.scale_log2, up));
       pop[e / 8][e % 8 / 2] = fp4_pack<DT>(x, y);
       l_run = fp4_add2<DT>(pop[e / 8][e % 8 / 2], l_run);
     }
@@ -507,7 +508,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
         }
     }
     if (lg == 0) {
-      lds.m[wave][li] = m_run * a.scale_log2;
+      lds.m[wave][li] = m_run;
       lds.l[wave][li] = l_run;
     }
   }
@@ -525,7 +526,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     f32x4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(lds.m[w][col] - mu);
+      const float f = __builtin_amdgcn_exp2f((lds.m[w][col] - mu) * a.scale_log2);
       L += lds.l[w][col] * f;
       O += *reinterpret_cast<const f32x4_t*>(&lds.o[w][col][d]) * f;
     }
@@ -627,7 +628,8 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4 c, Kv4Attn a) {
     for (int i = 0; i < U; ++i) {
       if (s0 + i * NG < ns) {
         const float mx = fmaxf(M, x[i].x), mu = mx == -INFINITY ? 0.f : mx;
-        const float f0 = __builtin_amdgcn_exp2f(M - mu), f1 = __builtin_amdgcn_exp2f(x[i].x - mu);
+        const float f0 = __builtin_amdgcn_exp2f((M - mu) * a.scale_log2);
+        const float f1 = __builtin_amdgcn_exp2f((x[i].x - mu) * a.scale_log2);
         L = L * f0 + x[i].y * f1;
         O = O * f0 + o[i] * f1;
         M = mx;
@@ -652,7 +654,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4 c, Kv4Attn a) {
   O = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
-    const float f = __builtin_amdgcn_exp2f(sm[hb][i] - mu);
+    const float f = __builtin_amdgcn_exp2f((sm[hb][i] - mu) * a.scale_log2);
     L += sl[hb][i] * f;
     O += *reinterpret_cast<const f32x4_t*>(&so[hb][i][d]) * f;
   }
@@ -779,6 +781,7 @@ M3X_API int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_
   if (dtype != M3X_BF16 && dtype != M3X_F16) return M3X_EUNSUPPORTED;
   if (heads % c.kv_heads) return M3X_EUNSUPPORTED;
   if (chunk <= 0 || chunk % 128 || max_ctx > c.cap) return M3X_EINVAL;
+  if (!(fabsf(scale) <= 0x1p127f)) return M3X_EINVAL;  // its factor would not be finite; NaN
   if (rows == 0) return M3X_OK;
   if (!q || !out || !slots || !pos) return M3X_ENULL;
   if (((sq_b | sq_h | so_b | so_h) & 7) || !m3x_aligned16(q) || !m3x_aligned16(out)) return M3X_EINVAL;

@@ -755,7 +755,8 @@ def kv4_attn(q, cache, out, slots, pos, scale, max_ctx, chunk, workspace):
     [rows, heads, head_dim] (bf16 or fp16, any row and head strides). A row with pos[r] < 0 or a slot outside the
     cache gets zeros. max_ctx: at least every pos[r] + 1; chunk: keys per split (kv4_attn_chunk); workspace: a tensor of
     kv4_attn_workspace bytes, or None when that is 0 (calls that may run at the same time need one each). Rows of one
-    slot at consecutive positions (a prompt's) that stand next to each other share one pass over the keys."""
+    slot at consecutive positions (a prompt's) that stand next to each other share one pass over the keys. |scale| is at
+    most 2^127."""
     rows, sp, pp = _kv4_rows("kv4_attn", cache, slots, pos)
     heads = q.shape[1] if q.dim() == 3 else 0
     if heads == 0 or heads % cache.kv_heads:
@@ -764,6 +765,8 @@ def kv4_attn(q, cache, out, slots, pos, scale, max_ctx, chunk, workspace):
     oa = _kv4_heads("kv4_attn", "out", out, cache, rows, heads, q.dtype)
     if not 1 <= max_ctx <= cache.cap or chunk < 128 or chunk % 128:
         raise ValueError(f"kv4_attn: max_ctx {max_ctx} must be in [1, {cache.cap}] and chunk {chunk} a multiple of 128")
+    if not abs(scale) <= 2.0 ** 127:
+        raise ValueError(f"kv4_attn: |scale| must be at most 2^127, got {scale}")
     ws, ws_bytes = 0, 0
     if max_ctx > chunk:
         need = kv4_attn_workspace(rows, heads, cache.head_dim, max_ctx, chunk)

@@ -1,0 +1,29 @@
+"""Arguments at the ends of what the 4-bit entry points take, on the CPU: refused before a launch, or computed on the
+host."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+P = ctypes.c_void_p(4096)  # never read: every call below is refused
+
+
+def _cache(cap=64, D=128):
+    from m3x import ops
+    return ops.Kv4Cache.empty(2, 2, cap, D, "cpu")
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 2.0 ** 127 * 1.0001, -3e38, 1e300])
+def test_attn_scale_refused(scale):
+    """A scale whose factor of the exponents is not finite."""
+    from m3x import ops
+    from m3x._lib import lib
+    c = _cache()
+    q = torch.zeros(3, 4, 128, dtype=torch.bfloat16)
+    at = torch.zeros(3, dtype=torch.long), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="scale"):
+        ops.kv4_attn(q, c, q, *at, scale, 64, 128, None)
+    a = ops.Kv4CacheArgs(4096, 4096, 4096, 4096, 1, 2, 128, 64)
+    assert lib().m3x_kv4_attn(ctypes.addressof(a), P, 512, 128, P, 512, 128, P, P, scale, 1, 4, 64, 128, None, 0, 0,
+                              None) == -1
