@@ -10,6 +10,7 @@
 //                               needs no transpose through LDS; a position's write stays whole words.
 //   vs  [cap / 4][D / 32][4]    the four positions' bytes of a group are one word
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 #include "m3x_norm.h"
@@ -802,10 +803,16 @@ M3X_API int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_
   int R = 1;
   while (R < qb && (long)rows * c.kv_heads * hb * splits >= 4096L * R) R *= 2;
   R = R < qb ? R : qb;
-  // a weight is exp2 of one fused multiply-add of the raw score: its factor must not be negative (the running maximum is
-  // the raw scores') or 0 (0 * -inf of a masked key); one this small leaves every weight of finite scores at 1
-  float weight = fabsf(scale) * 1.44269504088896341f;
-  if (weight < 0x1p-100f) weight = 0x1p-100f;
+  // The raw scores' differences are multiplied by |scale| log2(e): not by a negative factor (the running maximum is the raw
+  // scores') and not by 0 (0 * -inf of a masked key). fp32's smallest number stands for 0: no difference of finite scores
+  // makes more than 2^-20 of it. A factor below the normal numbers is made from its bits, whether or not the caller's thread
+  // flushes them to 0; what its few bits round away is no more than that either.
+  const double factor = fabs((double)scale) * 1.44269504088896341;
+  float weight = (float)factor;
+  if (factor < 0x1p-126) {
+    const uint32_t bits = std::max(1u, (uint32_t)(factor * 0x1p149));
+    memcpy(&weight, &bits, sizeof weight);
+  }
   const Kv4Attn a = {(const uint16_t*)q, sq_b, sq_h, (uint16_t*)out, so_b, so_h, slots, pos,
                      weight, scale < 0.f ? 0x80008000u : 0u, rows, heads, G, hb, qb, R, chunk, max_ctx, splits,
                      (uint32_t)((256 + Gc - 1) / Gc), (float*)workspace};

@@ -68,3 +68,27 @@ def test_attn_far_scores(gpu, dtype, scale):
             out, mag, ds = R.attention(_f64(q[r]), *vals[int(slots[r])], int(pos[r]), scale)
             bound = R.attention_bound(out, mag, np.full_like(ds, 2.0 ** -14), dtype, int(pos[r]) + 1)
             assert (np.abs(got[r] - out) <= bound).all(), (chunk, r, float(np.nanmax(np.abs(got[r] - out) / bound)))
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-40, -1e-38])
+def test_attn_scores_past_the_scale(gpu, scale):
+    """Raw scores of some 2^105 under scale 0, or under one so small that their products with it are below 2^-22: every
+    weight is the same."""
+    from m3x import ops
+    dtype, D, cap = torch.bfloat16, 64, 160
+    g = _g(2)
+    k, v = torch.randn(cap, 1, D, generator=g) * 2.0 ** 60, torch.randn(cap, 1, D, generator=g)
+    c = ops.Kv4Cache.empty(1, 1, cap, D, gpu)
+    zero = torch.zeros(cap, dtype=torch.long, device=gpu)
+    ops.kv4_append(k.to(dtype).to(gpu), v.to(dtype).to(gpu), c, zero, torch.arange(cap, dtype=torch.int32, device=gpu))
+    q = (torch.randn(3, 2, D, generator=g) * 2.0 ** 42).to(dtype).to(gpu)
+    if scale == -1e-38:
+        q = q * 2.0 ** -8
+    pos = torch.tensor([159, 40, 70])
+    V = R.cache_values(c, 0)[1][0]
+    for chunk in (128, 256):
+        got = _f64(_attend(q, c, torch.zeros(3, dtype=torch.long), pos, scale, chunk))
+        for r, p in enumerate(pos.tolist()):
+            out, mag = V[:p + 1].mean(0), np.abs(V[:p + 1]).mean(0)
+            bound = R.attention_bound(out, mag, 2.0 ** -14, dtype, p + 1)
+            assert (np.abs(got[r] - out) <= bound).all(), (r, float((np.abs(got[r] - out) / bound).max()))
