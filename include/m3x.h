@@ -555,7 +555,8 @@ size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, in
  * kv_heads); q and out [rows, heads, D] 16-bit (strides % 8 == 0, 16-byte aligned). pos[r] < 0 or a slot outside the
  * cache: zeros. max_ctx >= pos[r] + 1 for every row (keys past it are not attended), <= cap; chunk = keys per split,
  * a multiple of 128; at most 2^20 rows and 4095 splits; |scale| <= 2^127. A score q . K is an fp32 sum, and a weight's
- * exponent its fp32 difference from the largest times the scale. What a row does not see has no part in its result,
+ * exponent its fp32 difference from the largest times the scale. bf16 weights below 2^-102 of the largest count as 0; a
+ * sum of weighted values is finite up to 2^24 keys of any values. What a row does not see has no part in its result,
  * whatever it holds. Rows next to each other in the call, of one slot at consecutive positions (a prompt's), share one
  * pass over the keys; a row's bits do not depend on that, and not on the other rows. Fixed summation order. Two calls
  * that may run at the same time need a workspace each. */

@@ -423,8 +423,10 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
     m_run = mx;
     // A weight's exponent is the difference of the raw scores, which is exact near the maximum, times the factor: the
     // largest weight is one power of two whatever the scores' size. fp16 weights stand 2^15 higher (up to 32768), as do
-    // their sums: below 2^-14 fp16 loses relative precision, and many keys of small weight would lose their part.
-    constexpr float up = DT == M3X_F16 ? 15.f : 0.f;
+    // their sums: below 2^-14 fp16 loses relative precision, and many keys of small weight would lose their part. bf16
+    // weights stand 2^24 lower: the sum over 2^24 keys of the format's largest values, 6 x 2^125, is then finite, as their
+    // mean is. It costs weights below 2^-102, which become 0, and values below it some of their digits.
+    constexpr float up = DT == M3X_F16 ? 15.f : -24.f;
     fp4_u4 pop[NG / 2];
 #pragma unroll
     for (int e = 0; e < 4 * NG; e += 2) {

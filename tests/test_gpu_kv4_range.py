@@ -92,3 +92,30 @@ def test_attn_scores_past_the_scale(gpu, scale):
             out, mag = V[:p + 1].mean(0), np.abs(V[:p + 1]).mean(0)
             bound = R.attention_bound(out, mag, 2.0 ** -14, dtype, p + 1)
             assert (np.abs(got[r] - out) <= bound).all(), (r, float((np.abs(got[r] - out) / bound).max()))
+
+
+def test_attn_largest_values(gpu):
+    """Values at the format's largest, 6 x 2^125, whose plain sum passes fp32: the weighted mean is never larger than
+    they are, and keys of either sign cancel."""
+    from m3x import ops
+    dtype, D, KV, cap = torch.bfloat16, 128, 2, 512
+    top = 6 * 2.0 ** 125
+    c = ops.Kv4Cache.empty(1, KV, cap, D, gpu)
+    g = _g(7)
+    k = torch.randn(cap, KV, D, generator=g)
+    v = torch.full((cap, KV, D), top)
+    v[:, 1, ::2] *= 1 - 2 * (torch.arange(cap) % 2)[:, None].float()
+    ops.kv4_append(k.to(dtype).to(gpu), v.to(dtype).to(gpu), c, torch.zeros(cap, dtype=torch.long, device=gpu),
+                   torch.arange(cap, dtype=torch.int32, device=gpu))
+    assert (c.vs == 252).all()
+    K, V = R.cache_values(c, 0)
+    pos = torch.tensor([1, 5, 300, 301, 302, 511])
+    slots = torch.zeros(len(pos), dtype=torch.long)
+    q = torch.randn(len(pos), 4, D, generator=g).to(dtype).to(gpu)
+    for scale in (0.0, 0.09):
+        for chunk in (128, 512):
+            got = _f64(_attend(q, c, slots, pos, scale, chunk))
+            for r, p in enumerate(pos.tolist()):
+                out, mag, ds = R.attention(_f64(q[r]), K, V, p, scale)
+                bound = R.attention_bound(out, mag, ds, dtype, p + 1)
+                assert (np.abs(got[r] - out) <= bound).all(), (r, scale, chunk)
