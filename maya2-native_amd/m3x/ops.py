@@ -730,8 +730,8 @@ def kv4_read(cache, slots, pos, k, v):
 
 def kv4_attn_chunk(rows, heads, kv_heads, max_ctx, head_dim=128) -> int:
     """Keys per split of kv4_attn for `rows` rows of up to max_ctx keys: a workgroup (a row, a kv head, a split) per CU
-    at head_dim 128, two at 64 (whose arithmetic is the larger share), and at least 128 keys each; up to 1024 keys whole
-    (no join of splits behind). Rows known to be a prompt's count as one per 16 // (heads // kv_heads), the rows that
+    at head_dim 128, two at 64 (whose arithmetic is the larger share), at least 128 keys each and no more than there are
+    (rounded up to 128); up to 1024 keys whole (no join of splits behind). Rows known to be a prompt's count as one per 16 // (heads // kv_heads), the rows that
     share a pass: 64 of them at 4000 keys 14 us instead of 23.
 
     Measured on MI355X (graph-timed, us, 16/8 heads of 128, combine included): one row at 1024 keys 7.8 whole (128 keys
@@ -742,11 +742,14 @@ def kv4_attn_chunk(rows, heads, kv_heads, max_ctx, head_dim=128) -> int:
     if max_ctx <= 1024:
         return 1024
     blocks = rows * kv_heads * -(-heads // (16 * kv_heads))
-    return 128 * max(1, -(-blocks * max_ctx // (128 * (256 if head_dim == 128 else 512))))
+    tiles = -(-max_ctx // 128)
+    return 128 * min(tiles, max(1, -(-blocks * max_ctx // (128 * (256 if head_dim == 128 else 512)))))
 
 
 def kv4_attn_workspace(rows, heads, head_dim, max_ctx, chunk) -> int:
     """Bytes of workspace for kv4_attn (0: none)."""
+    if max(rows, heads, head_dim, max_ctx, chunk) >= 1 << 31:
+        raise ValueError(f"kv4_attn_workspace: counts below 2^31, got {(rows, heads, head_dim, max_ctx, chunk)}")
     return int(lib().m3x_kv4_attn_workspace(rows, heads, head_dim, max_ctx, chunk))
 
 
@@ -763,8 +766,9 @@ def kv4_attn(q, cache, out, slots, pos, scale, max_ctx, chunk, workspace):
         raise ValueError(f"kv4_attn: {heads} query heads over {cache.kv_heads} kv heads")
     qa = _kv4_heads("kv4_attn", "q", q, cache, rows, heads)
     oa = _kv4_heads("kv4_attn", "out", out, cache, rows, heads, q.dtype)
-    if not 1 <= max_ctx <= cache.cap or chunk < 128 or chunk % 128:
-        raise ValueError(f"kv4_attn: max_ctx {max_ctx} must be in [1, {cache.cap}] and chunk {chunk} a multiple of 128")
+    if not 1 <= max_ctx <= cache.cap or not 128 <= chunk < 1 << 31 or chunk % 128:
+        raise ValueError(f"kv4_attn: max_ctx {max_ctx} must be in [1, {cache.cap}] and chunk {chunk} a multiple of 128 "
+                         "below 2^31")
     if not abs(scale) <= 2.0 ** 127:
         raise ValueError(f"kv4_attn: |scale| must be at most 2^127, got {scale}")
     ws, ws_bytes = 0, 0

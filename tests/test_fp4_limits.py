@@ -27,3 +27,30 @@ def test_attn_scale_refused(scale):
     a = ops.Kv4CacheArgs(4096, 4096, 4096, 4096, 1, 2, 128, 64)
     assert lib().m3x_kv4_attn(ctypes.addressof(a), P, 512, 128, P, 512, 128, P, P, scale, 1, 4, 64, 128, None, 0, 0,
                               None) == -1
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,max_ctx", [(65536, 16, 8, 1 << 20), (100000, 16, 8, 1 << 20),
+                                                         (1 << 20, 64, 64, 1 << 30), (224, 16, 8, 2049), (1, 16, 8, 1 << 30)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attn_chunk_within_the_context(rows, heads, kv_heads, max_ctx, dim):
+    """The split rule stays within the context (and so within an int) at any count that attention takes, and the
+    workspace of its splits is what they need."""
+    from m3x import ops
+    chunk = ops.kv4_attn_chunk(rows, heads, kv_heads, max_ctx, dim)
+    assert 128 <= chunk < max_ctx + 128 and chunk % 128 == 0
+    splits = -(-max_ctx // chunk)
+    want = rows * heads * splits * (dim + 2) * 4 if splits > 1 else 0
+    assert ops.kv4_attn_workspace(rows, heads, dim, max_ctx, chunk) == want
+
+
+def test_attn_chunk_past_an_int():
+    """A chunk that an int does not hold is refused, not wrapped."""
+    from m3x import ops
+    c = _cache()
+    q = torch.zeros(3, 4, 128, dtype=torch.bfloat16)
+    at = torch.zeros(3, dtype=torch.long), torch.zeros(3, dtype=torch.int32)
+    for chunk in (1 << 31, 1 << 32, (1 << 32) + 128):
+        with pytest.raises(ValueError, match="chunk"):
+            ops.kv4_attn(q, c, q, *at, 1.0, 64, chunk, None)
+        with pytest.raises(ValueError):
+            ops.kv4_attn_workspace(3, 4, 128, 1 << 20, chunk)
