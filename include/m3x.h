@@ -569,7 +569,7 @@ int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_h, void*
  *   codes  [tiles][steps][64][16]           lane l: row l % 16 of the tile, inputs 32 (l / 16) .. + 31 of the step
  *   scales [tiles][ceil(steps / 4)][64][4]  the lane's scale byte of four consecutive steps
  * m3x_packed_weight4_bytes: size of the codes (scales = 0) or of the scales; -1 if K % 32. m3x_pack_weight4: from
- * bf16, fp16 or fp32 rows (ldw % 8 == 0, 16-byte aligned), once at load time. */
+ * bf16, fp16 or fp32 rows (ldw % 8 == 0, 16-byte aligned; fewer than 2^26 tiles x steps), once at load time. */
 long m3x_packed_weight4_bytes(int N, int K, int scales);
 int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes, void* scales, int dtype, void* stream);
 

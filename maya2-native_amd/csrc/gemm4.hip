@@ -170,8 +170,8 @@ __global__ __launch_bounds__(64) void pack_weight4_kernel(const Elt<DT>* __restr
                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                           int steps) {
   const int lane = threadIdx.x;
-  const int s = blockIdx.x;
-  const long tile = blockIdx.y;
+  const long tile = blockIdx.x / steps;
+  const int s = blockIdx.x - (int)tile * steps;
   const int row = 16 * (int)tile + (lane & 15), k = 128 * s + 32 * (lane >> 4);
   float x[32];
   uint32_t m = 0;
@@ -219,8 +219,8 @@ M3X_API int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes,
   if (!m3x_aligned16(w) || !m3x_aligned16(codes) || !m3x_aligned16(scales)) return M3X_EINVAL;
   const int steps = m3x_ceil_div(K, 128), tiles = m3x_ceil_div(N, 16);
   hipStream_t st = (hipStream_t)stream;
-  if (tiles > 65535) return M3X_EINVAL;
-  const dim3 grid(steps, tiles);
+  if ((long)tiles * steps >= 1L << 26) return M3X_EINVAL;  // a launch of fewer than 2^32 threads
+  const dim3 grid(tiles * steps);
   if (dtype == M3X_BF16)
     hipLaunchKernelGGL(pack_weight4_kernel<M3X_BF16>, grid, dim3(64), 0, st, (const uint16_t*)w, ldw, N, K,
                        (uint8_t*)codes, (uint8_t*)scales, steps);

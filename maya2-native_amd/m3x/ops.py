@@ -819,11 +819,14 @@ class PackedWeight4:
 
 
 def pack_weight4(w):
-    """w [N, K] (bf16, fp16 or fp32; row stride % 8 == 0, K % 32 == 0) in 4 bits; one launch on the current stream."""
+    """w [N, K] (bf16, fp16 or fp32; row stride % 8 == 0, K % 32 == 0, fewer than 2^26 tiles of 16 rows x 128 inputs) in 4 bits;
+    one launch on the current stream."""
     _rows2d(w, "w")
     N, K = w.shape
     if N < 1 or K < 32 or K % 32:
         raise ValueError(f"pack_weight4: K={K} must be a multiple of 32")
+    if -(-N // 16) * -(-K // 128) >= 1 << 26:
+        raise ValueError(f"pack_weight4: fewer than 2^26 tiles of 16 x 128, got {N} x {K}")
     if w.stride(0) % 8 or w.data_ptr() % 16:
         raise ValueError(f"pack_weight4: w needs 16-byte aligned rows (stride {w.stride(0)})")
     dt = _dt3(w)

@@ -54,3 +54,12 @@ def test_attn_chunk_past_an_int():
             ops.kv4_attn(q, c, q, *at, 1.0, 64, chunk, None)
         with pytest.raises(ValueError):
             ops.kv4_attn_workspace(3, 4, 128, 1 << 20, chunk)
+
+
+def test_pack_sizes_refused():
+    from m3x import ops
+    from m3x._lib import lib
+    for N, K in ((1 << 30, 32), (1 << 26, 2048), ((1 << 20) - 15, 128 << 10)):
+        assert lib().m3x_pack_weight4(P, 32, N, K, P, P, 0, None) == -1
+        with pytest.raises(ValueError, match="fewer than"):
+            ops.pack_weight4(torch.zeros(1, K, dtype=torch.bfloat16).expand(N, K))
