@@ -385,7 +385,7 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
 #pragma unroll
   for (int T = 0; T < ND; ++T) acc[T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  const int full = min(p0 + 1, kend);  // keys below it are seen by every row of the block
+  const int full = min(min(p0, plim) + 1, kend);  // keys below it are seen by every row of the block
   auto tile = [&](Buf& t, int k0) {
     const bool edge = k0 + KT > full;  // the tile is masked by column
     float sv[4 * NG];

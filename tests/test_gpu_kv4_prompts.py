@@ -90,3 +90,22 @@ def test_prompts_share_workgroups(gpu, dtype, D, G, runs, chunk, want):
         bound = R.attention_bound(out, mag, ds, dtype, keys)
         off = np.abs(_f64(got[at]) - out) / bound
         assert off.max() <= 1, (s, at[int(off.max((1, 2)).argmax())], float(off.max()))
+
+
+@pytest.mark.parametrize("G", [1, 2, 20])
+def test_positions_past_the_context(gpu, G):
+    """A position at or past max_ctx, the largest int among them, sees the keys below max_ctx."""
+    from m3x import ops
+    KV, D, cap, ctx = 2, 128, 128, 70
+    g = _g(3)
+    c = ops.Kv4Cache.empty(2, KV, cap, D, gpu)
+    k, v = (torch.randn(2 * cap, KV, D, generator=g).bfloat16().to(gpu) for _ in "kv")
+    ops.kv4_append(k, v, c, torch.arange(2, device=gpu).repeat_interleave(cap),
+                   torch.arange(cap, dtype=torch.int32, device=gpu).repeat(2))
+    slots = torch.tensor([0, 0, 0, 0, 1, 1, 0], device=gpu)
+    pos = torch.tensor([67, 68, 69, 70, 127, 2 ** 31 - 2, 2 ** 31 - 1], dtype=torch.int32, device=gpu)
+    q = torch.randn(7, KV * G, D, generator=g).bfloat16().to(gpu)
+    out, ref = torch.empty_like(q), torch.empty_like(q)
+    ops.kv4_attn(q, c, out, slots, pos, 0.1, ctx, 128, None)
+    ops.kv4_attn(q, c, ref, slots, pos.clamp(max=ctx - 1), 0.1, ctx, 128, None)
+    assert torch.equal(out, ref) and torch.isfinite(out).all()
