@@ -237,14 +237,14 @@ M3X_API int m3x_pack_weight4(const void* w, long ldw, int N, int K, void* codes,
 }
 
 namespace {
-// x turned over in LDS or not, measured on MI355X (us; not, turned): N 1024, K 8192 (1x1x8) 9 rows 8.4, 9.0, 12 rows 9.3,
-// 9.2, 16 rows 10.6, 9.6; N 5000, K 8192 (2x1x8) 1 row 10.3, 10.5, 5 rows 11.0, 10.8, 8 rows 13.9, 11.0, 16 rows 19.7,
-// 14.2; N 16384, K 8192 (4x1x16) 9 rows 16.0, 16.5, 16 rows 18.4, 17.3; 64 rows (8x2x8) 32.1, 28.7; N 11008, K 4096, 128 rows
-// gated (4x4x4, where it takes 304 of a wave's registers) 49, 57.
+// x turned over in LDS or not, measured on MI355X (us; not, turned): N 1024, K 8192 (1x1x8) 9 rows 8.1, 9.0, 12 rows 9.0,
+// 9.0, 16 rows 10.2, 9.5; N 5000, K 8192 (2x1x8) 5 rows 9.5, 10.5, 8 rows 9.7, 10.6, 12 rows 10.6, 10.9, 16 rows 12.1, 11.2,
+// gated 8 rows 12.6, 12.7, 12 rows 14.0, 13.5, 16 rows 15.3, 13.9; N 16384, K 8192 (4x1x16) 9 rows 17.4, 17.8, 16 rows 18.8,
+// 17.9; 64 rows (8x2x8) 32.9, 29.1; N 11008, K 4096, 128 rows gated (4x4x4, where it takes 304 of a wave's registers) 48, 58.
 template <int DT, int TW, int MT, int NW, int ACT> void launch4(const Lin4& a, hipStream_t st) {
   const dim3 grid(m3x_ceil_div(a.tiles, TW), m3x_ceil_div(a.M, 16 * MT)), block(64 * NW);
   if constexpr (MT == 1) {
-    if (a.M > (TW == 2 ? 4 : 12)) hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, true>), grid, block, 0, st, a);
+    if (a.M > 12) hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, false>), grid, block, 0, st, a);
   } else {
     hipLaunchKernelGGL((linear4_kernel<DT, TW, MT, NW, ACT, MT == 2>), grid, block, 0, st, a);
