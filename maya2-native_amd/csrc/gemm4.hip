@@ -253,21 +253,28 @@ template <int DT, int TW, int MT, int NW, int ACT> void launch4(const Lin4& a, h
 template <int DT, int ACT> void plan4(const Lin4& a, hipStream_t st) {
   // Weight tiles times 16-row blocks are dealt out over 256 CUs: a workgroup takes as many as leave every CU about one, so
   // that x, which every group of tiles reads anew, is read the fewest times. Past 16 a CU, and for few steps of K, where a
-  // large group's start and sums weigh more, smaller groups run in several rounds. Measured on MI355X (us; TW x MT x NW, the
-  // rule's first):
-  //   plain, K 8192  N 16384: 16 rows 4x1x16 17.3, 2x1x8 18.7, 1x1x8 25; 32 rows 4x2x8 21.5, 8x2x8 28, 4x1x16 30; 64 rows
-  //                  8x2x8 28.8, 4x2x8 35; 256 rows 8x2x8 111, 4x2x8 123. N 5000: 16 rows 2x1x8 11.6, 1x1x8 14.0
-  //   plain, K 4096  N 11008: 16 rows 4x1x16 9.8, 2x1x8 11.5; 32 rows 4x2x8 13.0, 4x1x16 17; 256 rows 4x2x8 48, 8x2x8 54
-  //   plain, K 1024  N 4096: 16 rows 1x1x8 3.5; 64 rows 2x1x8 4.8, 4x1x16 5.2; 128 rows 2x1x8 5.4, 4x2x8 5.6, 8x2x8 7.9; 256
-  //                  rows 4x2x8 7.0, 8x2x8 8.1
-  //   gated, K 8192  N 16384: 16 rows 2x1x8 27.3, 4x1x8 28.7; 32 rows 4x2x8 33.7, 2x2x8 34.9; 64 rows 4x4x4 46, 4x2x8 65
-  //   gated, K 1024  N 4096: 64 rows 2x2x8 5.8, 4x2x8 7.6; 128 rows 2x2x8 6.9, 4x2x8 7.8; 256 rows 2x2x8 11.2, 4x4x4 12.0
+  // large group's start and sums weigh more, smaller groups run in several rounds. A gated group of 4x4x4 leaves CUs idle below
+  // some 2800 units, which costs more than the smaller groups' rounds up to 25 steps. Measured on MI355X (us; TW x MT x NW,
+  // the rule's first):
+  //   plain, K 8192  N 16384: 16 rows 4x1x16 17.9, 2x1x8 18.9, 1x1x8 25; 32 rows 4x2x8 21.8, 8x2x8 28, 4x1x16 31; 64 rows
+  //                  8x2x8 29.1, 4x2x8 35; 256 rows 8x2x8 113, 4x2x8 125. N 5000: 16 rows 2x1x8 11.2, 1x1x8 13.8
+  //   plain, K 4096  N 11008: 16 rows 4x1x16 9.4, 2x1x8 11.2; 32 rows 4x2x8 12.8, 4x1x16 16; 256 rows 4x2x8 49, 8x2x8 56
+  //   plain, K 1024  N 4096: 16 rows 1x1x8 3.4, 2x1x8 3.8; 64 rows 2x1x8 4.5, 4x1x16 4.8; 128 rows 2x1x8 5.5, 4x2x8 5.4, 8x2x8
+  //                  7.7; 256 rows 4x2x8 7.1, 8x2x8 8.0
+  //   GELU           N 4096, K 1024: 16 rows 1x1x8 3.9, 2x1x8 4.3; 64 rows 2x1x8 5.0, 4x1x16 5.4; 256 rows 4x2x8 8.1, 8x2x8 8.9;
+  //                  N 16384, K 8192: 16 rows 4x1x16 19.5, 2x1x8 20.2; 64 rows 8x2x8 30.7, 4x2x8 37
+  //   gated, K 8192  N 16384: 16 rows 2x1x8 30.6, 4x1x8 29.4; 32 rows 4x2x8 34.3, 2x2x8 37.4; 64 rows 4x4x4 46, 4x2x8 65.
+  //                  N 11008: 64 rows (2752 units) 4x4x4 44, 2x2x8 50
+  //   gated, K 1024  N 4096: 64 rows 2x2x8 5.7, 4x2x8 7.4; 128 rows 2x2x8 7.6, 4x2x8 7.6; 256 rows 2x2x8 11.1, 4x4x4 12.0
+  //   gated, 9 to 32 steps (2x2x8, 4x4x4): 2560 units K 1152 11.6, 13.2, K 2048 15.2, 18.3, K 3200 22.4, 25.0, K 4096 27.6, 27.0;
+  //                  2752 units K 1536 13.8, 15.8, K 3200 23.1, 25.4; 3072 units K 1152 14.6, 13.0, K 2048 19.5, 18.8; 4096
+  //                  units K 1152 14.5, 13.5, K 2048 20.5, 20.4, K 2304 22.3, 20.2
   const int blocks = m3x_ceil_div(a.M, 16);
   const long units = (long)a.tiles * blocks;
   if (units <= 256) return launch4<DT, 1, 1, 8, ACT>(a, st);
   if constexpr (ACT == L4_SWIGLU) {
     if (units <= 512 || blocks == 1) launch4<DT, 2, 1, 8, ACT>(a, st);
-    else if (units <= (a.steps <= 8 ? 4096 : 1024) || (units > 2048 && units <= 4096 && a.steps <= 16))
+    else if (units <= (a.steps <= 8 ? 4096 : 1024) || (units > 2048 && units <= 2816 && a.steps <= 25))
       launch4<DT, 2, 2, 8, ACT>(a, st);
     else if (units <= 2048) launch4<DT, 4, 2, 8, ACT>(a, st);
     else launch4<DT, 4, 4, 4, ACT>(a, st);
