@@ -10,7 +10,8 @@
 // columns, as read from memory: per step and 16 rows of x four MFMA 16x16x32, the lane's inputs 8 i .. 8 i + 7 in the
 // i-th. The waves of a workgroup share the steps out and their sums meet in LDS, added in wave order (deterministic).
 // Products and sums are fp32; the one rounding is the store's. Measured on MI355X: 9 rows through 16384 x 8192 (71.3 MB
-// of weights) 15.6 us, 4.6 TB/s; one row through 4096 x 1024 3.1 us; 64 rows through 2816 x 1024 twice, gated, 5.9 us.
+// of weights) 15.6 us, 4.6 TB/s; one row through 4096 x 1024 3.1 us; 64 rows through 2816 x 1024 twice, gated, 5.5 us. Past 32
+// rows the weights are read once per 32 (gated 64) rows: 64 rows through 16384 x 8192 29 us, 256 rows 113.
 #include "m3x_fp4.h"
 
 namespace {

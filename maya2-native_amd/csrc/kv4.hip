@@ -26,8 +26,9 @@ struct M3xKv4 {
 };
 
 namespace {
-// Attention's workgroups: 4 waves, 4 on a SIMD (128 registers; no spill, 18 spilled registers cost 30 %). Measured at 224
-// rows of 2048 keys, heads 16/8 of 128, with 3 a SIMD (us): 79; 8 waves 92, 2 waves 93.
+// Attention's workgroups: 4 waves, 4 on a SIMD (128 registers; no spill, 18 spilled registers cost 30 %). Measured with 4
+// waves, 8 and 2, heads 16/8 of 128 (us): 224 rows of 2048 keys 79, 80, 89; of 300 keys 18, 23, 20; 8 x 200 prompt rows over
+// 500 keys 21, 26, 25.
 constexpr int KV4_NW = 4, KV4_OCC = 4;
 
 struct Kv4 {
@@ -72,8 +73,8 @@ __device__ __forceinline__ bool kv4_inside(const Kv4& c, long slot, int p) {
 }  // namespace
 
 // K and V rows into the cache, D / 8 threads per (row, kv head): a thread's eight numbers are one word of codes, four
-// threads' a group. Bound by the launch at few rows (1.7 us), by the rows' 16-bit bytes at many: 2048 rows of 8 heads of
-// 128 (8.4 MB in, 2.2 MB out) 4.9 us.
+// threads' a group. Bound by the launch at few rows (1.7 us), by one memory round trip beside the rows' bytes at many: 2048
+// rows of 8 heads of 128 (8.4 MB in, 2.2 MB out) 5.4 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const uint16_t* __restrict__ k, long sk_r, long sk_h,
                                                          const uint16_t* __restrict__ v, long sv_r, long sv_h, Kv4 c,
@@ -93,7 +94,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const uint16_t* __restr
 }
 
 // qk_norm_rope_cache_kernel's arithmetic and bits with the keys and values quantised into the 4-bit cache: one pass
-// over q|k|v instead of two, and no 16-bit keys in between. Bound as kv4_append_kernel.
+// over q|k|v instead of two, and no 16-bit keys in between. Bound as kv4_append_kernel; 16/8 heads of 128: 1 row 2.5 us, 224
+// rows 4.2, 2048 rows (27 MB) 10.0, as qk_norm_rope_cache_kernel's 2.6, 4.3 and 9.6.
 template <int D>
 __global__ __launch_bounds__(256) void qk_norm_rope_kv4_kernel(
     const uint16_t* __restrict__ qkv, long s_qkv, uint16_t* __restrict__ qo, long s_qo_b, long s_qo_h, Kv4 c,
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kv4_kernel(
 }
 
 // Positions of the cache as 16-bit rows (zeros for a row outside it). Bound by the rows' bytes: stored with the
-// non-temporal hint, passes over 16 x 4095 positions of 8 heads of 64 take 32.4 us (170 MB, 5.3 TB/s; a large copy's
+// non-temporal hint, passes over 16 x 4095 positions of 8 heads of 64 take 32.2 us (170 MB, 5.3 TB/s; a large copy's
 // 5.1), without it 45.6 (each pass then waits for the last one's lines to leave the caches).
 __device__ __forceinline__ void st16_nt(uint16_t* p, const u16x8& x) {
   __builtin_nontemporal_store(__builtin_bit_cast(fp4_u4, x), reinterpret_cast<fp4_u4*>(p));
@@ -183,16 +185,16 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4 c, const int64_t* __r
 // the largest weight is rounded too, and the error against 64 bits rises by a sixth.
 //
 // Bound, measured on MI355X with 16/8 heads of 128: the cache's bytes where rows fill the GPU (224 rows of 2048 keys
-// 77 us, 499 MB at 6.5 TB/s; of 4000 keys 143, 6.8 TB/s; the arithmetic without the loads 58, VALU busy 45 %).
-// Few rows: the start, the merge and the join beside the bytes (2 rows of 120000 keys, 32/4 heads of 64: 16.9 us of 65 MB
-// and 3.8 for the join; one row of 2048 keys 4.8 and 3.5). A prompt over a long context: a tile's own chain of steps, about
+// 77 us, 499 MB at 6.5 TB/s; of 4000 keys 145, 6.7 TB/s; VALU busy 47 %).
+// Few rows: the start, the merge and the join beside the bytes (2 rows of 120000 keys, 32/4 heads of 64: 16.3 us of 65 MB
+// and 4.0 for the join; one row of 2048 keys 4.5 and 3.4). A prompt over a long context: a tile's own chain of steps, about
 // 1 us at two waves a SIMD (512 rows over 4000 keys 34 us); over a short one a block's start and merge (1600 rows over up
-// to 500 keys 21 us).
+// to 500 keys 21 us). Every block of 16 columns converts its keys and values anew.
 namespace {
 template <int NI> struct Words { uint32_t w[NI]; };
 // A tile of the cache at `base`, the same in every lane; where `live` is false its loads give zeros and access nothing:
-// the loads ahead past a wave's last tile would read a tile again (1600 rows of 500 keys: 181 -> 151 us, 224 of 2048 80.5
-// -> 77).
+// the loads ahead past a wave's last tile would read a tile again (what it gave when it came: 1600 single rows of 500 keys
+// 181 -> 151 us, 224 of 2048 80.5 -> 77).
 typedef __amdgpu_buffer_rsrc_t Kv4Ref;
 __device__ __forceinline__ Kv4Ref kv4_ref(const uint8_t* base, bool live, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, live ? bytes : 0, 0x00020000);
@@ -563,8 +565,8 @@ __global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4At
 
   // The workgroup's candidates: R rows of an aligned group of qb. All first parts of groups, over the heads and the
   // splits, come before all second ones in launch order: a prompt's live workgroups, which its groups' first parts are,
-  // spread over the XCDs and do not stand behind those that leave at once (512 rows of a prompt over 4000 keys, heads
-  // 16/8 of 128: 49 -> 36 us against parts within a head; 64 rows over 500: 9.5 -> 7.1).
+  // spread over the XCDs and do not stand behind those that leave at once (heads 16/8 of 128, against a group's parts next
+  // to each other: 512 rows of a prompt over 4000 keys 39 us, 111; 64 rows over 500 6.7, 9.3).
   int part = 0, split = blockIdx.z;
   for (; split >= a.max_splits; split -= a.max_splits) ++part;
   const int first = blockIdx.x * a.qb;
@@ -589,8 +591,8 @@ __global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4At
     const long slot_u = (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)slot) |
                                (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(slot >> 32)) << 32);
     const int p0 = __builtin_amdgcn_readfirstlane(lds.pos[cand + 1]);
-    // A single row's keys are a stream of their own (non-temporal loads: 224 rows of 2048 keys 77 us, 88 without); a
-    // prompt's are read by its next blocks as well (16 x 512 rows over 512 keys: 67 us, 78 with).
+    // A single row's keys are a stream of their own (non-temporal loads: 224 rows of 2048 keys 80 us, 92 without); a
+    // prompt's are read by its next blocks as well (16 x 512 rows over 512 keys: 68 us, 78 with).
     if (n > 1) kv4_attn_row<DT, D, NW, false>(c, a, first + cand, n, slot_u, p0, kh, h0, Gc, split, wave, lds);
     else kv4_attn_row<DT, D, NW, true>(c, a, first + cand, 1, slot_u, p0, kh, h0, Gc, split, wave, lds);
   }
@@ -598,7 +600,7 @@ __global__ __launch_bounds__(64 * NW, KV4_OCC) void kv4_attn_kernel(Kv4 c, Kv4At
 
 // Joins the splits of a row's keys: NG groups of D / 4 threads a (row, head), each every NG-th split in order, then the
 // groups in order (the same order whatever the launch). Bound by the launch and two memory round trips; the first
-// splits are loaded beside the row's position, before it is known which of them there are. One row's 16 splits: 3.5 us.
+// splits are loaded beside the row's position, before it is known which of them there are. One row's 16 splits: 3.4 us.
 template <int DT, int D, int NG>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4 c, Kv4Attn a) {
   constexpr int TD = D / 4, HB = 256 / (TD * NG), U = 4;
@@ -799,9 +801,9 @@ M3X_API int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_
   }
   const int Gc = std::min(G, 16), qb = hb > 1 ? 1 : 16 / G;
   // R candidate rows a workgroup: fewer workgroups that leave at once, as long as 4096 are left for rows that are no
-  // prompt's and differ in length. Measured (us; 4096, 12288, R = 1): prompts of 64 rows x 64 seqs, 8/8 heads 21, 25, 50;
-  // 8 x 200 rows over 500 keys, 16/8 heads 26, 27, 33; 512 single rows over up to 1000 keys 63, 61, 61; 400 over up to
-  // 2000 79, 79, 79 (2048: 85, 1024: 95).
+  // prompt's and differ in length. Measured (us; 4096, 12288, R = 1): prompts of 64 rows x 64 seqs, 8/8 heads 15, 18, 38;
+  // 8 x 200 rows over 500 keys, 16/8 heads 21, 21, 25; 512 single rows over up to 1000 keys 58, 54, 55 (2048: 63); 400 over
+  // up to 2000 77, 76, 76 (2048: 81, 1024: 96).
   int R = 1;
   while (R < qb && (long)rows * c.kv_heads * hb * splits >= 4096L * R) R *= 2;
   R = R < qb ? R : qb;

@@ -731,14 +731,14 @@ def kv4_read(cache, slots, pos, k, v):
 def kv4_attn_chunk(rows, heads, kv_heads, max_ctx, head_dim=128) -> int:
     """Keys per split of kv4_attn for `rows` rows of up to max_ctx keys: a workgroup (a row, a kv head, a split) per CU
     at head_dim 128, two at 64 (whose arithmetic is the larger share), at least 128 keys each and no more than there are
-    (rounded up to 128); up to 1024 keys whole (no join of splits behind). Rows known to be a prompt's count as one per 16 // (heads // kv_heads), the rows that
-    share a pass: 64 of them at 4000 keys 14 us instead of 23.
+    (rounded up to 128); up to 1024 keys whole (no join of splits behind). Rows known to be a prompt's count as one per
+    16 // (heads // kv_heads), the rows that share a pass: 64 of them at 4000 keys 13.4 us instead of 22.5.
 
-    Measured on MI355X (graph-timed, us, 16/8 heads of 128, combine included): one row at 1024 keys 7.8 whole (128 keys
-    a split: 7.3), 32 rows 8.8 (512: 12.1); one row at 2048 7.7 (128; 512: 8.7, 2048: 11.6), 32 rows 13.5 whole (1024:
-    17.3); one row at 32000 12.0 (1024; 256: 15.9, 4096: 21.8), 4 rows 27.0 (4096; 1024: 28.5, 8192: 37.1); 224 rows at
-    2048 77 whole. 32/4 heads of 64: 2 rows at 120000 18.8 (2048; 1024: 22.7, 8192: 31.0), 16 rows at 32000 29.3 (4096;
-    512: 37.9)."""
+    Measured on MI355X (graph-timed, us, 16/8 heads of 128, combine included): one row at 1024 keys 7.2 whole (128 keys
+    a split: 6.4), 32 rows 8.8 (512: 12.5); one row at 2048 7.0 (128; 512: 8.2, 2048: 11.0), 32 rows 14.4 whole (1024:
+    18.2); one row at 32000 11.5 (1024; 256: 15.3, 4096: 21.8), 4 rows 27.7 (4096; 1024: 27.9, 8192: 37.9); 224 rows at
+    2048 77 whole. 32/4 heads of 64: 2 rows at 120000 19.2 (1920; 1024: 22.5, 8192: 31.9), 16 rows at 32000 30.9 (4096;
+    512: 40.0)."""
     if max_ctx <= 1024:
         return 1024
     blocks = rows * kv_heads * -(-heads // (16 * kv_heads))
