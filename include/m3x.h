@@ -513,7 +513,8 @@ int m3x_backbone_run(const M3xBackboneRun* args, void* stream);
  * <= 140); codes to nearest, ties to the even code, 6 above 5 s, so |x - value| <= s (fp16 numbers above 57344 and
  * bf16 numbers above 7 * 2^125 lose up to 2 s). A group holding a NaN or an infinity is stored with b = 255 and reads
  * as NaN. A call takes the numbers in its 16-bit type, rounded to nearest where the type is not the one they came from
- * (fp16 holds them all for 104 <= b <= 140). No counterpart in the reference, whose caches and weights are 16-bit (serve/fast_backbone.py:146-150).
+ * (fp16 holds them all for 104 <= b <= 140). No counterpart in the reference, whose caches and weights are 16-bit
+ * (serve/fast_backbone.py:146-150).
  *
  * The cache (per layer; cap % 32 == 0, head_dim D in {64, 128}; all four 16-byte aligned and contiguous), bytes:
  *   k4  [slots][kv_heads][cap][D / 2]               byte j: dims 2j (low half), 2j + 1
@@ -555,11 +556,12 @@ size_t m3x_kv4_attn_workspace(int rows, int heads, int head_dim, int max_ctx, in
  * kv_heads); q and out [rows, heads, D] 16-bit (strides % 8 == 0, 16-byte aligned). pos[r] < 0 or a slot outside the
  * cache: zeros. max_ctx >= pos[r] + 1 for every row (keys past it are not attended), <= cap; chunk = keys per split,
  * a multiple of 128; at most 2^20 rows and 4095 splits; |scale| <= 2^127. A score q . K is an fp32 sum, and a weight's
- * exponent its fp32 difference from the largest times the scale. bf16 weights below 2^-102 of the largest count as 0; a
- * sum of weighted values is finite up to 2^24 keys of any values. What a row does not see has no part in its result,
- * whatever it holds. Rows next to each other in the call, of one slot at consecutive positions (a prompt's), share one
- * pass over the keys; a row's bits do not depend on that, and not on the other rows. Fixed summation order. Two calls
- * that may run at the same time need a workspace each. */
+ * exponent its fp32 difference from the largest times the scale. Weights are rounded to the 16-bit type, and relative to
+ * the largest bf16 ones below 2^-102 count as 0 and fp16 ones are multiples of 2^-39; a sum of weighted values is finite up
+ * to 2^24 keys of any values. What a row does not see has no part in its result, whatever it holds. Rows next to each
+ * other in the call, of one slot at consecutive positions (a prompt's), share one pass over the keys; a row's bits do not
+ * depend on that, and not on the other rows. Fixed summation order. Two calls that may run at the same time need a
+ * workspace each. */
 int m3x_kv4_attn(const M3xKv4* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
                  const int64_t* slots, const int32_t* pos, float scale, int rows, int heads, int max_ctx, int chunk,
                  void* workspace, size_t ws_bytes, int dtype, void* stream);

@@ -469,7 +469,8 @@ __device__ __forceinline__ void kv4_attn_row(const Kv4& c, const Kv4Attn& a, int
 #pragma unroll
             for (int e = 0; e < 4 * NG; e += 2)
               if (e == (at & ~1)) mine = pop[e / 8][e % 8 / 2];
-            const float p = E<DT>::to_f((uint16_t)(__builtin_amdgcn_ds_bpermute(4 * (16 * q + li), (int)mine) >> (16 * (at & 1))));
+            const int pair = __builtin_amdgcn_ds_bpermute(4 * (16 * q + li), (int)mine);
+            const float p = E<DT>::to_f((uint16_t)(pair >> (16 * (at & 1))));
             if (key > klim) continue;
             const uint8_t* wp = c.v + ((base + key) >> 2) * (2 * D) + (key & 3) * NI;
             const uint8_t* sp = c.vs + ((base + key) >> 2) * (4 * NI) + (key & 3);
