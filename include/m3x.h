@@ -586,6 +586,68 @@ int m3x_linear4(const void* x, long ldx, const void* codes, const void* scales, 
 int m3x_linear4_act(const void* x, long ldx, const void* g_codes, const void* g_scales, const void* u_codes,
                     const void* u_scales, void* y, long ldy, int M, int I, int K, int kind, int dtype, void* stream);
 
+/* ---- paged 16-bit cache ------------------------------------------------------------------------------------------
+ * Positions live in pages that a table names: position p of slot s is at p % page_size of page
+ * table[s * width + p / page_size]. Per layer two pools k, v [pages][kv_heads][page_size][head_dim] in 16 bits, the last
+ * three dimensions contiguous, a page every page_stride elements (% 8 == 0, the same in both: a view of joined pools
+ * will do), 16-byte aligned. head_dim 64 or 128, page_size 16, 32, 64, 128 or 256, width * page_size <= 2^30. Slots may
+ * name the same page (a shared prefix). An entry outside [0, pages) is no page: what would lie there is not written, is
+ * read as zeros and seen by no row. No counterpart in the reference, whose cache is one block of `capacity` positions a
+ * slot (serve/fast_backbone.py:146-150). */
+typedef struct M3xPagedKv {
+  void* k;
+  void* v;
+  const int32_t* table; /* device */
+  long page_stride;
+  int pages, page_size, kv_heads, head_dim, slots, width, dtype;
+} M3xPagedKv;
+
+/* The rotation of the first `dim` dims (a multiple of 16, at most head_dim) of a head at position p: pair i turns by
+ * p * f_i, freq[i] (device, dim / 2 of them) = round(f_i / (2 pi) * 2^64) mod 2^64, a 64-bit binary fraction of a turn a
+ * position, so that angles are exact at any position. Pairs are (i, i + dim / 2), or (2 i, 2 i + 1) when interleaved.
+ * factor multiplies the rotated values. The structs are on the host and read during the call. */
+typedef struct M3xRotary {
+  const uint64_t* freq;
+  int dim, interleaved;
+  float factor;
+} M3xRotary;
+
+/* K and V rows [rows, kv_heads, head_dim] (cache's dtype, row and head strides % 8 == 0) to position pos[r] of slot
+ * slots[r]; a row whose slot, position or page is outside the cache is not written. Rows of one call are to be at
+ * different places. */
+int m3x_paged_append(const M3xPagedKv* cache, const void* k, long sk_r, long sk_h, const void* v, long sv_r, long sv_h,
+                     const int64_t* slots, const int32_t* pos, int rows, void* stream);
+
+/* q|k|v rows [q heads | k heads | v heads]: each head of q and k normed, x / sqrt(mean(x^2) + eps) * w (wq, wk
+ * [head_dim]; both NULL: not normed), rotated at pos[r] (0 for a negative one), q to q_out [rows, heads, head_dim], k and
+ * v to the cache as m3x_paged_append does. fp32 arithmetic, one rounding. q_out does not overlap qkv. */
+int m3x_qk_norm_rope_paged(const M3xPagedKv* cache, const void* qkv, long s_qkv, void* q_out, long s_qo_b, long s_qo_h,
+                           const int64_t* slots, const int32_t* pos, const M3xRotary* rotary, const void* wq,
+                           const void* wk, float eps, int rows, int heads, void* stream);
+
+/* k[r], v[r] ([kv_heads, head_dim], strides % 8 == 0) = position pos[r] of slot slots[r], zeros where there is none. */
+int m3x_paged_read(const M3xPagedKv* cache, const int64_t* slots, const int32_t* pos, void* k, long sk_r, long sk_h,
+                   void* v, long sv_r, long sv_h, int rows, void* stream);
+
+/* Bytes of workspace of m3x_paged_attn (0 for one split). */
+size_t m3x_paged_attn_workspace(int tiles, int kv_heads, int heads, int tile_rows, int cols, int head_dim, int splits);
+
+/* out[r, h] = softmax(scale q[r, h] . K^T) V over the positions j of slot slots[r] that the row at position p = pos[r]
+ * sees: j <= p and, with window > 0, j > p - window or j < sinks; kv head h / (heads / kv_heads). q and out
+ * [rows, heads, head_dim] (strides % 8 == 0, 16-byte aligned). A row that sees nothing (pos < 0, no page, a slot outside
+ * the cache) gets zeros; positions past the table's end do not exist.
+ * tiles (device): ntiles pairs (first row, rows <= tile_rows) of rows of one slot at consecutive positions, of which the
+ * first row's slot and position are read; NULL: ntiles single rows 0, 1, ... (tile_rows 1). Rows in no tile are left as
+ * they are; a pair with no rows is skipped. cols: columns (a tile's rows x query heads of a kv head) that a workgroup
+ * takes, 16 or 32 (few columns, bound by the keys' bytes) or 128 (prompts). A tile's keys are divided among up to
+ * `splits` <= 256 workgroups. Weights are rounded to the 16-bit type and summed as rounded; all else is fp32, in a fixed
+ * order. Scores times |scale| log2(e) are to be finite. What a row does not see has no part in its result, whatever it
+ * holds. Two calls that may run at the same time need a workspace each. */
+int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
+                   const int64_t* slots, const int32_t* pos, const int32_t* tiles, int ntiles, int tile_rows, int cols,
+                   float scale, int rows, int heads, int window, int sinks, int splits, void* workspace, size_t ws_bytes,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

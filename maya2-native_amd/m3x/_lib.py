@@ -12,7 +12,7 @@ import os
 import torch  # noqa: F401  (must precede the CDLL load, see above)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libm3x.so")
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -90,6 +90,11 @@ SIGNATURES = {
     "m3x_pack_weight4": (_I, [_P, _L, _I, _I, _P, _P, _I, _P]),
     "m3x_linear4": (_I, [_P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _P]),
     "m3x_linear4_act": (_I, [_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P]),
+    "m3x_paged_append": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _P]),
+    "m3x_qk_norm_rope_paged": (_I, [_P, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _F, _I, _I, _P]),
+    "m3x_paged_read": (_I, [_P, _P, _P, _P, _L, _L, _P, _L, _L, _I, _P]),
+    "m3x_paged_attn_workspace": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
+    "m3x_paged_attn": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "m3x_final_conv": (_I, [_P, _L, _P, _L, _P, _P, _F, _P, _L, _I, _I, _I, _I, _I, _I, _P]),
 }
 

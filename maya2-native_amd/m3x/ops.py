@@ -8,7 +8,7 @@ passes preallocated outputs and workspaces.
 from __future__ import annotations
 
 import ctypes
-
+import math
 
 import numpy as np
 
@@ -890,6 +890,306 @@ def linear4_act(x, w_gate, w_up, kind, y=None):
     _launch(dev, lib().m3x_linear4_act, xp, ldx, w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), *u, yp, ldy, M,
             w_gate.N, w_gate.K, kind, _DT[x.dtype])
     return y
+
+
+# ---------------------------------------------------------------- paged 16-bit cache
+class PagedKvArgs(ctypes.Structure):
+    """Mirror of M3xPagedKv (include/m3x.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "table")] + [("page_stride", ctypes.c_long)] + [
+        (n, ctypes.c_int) for n in ("pages", "page_size", "kv_heads", "head_dim", "slots", "width", "dtype")]
+
+
+class PagedKv:
+    """A layer's KV cache in pages (include/m3x.h): pools k, v [pages, kv_heads, page_size, head_dim] (bf16 or fp16; one
+    page stride, the rest contiguous) and the table [slots, width] (int32, contiguous) that names the page of every
+    page_size positions of a slot. Layers may share a table, slots a page; an entry outside the pool (-1) is no page.
+    head_dim 64 or 128, page_size 16, 32, 64, 128 or 256, up to 2^30 positions a slot (`cap`). The tensors are the
+    handle's for its life: their storage is not resized or replaced; the table's entries may change between calls."""
+    __slots__ = ("k", "v", "table", "pages", "page_size", "kv_heads", "head_dim", "slots", "cap", "dtype", "device",
+                 "_index", "_args", "_ref")
+
+    def __init__(self, k, v, table):
+        if k.dim() != 4:
+            raise ValueError(f"PagedKv: k must be [pages, kv_heads, page_size, head_dim], got {tuple(k.shape)}")
+        N, KV, P, D = k.shape
+        if D not in (64, 128) or P not in (16, 32, 64, 128, 256) or min(N, KV) < 1 or k.dtype not in _DT:
+            raise ValueError(f"PagedKv: head_dim {D} must be 64 or 128, page_size {P} a power of two from 16 to 256 and "
+                             f"the type bfloat16 or float16, got {k.dtype}")
+        for t, name in ((k, "k"), (v, "v")):
+            if t.shape != k.shape or t.dtype != k.dtype or t.device != k.device or t.stride() != k.stride():
+                raise ValueError(f"PagedKv: {name} must be {k.dtype} {tuple(k.shape)} with strides {k.stride()} on "
+                                 f"{k.device}")
+            if t.stride()[1:] != (P * D, D, 1) or t.stride(0) % 8 or t.stride(0) < KV * P * D or t.data_ptr() % 16:
+                raise ValueError(f"PagedKv: {name}'s pages must be contiguous and 16-byte aligned (strides {t.stride()})")
+        if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.device != k.device:
+            raise ValueError(f"PagedKv: table must be contiguous int32 [slots, width] on {k.device}")
+        S, W = table.shape
+        if min(S, W) < 1 or W * P > 1 << 30:
+            raise ValueError(f"PagedKv: a table of {S} x {W} pages of {P}: at least one slot, at most 2^30 positions")
+        self.k, self.v, self.table = k, v, table
+        self.pages, self.page_size, self.kv_heads, self.head_dim, self.slots = N, P, KV, D, S
+        self.cap, self.dtype, self.device, self._index = W * P, k.dtype, k.device, k.get_device()
+        self._args = PagedKvArgs(k.data_ptr(), v.data_ptr(), table.data_ptr(), k.stride(0), N, P, KV, D, S, W,
+                                 _DT[k.dtype])
+        self._ref = ctypes.addressof(self._args)
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, head_dim, table, dtype=torch.bfloat16):
+        """New pools (zeros) under `table`."""
+        return cls(*(torch.zeros(pages, kv_heads, page_size, head_dim, dtype=dtype, device=table.device) for _ in "kv"),
+                   table)
+
+    def memory_bytes(self):
+        """Bytes of the pools."""
+        return 2 * self.k.numel() * self.k.element_size()
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of M3xRotary (include/m3x.h)."""
+    _fields_ = [("freq", ctypes.c_void_p), ("dim", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("factor", ctypes.c_float)]
+
+
+def _turns(inv_freq):
+    """round(f / (2 pi) * 2^64) mod 2^64 of each (finite) f, exact, as int64 words. 2 pi by Machin's formula,
+    pi / 4 = 4 arctan(1/5) - arctan(1/239), in integers of 256 bits."""
+    one = 1 << 256
+
+    def arctan_inverse(n):
+        total = term = one // n
+        k = 1
+        while term:
+            term //= -n * n
+            k += 2
+            total += term // k
+        return total
+    two_pi = 8 * (4 * arctan_inverse(5) - arctan_inverse(239))
+    out = []
+    for f in inv_freq:
+        num, den = float(f).as_integer_ratio()
+        scaled = num * (one << 64)
+        whole = (2 * scaled + den * two_pi) // (2 * den * two_pi) & ((1 << 64) - 1)
+        out.append(whole - (1 << 64) if whole >> 63 else whole)
+    return out
+
+
+class Rotary:
+    """A rotation of the first 2 * len(inv_freq) dims of each head by position: inv_freq in radians a position (a tensor
+    or floats, taken as they are in 64 bits; 8 to 64 of them, a multiple of 8), pairs (i, i + dim / 2), or (2i, 2i + 1)
+    when interleaved; factor multiplies the rotated values. Angles are exact at any position. See rotary_freqs."""
+    __slots__ = ("freq", "dim", "interleaved", "factor", "_index", "_args", "_ref")
+
+    def __init__(self, inv_freq, interleaved=False, factor=1.0, device="cuda"):
+        f = torch.as_tensor(inv_freq).detach().to("cpu", torch.float64)
+        if f.dim() != 1 or f.numel() % 8 or not 8 <= f.numel() <= 64 or not torch.isfinite(f).all():
+            raise ValueError(f"Rotary: 8 to 64 finite frequencies, a multiple of 8, got {tuple(f.shape)}")
+        if not abs(float(factor)) < 3.4e38:
+            raise ValueError(f"Rotary: factor {factor}")
+        self.freq = torch.tensor(_turns(f.tolist()), dtype=torch.int64).to(device)
+        self.dim, self.interleaved, self.factor = 2 * f.numel(), bool(interleaved), float(factor)
+        self._index = self.freq.get_device()
+        self._args = RotaryArgs(self.freq.data_ptr(), self.dim, int(self.interleaved), self.factor)
+        self._ref = ctypes.addressof(self._args)
+
+
+def rotary_freqs(dim, theta, kind="plain", by=1.0, trained=None, fast=32.0, slow=1.0):
+    """(inv_freq float64 [dim / 2], factor) for Rotary, inv_freq_i = theta^(-2i / dim), for contexts `by` times as long
+    as the model was trained for. kind:
+      plain   as they are
+      linear  positions interpolated: inv_freq / by
+      base    theta * by^(dim / (dim - 2)): the slowest pair interpolated, the fastest as it is
+      parts   by each pair's turns r over the `trained` length: as they are from `fast` turns on, interpolated up to
+              `slow`, in between by (r - slow) / (fast - slow); factor 0.1 ln(by) + 1"""
+    if kind not in ("plain", "linear", "base", "parts"):
+        raise ValueError(f"rotary_freqs: kind {kind!r}")
+    if dim < 4 or dim % 2 or not theta > 0 or not by >= 1 or (kind == "parts" and (not trained or not fast > slow)):
+        raise ValueError(f"rotary_freqs: dim {dim}, theta {theta}, by {by}, trained {trained}, turns {slow} to {fast}")
+    if kind == "base":
+        theta = theta * by ** (dim / (dim - 2))
+    f = float(theta) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if kind == "linear":
+        return f / by, 1.0
+    if kind == "parts":
+        keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        return f * keep + f / by * (1 - keep), 0.1 * math.log(by) + 1
+    return f, 1.0
+
+
+def _paged_rows(name, cache, slots, pos):
+    """(rows, slots pointer, pos pointer) of a call's rows."""
+    if not isinstance(cache, PagedKv):
+        raise TypeError(f"{name}: the cache must be an ops.PagedKv")
+    if slots.dtype != torch.int64 or pos.dtype != torch.int32:
+        raise ValueError(f"{name}: slots must be int64 and pos int32, got {slots.dtype}, {pos.dtype}")
+    shape = slots.shape
+    if len(shape) != 1 or pos.shape != shape or not slots.is_contiguous() or not pos.is_contiguous():
+        raise ValueError(f"{name}: slots and pos must be contiguous [rows], got {tuple(shape)}, {tuple(pos.shape)}")
+    if slots.get_device() != cache._index or pos.get_device() != cache._index:
+        raise ValueError(f"{name}: slots on {slots.device}, pos on {pos.device}, the cache on {cache.device}")
+    return shape[0], slots.data_ptr(), pos.data_ptr()
+
+
+def paged_append(k, v, cache, slots, pos):
+    """K and V rows [rows, kv_heads, head_dim] (the cache's type, any row and head strides) to position pos[r] (int32) of
+    slot slots[r] (int64). A row whose slot, position or page is outside the cache is not written; rows at one place leave
+    a mixture there."""
+    rows, sp, pp = _paged_rows("paged_append", cache, slots, pos)
+    ka = _kv4_heads("paged_append", "k", k, cache, rows, cache.kv_heads, cache.dtype)
+    va = _kv4_heads("paged_append", "v", v, cache, rows, cache.kv_heads, cache.dtype)
+    _on_gpu("paged_append", cache)
+    _launch(cache._index, lib().m3x_paged_append, cache._ref, *ka, *va, sp, pp, rows)
+
+
+def qk_norm_rope_paged(qkv, q_out, cache, slots, pos, rotary, wq, wk, eps, heads):
+    """q|k|v rows [rows, (heads + 2 kv_heads) * head_dim] of a step: each head of q and k RMS-normed with wq, wk
+    [head_dim] (both None: not normed) and rotated at its row's position, queries to q_out [rows, heads, head_dim], keys
+    and values into the cache as paged_append does. Everything in the cache's type; fp32 arithmetic, rounded once.
+    q_out does not overlap qkv."""
+    name = "qk_norm_rope_paged"
+    rows, sp, pp = _paged_rows(name, cache, slots, pos)
+    D, width = cache.head_dim, (heads + 2 * cache.kv_heads) * cache.head_dim
+    if qkv.shape != (rows, width) or (rows and qkv.stride(1) != 1) or heads < 1:
+        raise ValueError(f"{name}: qkv must be [{rows}, {width}] with a contiguous last dimension, got {tuple(qkv.shape)}")
+    if not isinstance(rotary, Rotary) or rotary.dim > D:
+        raise ValueError(f"{name}: rotary must be an ops.Rotary of at most {D} dims")
+    qa = _kv4_heads(name, "q_out", q_out, cache, rows, heads, cache.dtype)
+    qp, s_qkv = qkv.data_ptr(), qkv.stride(0)
+    if qkv.dtype != cache.dtype or qkv.get_device() != cache._index or rotary._index != cache._index:
+        raise ValueError(f"{name}: qkv must be {cache.dtype} on {cache.device}, as the rotation, got {qkv.dtype} on "
+                         f"{qkv.device}")
+    if (s_qkv | qp >> 1) & 7:
+        raise ValueError(f"{name}: qkv needs 16-byte aligned rows (stride {s_qkv})")
+    wp = [0, 0]
+    if wq is not None or wk is not None:
+        for i, (t, what) in enumerate(((wq, "wq"), (wk, "wk"))):
+            if t is None or t.numel() != D or t.dtype != cache.dtype or not t.is_contiguous() or t.data_ptr() % 16 or \
+                    t.get_device() != cache._index:
+                raise ValueError(f"{name}: {what} must be {D} contiguous, 16-byte aligned {cache.dtype} on {cache.device}")
+            wp[i] = t.data_ptr()
+    _on_gpu(name, cache)
+    _launch(cache._index, lib().m3x_qk_norm_rope_paged, cache._ref, qp, s_qkv, *qa, sp, pp, rotary._ref, *wp, float(eps),
+            rows, heads)
+
+
+def paged_read(cache, slots, pos, k, v):
+    """k, v [rows, kv_heads, head_dim] (the cache's type, any row and head strides) = position pos[r] of slot slots[r];
+    zeros where there is none."""
+    rows, sp, pp = _paged_rows("paged_read", cache, slots, pos)
+    ka = _kv4_heads("paged_read", "k", k, cache, rows, cache.kv_heads, cache.dtype)
+    va = _kv4_heads("paged_read", "v", v, cache, rows, cache.kv_heads, cache.dtype)
+    _on_gpu("paged_read", cache)
+    _launch(cache._index, lib().m3x_paged_read, cache._ref, sp, pp, *ka, *va, rows)
+
+
+NARROW_COLS, WIDE_COLS = 32, 128  # columns (rows x query heads of a kv head) that a workgroup of either kernel takes
+
+
+def paged_tiles(runs, heads, kv_heads):
+    """The tiles of paged_attn for rows laid out as runs, (first row, rows, first position) each, of one slot at
+    consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to 32 columns is one narrow
+    tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first."""
+    G = heads // kv_heads
+    r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
+    r = r[r[:, 1] > 0]
+    few = (r[:, 1] * G <= NARROW_COLS) | (r[:, 1] == 1)
+    most = max(1, WIDE_COLS // G)
+    long = r[~few]
+    n = -(-long[:, 1] // most)
+    of = np.repeat(np.arange(len(long)), n)
+    at = np.arange(len(of)) - np.repeat(np.cumsum(n) - n, n)
+    a, b = at * long[of, 1] // n[of], (at + 1) * long[of, 1] // n[of]
+    order = np.argsort(-(long[of, 2] + b), kind="stable")
+    wide = np.stack([long[of, 0] + a, b - a], 1)[order]
+    return r[few, :2].astype(np.int32), wide.astype(np.int32)
+
+
+class PagedPlan:
+    """How paged_attn runs a step's rows, for all its layers and for every step of the same row layout: runs as in
+    paged_tiles (rows in none are left as they are), the heads, the largest context that the rows will see (a rule's
+    input, no limit), window and sinks (see paged_attn). `workspace`: bytes that a call needs; calls that may run at the
+    same time need one each."""
+    __slots__ = ("rows", "heads", "kv_heads", "head_dim", "window", "sinks", "launches", "workspace", "_index", "_calls",
+                 "_keep")
+
+    def __init__(self, runs, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
+        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
+        if kv_heads < 1 or heads < 1 or heads % kv_heads:
+            raise ValueError(f"PagedPlan: {heads} query heads over {kv_heads} kv heads")
+        if (r[:, :2] < 0).any() or (r[:, 0] + r[:, 1] >= 1 << 31).any():
+            raise ValueError("PagedPlan: runs are (first row, rows, first position)")
+        if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
+            raise ValueError(f"PagedPlan: window {window}, sinks {sinks}")
+        self._begin(int((r[:, 0] + r[:, 1]).max()) if len(r) else 0, heads, kv_heads, head_dim, window, sinks)
+        narrow, wide = paged_tiles(r, heads, kv_heads)
+        every = len(narrow) == self.rows and (narrow[:, 1] == 1).all() and (narrow[:, 0] == np.arange(self.rows)).all()
+        if len(narrow):
+            tiles = None if every else torch.from_numpy(np.ascontiguousarray(narrow)).to(device)
+            self._add(tiles, len(narrow), int(narrow[:, 1].max()), max_ctx)
+        if len(wide):
+            self._add(torch.from_numpy(np.ascontiguousarray(wide)).to(device), len(wide), int(wide[:, 1].max()), max_ctx,
+                      True)
+        self._finish(torch.device(device))
+
+    def _begin(self, rows, heads, kv_heads, head_dim, window, sinks):
+        self.rows, self.heads, self.kv_heads, self.head_dim = rows, heads, kv_heads, head_dim
+        self.window, self.sinks, self.launches = int(window), int(sinks), []
+
+    def _add(self, tiles, n, tile_rows, max_ctx, wide=False):
+        G = self.heads // self.kv_heads
+        cols = WIDE_COLS if wide else 16 if tile_rows * G <= 16 else NARROW_COLS
+        blocks = n * self.kv_heads * -(-tile_rows * G // cols)
+        keys = min(max_ctx, self.window + self.sinks + tile_rows) if self.window else max_ctx
+        self.launches.append((tiles, n, tile_rows, cols, paged_attn_splits(blocks, keys, cols)))
+
+    def _finish(self, device):
+        self.workspace = max([0] + [int(lib().m3x_paged_attn_workspace(n, self.kv_heads, self.heads, tr, cols,
+                                                                       self.head_dim, splits))
+                                    for _, n, tr, cols, splits in self.launches])
+        if device.type == "cuda":
+            self._index = torch.cuda.current_device() if device.index is None else device.index
+        else:
+            self._index = -1
+        self._calls = [(0 if t is None else t.data_ptr(), n, tr, cols, s) for t, n, tr, cols, s in self.launches]
+
+
+def paged_attn_splits(blocks, keys, cols) -> int:
+    """Workgroups that share a tile's keys, for `blocks` (tiles x kv heads x blocks of `cols` columns) of up to `keys`
+    keys each."""
+    if cols == WIDE_COLS:
+        return max(1, min(512 // max(blocks, 1), -(-keys // 256), 64))
+    return max(1, min(-(-768 // max(blocks, 1)), -(-keys // 256), 64))
+
+
+def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
+    """out[r, h] = softmax(scale q[r, h] . K^T) V over the positions j of slot slots[r] that row r at position p = pos[r]
+    sees: j <= p and, with a window (plan.window > 0), j > p - window or j < plan.sinks. q, out [rows, heads, head_dim]
+    (the cache's type, any row and head strides). A row that sees nothing gets zeros (pos[r] < 0, a slot outside the
+    cache, positions in no page); a row in none of the plan's runs is left as it is. The rows of a run are of one slot at
+    consecutive positions: its first row's are read. workspace: a tensor of plan.workspace bytes, or None when that is 0.
+    Scores times |scale| are finite numbers below 2^127, |scale| at most 2^126."""
+    rows, sp, pp = _paged_rows("paged_attn", cache, slots, pos)
+    if not isinstance(plan, PagedPlan):
+        raise TypeError("paged_attn: the plan must be an ops.PagedPlan")
+    heads = plan.heads
+    if plan.kv_heads != cache.kv_heads or plan.head_dim != cache.head_dim or plan.rows > rows or plan._index != cache._index:
+        raise ValueError(f"paged_attn: a plan of {plan.rows} rows, {heads} / {plan.kv_heads} heads of {plan.head_dim} for "
+                         f"{rows} rows over {cache.kv_heads} kv heads of {cache.head_dim} on {cache.device}")
+    qa = _kv4_heads("paged_attn", "q", q, cache, rows, heads, cache.dtype)
+    oa = _kv4_heads("paged_attn", "out", out, cache, rows, heads, cache.dtype)
+    if not abs(scale) <= 2.0 ** 126:
+        raise ValueError(f"paged_attn: |scale| must be at most 2^126, got {scale}")
+    ws, ws_bytes = 0, 0
+    if plan.workspace:
+        if workspace is not None:
+            ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if ws_bytes < plan.workspace:
+            raise ValueError(f"paged_attn: a workspace of {plan.workspace} bytes is needed, got {ws_bytes}")
+        if not workspace.is_contiguous() or ws % 16 or workspace.get_device() != cache._index:
+            raise ValueError(f"paged_attn: the workspace must be contiguous, 16-byte aligned and on {cache.device}")
+    _on_gpu("paged_attn", cache)
+    for tiles, n, tile_rows, cols, splits in plan._calls:
+        _launch(cache._index, lib().m3x_paged_attn, cache._ref, *qa, *oa, sp, pp, tiles, n, tile_rows, cols, scale, rows,
+                heads, plan.window, plan.sinks, splits, ws, ws_bytes)
 
 
 # ---------------------------------------------------------------- Mimi decode (serve/fast_codec.py)
