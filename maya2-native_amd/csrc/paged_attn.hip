@@ -45,18 +45,27 @@ struct Where {
   int tile, kh, block, first, n, p0;  // rows first .. first + n - 1 at positions p0 ..; n == 0: nothing to do
   long slot;
 };
-__device__ __forceinline__ int pg_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// x, the same in every lane, in a scalar register. The empty statement hides where x comes from: a value known to be
+// uniform is left in vector registers where a division made it, and what is computed from it too, up to the buffer
+// loads' addresses, each then in a loop over the lanes.
+__device__ __forceinline__ int pg_uniform(int x) {
+  asm("" : "+v"(x));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ long pg_uniform(long x) {
+  return (long)((uint64_t)(uint32_t)pg_uniform((int)x) | (uint64_t)(uint32_t)pg_uniform((int)(x >> 32)) << 32);
+}
 __device__ __forceinline__ Where pg_where(const Paged& c, const PagedAttn& a, uint32_t item) {
   Where w;
   const uint32_t th = item / (uint32_t)a.blocks;
-  w.block = (int)(item - th * a.blocks);
-  w.tile = (int)(th / (uint32_t)c.kv_heads);
-  w.kh = (int)(th - (uint32_t)w.tile * c.kv_heads);
+  w.block = pg_uniform((int)(item - th * a.blocks));
+  w.tile = pg_uniform((int)(th / (uint32_t)c.kv_heads));
+  w.kh = pg_uniform((int)(th - (uint32_t)w.tile * c.kv_heads));
   w.first = w.tile;
   w.n = 1;
   if (a.tiles) {
-    w.first = a.tiles[2 * w.tile];
-    w.n = a.tiles[2 * w.tile + 1];
+    w.first = pg_uniform(a.tiles[2 * w.tile]);
+    w.n = pg_uniform(a.tiles[2 * w.tile + 1]);
   }
   w.slot = -1;
   w.p0 = -1;
@@ -65,26 +74,27 @@ __device__ __forceinline__ Where pg_where(const Paged& c, const PagedAttn& a, ui
     return w;
   }
   w.n = min(min(w.n, a.tile_rows), a.rows - w.first);
-  w.slot = a.slots[w.first];
-  w.p0 = min(a.pos[w.first], 1 << 30);  // positions count past it in 32 bits, and the cache ends before
+  w.slot = pg_uniform((long)a.slots[w.first]);
+  w.p0 = min(pg_uniform(a.pos[w.first]), 1 << 30);  // positions count past it in 32 bits, and the cache ends before
   return w;
 }
 
 // a tile's keys in steps of KT positions
 template <int KT> struct Keys {
   int last;          // the last key that some row sees; -1: none
-  int sink, lo, nt;  // steps 0 .. sink - 1, then lo ..; their number
+  int sink, skip, nt;  // steps 0 .. sink - 1, then from sink + skip on; their number
   int per, active;   // steps a split; splits that have some
   __device__ __forceinline__ Keys(const Paged& c, const PagedAttn& a, const Where& w, int least) {
     const int cap = c.width << c.shift;
     last = w.slot < 0 || w.slot >= c.slots || w.n == 0 || w.p0 < -w.n ? -1 : min(w.p0 + w.n - 1, cap - 1);
-    lo = a.window ? max(0, w.p0 - a.window + 1) / KT : 0;
+    const int lo = a.window ? max(0, w.p0 - a.window + 1) / KT : 0;
     sink = a.window ? min((min(a.sinks, last + 1) + KT - 1) / KT, lo) : 0;
+    skip = pg_uniform(lo - sink);  // (opaque: it also serves lanes that branch, and would be made anew there)
     nt = last < 0 ? 0 : sink + max(0, last / KT + 1 - lo);
-    per = max(least, (nt + a.splits - 1) / a.splits);
-    active = (nt + per - 1) / per;
+    per = pg_uniform(max(least, (nt + a.splits - 1) / a.splits));
+    active = pg_uniform((nt + per - 1) / per);
   }
-  __device__ __forceinline__ int key(int i) const { return (i < sink ? i : i - sink + lo) * KT; }
+  __device__ __forceinline__ int key(int i) const { return (i + (i < sink ? 0 : skip)) * KT; }
 };
 
 // a column's row and head, and the keys it sees
@@ -181,10 +191,12 @@ template <int D> struct NarrowLds {
 // waves takes every fourth step of 32 keys, straight from memory to registers: K as the score product's operand, V as
 // rows whose numbers byte permutes pair over keys. The waves' results are merged through LDS.
 template <int DT, int D, int QT, bool NT>
-__global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Paged c, PagedAttn a) {
+__global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_kernel(Paged c, PagedAttn a) {
   constexpr int KT = 32, NW = NARROW_NW, KS = D / 32, NV = D / 32, COLS = 16 * QT;
-  // NV: words of V a lane holds of a key (2 NV dims)
-  const int wave = pg_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  // NV: words of V a lane holds of a key (2 NV dims); AHEAD: steps that a wave's loads run ahead (two fill the registers
+  // with 16 columns of 128 dims)
+  constexpr int AHEAD = D == 128 && QT == 2 ? 1 : 2;
+  const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Where w = pg_where(c, a, blockIdx.x);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
   const int split = blockIdx.y;
@@ -224,35 +236,38 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Page
   };
   const int inside = (1 << c.shift) - 1;
   const uint32_t k_at = li * (2 * D) + lg * 16, v_at = lg * (8 * D) + li * (D / 8);
-  PgWords<4> kw[2][KS];
-  PgWords<NV> vw[8];
-  const uint16_t* vbase[2];
-  int vbytes[2];
-  bool holes = false;  // a group of the step lies in no page
-  auto load_k = [&](int at) {
+  // AHEAD steps' numbers in turn: a step's keys are loaded behind the score products of the keys that they replace, its
+  // values behind the output products. Loads are never conditional (one whose registers are merged behind a
+  // branch is waited for there): past the wave's last step they are of no bytes.
+  struct Buf {
+    PgWords<4> kw[2][KS];
+    PgWords<NV> vw[8];
+    long off[2];   // where the two groups lie in the pools
+    int bytes[2];  // what is there of them
+    bool holes;    // one lies in no page
+  };
+  auto load_k = [&](Buf& b, int at) {
     if (left == 0) fetch_ids(at);
     const int key = at < i1 ? keys.key(at) : 0;
-    holes = false;
+    b.holes = false;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int id = __builtin_amdgcn_readlane(ids, 2 * (32 - left) + g), k0 = key + 16 * g;
-      const int bytes = id < 0 ? 0 : min(16, max(0, keys.last + 1 - k0)) * (2 * D);
-      holes |= id < 0 && k0 <= keys.last;
-      const long off = max(id, 0) * c.page_stride + (((long)w.kh << c.shift) + (k0 & inside)) * D;
-      vbase[g] = c.v + off;
-      vbytes[g] = bytes;
-      const auto ref = pg_ref_of(c.k + off, bytes);
+      b.bytes[g] = pg_uniform(id < 0 ? 0 : min(16, max(0, keys.last + 1 - k0)) * (2 * D));
+      b.holes |= id < 0 && k0 <= keys.last;
+      b.off[g] = pg_uniform(max(id, 0) * c.page_stride + (((long)w.kh << c.shift) + (k0 & inside)) * D);
+      const auto ref = pg_ref_of(c.k + b.off[g], b.bytes[g]);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kw[g][s] = pg_load<4, NT>(ref, k_at + 64 * s);
+      for (int s = 0; s < KS; ++s) b.kw[g][s] = pg_load<4, NT>(ref, k_at + 64 * s);
     }
     --left;
   };
-  auto load_v = [&]() {
+  auto load_v = [&](Buf& b) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const auto ref = pg_ref_of(vbase[g], vbytes[g]);
+      const auto ref = pg_ref_of(c.v + b.off[g], b.bytes[g]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) vw[4 * g + e] = pg_load<NV, NT>(ref, v_at + 2 * D * e);
+      for (int e = 0; e < 4; ++e) b.vw[4 * g + e] = pg_load<NV, NT>(ref, v_at + 2 * D * e);
     }
   };
 
@@ -267,17 +282,11 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Page
   }
   // keys up to `all` are seen by every row unless the window hides them; those up to `none` may be hidden by it
   const int all = min(w.p0, keys.last), none = a.window ? w.p0 + w.n - 1 - a.window : -1;
-  load_k(i);
-  load_v();
-  for (; i < i1; i += NW) {
+  auto step = [&](Buf& b, int i) {
     const int key = keys.key(i);
-    const bool holes_now = holes;
-    const bool edge = key + KT - 1 > all || (key <= none && key + KT > a.sinks) || holes_now;
+    const bool edge = key + KT - 1 > all || (key <= none && key + KT > a.sinks) || b.holes;
     uint32_t gone = 0;  // groups in no page
-    if (holes_now) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) gone |= vbytes[g] == 0 ? 1u << g : 0u;
-    }
+    if (b.holes) gone = (b.bytes[0] == 0 ? 1u : 0u) | (b.bytes[1] == 0 ? 2u : 0u);
     float s[QT][8];
 #pragma unroll
     for (int t = 0; t < QT; ++t)
@@ -285,13 +294,13 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Page
       for (int g = 0; g < 2; ++g) {
         f32x4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) x = mfma16x16x32<DT>(__builtin_bit_cast(u16x8, kw[g][k]), qop[t][k], x);
+        for (int k = 0; k < KS; ++k) x = mfma16x16x32<DT>(__builtin_bit_cast(u16x8, b.kw[g][k]), qop[t][k], x);
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[t][4 * g + r] = x[r];
       }
     __builtin_amdgcn_sched_barrier(0);
-    const uint16_t* vb[2] = {vbase[0], vbase[1]};
-    load_k(i + NW);
+    const long off[2] = {b.off[0], b.off[1]};
+    load_k(b, i + AHEAD * NW);
     __builtin_amdgcn_sched_barrier(0);
     if (edge) {
 #pragma unroll
@@ -335,13 +344,13 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Page
 #pragma unroll
       for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int x = 0; x < NV; ++x) any |= pg_wild<DT>(vw[e].w[x]);
+        for (int x = 0; x < NV; ++x) any |= pg_wild<DT>(b.vw[e].w[x]);
       wild = __ballot(any != 0) != 0;
       if (wild) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-          for (int x = 0; x < NV; ++x) vw[e].w[x] = pg_tame<DT>(vw[e].w[x]);
+          for (int x = 0; x < NV; ++x) b.vw[e].w[x] = pg_tame<DT>(b.vw[e].w[x]);
       }
     }
 #pragma unroll
@@ -349,8 +358,8 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Page
       pg_u4 lo, hi;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        lo[e] = __builtin_amdgcn_perm(vw[2 * e + 1].w[x], vw[2 * e].w[x], 0x05040100u);
-        hi[e] = __builtin_amdgcn_perm(vw[2 * e + 1].w[x], vw[2 * e].w[x], 0x07060302u);
+        lo[e] = __builtin_amdgcn_perm(b.vw[2 * e + 1].w[x], b.vw[2 * e].w[x], 0x05040100u);
+        hi[e] = __builtin_amdgcn_perm(b.vw[2 * e + 1].w[x], b.vw[2 * e].w[x], 0x07060302u);
       }
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -362,22 +371,43 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void paged_narrow_kernel(Page
     if (wild) {
       for (int k = 0; k < KT; ++k) {
         if (key + k > keys.last || (gone >> (k >> 4) & 1u)) continue;
-        const uint16_t* vp = (k < 16 ? vb[0] : vb[1]) + (long)(k & 15) * D;
+        const uint16_t* vp = c.v + (k < 16 ? off[0] : off[1]) + (k & 15) * D;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+          uint32_t x[NV];
+          if constexpr (NV == 4) *reinterpret_cast<pg_u4*>(x) = *reinterpret_cast<const pg_u4*>(vp + 2 * NV * (4 * lg + r));
+          else *reinterpret_cast<pg_u2*>(x) = *reinterpret_cast<const pg_u2*>(vp + 2 * NV * (4 * lg + r));
 #pragma unroll
-          for (int T = 0; T < 2 * NV; ++T) {
-            const float x = pg_wild_number<DT>(vp[2 * NV * (4 * lg + r) + T]);
+          for (int t = 0; t < QT; ++t)
+            if (!pg_hidden(key + k, min(cp[t], keys.last), pg_low(a, cp[t]), a.sinks)) {
 #pragma unroll
-            for (int t = 0; t < QT; ++t)
-              if (!pg_hidden(key + k, min(cp[t], keys.last), pg_low(a, cp[t]), a.sinks)) acc[t][T][r] += x;
-          }
+              for (int T = 0; T < 2 * NV; ++T) acc[t][T][r] += pg_wild_number<DT>((uint16_t)(x[T / 2] >> (16 * (T & 1))));
+            }
+        }
       }
       __builtin_amdgcn_s_waitcnt(0x0F70);
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_v();
+    load_v(b);
     __builtin_amdgcn_sched_barrier(0);
+  };
+  Buf b0, b1;
+  load_k(b0, i);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(b0);
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (AHEAD == 2) {
+    load_k(b1, i + NW);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(b1);
+    __builtin_amdgcn_sched_barrier(0);
+    for (; i + NW < i1; i += 2 * NW) {
+      step(b0, i);
+      step(b1, i + NW);
+    }
+    if (i < i1) step(b0, i);
+  } else {
+    for (; i < i1; i += NW) step(b0, i);
   }
 
   // merge the waves, 16 columns at a time: lane (column, lg) holds dims 2 NV (4 lg + r) + T
@@ -447,7 +477,7 @@ template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a) {
   constexpr int KT = WIDE_KT, KS = D / 32, ND = D / 16, COLS = 128, CH = D / 8, RPI = 64 / CH;  // RPI: rows a wave's load
   __shared__ __align__(16) uint16_t lk[2][KT * D], lv[2][KT * D];
-  const int wave = pg_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Where w = pg_where(c, a, blockIdx.x);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
   const int split = blockIdx.y;
@@ -525,7 +555,7 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
       const int k = key + 16 * g;
       if (k <= keys.last && (unsigned)row[k >> c.shift] >= (unsigned)c.pages) gone |= 1u << g;
     }
-    gone = pg_uniform(gone);
+    gone = (uint32_t)pg_uniform((int)gone);
     const bool edge = key + KT - 1 > min(pa, keys.last) || (key <= none && key + KT > a.sinks) || gone;
 
     float s[2][16];
