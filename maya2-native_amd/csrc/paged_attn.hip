@@ -164,7 +164,7 @@ template <int COLS, int D, int NT> __device__ __forceinline__ void pg_zero(const
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t pg_ref_of(const uint16_t* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, bytes, 0x00020000);
 }
-template <int NI> struct PgWords { uint32_t w[NI]; };
+template <int NI> struct __align__(4 * NI) PgWords { uint32_t w[NI]; };
 template <int NI, bool NT> __device__ __forceinline__ PgWords<NI> pg_load(__amdgpu_buffer_rsrc_t ref, uint32_t off) {
   constexpr int AUX = NT ? 2 : 0;
   PgWords<NI> r;
@@ -456,27 +456,23 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
 
 // ---------------------------------------------------------------------------------------------------------
 // Tiles of up to 128 columns and more: prompts. Bound by the matrix and vector units: each of the 4 waves owns 32 columns
-// and passes over all keys of the split; steps of 64 keys come to LDS (two in turn, loaded without registers) and every
+// and passes over all keys of the split; steps of 64 keys come to LDS (two in turn) and every
 // wave reads them from there, K's 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads.
-// Rows in LDS are permuted by 16-byte chunks (source address of a load, since a load writes LDS in lane order) so that
-// neither read meets a bank twice.
+// Rows in LDS are permuted by 16-byte chunks so that neither read meets a bank twice.
 namespace {
 constexpr int WIDE_KT = 64;
-__device__ const uint32_t pg_zeros[64] = {};  // a position's numbers where there is no position
-
-// the chunk of its row that a row's LDS chunk x holds, and the other way round
+// chunk x of a row lies at chunk x ^ wide_kx (wide_vx) of its row in LDS
 template <int D> __device__ __forceinline__ int wide_kx(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
 template <int D> __device__ __forceinline__ int wide_vx(int key) { return D == 128 ? 2 * (key & 7) : 2 * ((key >> 1) & 3); }
 
-typedef __attribute__((address_space(1))) const void pg_global;
-typedef __attribute__((address_space(3))) void pg_lds;
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 }  // namespace
 
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a) {
   constexpr int KT = WIDE_KT, KS = D / 32, ND = D / 16, COLS = 128, CH = D / 8, RPI = 64 / CH;  // RPI: rows a wave's load
-  __shared__ __align__(16) uint16_t lk[2][KT * D], lv[2][KT * D];
+  constexpr int RB = 2 * D, VB = KT * RB, STAGE = 2 * VB;  // bytes of a row, of a step's K, of a stage (K, then V)
+  __shared__ __align__(16) uint8_t lds[2 * STAGE];
   const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Where w = pg_where(c, a, blockIdx.x);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
@@ -509,25 +505,60 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
   const int pa = w.p0 + ja, pb = some ? w.p0 + jb : -1;
   const int none = a.window ? pb - a.window : -1, low = a.window ? pa - a.window : -1;
 
-  // step i's keys to stage `st`: the wave brings 16 keys of K and of V (a 16-key group, so one page)
+  // Lane x: the page of step base + x's group `wave` of 16 keys (-1: none), and which of its four groups lie in no page
   const int32_t* row = c.table + w.slot * c.width;
   const int inside = (1 << c.shift) - 1;
-  auto stage = [&](int i, int st) {
-    const int k0 = keys.key(i) + 16 * wave;
-    int id = k0 <= keys.last ? row[k0 >> c.shift] : -1;
-    if ((unsigned)id >= (unsigned)c.pages) id = -1;
-    id = pg_uniform(id);
-    const long off = max(id, 0) * c.page_stride + (((long)w.kh << c.shift) + (k0 & inside)) * D;
+  int ids = -1, gaps = 0, base = 0;
+  auto fetch_ids = [&](int from) {
+    base = from;
+    ids = -1;
+    gaps = 0;
+    const int at = from + lane;
+    if (at < i1) {
+      const int key = keys.key(at);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int k = key + 16 * g;
+        const bool in = k <= keys.last;
+        const int id = in ? row[k >> c.shift] : -1;
+        if ((unsigned)id >= (unsigned)c.pages) gaps |= in ? 1 << g : 0;
+        else if (g == wave) ids = id;
+      }
+    }
+  };
+  // a step's K and V: the wave brings 16 keys of each (one page), RPI a load; then to LDS. A chunk's place is its number
+  // XOR a number of its row, so the places of a lane's other rows, key quarters and dims are its first place XOR constants
+  // (made anew where they are used: kept, they would not fit the registers), and the other stage's XOR the stage's size.
+  const int r0 = lane / CH, ch = lane % CH, rv = 4 * lg + (li >> 2);
+  const uint32_t g_at = r0 * RB + ch * 16;
+  uint32_t put_k = (16 * wave + r0) * RB + (ch ^ wide_kx<D>(r0)) * 16;
+  uint32_t put_v = VB + (16 * wave + r0) * RB + (ch ^ wide_vx<D>(r0)) * 16;
+  uint32_t get_k = li * RB + (lg ^ wide_kx<D>(li)) * 16;
+  // the lane group's four keys, 16 dims: lane x brings dims 4 (x % 4) .. of key x / 4, and takes dim x of the four
+  uint32_t get_v = VB + rv * RB + (((li >> 1) & 1) ^ wide_vx<D>(rv)) * 16 + (li & 1) * 8;
+  PgWords<4> kb[16 / RPI], vb[16 / RPI];
+  auto bring = [&](int i) {
+    if (i - base == 64) fetch_ids(i);
+    const int k0 = keys.key(i) + 16 * wave, x = (i - base) & 63;
+    const int id = __builtin_amdgcn_readlane(ids, x);
+    const uint32_t g = (uint32_t)__builtin_amdgcn_readlane(gaps, x);
+    const int bytes = pg_uniform(id < 0 ? 0 : min(16, max(0, keys.last + 1 - k0)) * (2 * D));
+    const long off = pg_uniform(max(id, 0) * c.page_stride + (((long)w.kh << c.shift) + (k0 & inside)) * D);
+    const auto kr = pg_ref_of(c.k + off, bytes), vr = pg_ref_of(c.v + off, bytes);
+#pragma unroll
+    for (int x = 0; x < 16 / RPI; ++x) kb[x] = pg_load<4, false>(kr, g_at + x * RPI * RB);
+#pragma unroll
+    for (int x = 0; x < 16 / RPI; ++x) vb[x] = pg_load<4, false>(vr, g_at + x * RPI * RB);
+    return g;
+  };
+  auto store = [&]() {
 #pragma unroll
     for (int x = 0; x < 16 / RPI; ++x) {
-      const int r = x * RPI + lane / CH, ch = lane % CH;  // the lane's row of the group and its chunk in LDS
-      const bool there = id >= 0 && k0 + r <= keys.last;
-      const uint16_t* zero = reinterpret_cast<const uint16_t*>(pg_zeros) + ch * 8;
-      const uint16_t* kp = there ? c.k + off + r * D + (ch ^ wide_kx<D>(r)) * 8 : zero;
-      const uint16_t* vp = there ? c.v + off + r * D + (ch ^ wide_vx<D>(r)) * 8 : zero;
-      __builtin_amdgcn_global_load_lds((pg_global*)kp, (pg_lds*)&lk[st][(16 * wave + x * RPI) * D], 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((pg_global*)vp, (pg_lds*)&lv[st][(16 * wave + x * RPI) * D], 16, 0, 0);
+      *reinterpret_cast<PgWords<4>*>(lds + (put_k ^ (64 * x)) + x * RPI * RB) = kb[x];
+      *reinterpret_cast<PgWords<4>*>(lds + (put_v ^ (D == 128 ? 128 * (x & 1) : 0)) + x * RPI * RB) = vb[x];
     }
+    put_k ^= STAGE;
+    put_v ^= STAGE;
   };
 
   float m[2], l[2];
@@ -540,39 +571,54 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
     for (int T = 0; T < ND; ++T) acc[t][T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  stage(i0, 0);
+  fetch_ids(i0);
+  uint32_t next = bring(i0);
+  store();
+  __syncthreads();
   for (int i = i0; i < i1; ++i) {
-    const int st = (i - i0) & 1;
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // the wave's loads into this stage have arrived (vmcnt 0)
-    __syncthreads();                     // everyone's have, and everyone is done with the other stage
-    if (i + 1 < i1) stage(i + 1, st ^ 1);
+    asm("" : "+v"(put_k), "+v"(put_v), "+v"(get_k), "+v"(get_v));
+    const uint32_t gone = next;
+    next = bring(i + 1);
     const int key = keys.key(i);
-    // nothing for this wave: its rows end before the step, or the window hides it from all of them
-    if (key > pb || (key + KT - 1 <= low && key >= a.sinks)) continue;
-    uint32_t gone = 0;  // 16-key groups in no page
-#pragma unroll
-    for (int g = 0; g < KT / 16; ++g) {
-      const int k = key + 16 * g;
-      if (k <= keys.last && (unsigned)row[k >> c.shift] >= (unsigned)c.pages) gone |= 1u << g;
-    }
-    gone = (uint32_t)pg_uniform((int)gone);
+    // nothing for a wave whose rows end before the step, or from all of which the window hides it
+    if (!(key > pb || (key + KT - 1 <= low && key >= a.sinks))) {
     const bool edge = key + KT - 1 > min(pa, keys.last) || (key <= none && key + KT > a.sinks) || gone;
 
+    // operands are read a group ahead of the products that take them, held in place by the scheduling barriers
     float s[2][16];
+    u16x8 kop[2][KS];
+    auto read_k = [&](int g) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        kop[g & 1][k] = ld16(reinterpret_cast<const uint16_t*>(lds + (get_k ^ (64 * k)) + 16 * g * RB));
+    };
+    read_k(0);
 #pragma unroll
     for (int g = 0; g < KT / 16; ++g) {
-      u16x8 kop[KS];
+      if (g + 1 < KT / 16) read_k(g + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int k = 0; k < KS; ++k) kop[k] = ld16(&lk[st][(16 * g + li) * D + ((4 * k + lg) ^ wide_kx<D>(li)) * 8]);
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 2; ++t) x[t] = mfma16x16x32<DT>(kop[g & 1][k], qop[t][k], x[t]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) x = mfma16x16x32<DT>(kop[k], qop[t][k], x);
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[t][4 * g + r] = x[r];
-      }
+        for (int r = 0; r < 4; ++r) s[t][4 * g + r] = x[t][r];
     }
+    // V's operands, 64 keys of 16 dims
+    pg_u2 vop[2][4];
+    auto read_v = [&](int T) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        vop[T & 1][h] = __builtin_bit_cast(
+            pg_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (__attribute__((address_space(3))) pg_s4*)(lds + (get_v ^ (32 * T)) + 16 * h * RB)));
+    };
+    read_v(0);
+    __builtin_amdgcn_sched_barrier(0);
     if (edge) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -613,31 +659,27 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
       uint32_t any = 0;
 #pragma unroll
       for (int x = 0; x < KT * D / 512; ++x) {
-        const pg_u4 v = *reinterpret_cast<const pg_u4*>(&lv[st][(x * 64 + lane) * 8]);
+        const pg_u4 v = *reinterpret_cast<const pg_u4*>(lds + (get_v & STAGE) + VB + (x * 64 + lane) * 16);
         any |= pg_wild<DT>(v[0]) | pg_wild<DT>(v[1]) | pg_wild<DT>(v[2]) | pg_wild<DT>(v[3]);
       }
       wild = __ballot(any != 0) != 0;
     }
     auto products = [&](auto tame) {
 #pragma unroll
-      for (int T = 0; T < ND; ++T)
+      for (int T = 0; T < ND; ++T) {
+        if (T + 1 < ND) read_v(T + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
-          pg_u4 v;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // the lane group's four keys, 16 dims of T: lane x brings dims 4 (x % 4) .. of key x / 4, and takes dim x
-            const int r = 4 * lg + (li >> 2), kk = 32 * u + 16 * h + r;
-            const uint16_t* vp = &lv[st][kk * D + (((2 * T + ((li >> 1) & 1)) ^ wide_vx<D>(r)) * 8) + (li & 1) * 4];
-            const pg_u2 x = __builtin_bit_cast(
-                pg_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s4*)vp));
-            v[2 * h] = tame ? pg_tame<DT>(x[0]) : x[0];
-            v[2 * h + 1] = tame ? pg_tame<DT>(x[1]) : x[1];
-          }
+          const pg_u2 x = vop[T & 1][2 * u], y = vop[T & 1][2 * u + 1];
+          const pg_u4 v = tame ? pg_u4{pg_tame<DT>(x[0]), pg_tame<DT>(x[1]), pg_tame<DT>(y[0]), pg_tame<DT>(y[1])}
+                               : pg_u4{x[0], x[1], y[0], y[1]};
 #pragma unroll
           for (int t = 0; t < 2; ++t)
             acc[t][T] = mfma16x16x32<DT>(__builtin_bit_cast(u16x8, v), __builtin_bit_cast(u16x8, pop[t][u]), acc[t][T]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     if (!wild) {
       products(std::false_type{});
@@ -647,7 +689,8 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
         if (key + k > keys.last || (gone >> (k >> 4) & 1u)) continue;
 #pragma unroll
         for (int T = 0; T < ND; ++T) {
-          const uint16_t* vp = &lv[st][k * D + ((2 * T + (lg >> 1)) ^ wide_vx<D>(k & 15)) * 8 + (lg & 1) * 4];
+          const uint16_t* vp = reinterpret_cast<const uint16_t*>(
+              lds + (get_v & STAGE) + VB + k * RB + ((2 * T + (lg >> 1)) ^ wide_vx<D>(k & 15)) * 16 + (lg & 1) * 8);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float x = pg_wild_number<DT>(vp[r]);
@@ -658,6 +701,11 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
         }
       }
     }
+    }
+    store();
+    get_k ^= STAGE;
+    get_v ^= STAGE;
+    __syncthreads();
   }
 
   // lane (column, lg) holds dims 16 T + 4 lg + r
