@@ -181,6 +181,7 @@ template <int NI, bool NT> __device__ __forceinline__ PgWords<NI> pg_load(__amdg
 }
 
 constexpr int NARROW_NW = 4;
+constexpr int WIDE_LEAST = 2;  // steps a split at least
 template <int D> struct NarrowLds {
   __align__(16) float o[NARROW_NW][16][D + 4];
   float ref[NARROW_NW][16], l[NARROW_NW][16];
@@ -456,28 +457,61 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
 
 // ---------------------------------------------------------------------------------------------------------
 // Tiles of up to 128 columns and more: prompts. Bound by the matrix and vector units: each of the 4 waves owns 32 columns
-// and passes over all keys of the split; steps of 64 keys come to LDS (two in turn) and every
-// wave reads them from there, K's 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads.
-// Rows in LDS are permuted by 16-byte chunks so that neither read meets a bank twice.
+// and passes over all keys of the split in steps of 32, which come to LDS by loads that need no registers, two steps
+// ahead; every wave reads K there in 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads. A row's
+// chunks lie in LDS at their number XOR a number of the row, so that neither read meets a bank twice.
 namespace {
-constexpr int WIDE_KT = 64;
+constexpr int WIDE_KT = 32;
+// A weight's exponent is counted from a reference that the scores of a column pass by less than WIDE_SLACK: renewing it
+// whenever a maximum grows would mean scaling the outputs in most turns of a wave's 32 columns. Weights stand at 2^wide_up
+// of their size, as in the narrow kernel.
+constexpr float WIDE_SLACK = 8.f;
+template <int DT> constexpr float wide_up = pg_up<DT> - WIDE_SLACK;
+
 // chunk x of a row lies at chunk x ^ wide_kx (wide_vx) of its row in LDS
 template <int D> __device__ __forceinline__ int wide_kx(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
 template <int D> __device__ __forceinline__ int wide_vx(int key) { return D == 128 ? 2 * (key & 7) : 2 * ((key >> 1) & 3); }
 
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
+typedef float pg_f16 __attribute__((ext_vector_type(16)));
+
+// v_mfma_f32_32x32x16: A is 32 x 16, B 16 x 32; lane l holds A[l % 32][8 (l / 32) + e] and B[8 (l / 32) + e][l % 32], e = 0 ..
+// 7, and D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32], r = 0 .. 15. It takes the matrix unit 32 clocks and leaves the vector
+// unit 24 of them, where two 16 x 16 x 32 leave 16.
+template <int DT> __device__ __forceinline__ pg_f16 mfma32x32x16(const u16x8& a, const u16x8& b, pg_f16 c) {
+  if constexpr (DT == M3X_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Lane x's 16 bytes at `off` of a tile of `bytes` bytes at `base` to LDS, x * 16 bytes behind `to` (all uniform but off). The compiler
+// knows neither the load nor what it writes: the caller waits (pg_landed) and then meets the other waves before anyone
+// reads. The pauses in front are those between writes of scalar registers and a load that takes them. m0 is free: nothing
+// else in the kernels here uses it, and the compiler gives it to no variable.
+__device__ __forceinline__ void pg_to_lds(uint64_t base, uint32_t bytes, uint32_t off, uint32_t to) {
+  const pg_u4 ref = {(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, bytes, 0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(ref)
+               : "memory");
+}
+// waits until all but the wave's last N loads have arrived
+template <int N> __device__ __forceinline__ void pg_landed() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 }  // namespace
 
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a) {
-  constexpr int KT = WIDE_KT, KS = D / 32, ND = D / 16, COLS = 128, CH = D / 8, RPI = 64 / CH;  // RPI: rows a wave's load
-  constexpr int RB = 2 * D, VB = KT * RB, STAGE = 2 * VB;  // bytes of a row, of a step's K, of a stage (K, then V)
-  __shared__ __align__(16) uint8_t lds[2 * STAGE];
-  const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  constexpr int KT = WIDE_KT, KS = D / 16, ND = D / 32, COLS = 128, CH = D / 8, RPI = 64 / CH;  // RPI: rows a wave's load
+  constexpr int RB = 2 * D, SB = KT * RB, LI = 8 / RPI;  // bytes of a row and of a step's K; a wave's loads of them
+  constexpr int NK = 3, NV = 4;                          // stages: K of steps j + 1 .. j + 3, V of j - 1 .. j + 2
+  constexpr uint32_t SPARE = NV * SB;  // a stage of values without infinite and NaN ones, see below (from lv on)
+  __shared__ __align__(16) uint8_t lds[(NK + NV + 1) * SB];
+  uint8_t* const lk = lds;
+  uint8_t* const lv = lds + NK * SB;
+  const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
   const Where w = pg_where(c, a, blockIdx.x);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
   const int split = blockIdx.y;
-  const Keys<KT> keys(c, a, w, 1);
+  const Keys<KT> keys(c, a, w, WIDE_LEAST);
   if (keys.active == 0) {
     if (split == 0) pg_zero<COLS, D, 256>(a, w, threadIdx.x);
     return;
@@ -485,246 +519,284 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
   if (split >= keys.active) return;
   const int i0 = split * keys.per, i1 = min(keys.nt, i0 + keys.per);
 
-  // the wave's columns
-  const int c0 = w.block * COLS + 32 * wave;
-  u16x8 qop[2][KS];
-  int cp[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const Col col(a, w, c0 + 16 * t + li);
-    cp[t] = col.p;
-    const uint16_t* qp = a.q + (long)(w.first + (col.live ? col.j : 0)) * a.sq_b +
-                         (long)(w.kh * a.G + (col.live ? col.h : 0)) * a.sq_h;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-      qop[t][s] = __builtin_bit_cast(u16x8, __builtin_bit_cast(pg_u4, ld16(qp + 32 * s + 8 * lg)) ^ a.q_flip);
-  }
-  // the wave's rows: the first's position (keys up to it every row sees, unless the window hides them), the last's
-  const int jl = w.n - 1, ja = min((int)((uint32_t)c0 / (uint32_t)a.G), jl), jb = min((int)((uint32_t)(c0 + 31) / (uint32_t)a.G), jl);
-  const bool some = c0 < w.n * a.G;
-  const int pa = w.p0 + ja, pb = some ? w.p0 + jb : -1;
-  const int none = a.window ? pb - a.window : -1, low = a.window ? pa - a.window : -1;
-
-  // Lane x: the page of step base + x's group `wave` of 16 keys (-1: none), and which of its four groups lie in no page
+  // Lane x, for step base + x's group wave / 2 of 16 keys: where it lies in the pools, the bytes that are there, and in bits
+  // 16 and 17 which of the step's two groups lie in no page
   const int32_t* row = c.table + w.slot * c.width;
-  const int inside = (1 << c.shift) - 1;
-  int ids = -1, gaps = 0, base = 0;
-  auto fetch_ids = [&](int from) {
+  int off_lo = 0, off_hi = 0, info = 0, base = 0;
+  auto fetch = [&](int from) {
     base = from;
-    ids = -1;
-    gaps = 0;
+    info = 0;
     const int at = from + lane;
     if (at < i1) {
       const int key = keys.key(at);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2; ++g) {
         const int k = key + 16 * g;
-        const bool in = k <= keys.last;
-        const int id = in ? row[k >> c.shift] : -1;
-        if ((unsigned)id >= (unsigned)c.pages) gaps |= in ? 1 << g : 0;
-        else if (g == wave) ids = id;
-      }
-    }
-  };
-  // a step's K and V: the wave brings 16 keys of each (one page), RPI a load; then to LDS. A chunk's place is its number
-  // XOR a number of its row, so the places of a lane's other rows, key quarters and dims are its first place XOR constants
-  // (made anew where they are used: kept, they would not fit the registers), and the other stage's XOR the stage's size.
-  const int r0 = lane / CH, ch = lane % CH, rv = 4 * lg + (li >> 2);
-  const uint32_t g_at = r0 * RB + ch * 16;
-  uint32_t put_k = (16 * wave + r0) * RB + (ch ^ wide_kx<D>(r0)) * 16;
-  uint32_t put_v = VB + (16 * wave + r0) * RB + (ch ^ wide_vx<D>(r0)) * 16;
-  uint32_t get_k = li * RB + (lg ^ wide_kx<D>(li)) * 16;
-  // the lane group's four keys, 16 dims: lane x brings dims 4 (x % 4) .. of key x / 4, and takes dim x of the four
-  uint32_t get_v = VB + rv * RB + (((li >> 1) & 1) ^ wide_vx<D>(rv)) * 16 + (li & 1) * 8;
-  PgWords<4> kb[16 / RPI], vb[16 / RPI];
-  auto bring = [&](int i) {
-    if (i - base == 64) fetch_ids(i);
-    const int k0 = keys.key(i) + 16 * wave, x = (i - base) & 63;
-    const int id = __builtin_amdgcn_readlane(ids, x);
-    const uint32_t g = (uint32_t)__builtin_amdgcn_readlane(gaps, x);
-    const int bytes = pg_uniform(id < 0 ? 0 : min(16, max(0, keys.last + 1 - k0)) * (2 * D));
-    const long off = pg_uniform(max(id, 0) * c.page_stride + (((long)w.kh << c.shift) + (k0 & inside)) * D);
-    const auto kr = pg_ref_of(c.k + off, bytes), vr = pg_ref_of(c.v + off, bytes);
-#pragma unroll
-    for (int x = 0; x < 16 / RPI; ++x) kb[x] = pg_load<4, false>(kr, g_at + x * RPI * RB);
-#pragma unroll
-    for (int x = 0; x < 16 / RPI; ++x) vb[x] = pg_load<4, false>(vr, g_at + x * RPI * RB);
-    return g;
-  };
-  auto store = [&]() {
-#pragma unroll
-    for (int x = 0; x < 16 / RPI; ++x) {
-      *reinterpret_cast<PgWords<4>*>(lds + (put_k ^ (64 * x)) + x * RPI * RB) = kb[x];
-      *reinterpret_cast<PgWords<4>*>(lds + (put_v ^ (D == 128 ? 128 * (x & 1) : 0)) + x * RPI * RB) = vb[x];
-    }
-    put_k ^= STAGE;
-    put_v ^= STAGE;
-  };
-
-  float m[2], l[2];
-  f32x4_t acc[2][ND];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    m[t] = -3.402823466e38f;
-    l[t] = 0.f;
-#pragma unroll
-    for (int T = 0; T < ND; ++T) acc[t][T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  fetch_ids(i0);
-  uint32_t next = bring(i0);
-  store();
-  __syncthreads();
-  for (int i = i0; i < i1; ++i) {
-    asm("" : "+v"(put_k), "+v"(put_v), "+v"(get_k), "+v"(get_v));
-    const uint32_t gone = next;
-    next = bring(i + 1);
-    const int key = keys.key(i);
-    // nothing for a wave whose rows end before the step, or from all of which the window hides it
-    if (!(key > pb || (key + KT - 1 <= low && key >= a.sinks))) {
-    const bool edge = key + KT - 1 > min(pa, keys.last) || (key <= none && key + KT > a.sinks) || gone;
-
-    // operands are read a group ahead of the products that take them, held in place by the scheduling barriers
-    float s[2][16];
-    u16x8 kop[2][KS];
-    auto read_k = [&](int g) {
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        kop[g & 1][k] = ld16(reinterpret_cast<const uint16_t*>(lds + (get_k ^ (64 * k)) + 16 * g * RB));
-    };
-    read_k(0);
-#pragma unroll
-    for (int g = 0; g < KT / 16; ++g) {
-      if (g + 1 < KT / 16) read_k(g + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) x[t] = mfma16x16x32<DT>(kop[g & 1][k], qop[t][k], x[t]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[t][4 * g + r] = x[t][r];
-    }
-    // V's operands, 64 keys of 16 dims
-    pg_u2 vop[2][4];
-    auto read_v = [&](int T) {
-#pragma unroll
-      for (int h = 0; h < 4; ++h)
-        vop[T & 1][h] = __builtin_bit_cast(
-            pg_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                       (__attribute__((address_space(3))) pg_s4*)(lds + (get_v ^ (32 * T)) + 16 * h * RB)));
-    };
-    read_v(0);
-    __builtin_amdgcn_sched_barrier(0);
-    if (edge) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int p = min(cp[t], keys.last), lw = pg_low(a, cp[t]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = key + 16 * (e >> 2) + 4 * lg + (e & 3);
-          if (pg_hidden(k, p, lw, a.sinks) || (gone >> (e >> 2) & 1u)) s[t][e] = -INFINITY;
+        if (k > keys.last) continue;
+        const int id = row[k >> c.shift];
+        if ((unsigned)id >= (unsigned)c.pages) {
+          info |= 0x10000 << g;
+        } else if (g == wave >> 1) {
+          const long off = 2 * (id * c.page_stride + (((long)w.kh << c.shift) + (k & ((1 << c.shift) - 1))) * D);
+          off_lo = (int)off;
+          off_hi = (int)(off >> 32);
+          info |= min(16, keys.last + 1 - k) * RB;
         }
       }
     }
-    pg_u4 pop[2][2];
+  };
+  // The wave brings 8 rows of a step's K and V. A load writes LDS in the lanes' order: the lanes' addresses do the XOR.
+  uint32_t from_k[LI], from_v[LI];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float mx = s[t][0];
+  for (int x = 0; x < LI; ++x) {
+    const int r = 8 * (wave & 1) + x * RPI + lane / CH;  // of the 16-key group
+    from_k[x] = r * RB + ((lane % CH) ^ wide_kx<D>(r)) * 16;
+    from_v[x] = r * RB + ((lane % CH) ^ wide_vx<D>(r)) * 16;
+  }
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const uint32_t to = pg_uniform((int)(lds_at + 8 * wave * RB));
+  uint32_t sk = 0, sv = NK * SB;  // the stages that the next K and V go to
+  uint64_t v_from = 0;            // V of the step whose K came last
+  uint32_t v_bytes = 0;
+  auto bring_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
-      mx = fmaxf(m[t], xor32_max(xor16_max(mx)));
-      if (__ballot(mx > m[t])) {
-        const float f = __builtin_amdgcn_exp2f(pg_ref(m[t], a.c) - pg_ref(mx, a.c));
-        l[t] *= f;
+    for (int x = 0; x < LI; ++x) pg_to_lds(v_from, v_bytes, from_v[x], to + sv + x * RPI * RB);
+    sv = sv == (NK + NV - 1) * SB ? NK * SB : sv + SB;
+  };
+  auto bring_k = [&](int i) __attribute__((always_inline)) {  // returns which groups lie in no page
+    const int x = i - base;
+    const uint64_t off = (uint32_t)__builtin_amdgcn_readlane(off_lo, x) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, x) << 32;
+    const uint32_t y = (uint32_t)__builtin_amdgcn_readlane(info, x);
+    v_from = (uint64_t)c.v + off;
+    v_bytes = y & 0xFFFFu;
 #pragma unroll
-        for (int T = 0; T < ND; ++T) acc[t][T] *= f;
-        m[t] = mx;
-      }
-      const float sub = pg_up<DT> - pg_ref(m[t], a.c);
+    for (int x = 0; x < LI; ++x) pg_to_lds((uint64_t)c.k + off, v_bytes, from_k[x], to + sk + x * RPI * RB);
+    sk = sk == (NK - 1) * SB ? 0 : sk + SB;
+    return y >> 16;
+  };
+
+  // the wave's columns
+  const int c0 = w.block * COLS + 32 * wave;
+  const Col col(a, w, c0 + li);
+  const int cp = col.p;
+  const uint16_t* qp = a.q + (long)(w.first + (col.live ? col.j : 0)) * a.sq_b + (long)(w.kh * a.G + (col.live ? col.h : 0)) * a.sq_h;
+  u16x8 qop[KS];
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const uint32_t x = pg_pack<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], a.c, sub)),
-                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1], a.c, sub)));
-        pop[t][e / 8][e % 8 / 2] = x;
-        l[t] = pg_add2<DT>(x, l[t]);
-      }
+  for (int s = 0; s < KS; ++s)
+    qop[s] = __builtin_bit_cast(u16x8, __builtin_bit_cast(pg_u4, ld16(qp + 16 * s + 8 * lh)) ^ a.q_flip);
+  // the wave's rows: the first's position (keys up to it every row sees, unless the window hides them), the last's
+  const int jl = w.n - 1, ja = min((int)((uint32_t)c0 / (uint32_t)a.G), jl), jb = min((int)((uint32_t)(c0 + 31) / (uint32_t)a.G), jl);
+  const int pa = min(pg_uniform(w.p0 + ja), keys.last), pb = min(pg_uniform(c0 < w.n * a.G ? w.p0 + jb : -1), keys.last);
+  const int none = a.window ? pg_uniform(w.p0 + jb) - a.window : -1;
+  // the wave's steps: those up to its last row's key (pb lies at or behind the window's begin)
+  const int steps = pb < 0 ? 0 : max(0, min(i1 - i0, pb / KT - keys.skip - i0 + 1));
+  // the turns whose step some row sees only a part of: from edge on, and from cut on up to uncut
+  const int edge = min(steps, max(0, (pa + 1) / KT - keys.skip - i0));
+  const int cut = a.sinks / KT - i0, uncut = none < 0 ? cut : none / KT + 1 - keys.skip - i0;
+
+  const uint32_t get_k = li * RB + (lh ^ wide_kx<D>(li)) * 16;
+  // Sixteen lanes, four keys, 16 dims: lane x brings dims 4 (x % 4) .. of key x / 4, and takes dim x of the four. The lower
+  // 32 lanes take keys 0 .. 3 (and 8 .. 11) of 16, the upper ones 4 .. 7 (and 12 .. 15), as their weights are.
+  const int rv = 4 * lh + (lane >> 2 & 3);
+  const uint32_t get_v = rv * RB + ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ wide_vx<D>(rv)) * 16 + (lane & 1) * 8;
+
+  float add = wide_up<DT> - pg_ref(-3.402823466e38f, a.c), l = 0.f;  // wide_up less the column's reference, its sum
+  pg_f16 acc[ND];
+#pragma unroll
+  for (int T = 0; T < ND; ++T)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[T][e] = 0.f;
+
+  // The wave's work on step j stands in three turns: its scores are made in j - 1's, its weights in its own, its outputs in
+  // j + 1's, so that in each turn the matrix unit has one step's keys and another's values to work on while the vector unit
+  // makes a third one's weights: all in one block of code, which what is rare only prepares or corrects. A product and
+  // half of a pair of weights (two multiply-adds, two exponentials, packing, sum: 32 clocks) are a slot of that block, and the
+  // slots stay in order.
+  bool wild = false;                               // step j - 1 has values that stand apart
+  int old_key = 0;                                 // its first key
+  uint32_t old_gap = 0;
+  u16x8 kop[KS];
+  auto read_k = [&](uint32_t gk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) kop[k] = ld16(reinterpret_cast<const uint16_t*>(lk + (gk ^ (32 * k))));
+  };
+  pg_u2 vop[2 * ND][2];  // of 32 dims, 16 keys
+  auto read_v = [&](int n, uint32_t gv) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      vop[n][q] = __builtin_bit_cast(
+          pg_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s4*)(
+                     lv + (gv ^ (64 * (n / 2))) + (16 * (n % 2) + 8 * q) * RB)));
+  };
+  auto output = [&](int n, const pg_u4 (&pop)[2]) __attribute__((always_inline)) {
+    const pg_u4 v = {vop[n][0][0], vop[n][0][1], vop[n][1][0], vop[n][1][1]};
+    acc[n / 2] = mfma32x32x16<DT>(__builtin_bit_cast(u16x8, v), __builtin_bit_cast(u16x8, pop[n % 2]), acc[n / 2]);
+  };
+  float ex[2];
+  auto half_weight = [&](int n, const pg_f16& s, pg_u4 (&pop)[2]) __attribute__((always_inline)) {
+    const int e = n / 2;
+    if (n % 2 == 0) {
+      ex[0] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], a.c, add));
+      ex[1] = __builtin_fmaf(s[2 * e + 1], a.c, add);
+      asm volatile("" : "+v"(ex[0]), "+v"(ex[1]));  // made in this slot, not where it is taken
+    } else {
+      uint32_t x = pg_pack<DT>(ex[0], __builtin_amdgcn_exp2f(ex[1]));
+      l = pg_add2<DT>(x, l);
+      asm volatile("" : "+v"(x), "+v"(l));
+      pop[e / 4][e % 4] = x;
     }
-    // as in the narrow kernel: infinite and NaN values stand apart where some row does not see their key
-    bool wild = false;
-    if (edge) {
+  };
+  // Turn j over the keys from `key` on; ks: stage of the next step's keys; vs, vn: of the values of the step before and of
+  // its own; s: the step's scores, next: the next one's; pop: the weights of the one before, made: its own. A wave's last turn, j == steps, sees no key and only makes the
+  // outputs of the one before.
+  auto turn = [&](int j, int key, uint32_t ks, uint32_t vs, uint32_t vn, uint32_t gap, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
+    if (j > steps) return;
+    read_k(get_k + ks);  // first: what follows covers their way
+    __builtin_amdgcn_sched_barrier(0);
+    const bool was_wild = wild;
+    wild = false;
+    if (j >= edge || (j >= cut && j < uncut) || gap) {
+      const int p = min(cp, j == steps ? -1 : keys.last), lw = pg_low(a, cp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = key + 8 * (e >> 2) + 4 * lh + (e & 3);
+        if (pg_hidden(k, p, lw, a.sinks) || (gap >> (e >> 3) & 1u)) s[e] = -INFINITY;
+      }
       uint32_t any = 0;
 #pragma unroll
-      for (int x = 0; x < KT * D / 512; ++x) {
-        const pg_u4 v = *reinterpret_cast<const pg_u4*>(lds + (get_v & STAGE) + VB + (x * 64 + lane) * 16);
+      for (int x = 0; x < SB / 1024; ++x) {
+        const pg_u4 v = *reinterpret_cast<const pg_u4*>(lv + vn + (x * 64 + lane) * 16);
         any |= pg_wild<DT>(v[0]) | pg_wild<DT>(v[1]) | pg_wild<DT>(v[2]) | pg_wild<DT>(v[3]);
       }
       wild = __ballot(any != 0) != 0;
     }
-    auto products = [&](auto tame) {
+    // Infinite and NaN values of a step that not all rows see stand apart: 0 in the product, whose values the wave then
+    // takes from the spare stage (every wave that does so in this turn writes the same there), and added below to the
+    // columns that see them, as in the narrow kernel. The first turn's outputs are made of weights and values of 0.
+    if (was_wild || j == 0) {
 #pragma unroll
-      for (int T = 0; T < ND; ++T) {
-        if (T + 1 < ND) read_v(T + 1);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int x = 0; x < SB / 1024; ++x) {
+        pg_u4 v = *reinterpret_cast<const pg_u4*>(lv + vs + (x * 64 + lane) * 16);
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) {
-          const pg_u2 x = vop[T & 1][2 * u], y = vop[T & 1][2 * u + 1];
-          const pg_u4 v = tame ? pg_u4{pg_tame<DT>(x[0]), pg_tame<DT>(x[1]), pg_tame<DT>(y[0]), pg_tame<DT>(y[1])}
-                               : pg_u4{x[0], x[1], y[0], y[1]};
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            acc[t][T] = mfma16x16x32<DT>(__builtin_bit_cast(u16x8, v), __builtin_bit_cast(u16x8, pop[t][u]), acc[t][T]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 4; ++e) v[e] = j ? pg_tame<DT>(v[e]) : 0u;
+        *reinterpret_cast<pg_u4*>(lv + SPARE + (x * 64 + lane) * 16) = v;
       }
-    };
-    if (!wild) {
-      products(std::false_type{});
-    } else {
-      products(std::true_type{});
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    // A reference is renewed once a score passes it by WIDE_SLACK: the column's sum so far goes by the new one, and behind
+    // this turn its outputs
+    constexpr float most = wide_up<DT> + WIDE_SLACK;
+    const bool grew = __ballot(__builtin_fmaf(mx, a.c, add) > most) != 0;
+    float f = 1.f;
+    if (grew) {
+      const float x = fminf(add, wide_up<DT> - pg_ref(xor32_max(mx), a.c));
+      f = __builtin_amdgcn_exp2f(x - add);
+      l *= f;
+      add = x;
+    }
+    const uint32_t gv = get_v + (was_wild || j == 0 ? SPARE : vs);
+    constexpr int SLOTS = KS + 2 * ND, LEAD = 4;  // LEAD: slots that a value's read is ahead of its product
+#pragma unroll
+    for (int e = 0; e < 16; ++e) next[e] = 0.f;
+#pragma unroll
+    for (int n = 0; n < LEAD - KS; ++n) read_v(n, gv);
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      if (i + LEAD >= KS && i + LEAD < SLOTS) read_v(i + LEAD - KS, gv);
+      if (i < KS) next = mfma32x32x16<DT>(kop[i], qop[i], next);
+      else output(i - KS, pop);
+#pragma unroll
+      for (int h = 0; h < 16 / SLOTS; ++h) half_weight(i * (16 / SLOTS) + h, s, made);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (was_wild) {
       for (int k = 0; k < KT; ++k) {
-        if (key + k > keys.last || (gone >> (k >> 4) & 1u)) continue;
+        if (old_key + k > keys.last || (old_gap >> (k >> 4) & 1u)) continue;
+        if (pg_hidden(old_key + k, min(cp, keys.last), pg_low(a, cp), a.sinks)) continue;
 #pragma unroll
-        for (int T = 0; T < ND; ++T) {
-          const uint16_t* vp = reinterpret_cast<const uint16_t*>(
-              lds + (get_v & STAGE) + VB + k * RB + ((2 * T + (lg >> 1)) ^ wide_vx<D>(k & 15)) * 16 + (lg & 1) * 8);
+        for (int n = 0; n < 4 * ND; ++n) {
+          const pg_u2 x = *reinterpret_cast<const pg_u2*>(lv + vs + k * RB + (n ^ wide_vx<D>(k & 15)) * 16 + lh * 8);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = pg_wild_number<DT>(vp[r]);
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-              if (!pg_hidden(key + k, min(cp[t], keys.last), pg_low(a, cp[t]), a.sinks)) acc[t][T][r] += x;
-          }
+          for (int r = 0; r < 4; ++r) acc[n / 4][4 * (n % 4) + r] += pg_wild_number<DT>((uint16_t)(x[r / 2] >> (16 * (r & 1))));
         }
       }
     }
+    if (grew) {
+#pragma unroll
+      for (int T = 0; T < ND; ++T) acc[T] *= f;
     }
-    store();
-    get_k ^= STAGE;
-    get_v ^= STAGE;
-    __syncthreads();
-  }
+    old_key = key;
+    old_gap = gap;
+  };
 
-  // lane (column, lg) holds dims 16 T + 4 lg + r
+  fetch(i0);
+  // the queries came before the pages' numbers: taken here, or the compiler waits for them behind the loads it does not know
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float L = xor32_sum(xor16_sum(l[t]));
-    const int col = c0 + 16 * t + li;
-    const Col cc(a, w, col);
-    if (!cc.live) continue;
-    if (keys.active == 1) {
-      uint16_t* op = a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + 4 * lg;
+  for (int k = 0; k < KS; ++k) {
+    pg_u4 x = __builtin_bit_cast(pg_u4, qop[k]);
+    asm volatile("" : "+v"(x));
+    qop[k] = __builtin_bit_cast(u16x8, x);
+  }
+  uint32_t gap0 = bring_k(i0);
+  bring_v();
+  uint32_t gap1 = bring_k(i0 + 1);
+  bring_v();
+  uint32_t gap2 = bring_k(i0 + 2);
+  pg_landed<4 * LI>();
+  __syncthreads();
+  pg_f16 s0, s1;
+  pg_u4 p0[2] = {pg_u4{0, 0, 0, 0}, pg_u4{0, 0, 0, 0}}, p1[2];
+  read_k(get_k);
 #pragma unroll
-      for (int T = 0; T < ND; ++T) pg_store4<DT>(op + 16 * T, acc[t][T], L);
-    } else {
-      const long ncols = (long)gridDim.x * COLS, at = ((long)blockIdx.x * COLS + 32 * wave + 16 * t + li) * a.splits + split;
+  for (int e = 0; e < 16; ++e) s0[e] = 0.f;
 #pragma unroll
-      for (int T = 0; T < ND; ++T) *reinterpret_cast<f32x4_t*>(a.part + at * D + 16 * T + 4 * lg) = acc[t][T];
-      if (lg == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(pg_ref(m[t], a.c), L);
+  for (int k = 0; k < KS; ++k) s0 = mfma32x32x16<DT>(kop[k], qop[k], s0);
+  uint32_t ks = SB, vs = (NV - 1) * SB, vn = 0;  // stages of K of step j + 1, V of j - 1, V of j
+  const int n = i1 - i0;
+  auto round = [&](int j, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
+    pg_landed<2 * LI>();  // K of step j + 1 and V of step j (behind them: V of j + 1, K of j + 2)
+    __syncthreads();  // for everyone; and everyone is done with K of step j and V of j - 2
+    const uint32_t gap = gap0;
+    gap0 = gap1;
+    gap1 = gap2;
+    bring_v();
+    gap2 = bring_k(i0 + j + 3);
+    turn(j, keys.key(i0 + j), ks, vs, vn, gap, s, next, pop, made);
+    ks = ks == (NK - 1) * SB ? 0 : ks + SB;
+    vs = vn;
+    vn = vn == (NV - 1) * SB ? 0 : vn + SB;
+  };
+  // two rounds at a time, which hand each other scores and weights
+  for (int j = 0; j <= n; j += 2) {
+    if (i0 + j + 4 - base >= 64) fetch(i0 + j + 3);
+    round(j, s0, s1, p0, p1);
+    if (j < n) round(j + 1, s1, s0, p1, p0);
+  }
+  pg_landed<0>();
+
+  // lane (column, lh) holds dims 8 n + 4 lh + r
+  const float L = xor32_sum(l);
+  if (!col.live) return;
+  if (keys.active == 1) {
+    uint16_t* op = a.out + (long)(w.first + col.j) * a.so_b + (long)(w.kh * a.G + col.h) * a.so_h + 4 * lh;
+#pragma unroll
+    for (int n = 0; n < 4 * ND; ++n) {
+      const pg_f16& x = acc[n / 4];
+      pg_store4<DT>(op + 8 * n, f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]}, L);
     }
+  } else {
+    const long ncols = (long)gridDim.x * COLS, at = ((long)blockIdx.x * COLS + 32 * wave + li) * a.splits + split;
+#pragma unroll
+    for (int n = 0; n < 4 * ND; ++n) {
+      const pg_f16& x = acc[n / 4];
+      *reinterpret_cast<f32x4_t*>(a.part + at * D + 8 * n + 4 * lh) =
+          f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
+    }
+    if (lh == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(wide_up<DT> - add, L);
   }
 }
 
@@ -767,7 +839,7 @@ template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, i
   else hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, false>), grid, dim3(256), 0, st, c, a);
   if (a.splits == 1) return;
   const dim3 jg(items * (cols / (1024 / D)));
-  if (cols == 128) hipLaunchKernelGGL((paged_join_kernel<DT, D, WIDE_KT, 1>), jg, dim3(256), 0, st, c, a, cols);
+  if (cols == 128) hipLaunchKernelGGL((paged_join_kernel<DT, D, WIDE_KT, WIDE_LEAST>), jg, dim3(256), 0, st, c, a, cols);
   else hipLaunchKernelGGL((paged_join_kernel<DT, D, 32, NARROW_NW>), jg, dim3(256), 0, st, c, a, cols);
 }
 // workgroups a split: tiles x kv heads x blocks of the columns; 0: out of range
