@@ -456,8 +456,9 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Tiles of up to 128 columns and more: prompts. Bound by the matrix and vector units: each of the 4 waves owns 32 columns
-// and passes over all keys of the split in steps of 32, which come to LDS by loads that need no registers, two steps
+// Tiles of up to 128 columns and more: prompts. Bound by the matrix and vector units: each of 4 waves owns 32 columns and
+// passes over the keys of the split (of its half: where the call has few workgroups, KG = 2 groups of 4 waves share the
+// keys) in steps of 32, which come to LDS by loads that need no registers, two steps
 // ahead; every wave reads K there in 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads. A row's
 // chunks lie in LDS at their number XOR a number of the row, so that neither read meets a bank twice.
 namespace {
@@ -498,26 +499,30 @@ __device__ __forceinline__ void pg_to_lds(uint64_t base, uint32_t bytes, uint32_
 template <int N> __device__ __forceinline__ void pg_landed() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 }  // namespace
 
-template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a) {
+template <int DT, int D, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedAttn a) {
   constexpr int KT = WIDE_KT, KS = D / 16, ND = D / 32, COLS = 128, CH = D / 8, RPI = 64 / CH;  // RPI: rows a wave's load
   constexpr int RB = 2 * D, SB = KT * RB, LI = 8 / RPI;  // bytes of a row and of a step's K; a wave's loads of them
   constexpr int NK = 3, NV = 4;                          // stages: K of steps j + 1 .. j + 3, V of j - 1 .. j + 2
   constexpr uint32_t SPARE = NV * SB;  // a stage of values without infinite and NaN ones, see below (from lv on)
-  __shared__ __align__(16) uint8_t lds[(NK + NV + 1) * SB];
-  uint8_t* const lk = lds;
-  uint8_t* const lv = lds + NK * SB;
-  const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
+  constexpr int LDS = (NK + NV + 1) * SB;      // a key group's
+  __shared__ __align__(16) uint8_t lds[KG * LDS];
+  const int group = KG == 1 ? 0 : pg_uniform((int)(threadIdx.x >> 8)), wave = pg_uniform((int)(threadIdx.x >> 6 & 3));
+  uint8_t* const lk = lds + group * LDS;
+  uint8_t* const lv = lk + NK * SB;
+  const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
   const Where w = pg_where(c, a, blockIdx.x);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
   const int split = blockIdx.y;
   const Keys<KT> keys(c, a, w, WIDE_LEAST);
   if (keys.active == 0) {
-    if (split == 0) pg_zero<COLS, D, 256>(a, w, threadIdx.x);
+    if (split == 0) pg_zero<COLS, D, 256 * KG>(a, w, threadIdx.x);
     return;
   }
   if (split >= keys.active) return;
-  const int i0 = split * keys.per, i1 = min(keys.nt, i0 + keys.per);
+  // the split's steps, divided among the key groups; n: the most that one has
+  const int from = split * keys.per, till = min(keys.nt, from + keys.per);
+  const int n = (till - from + KG - 1) / KG, i0 = min(till, from + group * n), i1 = min(till, i0 + n);
 
   // Lane x, for step base + x's group wave / 2 of 16 keys: where it lies in the pools, the bytes that are there, and in bits
   // 16 and 17 which of the step's two groups lie in no page
@@ -554,7 +559,7 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
     from_v[x] = r * RB + ((lane % CH) ^ wide_vx<D>(r)) * 16;
   }
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  const uint32_t to = pg_uniform((int)(lds_at + 8 * wave * RB));
+  const uint32_t to = pg_uniform((int)(lds_at + group * LDS + 8 * wave * RB));
   uint32_t sk = 0, sv = NK * SB;  // the stages that the next K and V go to
   uint64_t v_from = 0;            // V of the step whose K came last
   uint32_t v_bytes = 0;
@@ -756,7 +761,6 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
 #pragma unroll
   for (int k = 0; k < KS; ++k) s0 = mfma32x32x16<DT>(kop[k], qop[k], s0);
   uint32_t ks = SB, vs = (NV - 1) * SB, vn = 0;  // stages of K of step j + 1, V of j - 1, V of j
-  const int n = i1 - i0;
   auto round = [&](int j, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
     pg_landed<2 * LI>();  // K of step j + 1 and V of step j (behind them: V of j + 1, K of j + 2)
     __syncthreads();  // for everyone; and everyone is done with K of step j and V of j - 2
@@ -778,6 +782,31 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(Paged c, PagedAttn a
   }
   pg_landed<0>();
 
+  if constexpr (KG == 2) {  // the second group's sums by way of LDS to the first
+    __syncthreads();
+    f32x4_t* const at = reinterpret_cast<f32x4_t*>(lds) + wave * (4 * ND * 64) + lane;
+    float2* const ml = reinterpret_cast<float2*>(lds + 4 * (4 * ND * 64) * 16) + wave * 64 + lane;
+    if (group) {
+#pragma unroll
+      for (int n = 0; n < 4 * ND; ++n) {
+        const pg_f16& x = acc[n / 4];
+        at[64 * n] = f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
+      }
+      *ml = make_float2(add, l);
+    }
+    __syncthreads();
+    if (group) return;
+    const float2 o = *ml;
+    const float x = fminf(add, o.x), f0 = __builtin_amdgcn_exp2f(x - add), f1 = __builtin_amdgcn_exp2f(x - o.x);
+    add = x;
+    l = l * f0 + o.y * f1;
+#pragma unroll
+    for (int n = 0; n < 4 * ND; ++n) {
+      const f32x4_t y = at[64 * n];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[n / 4][n % 4 * 4 + r] = acc[n / 4][n % 4 * 4 + r] * f0 + y[r] * f1;
+    }
+  }
   // lane (column, lh) holds dims 8 n + 4 lh + r
   const float L = xor32_sum(l);
   if (!col.live) return;
@@ -833,7 +862,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, PagedAttn a, i
 namespace {
 template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, int items, int cols, bool single, hipStream_t st) {
   const dim3 grid(items, a.splits);
-  if (cols == 128) hipLaunchKernelGGL((paged_wide_kernel<DT, D>), grid, dim3(256), 0, st, c, a);
+  if (cols == 128) {
+    // Up to a workgroup a CU, two groups of waves share its keys
+    if ((long)items * a.splits <= 256) hipLaunchKernelGGL((paged_wide_kernel<DT, D, 2>), grid, dim3(512), 0, st, c, a);
+    else hipLaunchKernelGGL((paged_wide_kernel<DT, D, 1>), grid, dim3(256), 0, st, c, a);
+  }
   else if (cols == 32) hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 2, false>), grid, dim3(256), 0, st, c, a);
   else if (single) hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, true>), grid, dim3(256), 0, st, c, a);
   else hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, false>), grid, dim3(256), 0, st, c, a);
