@@ -37,6 +37,7 @@ struct PagedAttn {
   float c;               // |scale| log2(e), not 0
   uint32_t q_flip;       // the sign bits of two query elements where scale < 0
   int rows, heads, G, tile_rows, blocks, window, sinks, splits;
+  uint32_t over_G;  // ceil(2^32 / G): x / G = x * over_G >> 32 for x, G < 2^16 (0 for G = 1)
   float* part;  // [columns][splits][D], then [columns][splits][2]: (reference, sum)
 };
 
@@ -55,17 +56,21 @@ __device__ __forceinline__ int pg_uniform(int x) {
 __device__ __forceinline__ long pg_uniform(long x) {
   return (long)((uint64_t)(uint32_t)pg_uniform((int)x) | (uint64_t)(uint32_t)pg_uniform((int)(x >> 32)) << 32);
 }
-__device__ __forceinline__ Where pg_where(const Paged& c, const PagedAttn& a, uint32_t item) {
+// x: kv head + kv_heads * block, y: tile (z: split)
+__device__ __forceinline__ Where pg_where(const Paged& c, const PagedAttn& a, int x, int tile) {
   Where w;
-  const uint32_t th = item / (uint32_t)a.blocks;
-  w.block = pg_uniform((int)(item - th * a.blocks));
-  w.tile = pg_uniform((int)(th / (uint32_t)c.kv_heads));
-  w.kh = pg_uniform((int)(th - (uint32_t)w.tile * c.kv_heads));
-  w.first = w.tile;
+  w.tile = tile;
+  w.block = 0;
+  w.kh = x;
+  if (a.blocks > 1) {
+    w.block = pg_uniform(x / c.kv_heads);
+    w.kh = x - w.block * c.kv_heads;
+  }
+  w.first = tile;
   w.n = 1;
   if (a.tiles) {
-    w.first = pg_uniform(a.tiles[2 * w.tile]);
-    w.n = pg_uniform(a.tiles[2 * w.tile + 1]);
+    w.first = pg_uniform(a.tiles[2 * tile]);
+    w.n = pg_uniform(a.tiles[2 * tile + 1]);
   }
   w.slot = -1;
   w.p0 = -1;
@@ -77,6 +82,9 @@ __device__ __forceinline__ Where pg_where(const Paged& c, const PagedAttn& a, ui
   w.slot = pg_uniform((long)a.slots[w.first]);
   w.p0 = min(pg_uniform(a.pos[w.first]), 1 << 30);  // positions count past it in 32 bits, and the cache ends before
   return w;
+}
+__device__ __forceinline__ int pg_row(const PagedAttn& a, int col) {
+  return a.over_G ? (int)__umulhi((uint32_t)col, a.over_G) : col;
 }
 
 // a tile's keys in steps of KT positions
@@ -91,8 +99,12 @@ template <int KT> struct Keys {
     sink = a.window ? min((min(a.sinks, last + 1) + KT - 1) / KT, lo) : 0;
     skip = pg_uniform(lo - sink);  // (opaque: it also serves lanes that branch, and would be made anew there)
     nt = last < 0 ? 0 : sink + max(0, last / KT + 1 - lo);
-    per = pg_uniform(max(least, (nt + a.splits - 1) / a.splits));
-    active = pg_uniform((nt + per - 1) / per);
+    per = nt;
+    active = nt > 0;
+    if (a.splits > 1) {
+      per = pg_uniform(max(least, (nt + a.splits - 1) / a.splits));
+      active = pg_uniform((nt + per - 1) / per);
+    }
   }
   __device__ __forceinline__ int key(int i) const { return (i + (i < sink ? 0 : skip)) * KT; }
 };
@@ -102,16 +114,37 @@ struct Col {
   int j, h, p;  // row of the tile, head of the kv head's G, position
   bool live;
   __device__ __forceinline__ Col(const PagedAttn& a, const Where& w, int col) {
-    j = (int)((uint32_t)col / (uint32_t)a.G);
+    j = pg_row(a, col);
     h = col - j * a.G;
     live = j < w.n;
     p = live ? w.p0 + j : -1;
   }
 };
-// whether keys key .. of a step may be hidden from some row that another row sees, or lie outside
+// whether a row at p does not see a key; low: pg_low
 __device__ __forceinline__ bool pg_hidden(int key, int p, int low, int sinks) { return key > p || (key <= low && key >= sinks); }
 // the largest position that the window hides from a row at p (-1: none)
 __device__ __forceinline__ int pg_low(const PagedAttn& a, int p) { return a.window ? p - a.window : -1; }
+
+// Scores s[e] of the keys from + 8 (e / 4) * STEP / 8 + e % 4 that a row at p does not see become -inf: later ones, and where
+// the window cuts (uniform) those up to `low` behind the sinks. holes: bits of 16-key groups in no page.
+template <int N, int STEP, typename T>
+__device__ __forceinline__ void pg_mask(T& s, int from, int p, int low, int sinks, bool cuts, uint32_t holes) {
+  const int late = p - from;
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (STEP * (e >> 2) + (e & 3) > late) s[e] = -INFINITY;
+  if (cuts) {
+    const int early = low - from, kept = sinks - from;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (STEP * (e >> 2) + (e & 3) <= early && STEP * (e >> 2) + (e & 3) >= kept) s[e] = -INFINITY;
+  }
+  if (holes) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (holes >> (STEP * (e >> 2) >> 4) & 1u) s[e] = -INFINITY;
+  }
+}
 
 template <int DT> __device__ __forceinline__ uint32_t pg_pack(float x, float y) {
   if constexpr (DT == M3X_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((pg_f2{x, y}), pg_h2));
@@ -123,6 +156,13 @@ template <int DT> __device__ __forceinline__ float pg_add2(uint32_t w, float acc
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(pg_h2, w), __builtin_bit_cast(pg_h2, 0x3C003C00u), acc, false);
   else
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pg_bf2, w), __builtin_bit_cast(pg_bf2, 0x3F803F80u), acc, false);
+}
+// acc, or NaN where one of the two numbers of w is infinite or NaN (0 times it)
+template <int DT> __device__ __forceinline__ float pg_probe(uint32_t w, float acc) {
+  if constexpr (DT == M3X_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(pg_h2, w), __builtin_bit_cast(pg_h2, 0u), acc, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pg_bf2, w), __builtin_bit_cast(pg_bf2, 0u), acc, false);
 }
 // bits 15 and 31: which of the two numbers of w are infinite or NaN (an exponent of ones carries into the sign's place)
 template <int DT> __device__ __forceinline__ uint32_t pg_wild(uint32_t w) {
@@ -198,9 +238,9 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
   // with 16 columns of 128 dims)
   constexpr int AHEAD = D == 128 && QT == 2 ? 1 : 2;
   const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-  const Where w = pg_where(c, a, blockIdx.x);
+  const Where w = pg_where(c, a, blockIdx.x, blockIdx.y);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
-  const int split = blockIdx.y;
+  const int split = blockIdx.z;
   const Keys<KT> keys(c, a, w, NW);
   if (keys.active == 0) {
     if (split == 0) pg_zero<COLS, D, 64 * NW>(a, w, threadIdx.x);
@@ -285,7 +325,8 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
   const int all = min(w.p0, keys.last), none = a.window ? w.p0 + w.n - 1 - a.window : -1;
   auto step = [&](Buf& b, int i) {
     const int key = keys.key(i);
-    const bool edge = key + KT - 1 > all || (key <= none && key + KT > a.sinks) || b.holes;
+    const bool cuts = key <= none && key + KT > a.sinks;
+    const bool edge = key + KT - 1 > all || cuts || b.holes;
     uint32_t gone = 0;  // groups in no page
     if (b.holes) gone = (b.bytes[0] == 0 ? 1u : 0u) | (b.bytes[1] == 0 ? 2u : 0u);
     float s[QT][8];
@@ -305,14 +346,8 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
     __builtin_amdgcn_sched_barrier(0);
     if (edge) {
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const int p = min(cp[t], keys.last), low = pg_low(a, cp[t]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = key + 16 * (e >> 2) + 4 * lg + (e & 3);
-          if (pg_hidden(k, p, low, a.sinks) || (gone >> (e >> 2) & 1u)) s[t][e] = -INFINITY;
-        }
-      }
+      for (int t = 0; t < QT; ++t)
+        pg_mask<8, 16>(s[t], key + 4 * lg, min(cp[t], keys.last), pg_low(a, cp[t]), a.sinks, cuts, gone);
     }
     pg_u4 pop[QT];
 #pragma unroll
@@ -341,12 +376,12 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
     // 0 in the product and added below to the columns that see them (p V of a weight p > 0 is V for these V)
     bool wild = false;
     if (edge) {
-      uint32_t any = 0;
+      float any = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int x = 0; x < NV; ++x) any |= pg_wild<DT>(b.vw[e].w[x]);
-      wild = __ballot(any != 0) != 0;
+        for (int x = 0; x < NV; ++x) any = pg_probe<DT>(b.vw[e].w[x], any);
+      wild = __ballot(any != any) != 0;
       if (wild) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -413,7 +448,7 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
 
   // merge the waves, 16 columns at a time: lane (column, lg) holds dims 2 NV (4 lg + r) + T
   __shared__ NarrowLds<D> lds;
-  const long ncols = (long)gridDim.x * COLS;
+  const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     if (t) __syncthreads();
@@ -447,7 +482,7 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
       if (keys.active == 1) {
         pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
       } else {
-        const long at = ((long)blockIdx.x * COLS + 16 * t + col) * a.splits + split;
+        const long at = (place * COLS + 16 * t + col) * a.splits + split;
         *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = O;
         if (d == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(M, L);
       }
@@ -471,7 +506,7 @@ template <int DT> constexpr float wide_up = pg_up<DT> - WIDE_SLACK;
 
 // chunk x of a row lies at chunk x ^ wide_kx (wide_vx) of its row in LDS
 template <int D> __device__ __forceinline__ int wide_kx(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
-template <int D> __device__ __forceinline__ int wide_vx(int key) { return D == 128 ? 2 * (key & 7) : 2 * ((key >> 1) & 3); }
+template <int D> __device__ __forceinline__ int wide_vx(int key) { return D == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
 
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 typedef float pg_f16 __attribute__((ext_vector_type(16)));
@@ -486,14 +521,16 @@ template <int DT> __device__ __forceinline__ pg_f16 mfma32x32x16(const u16x8& a,
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Lane x's 16 bytes at `off` of a tile of `bytes` bytes at `base` to LDS, x * 16 bytes behind `to` (all uniform but off). The compiler
-// knows neither the load nor what it writes: the caller waits (pg_landed) and then meets the other waves before anyone
-// reads. The pauses in front are those between writes of scalar registers and a load that takes them. m0 is free: nothing
-// else in the kernels here uses it, and the compiler gives it to no variable.
-__device__ __forceinline__ void pg_to_lds(uint64_t base, uint32_t bytes, uint32_t off, uint32_t to) {
+// Lane x's 16 bytes at `off` of a tile of `bytes` bytes at `base` to LDS, `by` + x * 16 bytes behind `to` (all uniform but
+// off). The compiler knows neither the load nor what it writes: the caller waits (pg_landed) and then meets the other waves
+// before anyone reads. PAUSE: idle slots between what writes the scalar registers and the load that takes them, 4 where a
+// vector instruction may have written the tile's, 0 where they stand since the load before (m0 needs one). m0 is free:
+// nothing else in the kernels here uses it, and the compiler gives it to no variable.
+template <int PAUSE> __device__ __forceinline__ void pg_to_lds(uint64_t base, uint32_t bytes, uint32_t off, uint32_t to, int by) {
   const pg_u4 ref = {(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, bytes, 0x00020000u};
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(ref)
-               : "memory");
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop %4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(ref),
+               "i"(by), "n"(PAUSE)
+               : "memory", "scc");
 }
 // waits until all but the wave's last N loads have arrived
 template <int N> __device__ __forceinline__ void pg_landed() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -503,17 +540,17 @@ template <int DT, int D, int KG>
 __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedAttn a) {
   constexpr int KT = WIDE_KT, KS = D / 16, ND = D / 32, COLS = 128, CH = D / 8, RPI = 64 / CH;  // RPI: rows a wave's load
   constexpr int RB = 2 * D, SB = KT * RB, LI = 8 / RPI;  // bytes of a row and of a step's K; a wave's loads of them
-  constexpr int NK = 3, NV = 4;                          // stages: K of steps j + 1 .. j + 3, V of j - 1 .. j + 2
-  constexpr uint32_t SPARE = NV * SB;  // a stage of values without infinite and NaN ones, see below (from lv on)
-  constexpr int LDS = (NK + NV + 1) * SB;      // a key group's
+  // rings of stages, a step's at its number % 4: in turn j K of steps j + 1 .. j + 3 and V of j - 1 .. j + 2 are there or come
+  constexpr int NK = 4, NV = 4, RING = 4 * SB;
+  constexpr int LDS = (NK + NV + 1) * SB;  // a key group's; the last stage: values without infinite and NaN ones, see below
   __shared__ __align__(16) uint8_t lds[KG * LDS];
   const int group = KG == 1 ? 0 : pg_uniform((int)(threadIdx.x >> 8)), wave = pg_uniform((int)(threadIdx.x >> 6 & 3));
   uint8_t* const lk = lds + group * LDS;
   uint8_t* const lv = lk + NK * SB;
   const int lane = threadIdx.x & 63, li = lane & 31, lh = lane >> 5;
-  const Where w = pg_where(c, a, blockIdx.x);
+  const Where w = pg_where(c, a, blockIdx.x, blockIdx.y);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
-  const int split = blockIdx.y;
+  const int split = blockIdx.z;
   const Keys<KT> keys(c, a, w, WIDE_LEAST);
   if (keys.active == 0) {
     if (split == 0) pg_zero<COLS, D, 256 * KG>(a, w, threadIdx.x);
@@ -524,13 +561,14 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   const int from = split * keys.per, till = min(keys.nt, from + keys.per);
   const int n = (till - from + KG - 1) / KG, i0 = min(till, from + group * n), i1 = min(till, i0 + n);
 
-  // Lane x, for step base + x's group wave / 2 of 16 keys: where it lies in the pools, the bytes that are there, and in bits
-  // 16 and 17 which of the step's two groups lie in no page
+  // Lane x, for step base + x's group wave / 2 of 16 keys: where it lies in the pools, the bytes that are there
   const int32_t* row = c.table + w.slot * c.width;
   int off_lo = 0, off_hi = 0, info = 0, base = 0;
+  bool holes = false;  // some group lies in no page
   auto fetch = [&](int from) {
     base = from;
     info = 0;
+    bool hole = false;
     const int at = from + lane;
     if (at < i1) {
       const int key = keys.key(at);
@@ -540,15 +578,16 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
         if (k > keys.last) continue;
         const int id = row[k >> c.shift];
         if ((unsigned)id >= (unsigned)c.pages) {
-          info |= 0x10000 << g;
+          hole = true;
         } else if (g == wave >> 1) {
           const long off = 2 * (id * c.page_stride + (((long)w.kh << c.shift) + (k & ((1 << c.shift) - 1))) * D);
           off_lo = (int)off;
           off_hi = (int)(off >> 32);
-          info |= min(16, keys.last + 1 - k) * RB;
+          info = min(16, keys.last + 1 - k) * RB;
         }
       }
     }
+    holes |= __ballot(hole) != 0;
   };
   // The wave brings 8 rows of a step's K and V. A load writes LDS in the lanes' order: the lanes' addresses do the XOR.
   uint32_t from_k[LI], from_v[LI];
@@ -560,24 +599,19 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   }
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const uint32_t to = pg_uniform((int)(lds_at + group * LDS + 8 * wave * RB));
-  uint32_t sk = 0, sv = NK * SB;  // the stages that the next K and V go to
-  uint64_t v_from = 0;            // V of the step whose K came last
+  uint64_t v_from = 0;  // V of the step whose K came last
   uint32_t v_bytes = 0;
-  auto bring_v = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < LI; ++x) pg_to_lds(v_from, v_bytes, from_v[x], to + sv + x * RPI * RB);
-    sv = sv == (NK + NV - 1) * SB ? NK * SB : sv + SB;
+  auto bring_v = [&](uint32_t stage) __attribute__((always_inline)) {
+    pg_to_lds<4>(v_from, v_bytes, from_v[0], to + stage, RING);
+    if constexpr (LI == 2) pg_to_lds<0>(v_from, v_bytes, from_v[1], to + stage, RING + RPI * RB);
   };
-  auto bring_k = [&](int i) __attribute__((always_inline)) {  // returns which groups lie in no page
+  auto bring_k = [&](int i, uint32_t stage) __attribute__((always_inline)) {
     const int x = i - base;
     const uint64_t off = (uint32_t)__builtin_amdgcn_readlane(off_lo, x) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, x) << 32;
-    const uint32_t y = (uint32_t)__builtin_amdgcn_readlane(info, x);
+    v_bytes = (uint32_t)__builtin_amdgcn_readlane(info, x);
     v_from = (uint64_t)c.v + off;
-    v_bytes = y & 0xFFFFu;
-#pragma unroll
-    for (int x = 0; x < LI; ++x) pg_to_lds((uint64_t)c.k + off, v_bytes, from_k[x], to + sk + x * RPI * RB);
-    sk = sk == (NK - 1) * SB ? 0 : sk + SB;
-    return y >> 16;
+    pg_to_lds<4>((uint64_t)c.k + off, v_bytes, from_k[0], to + stage, 0);
+    if constexpr (LI == 2) pg_to_lds<0>((uint64_t)c.k + off, v_bytes, from_k[1], to + stage, RPI * RB);
   };
 
   // the wave's columns
@@ -590,14 +624,15 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   for (int s = 0; s < KS; ++s)
     qop[s] = __builtin_bit_cast(u16x8, __builtin_bit_cast(pg_u4, ld16(qp + 16 * s + 8 * lh)) ^ a.q_flip);
   // the wave's rows: the first's position (keys up to it every row sees, unless the window hides them), the last's
-  const int jl = w.n - 1, ja = min((int)((uint32_t)c0 / (uint32_t)a.G), jl), jb = min((int)((uint32_t)(c0 + 31) / (uint32_t)a.G), jl);
+  const int jl = w.n - 1, ja = min(pg_row(a, c0), jl), jb = min(pg_row(a, c0 + 31), jl);
   const int pa = min(pg_uniform(w.p0 + ja), keys.last), pb = min(pg_uniform(c0 < w.n * a.G ? w.p0 + jb : -1), keys.last);
   const int none = a.window ? pg_uniform(w.p0 + jb) - a.window : -1;
   // the wave's steps: those up to its last row's key (pb lies at or behind the window's begin)
   const int steps = pb < 0 ? 0 : max(0, min(i1 - i0, pb / KT - keys.skip - i0 + 1));
-  // the turns whose step some row sees only a part of: from edge on, and from cut on up to uncut
+  // The turns whose step every row sees whole: from plain on up to edge. Before them the window hides something (or
+  // nothing: steps of the sinks), and turn 0 begins.
   const int edge = min(steps, max(0, (pa + 1) / KT - keys.skip - i0));
-  const int cut = a.sinks / KT - i0, uncut = none < 0 ? cut : none / KT + 1 - keys.skip - i0;
+  int plain = max(1, none < 0 ? 0 : none / KT + 1 - keys.skip - i0);
 
   const uint32_t get_k = li * RB + (lh ^ wide_kx<D>(li)) * 16;
   // Sixteen lanes, four keys, 16 dims: lane x brings dims 4 (x % 4) .. of key x / 4, and takes dim x of the four. The lower
@@ -617,9 +652,7 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   // makes a third one's weights: all in one block of code, which what is rare only prepares or corrects. A product and
   // half of a pair of weights (two multiply-adds, two exponentials, packing, sum: 32 clocks) are a slot of that block, and the
   // slots stay in order.
-  bool wild = false;                               // step j - 1 has values that stand apart
-  int old_key = 0;                                 // its first key
-  uint32_t old_gap = 0;
+  bool wild = false;  // step j - 1 has values that stand apart
   u16x8 kop[KS];
   auto read_k = [&](uint32_t gk) __attribute__((always_inline)) {
 #pragma unroll
@@ -651,43 +684,51 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       pop[e / 4][e % 4] = x;
     }
   };
-  // Turn j over the keys from `key` on; ks: stage of the next step's keys; vs, vn: of the values of the step before and of
-  // its own; s: the step's scores, next: the next one's; pop: the weights of the one before, made: its own. A wave's last turn, j == steps, sees no key and only makes the
-  // outputs of the one before.
-  auto turn = [&](int j, int key, uint32_t ks, uint32_t vs, uint32_t vn, uint32_t gap, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
+  // which of the two groups of 16 keys from `key` on lie in no page
+  auto gaps = [&](int key) {
+    uint32_t r = 0;
+    for (int g = 0; g < 2; ++g) {
+      const int k = key + 16 * g;
+      if (k <= keys.last && (unsigned)pg_uniform(row[k >> c.shift]) >= (unsigned)c.pages) r |= 1u << g;
+    }
+    return r;
+  };
+  // Turn j, vn = j % 4 stages; s: the step's scores, next: the next one's; pop: the weights of the one before, made: its
+  // own. A wave's last turn, j == steps, sees no key and only makes the outputs of the one before.
+  auto turn = [&](int j, uint32_t vn, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
     if (j > steps) return;
-    read_k(get_k + ks);  // first: what follows covers their way
+    read_k(get_k + (vn + SB & RING - 1));  // first: what follows covers their way
     __builtin_amdgcn_sched_barrier(0);
+    uint32_t vs = vn - SB & RING - 1;  // where the values of the step before lie
     const bool was_wild = wild;
-    wild = false;
-    if (j >= edge || (j >= cut && j < uncut) || gap) {
-      const int p = min(cp, j == steps ? -1 : keys.last), lw = pg_low(a, cp);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int k = key + 8 * (e >> 2) + 4 * lh + (e & 3);
-        if (pg_hidden(k, p, lw, a.sinks) || (gap >> (e >> 3) & 1u)) s[e] = -INFINITY;
-      }
-      uint32_t any = 0;
+    if (j < plain || j >= edge || holes) {
+      const int key = keys.key(i0 + j);
+      pg_mask<16, 8>(s, key + 4 * lh, min(cp, j == steps ? -1 : keys.last), pg_low(a, cp), a.sinks, a.window != 0, holes ? gaps(key) : 0u);
+      float any = 0.f;
 #pragma unroll
       for (int x = 0; x < SB / 1024; ++x) {
         const pg_u4 v = *reinterpret_cast<const pg_u4*>(lv + vn + (x * 64 + lane) * 16);
-        any |= pg_wild<DT>(v[0]) | pg_wild<DT>(v[1]) | pg_wild<DT>(v[2]) | pg_wild<DT>(v[3]);
-      }
-      wild = __ballot(any != 0) != 0;
-    }
-    // Infinite and NaN values of a step that not all rows see stand apart: 0 in the product, whose values the wave then
-    // takes from the spare stage (every wave that does so in this turn writes the same there), and added below to the
-    // columns that see them, as in the narrow kernel. The first turn's outputs are made of weights and values of 0.
-    if (was_wild || j == 0) {
 #pragma unroll
-      for (int x = 0; x < SB / 1024; ++x) {
-        pg_u4 v = *reinterpret_cast<const pg_u4*>(lv + vs + (x * 64 + lane) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = j ? pg_tame<DT>(v[e]) : 0u;
-        *reinterpret_cast<pg_u4*>(lv + SPARE + (x * 64 + lane) * 16) = v;
+        for (int e = 0; e < 4; ++e) any = pg_probe<DT>(v[e], any);
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      // Infinite and NaN values of a step that not all rows see stand apart: 0 in the product, whose values the wave then
+      // takes from the spare stage (every wave that does so in this turn writes the same there), and added below to the
+      // columns that see them, as in the narrow kernel. The first turn's outputs are made of weights and values of 0.
+      if (wild || j == 0) {
+        const uint32_t keep = j ? ~0u : 0u;
+#pragma unroll 1
+        for (int x = lane * 16; x < SB; x += 1024) {
+          pg_u4 v = *reinterpret_cast<const pg_u4*>(lv + vs + x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = pg_tame<DT>(v[e]) & keep;
+          *reinterpret_cast<pg_u4*>(lv + RING + x) = v;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        vs = RING;
+      }
+      wild = __ballot(any != any) != 0;
+      if (wild) plain = max(plain, j + 2);  // the next turn comes here too
     }
     float mx = s[0];
 #pragma unroll
@@ -696,14 +737,14 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
     // this turn its outputs
     constexpr float most = wide_up<DT> + WIDE_SLACK;
     const bool grew = __ballot(__builtin_fmaf(mx, a.c, add) > most) != 0;
-    float f = 1.f;
+    float f;
     if (grew) {
       const float x = fminf(add, wide_up<DT> - pg_ref(xor32_max(mx), a.c));
       f = __builtin_amdgcn_exp2f(x - add);
       l *= f;
       add = x;
     }
-    const uint32_t gv = get_v + (was_wild || j == 0 ? SPARE : vs);
+    const uint32_t gv = get_v + vs;
     constexpr int SLOTS = KS + 2 * ND, LEAD = 4;  // LEAD: slots that a value's read is ahead of its product
 #pragma unroll
     for (int e = 0; e < 16; ++e) next[e] = 0.f;
@@ -719,12 +760,15 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       __builtin_amdgcn_sched_barrier(0);
     }
     if (was_wild) {
+      const int key = keys.key(i0 + j - 1);
+      const uint32_t gap = holes ? gaps(key) : 0u;
       for (int k = 0; k < KT; ++k) {
-        if (old_key + k > keys.last || (old_gap >> (k >> 4) & 1u)) continue;
-        if (pg_hidden(old_key + k, min(cp, keys.last), pg_low(a, cp), a.sinks)) continue;
+        if (key + k > keys.last || (gap >> (k >> 4) & 1u)) continue;
+        if (pg_hidden(key + k, min(cp, keys.last), pg_low(a, cp), a.sinks)) continue;
 #pragma unroll
         for (int n = 0; n < 4 * ND; ++n) {
-          const pg_u2 x = *reinterpret_cast<const pg_u2*>(lv + vs + k * RB + (n ^ wide_vx<D>(k & 15)) * 16 + lh * 8);
+          const pg_u2 x = *reinterpret_cast<const pg_u2*>(lv + (vn - SB & RING - 1) + k * RB +
+                                                          (n ^ wide_vx<D>(k & 15)) * 16 + lh * 8);
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[n / 4][4 * (n % 4) + r] += pg_wild_number<DT>((uint16_t)(x[r / 2] >> (16 * (r & 1))));
         }
@@ -734,8 +778,6 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
 #pragma unroll
       for (int T = 0; T < ND; ++T) acc[T] *= f;
     }
-    old_key = key;
-    old_gap = gap;
   };
 
   fetch(i0);
@@ -746,11 +788,11 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
     asm volatile("" : "+v"(x));
     qop[k] = __builtin_bit_cast(u16x8, x);
   }
-  uint32_t gap0 = bring_k(i0);
-  bring_v();
-  uint32_t gap1 = bring_k(i0 + 1);
-  bring_v();
-  uint32_t gap2 = bring_k(i0 + 2);
+  bring_k(i0, 0);
+  bring_v(0);
+  bring_k(i0 + 1, SB);
+  bring_v(SB);
+  bring_k(i0 + 2, 2 * SB);
   pg_landed<4 * LI>();
   __syncthreads();
   pg_f16 s0, s1;
@@ -760,25 +802,29 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   for (int e = 0; e < 16; ++e) s0[e] = 0.f;
 #pragma unroll
   for (int k = 0; k < KS; ++k) s0 = mfma32x32x16<DT>(kop[k], qop[k], s0);
-  uint32_t ks = SB, vs = (NV - 1) * SB, vn = 0;  // stages of K of step j + 1, V of j - 1, V of j
-  auto round = [&](int j, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
+  auto round = [&](int j, uint32_t vn, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
     pg_landed<2 * LI>();  // K of step j + 1 and V of step j (behind them: V of j + 1, K of j + 2)
-    __syncthreads();  // for everyone; and everyone is done with K of step j and V of j - 2
-    const uint32_t gap = gap0;
-    gap0 = gap1;
-    gap1 = gap2;
-    bring_v();
-    gap2 = bring_k(i0 + j + 3);
-    turn(j, keys.key(i0 + j), ks, vs, vn, gap, s, next, pop, made);
-    ks = ks == (NK - 1) * SB ? 0 : ks + SB;
-    vs = vn;
-    vn = vn == (NV - 1) * SB ? 0 : vn + SB;
+    __syncthreads();      // for everyone; and everyone is done with K of step j and V of j - 2
+    bring_v(vn ^ 2 * SB);
+    bring_k(i0 + j + 3, vn + 3 * SB & RING - 1);
+    turn(j, vn, s, next, pop, made);
   };
-  // two rounds at a time, which hand each other scores and weights
-  for (int j = 0; j <= n; j += 2) {
-    if (i0 + j + 4 - base >= 64) fetch(i0 + j + 3);
-    round(j, s0, s1, p0, p1);
-    if (j < n) round(j + 1, s1, s0, p1, p0);
+  // Two rounds at a time, which hand each other scores and weights. A call of few workgroups is short: its time is the
+  // code's first fetch into the instruction cache, so there the round stands once and moves them.
+  if constexpr (KG == 1) {
+    for (int j = 0, vn = 0; j <= n; j += 2, vn ^= 2 * SB) {
+      if (i0 + j + 4 - base >= 64) fetch(i0 + j + 3);
+      round(j, vn, s0, s1, p0, p1);
+      if (j < n) round(j + 1, vn + SB, s1, s0, p1, p0);
+    }
+  } else {
+    for (int j = 0, vn = 0; j <= n; ++j, vn = vn + SB & RING - 1) {
+      if (i0 + j + 3 - base >= 64) fetch(i0 + j + 3);
+      round(j, vn, s0, s1, p0, p1);
+      s0 = s1;
+      p0[0] = p1[0];
+      p0[1] = p1[1];
+    }
   }
   pg_landed<0>();
 
@@ -818,7 +864,8 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       pg_store4<DT>(op + 8 * n, f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]}, L);
     }
   } else {
-    const long ncols = (long)gridDim.x * COLS, at = ((long)blockIdx.x * COLS + 32 * wave + li) * a.splits + split;
+    const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
+    const long at = (place * COLS + 32 * wave + li) * a.splits + split;
 #pragma unroll
     for (int n = 0; n < 4 * ND; ++n) {
       const pg_f16& x = acc[n / 4];
@@ -833,15 +880,16 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
 template <int DT, int D, int KT, int LEAST>
 __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, PagedAttn a, int cols) {
   constexpr int TD = D / 4, CB = 256 / TD;
-  const uint32_t per = cols / CB, item = blockIdx.x / per;
-  const Where w = pg_where(c, a, item);
+  const int per = cols / CB;  // z: which CB of the block's columns
+  const Where w = pg_where(c, a, blockIdx.x, blockIdx.y);
   if (w.n == 0) return;
   const Keys<KT> keys(c, a, w, LEAST);
   if (keys.active <= 1) return;  // written by the attention itself
-  const int col = (blockIdx.x - item * per) * CB + threadIdx.x / TD, d = threadIdx.x % TD * 4;
+  const int col = blockIdx.z * CB + threadIdx.x / TD, d = threadIdx.x % TD * 4;
   const Col cc(a, w, w.block * cols + col);
   if (!cc.live) return;
-  const long ncols = (long)(gridDim.x / per) * cols, at = ((long)item * cols + col) * a.splits;
+  const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * per * CB;
+  const long at = (place * cols + col) * a.splits;
   const float* po = a.part + at * D + d;
   const float* ml = a.part + ncols * a.splits * D + at * 2;
   float M = -INFINITY, L = 0.f;
@@ -860,24 +908,29 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, PagedAttn a, i
 
 // ---------------------------------------------------------------------------------------------------------
 namespace {
-template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, int items, int cols, bool single, hipStream_t st) {
-  const dim3 grid(items, a.splits);
+template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, int tiles, int cols, bool single, hipStream_t st) {
+  const int x = c.kv_heads * a.blocks;
+  const dim3 grid(x, tiles, a.splits);
   if (cols == 128) {
     // Up to a workgroup a CU, two groups of waves share its keys
-    if ((long)items * a.splits <= 256) hipLaunchKernelGGL((paged_wide_kernel<DT, D, 2>), grid, dim3(512), 0, st, c, a);
+    if ((long)x * tiles * a.splits <= 256) hipLaunchKernelGGL((paged_wide_kernel<DT, D, 2>), grid, dim3(512), 0, st, c, a);
     else hipLaunchKernelGGL((paged_wide_kernel<DT, D, 1>), grid, dim3(256), 0, st, c, a);
+  } else if (cols == 32) {
+    hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 2, false>), grid, dim3(256), 0, st, c, a);
+  } else if (single) {
+    hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, true>), grid, dim3(256), 0, st, c, a);
+  } else {
+    hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, false>), grid, dim3(256), 0, st, c, a);
   }
-  else if (cols == 32) hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 2, false>), grid, dim3(256), 0, st, c, a);
-  else if (single) hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, true>), grid, dim3(256), 0, st, c, a);
-  else hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, false>), grid, dim3(256), 0, st, c, a);
   if (a.splits == 1) return;
-  const dim3 jg(items * (cols / (1024 / D)));
+  const dim3 jg(x, tiles, cols / (1024 / D));
   if (cols == 128) hipLaunchKernelGGL((paged_join_kernel<DT, D, WIDE_KT, WIDE_LEAST>), jg, dim3(256), 0, st, c, a, cols);
   else hipLaunchKernelGGL((paged_join_kernel<DT, D, 32, NARROW_NW>), jg, dim3(256), 0, st, c, a, cols);
 }
 // workgroups a split: tiles x kv heads x blocks of the columns; 0: out of range
 long paged_items(long tiles, int kv_heads, int heads, int tile_rows, int cols) {
-  if (tiles < 0 || kv_heads <= 0 || heads <= 0 || tile_rows <= 0 || heads % kv_heads) return 0;
+  if (tiles < 0 || tiles > 65535 || kv_heads <= 0 || heads <= 0 || tile_rows <= 0 || heads % kv_heads) return 0;
+  if ((long)tile_rows * (heads / kv_heads) >= 65536 - cols) return 0;  // columns are counted in 16 bits
   if (cols != 16 && cols != 32 && cols != 128) return 0;
   const long per_tile = kv_heads * (((long)tile_rows * (heads / kv_heads) + cols - 1) / cols);
   return tiles * per_tile < 1L << 24 ? tiles * per_tile : 0;
@@ -917,14 +970,15 @@ M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, lo
   const int G = heads / c.kv_heads;
   const PagedAttn a = {(const uint16_t*)q, sq_b, sq_h, (uint16_t*)out, so_b, so_h, slots, pos, tiles, factor,
                        scale < 0.f ? 0x80008000u : 0u, rows, heads, G, tile_rows, (tile_rows * G + cols - 1) / cols,
-                       std::min(window, 1 << 30), std::min(sinks, 1 << 30), splits, (float*)workspace};
+                       std::min(window, 1 << 30), std::min(sinks, 1 << 30), splits,
+                       G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G), (float*)workspace};
   hipStream_t st = (hipStream_t)stream;
   const bool single = tile_rows == 1;
   const int D = cache->head_dim;
-  if (cache->dtype == M3X_BF16 && D == 128) paged_launch<M3X_BF16, 128>(c, a, (int)items, cols, single, st);
-  else if (cache->dtype == M3X_BF16) paged_launch<M3X_BF16, 64>(c, a, (int)items, cols, single, st);
-  else if (D == 128) paged_launch<M3X_F16, 128>(c, a, (int)items, cols, single, st);
-  else paged_launch<M3X_F16, 64>(c, a, (int)items, cols, single, st);
+  if (cache->dtype == M3X_BF16 && D == 128) paged_launch<M3X_BF16, 128>(c, a, ntiles, cols, single, st);
+  else if (cache->dtype == M3X_BF16) paged_launch<M3X_BF16, 64>(c, a, ntiles, cols, single, st);
+  else if (D == 128) paged_launch<M3X_F16, 128>(c, a, ntiles, cols, single, st);
+  else paged_launch<M3X_F16, 64>(c, a, ntiles, cols, single, st);
   M3X_CHECK_LAUNCH();
   return M3X_OK;
 }
