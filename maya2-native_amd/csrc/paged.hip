@@ -51,15 +51,23 @@ __global__ __launch_bounds__(256) void qk_norm_rope_paged_kernel(
   const bool first = d0 < half;
   const int dp = turned && !rot.interleaved ? (first ? d0 + half : d0 - half) : d0;
   const uint16_t* src = qkv + r * s_qkv;
-  u16x8 xv[HB], pv[HB];
+  const int p = pos[r];
+  const long slot = slots[r];
+  u16x8 xv[HB], pv[HB], vv[HB];
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
     const long at = (long)min(j0 + i, NH - 1) * D;
     xv[i] = ld16(src + at + d0);
     pv[i] = ld16(src + at + dp);
   }
-  const int p = pos[r];
-  const long slot = slots[r];
+  // the rows' last loads beside the first: values (of key heads) and their place, asked for before the arithmetic
+  const bool keys = j0 + HB > H;
+  long at = -1;
+  if (keys) {
+#pragma unroll
+    for (int i = 0; i < HB; ++i) vv[i] = ld16(src + (long)(min(max(j0 + i, H), NH - 1) + KV) * D + d0);
+    at = c.at<D>(slot, 0, p);
+  }
   float cs[8], sn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
@@ -109,10 +117,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_paged_kernel(
     if (j < H) {
       st16(qo + row * s_qo_b + (long)j * s_qo_h + d0, o);
     } else {
-      const long at = c.at<D>(slot, j - H, p);
+      const long to = at + ((long)(j - H) << c.shift) * D + d0;
       if (at >= 0) {
-        st16(c.k + at + d0, o);
-        st16(c.v + at + d0, ld16(src + (long)(j + KV) * D + d0));
+        st16(c.k + to, o);
+        st16(c.v + to, vv[i]);
       }
     }
   }

@@ -38,7 +38,8 @@ struct PagedAttn {
   uint32_t q_flip;       // the sign bits of two query elements where scale < 0
   int rows, heads, G, tile_rows, blocks, window, sinks, splits;
   uint32_t over_G;  // ceil(2^32 / G): x / G = x * over_G >> 32 for x, G < 2^16 (0 for G = 1)
-  float* part;  // [columns][splits][D], then [columns][splits][2]: (reference, sum)
+  float* part;   // [columns][splits][D], then [columns][splits][2]: (reference, sum)
+  int* arrived;  // narrow: a counter for each (tile, kv head, block), 0 between calls
 };
 
 // a workgroup's place: a tile, a kv head, a block of the tile's columns; all uniform
@@ -220,9 +221,38 @@ template <int NI, bool NT> __device__ __forceinline__ PgWords<NI> pg_load(__amdg
   return r;
 }
 
+// Device-scope accesses (SC1), coherent across the XCDs' L2s: partial results that another workgroup of the launch joins.
+// A store has arrived where every such load finds it once the storing wave's vmcnt is 0.
+constexpr int PG_SC1 = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t pg_span(float* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00020000);
+}
+
+// dims d .. d + 3 of a column's output from its splits' partial results, in their order; AUX: how they are read. The
+// addresses are a place's (uniform, 64-bit) and a column's within it (below 2^31 bytes: 32 columns of 256 splits).
+template <int DT, int D, int AUX>
+__device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, const Col& cc, long place, int cols, int col, long ncols, int active,
+                                        int d) {
+  const auto po = pg_span(a.part + place * cols * a.splits * D), ml = pg_span(a.part + ncols * a.splits * D + place * cols * a.splits * 2);
+  float M = -INFINITY, L = 0.f;
+  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < active; ++s) {
+    const int at = col * a.splits + s;
+    const float2 x = __builtin_bit_cast(float2, (pg_u2)__builtin_amdgcn_raw_buffer_load_b64(ml, at * 8, 0, AUX));
+    const f32x4_t o = __builtin_bit_cast(f32x4_t, (pg_u4)__builtin_amdgcn_raw_buffer_load_b128(po, (at * D + d) * 4, 0, AUX));
+    const float mx = fmaxf(M, x.x), f0 = __builtin_amdgcn_exp2f(M - mx), f1 = __builtin_amdgcn_exp2f(x.x - mx);
+    L = L * f0 + x.y * f1;
+    O = O * f0 + o * f1;
+    M = mx;
+  }
+  pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
+}
+
 constexpr int NARROW_NW = 4;
 constexpr int WIDE_LEAST = 2;  // steps a split at least
 template <int D> struct NarrowLds {
+  int order;
   __align__(16) float o[NARROW_NW][16][D + 4];
   float ref[NARROW_NW][16], l[NARROW_NW][16];
 };
@@ -482,11 +512,26 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
       if (keys.active == 1) {
         pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
       } else {
-        const long at = (place * COLS + 16 * t + col) * a.splits + split;
-        *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = O;
-        if (d == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(M, L);
+        const int at = (16 * t + col) * a.splits + split;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(pg_u4, O), pg_span(a.part + place * COLS * a.splits * D),
+                                               (at * D + d) * 4, 0, PG_SC1);
+        if (d == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(pg_u2, make_float2(M, L)),
+                                                pg_span(a.part + ncols * a.splits * D + place * COLS * a.splits * 2), at * 8, 0, PG_SC1);
       }
     }
+  }
+  // The split that is done last joins them, in their order whichever it is. Its place's counter is 0 again afterwards.
+  if (keys.active == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) lds.order = __hip_atomic_fetch_add(a.arrived + place, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (lds.order != keys.active - 1) return;
+  if (threadIdx.x == 0) __hip_atomic_store(a.arrived + place, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int x = threadIdx.x; x < COLS * (D / 4); x += 64 * NW) {
+    const Col cc(a, w, w.block * COLS + x / (D / 4));
+    if (cc.live) pg_join<DT, D, PG_SC1>(a, w, cc, place, COLS, x / (D / 4), ncols, keys.active, x % (D / 4) * 4);
   }
 }
 
@@ -885,25 +930,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, PagedAttn a, i
   if (w.n == 0) return;
   const Keys<KT> keys(c, a, w, LEAST);
   if (keys.active <= 1) return;  // written by the attention itself
-  const int col = blockIdx.z * CB + threadIdx.x / TD, d = threadIdx.x % TD * 4;
+  const int col = blockIdx.z * CB + threadIdx.x / TD;
   const Col cc(a, w, w.block * cols + col);
   if (!cc.live) return;
-  const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * per * CB;
-  const long at = (place * cols + col) * a.splits;
-  const float* po = a.part + at * D + d;
-  const float* ml = a.part + ncols * a.splits * D + at * 2;
-  float M = -INFINITY, L = 0.f;
-  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < keys.active; ++s) {
-    const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
-    const f32x4_t o = *reinterpret_cast<const f32x4_t*>(po + (long)s * D);
-    const float mx = fmaxf(M, x.x), f0 = __builtin_amdgcn_exp2f(M - mx), f1 = __builtin_amdgcn_exp2f(x.x - mx);
-    L = L * f0 + x.y * f1;
-    O = O * f0 + o * f1;
-    M = mx;
-  }
-  pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
+  const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * cols;
+  pg_join<DT, D, 0>(a, w, cc, place, cols, col, ncols, keys.active, threadIdx.x % TD * 4);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -922,10 +953,9 @@ template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, i
   } else {
     hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 1, false>), grid, dim3(256), 0, st, c, a);
   }
-  if (a.splits == 1) return;
-  const dim3 jg(x, tiles, cols / (1024 / D));
-  if (cols == 128) hipLaunchKernelGGL((paged_join_kernel<DT, D, WIDE_KT, WIDE_LEAST>), jg, dim3(256), 0, st, c, a, cols);
-  else hipLaunchKernelGGL((paged_join_kernel<DT, D, 32, NARROW_NW>), jg, dim3(256), 0, st, c, a, cols);
+  if (a.splits > 1 && cols == 128)
+    hipLaunchKernelGGL((paged_join_kernel<DT, D, WIDE_KT, WIDE_LEAST>), dim3(x, tiles, cols / (1024 / D)), dim3(256), 0, st, c,
+                       a, cols);
 }
 // workgroups a split: tiles x kv heads x blocks of the columns; 0: out of range
 long paged_items(long tiles, int kv_heads, int heads, int tile_rows, int cols) {
@@ -945,7 +975,7 @@ M3X_API size_t m3x_paged_attn_workspace(int tiles, int kv_heads, int heads, int 
 M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
                            const int64_t* slots, const int32_t* pos, const int32_t* tiles, int ntiles, int tile_rows,
                            int cols, float scale, int rows, int heads, int window, int sinks, int splits, void* workspace,
-                           size_t ws_bytes, void* stream) {
+                           size_t ws_bytes, int32_t* arrived, void* stream) {
   Paged c;
   if (const int st = paged_take(cache, c)) return st;
   if (rows < 0 || ntiles < 0 || heads <= 0 || window < 0 || sinks < 0 || heads > 65535) return M3X_EINVAL;
@@ -959,7 +989,8 @@ M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, lo
   const long items = paged_items(ntiles, c.kv_heads, heads, tile_rows, cols);
   if (items == 0) return M3X_EINVAL;
   if (splits > 1) {
-    if (!workspace) return M3X_ENULL;
+    if (!workspace || (cols != 128 && !arrived)) return M3X_ENULL;
+    if (((uintptr_t)arrived & 3u)) return M3X_EINVAL;
     if (ws_bytes < m3x_paged_attn_workspace(ntiles, c.kv_heads, heads, tile_rows, cols, cache->head_dim, splits))
       return M3X_EWORKSPACE;
     if (!m3x_aligned16(workspace)) return M3X_EINVAL;
@@ -971,7 +1002,7 @@ M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, lo
   const PagedAttn a = {(const uint16_t*)q, sq_b, sq_h, (uint16_t*)out, so_b, so_h, slots, pos, tiles, factor,
                        scale < 0.f ? 0x80008000u : 0u, rows, heads, G, tile_rows, (tile_rows * G + cols - 1) / cols,
                        std::min(window, 1 << 30), std::min(sinks, 1 << 30), splits,
-                       G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G), (float*)workspace};
+                       G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G), (float*)workspace, arrived};
   hipStream_t st = (hipStream_t)stream;
   const bool single = tile_rows == 1;
   const int D = cache->head_dim;

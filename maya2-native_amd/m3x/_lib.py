@@ -94,7 +94,7 @@ SIGNATURES = {
     "m3x_qk_norm_rope_paged": (_I, [_P, _P, _L, _P, _L, _L, _P, _P, _P, _P, _P, _F, _I, _I, _P]),
     "m3x_paged_read": (_I, [_P, _P, _P, _P, _L, _L, _P, _L, _L, _I, _P]),
     "m3x_paged_attn_workspace": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
-    "m3x_paged_attn": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _I, _I, _P, _Z, _P]),
+    "m3x_paged_attn": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _I, _I, _I, _F, _I, _I, _I, _I, _I, _P, _Z, _P, _P]),
     "m3x_final_conv": (_I, [_P, _L, _P, _L, _P, _P, _F, _P, _L, _I, _I, _I, _I, _I, _I, _P]),
 }
 

@@ -1093,6 +1093,8 @@ def paged_tiles(runs, heads, kv_heads):
     r = r[r[:, 1] > 0]
     few = (r[:, 1] * G <= NARROW_COLS) | (r[:, 1] == 1)
     most = max(1, WIDE_COLS // G)
+    if not few.all():  # rows that see nothing go along with the prompts, for their zeros, instead of a launch of their own
+        few &= r[:, 2] + r[:, 1] > 0
     long = r[~few]
     n = -(-long[:, 1] // most)
     of = np.repeat(np.arange(len(long)), n)
@@ -1106,10 +1108,10 @@ def paged_tiles(runs, heads, kv_heads):
 class PagedPlan:
     """How paged_attn runs a step's rows, for all its layers and for every step of the same row layout: runs as in
     paged_tiles (rows in none are left as they are), the heads, the largest context that the rows will see (a rule's
-    input, no limit), window and sinks (see paged_attn). `workspace`: bytes that a call needs; calls that may run at the
-    same time need one each."""
+    input, no limit), window and sinks (see paged_attn). `workspace`: bytes that a call needs. The plan holds counters that
+    a call leaves as it found them: calls that may run at the same time need a plan and a workspace each."""
     __slots__ = ("rows", "heads", "kv_heads", "head_dim", "window", "sinks", "launches", "workspace", "_index", "_calls",
-                 "_keep")
+                 "_arrived")
 
     def __init__(self, runs, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
         r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
@@ -1126,20 +1128,24 @@ class PagedPlan:
             tiles = None if every else torch.from_numpy(np.ascontiguousarray(narrow)).to(device)
             self._add(tiles, len(narrow), int(narrow[:, 1].max()), max_ctx)
         if len(wide):
+            ends = r[r[:, 1] > 0, 2] + r[r[:, 1] > 0, 1]
             self._add(torch.from_numpy(np.ascontiguousarray(wide)).to(device), len(wide), int(wide[:, 1].max()), max_ctx,
-                      True)
+                      True, int(ends[ends > 0].mean()) if (ends > 0).any() else 0)
         self._finish(torch.device(device))
 
     def _begin(self, rows, heads, kv_heads, head_dim, window, sinks):
         self.rows, self.heads, self.kv_heads, self.head_dim = rows, heads, kv_heads, head_dim
         self.window, self.sinks, self.launches = int(window), int(sinks), []
 
-    def _add(self, tiles, n, tile_rows, max_ctx, wide=False):
+    def _add(self, tiles, n, tile_rows, max_ctx, wide=False, mean_ctx=None):
         G = self.heads // self.kv_heads
         cols = WIDE_COLS if wide else 16 if tile_rows * G <= 16 else NARROW_COLS
         blocks = n * self.kv_heads * -(-tile_rows * G // cols)
-        keys = min(max_ctx, self.window + self.sinks + tile_rows) if self.window else max_ctx
-        self.launches.append((tiles, n, tile_rows, cols, paged_attn_splits(blocks, keys, cols)))
+        seen = self.window + self.sinks + tile_rows if self.window else max_ctx
+        keys, mean = min(max_ctx, seen), min(max_ctx if mean_ctx is None else mean_ctx, seen)
+        columns = blocks * min(cols, tile_rows * G)
+        self.launches.append((tiles, n, tile_rows, cols,
+                              paged_attn_splits(blocks, keys, cols, mean, columns, self.head_dim)))
 
     def _finish(self, device):
         self.workspace = max([0] + [int(lib().m3x_paged_attn_workspace(n, self.kv_heads, self.heads, tr, cols,
@@ -1149,15 +1155,43 @@ class PagedPlan:
             self._index = torch.cuda.current_device() if device.index is None else device.index
         else:
             self._index = -1
-        self._calls = [(0 if t is None else t.data_ptr(), n, tr, cols, s) for t, n, tr, cols, s in self.launches]
+        G, split = self.heads // self.kv_heads, [x for x in self.launches if x[4] > 1 and x[3] != WIDE_COLS]
+        need = max([0] + [n * self.kv_heads * -(-tr * G // cols) for _, n, tr, cols, _ in split])
+        self._arrived = torch.zeros(need, dtype=torch.int32, device=device) if need else None
+        at = self._arrived.data_ptr() if need else 0
+        self._calls = [(0 if t is None else t.data_ptr(), n, tr, cols, s, at) for t, n, tr, cols, s in self.launches]
 
 
-def paged_attn_splits(blocks, keys, cols) -> int:
-    """Workgroups that share a tile's keys, for `blocks` (tiles x kv heads x blocks of `cols` columns) of up to `keys`
-    keys each."""
-    if cols == WIDE_COLS:
-        return max(1, min(512 // max(blocks, 1), -(-keys // 256), 64))
-    return max(1, min(-(-768 // max(blocks, 1)), -(-keys // 256), 64))
+def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=128) -> int:
+    """Workgroups that share a tile's keys, for `blocks` (tiles x kv heads x blocks of `cols` columns) of up to `keys` keys
+    each.
+
+    Few columns: a workgroup a CU; two where there are one to two and a half without; at least 256 keys each. Measured on
+    MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3 whole, 14.5 / 11.0 / 8.6 / 8.5 / 8.4 at 2 / 4 / 8
+    / 16 / 32 splits; 16 rows 34.4, 24.2, 25.9, 28.9, 35.3 (16 splits); 48 of a 1024-key window 43.8, 40.3, 42.9 (3), 45.3
+    (4); 224 rows 275, 290. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at 16 / 32 / 64 / 128.
+
+    Prompts: the least of what the tiles' turns of 32 keys take (1.05 us for one of two groups of waves that share a
+    workgroup's keys, which they do up to a workgroup a CU; 0.52 for each of more workgroups that share a CU; the longest
+    tile alone 0.75) and, from two on, the join's launch and partial results (3 us, 3 TB/s). Measured: 512 rows over 2048
+    keys 43.9 / 33.5 / 27.1 / 32.5 at 1 / 2 / 4 / 8; 64 rows over 4000 22.5 / 20.3 / 23.8 at 8 / 16 / 32; 8 x 200 rows over
+    500 22.9 / 31.9 at 1 / 2; 30 x 5 rows over up to 3001, 32/4 heads of 64, 47.6 / 36.9 / 30.6 / 28.1 / 31.8 at 1 / 2 / 4
+    / 6 / 8."""
+    blocks = max(blocks, 1)
+    if cols != WIDE_COLS:
+        if blocks > 256:
+            return 2 if blocks <= 640 and keys >= 1024 else 1
+        return max(1, min(256 // blocks, -(-keys // 256), 64))
+    mean_keys = keys if mean_keys is None else mean_keys
+
+    def time(s):
+        work = blocks * s
+        if work <= 256:
+            turns = 1.05 * keys / (64 * s)
+        else:
+            turns = max(0.52 * -(-work // 256) * mean_keys / (32 * s), 0.75 * keys / (32 * s))
+        return turns + (3 + s * columns * head_dim * 8 / 3e6 if s > 1 else 0)
+    return min((s for s in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64) if s == 1 or s * 128 <= keys), key=time)
 
 
 def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
@@ -1187,9 +1221,9 @@ def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
         if not workspace.is_contiguous() or ws % 16 or workspace.get_device() != cache._index:
             raise ValueError(f"paged_attn: the workspace must be contiguous, 16-byte aligned and on {cache.device}")
     _on_gpu("paged_attn", cache)
-    for tiles, n, tile_rows, cols, splits in plan._calls:
+    for tiles, n, tile_rows, cols, splits, arrived in plan._calls:
         _launch(cache._index, lib().m3x_paged_attn, cache._ref, *qa, *oa, sp, pp, tiles, n, tile_rows, cols, scale, rows,
-                heads, plan.window, plan.sinks, splits, ws, ws_bytes)
+                heads, plan.window, plan.sinks, splits, ws, ws_bytes, arrived)
 
 
 # ---------------------------------------------------------------- Mimi decode (serve/fast_codec.py)
