@@ -742,9 +742,9 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   // own. A wave's last turn, j == steps, sees no key and only makes the outputs of the one before.
   auto turn = [&](int j, uint32_t vn, pg_f16& s, pg_f16& next, const pg_u4 (&pop)[2], pg_u4 (&made)[2]) __attribute__((always_inline)) {
     if (j > steps) return;
-    read_k(get_k + (vn + SB & RING - 1));  // first: what follows covers their way
+    read_k(get_k + ((vn + SB) & (RING - 1)));  // first: what follows covers their way
     __builtin_amdgcn_sched_barrier(0);
-    uint32_t vs = vn - SB & RING - 1;  // where the values of the step before lie
+    uint32_t vs = (vn - SB) & (RING - 1);  // where the values of the step before lie
     const bool was_wild = wild;
     if (j < plain || j >= edge || holes) {
       const int key = keys.key(i0 + j);
@@ -812,7 +812,7 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
         if (pg_hidden(key + k, min(cp, keys.last), pg_low(a, cp), a.sinks)) continue;
 #pragma unroll
         for (int n = 0; n < 4 * ND; ++n) {
-          const pg_u2 x = *reinterpret_cast<const pg_u2*>(lv + (vn - SB & RING - 1) + k * RB +
+          const pg_u2 x = *reinterpret_cast<const pg_u2*>(lv + ((vn - SB) & (RING - 1)) + k * RB +
                                                           (n ^ wide_vx<D>(k & 15)) * 16 + lh * 8);
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[n / 4][4 * (n % 4) + r] += pg_wild_number<DT>((uint16_t)(x[r / 2] >> (16 * (r & 1))));
@@ -851,7 +851,7 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
     pg_landed<2 * LI>();  // K of step j + 1 and V of step j (behind them: V of j + 1, K of j + 2)
     __syncthreads();      // for everyone; and everyone is done with K of step j and V of j - 2
     bring_v(vn ^ 2 * SB);
-    bring_k(i0 + j + 3, vn + 3 * SB & RING - 1);
+    bring_k(i0 + j + 3, (vn + 3 * SB) & (RING - 1));
     turn(j, vn, s, next, pop, made);
   };
   // Two rounds at a time, which hand each other scores and weights. A call of few workgroups is short: its time is the
@@ -863,7 +863,7 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       if (j < n) round(j + 1, vn + SB, s1, s0, p1, p0);
     }
   } else {
-    for (int j = 0, vn = 0; j <= n; ++j, vn = vn + SB & RING - 1) {
+    for (int j = 0, vn = 0; j <= n; ++j, vn = (vn + SB) & (RING - 1)) {
       if (i0 + j + 3 - base >= 64) fetch(i0 + j + 3);
       round(j, vn, s0, s1, p0, p1);
       s0 = s1;
@@ -925,12 +925,11 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
 template <int DT, int D, int KT, int LEAST>
 __global__ __launch_bounds__(256) void paged_join_kernel(Paged c, PagedAttn a, int cols) {
   constexpr int TD = D / 4, CB = 256 / TD;
-  const int per = cols / CB;  // z: which CB of the block's columns
   const Where w = pg_where(c, a, blockIdx.x, blockIdx.y);
   if (w.n == 0) return;
   const Keys<KT> keys(c, a, w, LEAST);
   if (keys.active <= 1) return;  // written by the attention itself
-  const int col = blockIdx.z * CB + threadIdx.x / TD;
+  const int col = blockIdx.z * CB + threadIdx.x / TD;  // z: which CB of the block's columns
   const Col cc(a, w, w.block * cols + col);
   if (!cc.live) return;
   const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * cols;

@@ -980,7 +980,7 @@ class Rotary:
     __slots__ = ("freq", "dim", "interleaved", "factor", "_index", "_args", "_ref")
 
     def __init__(self, inv_freq, interleaved=False, factor=1.0, device="cuda"):
-        f = torch.as_tensor(inv_freq).detach().to("cpu", torch.float64)
+        f = torch.as_tensor(inv_freq, dtype=torch.float64).detach().cpu()
         if f.dim() != 1 or f.numel() % 8 or not 8 <= f.numel() <= 64 or not torch.isfinite(f).all():
             raise ValueError(f"Rotary: 8 to 64 finite frequencies, a multiple of 8, got {tuple(f.shape)}")
         if not abs(float(factor)) < 3.4e38:
@@ -1084,16 +1084,17 @@ def paged_read(cache, slots, pos, k, v):
 NARROW_COLS, WIDE_COLS = 32, 128  # columns (rows x query heads of a kv head) that a workgroup of either kernel takes
 
 
-def paged_tiles(runs, heads, kv_heads):
+def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, apart=False):
     """The tiles of paged_attn for rows laid out as runs, (first row, rows, first position) each, of one slot at
-    consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to 32 columns is one narrow
-    tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first."""
+    consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to narrow_cols columns is one narrow
+    tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first. Rows that
+    see nothing go with the wide tiles, where there are some (apart: not)."""
     G = heads // kv_heads
     r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
     r = r[r[:, 1] > 0]
-    few = (r[:, 1] * G <= NARROW_COLS) | (r[:, 1] == 1)
+    few = (r[:, 1] * G <= narrow_cols) | (r[:, 1] == 1)
     most = max(1, WIDE_COLS // G)
-    if not few.all():  # rows that see nothing go along with the prompts, for their zeros, instead of a launch of their own
+    if not few.all() and not apart:  # rows that see nothing go along with the prompts, for their zeros, instead of a launch of their own
         few &= r[:, 2] + r[:, 1] > 0
     long = r[~few]
     n = -(-long[:, 1] // most)
@@ -1132,6 +1133,35 @@ class PagedPlan:
             self._add(torch.from_numpy(np.ascontiguousarray(wide)).to(device), len(wide), int(wide[:, 1].max()), max_ctx,
                       True, int(ends[ends > 0].mean()) if (ends > 0).any() else 0)
         self._finish(torch.device(device))
+
+    @classmethod
+    def reserve(cls, rows, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
+        """A plan for any layout of up to `rows` rows, what a captured graph launches: before a call, `tiles` of its runs go
+        into the tensors of its two `launches` (narrow, wide)."""
+        if kv_heads < 1 or heads < 1 or heads % kv_heads or rows < 1:
+            raise ValueError(f"PagedPlan: {rows} rows, {heads} query heads over {kv_heads} kv heads")
+        self = cls([], heads, kv_heads, head_dim, max_ctx, window, sinks, device)
+        G = heads // kv_heads
+        self.rows, few, most = rows, max(1, 16 // G), max(1, WIDE_COLS // G)
+        narrow = torch.zeros(rows, 2, dtype=torch.int32, device=device)
+        # a long run has few + 1 rows at least, and one tile more than whole ones; rows that see nothing are tiles too
+        wide = torch.zeros(rows // (few + 1) + rows // most + 1 if rows > few else 1, 2, dtype=torch.int32, device=device)
+        self._add(narrow, rows, min(few, rows), max_ctx)
+        self._add(wide, len(wide), min(most, rows), max_ctx, True)
+        self._finish(torch.device(device))
+        return self
+
+    def tiles(self, runs):
+        """paged_tiles for a reserved plan: (narrow, wide) of its tensors' sizes, (0, 0) behind the tiles."""
+        out = []
+        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
+        for x, (t, n, _, _, _) in zip(paged_tiles(r, self.heads, self.kv_heads, 16, True), self.launches):
+            if len(x) > n:
+                raise ValueError(f"PagedPlan: {len(x)} tiles, reserved for {n}")
+            full = np.zeros((n, 2), dtype=np.int32)
+            full[:len(x)] = x
+            out.append(full)
+        return out
 
     def _begin(self, rows, heads, kv_heads, head_dim, window, sinks):
         self.rows, self.heads, self.kv_heads, self.head_dim = rows, heads, kv_heads, head_dim

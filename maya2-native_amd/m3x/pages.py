@@ -1,0 +1,126 @@
+"""Pages of a paged KV cache: which page holds which positions of which slot (host side), and the device table that
+says so to the kernels (ops.PagedKv, one table for all layers).
+
+A slot's positions live in pages of page_size positions, taken from a pool as the slot grows. Slots may share pages (a
+prefix installed once): a page is free again when the last slot that names it lets go. Pages are only ever written by
+the one slot that took them new, so shared ones never change. Changes to the table are collected on the host and sent
+by `flush`, in stream order before the step that needs them."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from .staging import Upload
+
+
+class PagePool:
+    SEND = 4096  # table entries a copy
+
+    def __init__(self, pages, page_size, slots, capacity, device):
+        if pages < 1 or slots < 1 or capacity < 1:
+            raise ValueError(f"PagePool: {pages} pages for {slots} slots of {capacity} positions")
+        self.pages, self.page_size, self.slots = int(pages), int(page_size), int(slots)
+        self.width = -(-int(capacity) // self.page_size)
+        self.table = torch.full((self.slots, self.width), -1, dtype=torch.int32, device=device)
+        self._host = np.full((self.slots, self.width), -1, dtype=np.int32)
+        self._uses = np.zeros(self.pages, dtype=np.int32)  # slots that name a page
+        self._free = list(range(self.pages - 1, -1, -1))
+        self._end = [0] * self.slots    # table entries a slot has taken so far (some may be released again)
+        self._begin = [0] * self.slots  # first entry behind those that were released
+        self._changed = {}              # flat table index -> page, not yet sent
+        self._index = self._value = None
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def held(self, slot):
+        """Pages that the slot names."""
+        return int((self._host[slot] >= 0).sum())
+
+    def has(self, slot, length):
+        """Whether the slot's first `length` positions all lie in pages."""
+        return bool((self._host[slot, :-(-length // self.page_size)] >= 0).all())
+
+    def _set(self, slot, at, page):
+        self._host[slot, at] = page
+        self._changed[slot * self.width + at] = page
+
+    def _drop(self, slot, at):
+        page = int(self._host[slot, at])
+        if page >= 0:
+            self._uses[page] -= 1
+            if self._uses[page] == 0:
+                self._free.append(page)
+            self._set(slot, at, -1)
+
+    def grow(self, wants):
+        """wants: (slot, length) pairs. Takes the pages that the slots' first `length` positions still need; RuntimeError,
+        with nothing taken, when the pool has too few."""
+        todo, ends = [], {}
+        for slot, length in wants:
+            end = -(-int(length) // self.page_size)
+            if end > self.width:
+                raise ValueError(f"slot {slot}: {length} positions exceed the table's {self.width * self.page_size}")
+            todo += [(slot, at) for at in range(ends.get(slot, self._end[slot]), end)]
+            ends[slot] = max(end, ends.get(slot, 0))
+        if len(todo) > len(self._free):
+            raise RuntimeError(f"the page pool is exhausted: {len(todo)} pages needed, {len(self._free)} of {self.pages} free")
+        for slot, at in todo:
+            page = self._free.pop()
+            self._uses[page] = 1
+            self._set(slot, at, page)
+            self._end[slot] = at + 1
+
+    def trim(self, slot, first, keep=0):
+        """Lets go of the pages that hold only positions below `first`, but for those of the first `keep`."""
+        end = min(int(first) // self.page_size, self._end[slot])
+        begin = max(self._begin[slot], -(-int(keep) // self.page_size))
+        for at in range(begin, end):
+            self._drop(slot, at)
+        self._begin[slot] = max(begin, end) if end > begin else self._begin[slot]
+
+    def release(self, slot):
+        """Lets go of all of the slot's pages."""
+        for at in range(self._end[slot]):
+            self._drop(slot, at)
+        self._end[slot] = self._begin[slot] = 0
+
+    def share(self, slot, source, length):
+        """Gives the (empty) slot the whole pages of the source's first `length` positions and, for what is left of them, a
+        new page. Returns (page of the source, new page) when that is something, to be copied, else None. RuntimeError
+        when the pool has no page for it, ValueError when the source has let go of one."""
+        whole, rest = divmod(int(length), self.page_size)
+        if self._end[slot]:
+            raise ValueError(f"slot {slot} holds pages")
+        if not self.has(source, length):
+            raise ValueError(f"slot {source} does not hold its first {length} positions")
+        if rest and not self._free:
+            raise RuntimeError(f"the page pool is exhausted: 1 page needed, 0 of {self.pages} free")
+        for at in range(whole):
+            page = int(self._host[source, at])
+            self._uses[page] += 1
+            self._set(slot, at, page)
+        self._end[slot] = whole
+        if not rest:
+            return None
+        self.grow([(slot, length)])
+        return int(self._host[source, whole]), int(self._host[slot, whole])
+
+    @torch.inference_mode()
+    def flush(self):
+        """Sends the table's changes on the current stream."""
+        while self._changed:
+            if self._index is None:
+                dev = self.table.device
+                self._index = Upload(torch.zeros(self.SEND, dtype=torch.int64, device=dev))
+                self._value = Upload(torch.zeros(self.SEND, dtype=torch.int32, device=dev))
+            part = list(self._changed.items())[:self.SEND]
+            n = len(part)
+            self._index.buffer()[:n] = [at for at, _ in part]
+            self._value.buffer()[:n] = [page for _, page in part]
+            self._index.send(n)
+            self._value.send(n)
+            self.table.view(-1).index_copy_(0, self._index.dev[:n], self._value.dev[:n])
+            for at, _ in part:
+                del self._changed[at]

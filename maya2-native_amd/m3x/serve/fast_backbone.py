@@ -33,6 +33,13 @@ one kernel path.
 with kv4_attn, which finds a prompt's rows by itself, so decode, mixed and spread-out steps share one graph a bucket;
 one-row steps take the same launches. What is installed is quantised, what is exported is the numbers held, and an
 exported prefix installs as exactly itself.
+
+`page_size` (no counterpart in the reference) keeps the cache in pages (ops.PagedKv, one per layer in `paged`; `k` and `v`
+are then empty): a slot takes memory as it grows, from a pool of `pages` pages, `fork` gives a slot another one's prefix
+without copying its whole pages, and with a `window` a row sees the last `window` positions and the first `sinks`, and
+pages that no row will see again go back to the pool, so that a stream's memory stays the same however long it gets. A
+step writes the cache with qk_norm_rope_paged (the model's frequencies, angles exact at any position) and attends with
+paged_attn; one-row steps take the same launches.
 """
 from __future__ import annotations
 
@@ -43,6 +50,7 @@ import torch
 
 from .. import ops
 from .._lib import lib
+from ..pages import PagePool
 from ..staging import Buckets, ErrorWatch, RowTable, Upload, capture, check_slots
 
 TILE = 32  # keys per attention tile: the per-slot extent of the cache allocation is a multiple of this
@@ -98,25 +106,35 @@ def _join(modules):
 
 class _StepGraph:
     """One (row bucket, context bucket[, inline prefills | item launch]) step: buffers, row table, item upload,
-    graph, and the key of the decode item list last uploaded."""
-    __slots__ = ("bufs", "items", "graph", "items_key")
+    graph, the key of the decode item list last uploaded, and the uploads of a paged step's tiles."""
+    __slots__ = ("bufs", "items", "graph", "items_key", "tiles")
 
     def __init__(self, bufs):
-        self.bufs, self.items, self.graph, self.items_key = bufs, None, None, None
+        self.bufs, self.items, self.graph, self.items_key, self.tiles = bufs, None, None, None, ()
 
 
 class StaticBackbone:
     def __init__(self, backbone, max_slots, capacity=1536,
                  batch_buckets=(1, 2, 4, 8, 16, 24, 32, 48, 64, 80, 96), ctx_buckets=(512, 768, 1024, 1536),
-                 attention='gather', fused_norm=False, use_graphs=True, fuse_proj=False, fuse_rope=False, kv_bits=16):
+                 attention='gather', fused_norm=False, use_graphs=True, fuse_proj=False, fuse_rope=False, kv_bits=16,
+                 page_size=None, pages=None, window=0, sinks=0):
+        """page_size: 16, 32, 64, 128 or 256 positions (None: the static cache); pages: the pool's (default: enough for
+        every slot at capacity); window, sinks: positions that a row sees (0: all)."""
         if kv_bits not in (16, 4):
             raise ValueError(f'kv_bits must be 16 or 4, got {kv_bits}')
+        if page_size is None and (pages is not None or window or sinks):
+            raise ValueError('pages, window and sinks need a page_size')
+        if page_size is not None and (kv_bits != 16 or page_size not in (16, 32, 64, 128, 256)):
+            raise ValueError(f'page_size must be 16, 32, 64, 128 or 256 with kv_bits 16, got {page_size}, {kv_bits}')
+        if window < 0 or sinks < 0 or (sinks and not window):
+            raise ValueError(f'window {window} and sinks {sinks}: a window of positions, and the first ones beside it')
         if attention not in ('gather', 'triton'):
             raise ValueError('attention must be gather or triton')
         lib()  # the kernels are the only path: fail here if the library is missing
         self.attention, self.fused_norm, self.use_graphs = attention, fused_norm, use_graphs
         self.fuse_proj = self.fuse_rope = True
-        self.kv_bits = kv_bits
+        self.kv_bits, self.page_size, self.window, self.sinks = kv_bits, page_size, int(window), int(sinks)
+        self._wanted_pages = pages
         with torch.inference_mode():
             self._read_model(backbone)
             self.max_slots, self.capacity, self.dummy = int(max_slots), int(capacity), int(max_slots)
@@ -197,7 +215,20 @@ class StaticBackbone:
         self._extent = -(-self.capacity // TILE) * TILE
         full = (self.max_slots + 1, self.kv_heads, self._extent, self.head_dim)
         self.kv4 = [ops.Kv4Cache.empty(*full, self.device) for _ in self.layers] if self.kv_bits == 4 else []
-        wide = self.layers if self.kv_bits == 16 else ()
+        self.pages, self.paged = None, []
+        if self.page_size is not None:
+            n = self._wanted_pages
+            if n is None:
+                n = self.max_slots * -(-self.capacity // self.page_size)
+            self.pages = PagePool(n, self.page_size, self.max_slots + 1, self.capacity, self.device)
+            self.paged = [ops.PagedKv.empty(n, self.kv_heads, self.page_size, self.head_dim, self.pages.table, self.dtype)
+                          for _ in self.layers]
+            rope = self.lm.rotary_emb
+            if getattr(rope, 'inv_freq', None) is None:
+                raise ValueError('a paged cache needs the rotary embedding\'s inv_freq')
+            self.rotary = ops.Rotary(rope.inv_freq, factor=float(getattr(rope, 'attention_scaling', 1.0)),
+                                     device=self.device)
+        wide = self.layers if self.kv_bits == 16 and self.page_size is None else ()
         self._kfull = [torch.zeros(full, dtype=self.dtype, device=self.device) for _ in wide]
         self._vfull = [torch.zeros(full, dtype=self.dtype, device=self.device) for _ in wide]
         self.k = [t[:, :, :self.capacity] for t in self._kfull]
@@ -213,6 +244,22 @@ class StaticBackbone:
         self.lengths[slot] = n
         self.lengths_cpu[slot] = n
 
+    def _trim(self, slot):
+        """Pages that no later row of the slot sees go back to the pool (a row at position p sees p - window + 1 on)."""
+        if self.window:
+            self.pages.trim(slot, self.lengths_cpu[slot] - self.window + 1, self.sinks)
+
+    def reserve(self, slots, ahead=1):
+        """Paged cache: takes the pages that the slots' next `ahead` positions need (and lets go of those behind their
+        windows) and sends the table, in stream order before what follows. Steps do it by themselves; programs that
+        replay a captured step do it first. RuntimeError when the pool has too few pages."""
+        if self.pages is None:
+            return
+        for s in slots:
+            self._trim(s)
+        self.pages.grow([(s, self.lengths_cpu[s] + ahead) for s in slots])
+        self.pages.flush()
+
     def _positions_of(self, slot, length):
         """(slots, positions) of a slot's first `length` positions, as the 4-bit cache's rows."""
         return (torch.full((length,), int(slot), dtype=torch.long, device=self.device),
@@ -223,13 +270,17 @@ class StaticBackbone:
         check_slots([slot], self.max_slots)
         if length > self.capacity:
             raise ValueError(f'length {length} exceeds capacity {self.capacity}')
-        if self.kv_bits == 4:
+        if self.kv_bits == 4 or self.pages is not None:
+            if self.pages is not None:
+                self.pages.release(slot)
+                self._set_length(slot, 0)
+                self.reserve([slot], length)
             if length:
                 at = self._positions_of(slot, length)
-                for c, (keys, values) in zip(self.kv4, pairs):
+                for c, (keys, values) in zip(self.paged or self.kv4, pairs):
                     rows = [t[:, :length].to(self.device, self.dtype).transpose(0, 1).contiguous()
                             for t in (keys, values)]
-                    ops.kv4_append(*rows, c, *at)
+                    (ops.kv4_append if self.kv_bits == 4 else ops.paged_append)(*rows, c, *at)
             self._set_length(slot, length)
             return
         for i, (keys, values) in enumerate(pairs):
@@ -246,7 +297,31 @@ class StaticBackbone:
 
     @torch.inference_mode()
     def free(self, slot):
+        if self.pages is not None:
+            self.pages.release(slot)
         self._set_length(slot, 0)
+
+    @torch.inference_mode()
+    def fork(self, slot, source, length=None):
+        """Paged cache: gives the slot the source's first `length` (default: all) positions, sharing the whole pages of
+        them (a voice's prefix, in the cache once for all streams that speak with it) and copying the last one's rest."""
+        if self.pages is None:
+            raise ValueError('fork needs a paged cache')
+        check_slots([slot, source], self.max_slots)
+        n = self.lengths_cpu[source] if length is None else int(length)
+        if not 0 <= n <= self.lengths_cpu[source]:
+            raise ValueError(f'length {n} outside the slot\'s {self.lengths_cpu[source]} cached positions')
+        if not self.pages.has(source, n):
+            raise ValueError(f'slot {source} has let go of positions behind its window')
+        self.pages.release(slot)
+        self._set_length(slot, 0)
+        rest = self.pages.share(slot, source, n)
+        if rest is not None:
+            for c in self.paged:
+                c.k[rest[1]].copy_(c.k[rest[0]])
+                c.v[rest[1]].copy_(c.v[rest[0]])
+        self.pages.flush()
+        self._set_length(slot, n)
 
     @torch.inference_mode()
     def load_prefix(self, slot, kv, length):
@@ -262,12 +337,15 @@ class StaticBackbone:
         n = self.lengths_cpu[slot] if length is None else int(length)
         if not 0 <= n <= self.lengths_cpu[slot]:
             raise ValueError(f'length {n} outside the slot\'s {self.lengths_cpu[slot]} cached positions')
-        if self.kv_bits == 4:
+        if self.pages is not None and not self.pages.has(slot, n):
+            raise ValueError(f'slot {slot} has let go of positions behind its window')
+        if self.kv_bits == 4 or self.pages is not None:
             at, out = self._positions_of(slot, n), []
-            for c in self.kv4:
+            for c in self.paged or self.kv4:
                 k, v = (torch.empty(1, self.kv_heads, n, self.head_dim, dtype=self.dtype, device=self.device)
                         for _ in 'kv')
-                ops.kv4_read(c, *at, k[0].transpose(0, 1), v[0].transpose(0, 1))
+                read = ops.kv4_read if self.kv_bits == 4 else ops.paged_read
+                read(c, *at, k[0].transpose(0, 1), v[0].transpose(0, 1))
                 out.append((k, v))
             return out
         return [(self.k[i][slot:slot + 1, :, :n].clone(), self.v[i][slot:slot + 1, :, :n].clone())
@@ -284,6 +362,8 @@ class StaticBackbone:
             raise ValueError(f'x must be [T>0, {self.hidden}], got {tuple(x.shape)}')
         if self.lengths_cpu[slot] + x.shape[0] > self.capacity:
             raise ValueError(f'context {self.lengths_cpu[slot] + x.shape[0]} exceeds capacity {self.capacity}')
+        if not self.window:
+            self.reserve([slot], x.shape[0])  # all or nothing
         piece = self.batch_buckets[-1]
         last = None
         for t0 in range(0, x.shape[0], piece):
@@ -311,6 +391,13 @@ class StaticBackbone:
         b.part = torch.empty(ops.tile_stats_elems(rows, hid), dtype=torch.float32, device=dev)
         b.q = torch.empty(rows, H, D, dtype=dt, device=dev)
         b.items = None
+        if self.pages is not None:
+            args = (H, KV, D, ctx, self.window, self.sinks, dev)
+            b.plan = ops.PagedPlan.reserve(rows, *args) if mixed else ops.PagedPlan([(r, 1, 0) for r in range(rows)], *args)
+            b.attn_ws = torch.empty(max(b.plan.workspace, 16) // 4, dtype=torch.float32, device=dev)
+            if mixed:  # until a step stages its own: a tile a row
+                b.plan.launches[0][0].copy_(torch.from_numpy(b.plan.tiles([(r, 1, 0) for r in range(rows)])[0]))
+            return b
         if self.kv_bits == 4:
             b.chunk = ops.kv4_attn_chunk(rows, H, KV, ctx, D)
             b.attn_ws = torch.empty(max(ops.kv4_attn_workspace(rows, H, D, ctx, b.chunk), 16) // 4, dtype=torch.float32,
@@ -333,7 +420,7 @@ class StaticBackbone:
         """Whether a step of `rows` rows runs as one persistent kernel: one row (the one-seat frame), the
         Qwen3-0.6B geometry the kernel implements (hidden 1024 with the folded norms, 16 q / 8 kv heads of 128,
         SwiGLU 3072, bf16), a per-slot extent of at most 4096 positions, one workgroup per CU on a 256-CU part."""
-        return (self.persistent and rows == 1 and self.kv_bits == 16
+        return (self.persistent and rows == 1 and self.kv_bits == 16 and self.pages is None
                 and self.fused_norms and self.dtype == torch.bfloat16 and self.heads == 16 and self.kv_heads == 8
                 and self.head_dim == 128 and self.inter == 3072 and self._extent <= 4096 and self._nwg == 256)
 
@@ -377,14 +464,20 @@ class StaticBackbone:
         self._run_sync[2].zero_()
         self._watch.evt = None
 
-    def _attend4(self, b, i, x_norm):
-        """q|k|v of layer i (x_norm: the first layer's normed input, else the residual with its norm to come), the
-        4-bit cache write and the attention over it."""
+    def _attend(self, b, i, x_norm):
+        """q|k|v of layer i (x_norm: the first layer's normed input, else the residual with its norm to come), the write of
+        the 4-bit or paged cache and the attention over it."""
         attn = self.layers[i].self_attn
         if x_norm is not None or not self.fused_norms:
             ops.linear(b.y if x_norm is None else x_norm, self.pqkv[i], b.qkv)
         else:
             ops.linear_normed(b.h, b.part, self.eps, ops.NORM_RMS, self.pqkv[i], y=b.qkv)
+        if self.pages is not None:
+            ops.qk_norm_rope_paged(b.qkv, b.q, self.paged[i], b.slots, b.pos, self.rotary, attn.q_norm.weight,
+                                   attn.k_norm.weight, self.eps, self.heads)
+            ops.paged_attn(b.q, self.paged[i], b.o.view(b.rows, self.heads, self.head_dim), b.slots, b.pos, self.scaling,
+                           b.plan, b.attn_ws)
+            return
         ops.qk_norm_rope_kv4(b.qkv, b.q, self.kv4[i], b.slots, b.pos, self.cos, self.sin, attn.q_norm.weight,
                              attn.k_norm.weight, self.eps, self.heads)
         ops.kv4_attn(b.q, self.kv4[i], b.o.view(b.rows, self.heads, self.head_dim), b.slots, b.pos, self.scaling, b.ctx,
@@ -408,8 +501,8 @@ class StaticBackbone:
                 ops.add_rms(b.x, None, w_in, eps, y=b.y)
             elif not fused:
                 ops.add_rms(b.h, b.pend, w_in, eps, h_out=b.h, y=b.y)
-            if self.kv_bits == 4:
-                self._attend4(b, i, b.y if i == 0 else None)
+            if self.kv_bits == 4 or self.pages is not None:
+                self._attend(b, i, b.y if i == 0 else None)
             else:
                 kc, vc = self._kfull[i], self._vfull[i]
                 qk = (b.qkv, b.q, kc, vc, b.slots, b.pos, self.cos, self.sin, attn.q_norm.weight, attn.k_norm.weight,
@@ -444,6 +537,8 @@ class StaticBackbone:
     def _graph(self, rows, ctx, mixed=False, items=False):
         if self.kv_bits == 4:
             mixed = items = False  # one launch attends every kind of step
+        if self.pages is not None:
+            items = False
         key = (rows, ctx, 'mixed') if mixed else ((rows, ctx, 'items') if items else (rows, ctx))
         g = self.graphs.get(key)
         if g is not None:
@@ -451,6 +546,8 @@ class StaticBackbone:
         g = _StepGraph(self.make_buffers(rows, ctx, mixed, items))
         if g.bufs.items is not None:
             g.items = Upload(g.bufs.items, ring=2)
+        if self.pages is not None and mixed:
+            g.tiles = tuple(Upload(x[0], ring=2) for x in g.bufs.plan.launches)
         if self.use_graphs:
             if self.pool is None:
                 self.pool = torch.cuda.graph_pool_handle()
@@ -468,7 +565,7 @@ class StaticBackbone:
         for rows in self._rows.largest_first(batch_buckets):
             for ctx in self._ctx.largest_first({min(int(c), self.capacity) for c in (ctx_buckets or self.ctx_buckets)}):
                 self._graph(rows, ctx)
-                if rows >= ITEM_MIN_ROWS and not self._persistent_ok(rows):
+                if rows >= ITEM_MIN_ROWS and self.pages is None and not self._persistent_ok(rows):
                     self._graph(rows, ctx, items=True)
                 if mixed:
                     self._graph(rows, ctx, True)
@@ -477,7 +574,7 @@ class StaticBackbone:
     def _spread(self, rows, runs):
         """Whether a decode step of `rows` rows (runs as _rows_of gives them) takes the item launch: its longest
         context more than ITEM_SKEW times the mean."""
-        if rows < ITEM_MIN_ROWS or self.kv_bits == 4 or self._persistent_ok(rows):
+        if rows < ITEM_MIN_ROWS or self.kv_bits == 4 or self.pages is not None or self._persistent_ok(rows):
             return False
         ctxs = np.asarray(runs, dtype=np.int64).reshape(-1, 3)[:, 2] + 1
         return int(ctxs.max()) > ITEM_SKEW * (int(ctxs.sum()) / len(ctxs))
@@ -521,13 +618,25 @@ class StaticBackbone:
         row_slot, row_off, runs, need = self._rows_of(slots, prefills)
         n = len(row_slot)
         rows = self._rows.pick(n, 'batch')
+        if self.pages is not None:
+            grown = [(s, self.lengths_cpu[s] + 1) for s in slots] + [(s, self.lengths_cpu[s] + t.shape[0]) for s, t in prefills]
+            for s, _ in grown:
+                self._trim(s)
+            self.pages.grow(grown)
+            self.pages.flush()
         spread = not prefills and self._spread(rows, runs)
         g = self._graph(rows, self._ctx.pick(need, 'context'), bool(prefills), spread)
         b = g.bufs
         # a decode step keyed by its seats restages nothing when they repeat
         b.table.stage(dict(slot=row_slot, real=np.ones(n, dtype=np.int64), offset=row_off),
                       key=None if prefills else ('decode', tuple(slots)))
-        if (prefills or spread) and self.kv_bits == 16:
+        if g.tiles:
+            pad = np.arange(n, b.rows)  # rows on the dummy slot, which has no page
+            every = np.concatenate([runs, np.stack([pad, np.ones_like(pad), np.zeros_like(pad)], 1)])
+            for up, tiles in zip(g.tiles, b.plan.tiles(every)):
+                up.buffer()[:] = tiles
+                up.send()
+        elif (prefills or spread) and self.kv_bits == 16:
             # a decode step's list stays valid while every row keeps its number of splits (the kernels take each
             # split's keys and a row's split count from the positions at run time): it is rebuilt only when a row
             # crosses a split boundary or the seats change
@@ -594,4 +703,4 @@ class StaticBackbone:
 
     def memory_bytes(self):
         return sum(t.numel() * t.element_size() for t in self._kfull + self._vfull) \
-            + sum(c.memory_bytes() for c in self.kv4)
+            + sum(c.memory_bytes() for c in self.kv4 + self.paged)
