@@ -1168,6 +1168,8 @@ class PagedPlan:
         self.window, self.sinks, self.launches = int(window), int(sinks), []
 
     def _add(self, tiles, n, tile_rows, max_ctx, wide=False, mean_ctx=None):
+        if n > 65535:
+            raise ValueError(f"PagedPlan: {n} tiles, a call holds 65535")
         G = self.heads // self.kv_heads
         cols = WIDE_COLS if wide else 16 if tile_rows * G <= 16 else NARROW_COLS
         blocks = n * self.kv_heads * -(-tile_rows * G // cols)
