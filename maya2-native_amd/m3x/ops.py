@@ -1019,14 +1019,27 @@ def _paged_rows(name, cache, slots, pos):
     """(rows, slots pointer, pos pointer) of a call's rows."""
     if not isinstance(cache, PagedKv):
         raise TypeError(f"{name}: the cache must be an ops.PagedKv")
-    if slots.dtype != torch.int64 or pos.dtype != torch.int32:
-        raise ValueError(f"{name}: slots must be int64 and pos int32, got {slots.dtype}, {pos.dtype}")
-    shape = slots.shape
-    if len(shape) != 1 or pos.shape != shape or not slots.is_contiguous() or not pos.is_contiguous():
-        raise ValueError(f"{name}: slots and pos must be contiguous [rows], got {tuple(shape)}, {tuple(pos.shape)}")
-    if slots.get_device() != cache._index or pos.get_device() != cache._index:
+    shape, dev = slots.shape, cache._index
+    if slots.dtype != torch.int64 or pos.dtype != torch.int32 or len(shape) != 1 or pos.shape != shape or \
+            not slots.is_contiguous() or not pos.is_contiguous():
+        raise ValueError(f"{name}: slots and pos must be contiguous int64 and int32 [rows], got {slots.dtype} {tuple(shape)}, "
+                         f"{pos.dtype} {tuple(pos.shape)}")
+    if slots.get_device() != dev or pos.get_device() != dev:
         raise ValueError(f"{name}: slots on {slots.device}, pos on {pos.device}, the cache on {cache.device}")
     return shape[0], slots.data_ptr(), pos.data_ptr()
+
+
+def _paged_heads(name, what, t, cache, shape):
+    """(pointer, row stride, head stride) of rows of this shape [rows, heads, head_dim]."""
+    if t.shape != shape or t.dtype != cache.dtype:
+        raise ValueError(f"{name}: {what} must be {cache.dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != cache._index:
+        raise ValueError(f"{name}: {what} on {t.device}, the cache on {cache.device}")
+    sr, sh, sd = t.stride()
+    ptr = t.data_ptr()
+    if (sr | sh | ptr >> 1) & 7 or (sd != 1 and shape[0]):
+        raise ValueError(f"{name}: {what} needs a contiguous last dimension and 16-byte aligned rows (strides {t.stride()})")
+    return ptr, sr, sh
 
 
 def paged_append(k, v, cache, slots, pos):
@@ -1034,8 +1047,9 @@ def paged_append(k, v, cache, slots, pos):
     slot slots[r] (int64). A row whose slot, position or page is outside the cache is not written; rows at one place leave
     a mixture there."""
     rows, sp, pp = _paged_rows("paged_append", cache, slots, pos)
-    ka = _kv4_heads("paged_append", "k", k, cache, rows, cache.kv_heads, cache.dtype)
-    va = _kv4_heads("paged_append", "v", v, cache, rows, cache.kv_heads, cache.dtype)
+    shape = rows, cache.kv_heads, cache.head_dim
+    ka = _paged_heads("paged_append", "k", k, cache, shape)
+    va = _paged_heads("paged_append", "v", v, cache, shape)
     _on_gpu("paged_append", cache)
     _launch(cache._index, lib().m3x_paged_append, cache._ref, *ka, *va, sp, pp, rows)
 
@@ -1048,26 +1062,28 @@ def qk_norm_rope_paged(qkv, q_out, cache, slots, pos, rotary, wq, wk, eps, heads
     name = "qk_norm_rope_paged"
     rows, sp, pp = _paged_rows(name, cache, slots, pos)
     D, width = cache.head_dim, (heads + 2 * cache.kv_heads) * cache.head_dim
-    if qkv.shape != (rows, width) or (rows and qkv.stride(1) != 1) or heads < 1:
-        raise ValueError(f"{name}: qkv must be [{rows}, {width}] with a contiguous last dimension, got {tuple(qkv.shape)}")
+    if qkv.shape != (rows, width) or heads < 1:
+        raise ValueError(f"{name}: qkv must be [{rows}, {width}], got {tuple(qkv.shape)}")
     if not isinstance(rotary, Rotary) or rotary.dim > D:
         raise ValueError(f"{name}: rotary must be an ops.Rotary of at most {D} dims")
-    qa = _kv4_heads(name, "q_out", q_out, cache, rows, heads, cache.dtype)
-    qp, s_qkv = qkv.data_ptr(), qkv.stride(0)
+    qa = _paged_heads(name, "q_out", q_out, cache, (rows, heads, D))
+    qp, (s_qkv, s_one) = qkv.data_ptr(), qkv.stride()
     if qkv.dtype != cache.dtype or qkv.get_device() != cache._index or rotary._index != cache._index:
         raise ValueError(f"{name}: qkv must be {cache.dtype} on {cache.device}, as the rotation, got {qkv.dtype} on "
                          f"{qkv.device}")
-    if (s_qkv | qp >> 1) & 7:
-        raise ValueError(f"{name}: qkv needs 16-byte aligned rows (stride {s_qkv})")
-    wp = [0, 0]
+    if (s_qkv | qp >> 1) & 7 or (s_one != 1 and rows):
+        raise ValueError(f"{name}: qkv needs a contiguous last dimension and 16-byte aligned rows (strides {qkv.stride()})")
+    wqp = wkp = 0
     if wq is not None or wk is not None:
-        for i, (t, what) in enumerate(((wq, "wq"), (wk, "wk"))):
-            if t is None or t.numel() != D or t.dtype != cache.dtype or not t.is_contiguous() or t.data_ptr() % 16 or \
-                    t.get_device() != cache._index:
-                raise ValueError(f"{name}: {what} must be {D} contiguous, 16-byte aligned {cache.dtype} on {cache.device}")
-            wp[i] = t.data_ptr()
-    _on_gpu(name, cache)
-    _launch(cache._index, lib().m3x_qk_norm_rope_paged, cache._ref, qp, s_qkv, *qa, sp, pp, rotary._ref, *wp, float(eps),
+        if wq is None or wk is None or wq.numel() != D or wk.numel() != D:
+            raise ValueError(f"{name}: wq and wk are two vectors of {D}, or both None")
+        wqp, wkp = wq.data_ptr(), wk.data_ptr()
+        if (wqp | wkp) & 15 or wq.dtype != cache.dtype or wk.dtype != cache.dtype or not wq.is_contiguous() or \
+                not wk.is_contiguous() or wq.get_device() != cache._index or wk.get_device() != cache._index:
+            raise ValueError(f"{name}: wq and wk must be contiguous, 16-byte aligned {cache.dtype} on {cache.device}")
+    if cache._index < 0:
+        _on_gpu(name, cache)
+    _launch(cache._index, lib().m3x_qk_norm_rope_paged, cache._ref, qp, s_qkv, *qa, sp, pp, rotary._ref, wqp, wkp, eps,
             rows, heads)
 
 
@@ -1075,8 +1091,9 @@ def paged_read(cache, slots, pos, k, v):
     """k, v [rows, kv_heads, head_dim] (the cache's type, any row and head strides) = position pos[r] of slot slots[r];
     zeros where there is none."""
     rows, sp, pp = _paged_rows("paged_read", cache, slots, pos)
-    ka = _kv4_heads("paged_read", "k", k, cache, rows, cache.kv_heads, cache.dtype)
-    va = _kv4_heads("paged_read", "v", v, cache, rows, cache.kv_heads, cache.dtype)
+    shape = rows, cache.kv_heads, cache.head_dim
+    ka = _paged_heads("paged_read", "k", k, cache, shape)
+    va = _paged_heads("paged_read", "v", v, cache, shape)
     _on_gpu("paged_read", cache)
     _launch(cache._index, lib().m3x_paged_read, cache._ref, sp, pp, *ka, *va, rows)
 
@@ -1240,8 +1257,9 @@ def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
     if plan.kv_heads != cache.kv_heads or plan.head_dim != cache.head_dim or plan.rows > rows or plan._index != cache._index:
         raise ValueError(f"paged_attn: a plan of {plan.rows} rows, {heads} / {plan.kv_heads} heads of {plan.head_dim} for "
                          f"{rows} rows over {cache.kv_heads} kv heads of {cache.head_dim} on {cache.device}")
-    qa = _kv4_heads("paged_attn", "q", q, cache, rows, heads, cache.dtype)
-    oa = _kv4_heads("paged_attn", "out", out, cache, rows, heads, cache.dtype)
+    shape = rows, heads, plan.head_dim
+    qa = _paged_heads("paged_attn", "q", q, cache, shape)
+    oa = _paged_heads("paged_attn", "out", out, cache, shape)
     if not abs(scale) <= 2.0 ** 126:
         raise ValueError(f"paged_attn: |scale| must be at most 2^126, got {scale}")
     ws, ws_bytes = 0, 0
