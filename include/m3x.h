@@ -639,9 +639,10 @@ size_t m3x_paged_attn_workspace(int tiles, int kv_heads, int heads, int tile_row
  * tiles (device): ntiles pairs (first row, rows <= tile_rows) of rows of one slot at consecutive positions, of which the
  * first row's slot and position are read; NULL: ntiles single rows 0, 1, ... (tile_rows 1). Rows in no tile are left as
  * they are; a pair with no rows is skipped. cols: columns (a tile's rows x query heads of a kv head) that a workgroup
- * takes, 16 or 32 (few columns, bound by the keys' bytes) or 128 (prompts); at most 65535 tiles, and fewer than 2^16 - cols
- * columns a tile. A tile's keys are divided among up to `splits` <= 256 workgroups; arrived (device, for cols 16 and 32 and
- * splits > 1): tiles x kv_heads x ceil(tile_rows x heads / kv_heads / cols) int32, zeroed before the first call and left so. Weights are rounded to the 16-bit type and summed as rounded; all else is fp32, in a fixed
+ * takes, 16, 32 or, with heads of 64, 48 (few columns, bound by the keys' bytes) or 128 (prompts); at most 65535 tiles, and
+ * fewer than 2^16 - cols columns a tile. A tile's keys are divided among up to `splits` <= 256 workgroups; arrived (device,
+ * for splits > 1 and cols other than 128): tiles x kv_heads x ceil(tile_rows x heads / kv_heads / cols) int32, zeroed before
+ * the first call and left so. Weights are rounded to the 16-bit type and summed as rounded; all else is fp32, in a fixed
  * order. Scores times |scale| log2(e) are to be finite. What a row does not see has no part in its result, whatever it
  * holds. Two calls that may run at the same time need a workspace and counters each. */
 int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,

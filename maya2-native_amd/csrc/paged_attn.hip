@@ -224,27 +224,38 @@ template <int NI, bool NT> __device__ __forceinline__ PgWords<NI> pg_load(__amdg
 // Device-scope accesses (SC1), coherent across the XCDs' L2s: partial results that another workgroup of the launch joins.
 // A store has arrived where every such load finds it once the storing wave's vmcnt is 0.
 constexpr int PG_SC1 = 16;
+constexpr int PG_SPAN = 0x7f000000;  // bytes that a place's partial results stay below
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t pg_span(float* p) {
-  return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, PG_SPAN, 0x00020000);
 }
 
 // dims d .. d + 3 of a column's output from its splits' partial results, in their order; AUX: how they are read. The
-// addresses are a place's (uniform, 64-bit) and a column's within it (below 2^31 bytes: 32 columns of 256 splits).
+// addresses are a place's (uniform, 64-bit) and a column's within it (below PG_SPAN bytes: 128 columns of 256 splits).
 template <int DT, int D, int AUX>
 __device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, const Col& cc, long place, int cols, int col, long ncols, int active,
                                         int d) {
   const auto po = pg_span(a.part + place * cols * a.splits * D), ml = pg_span(a.part + ncols * a.splits * D + place * cols * a.splits * 2);
   float M = -INFINITY, L = 0.f;
   f32x4_t O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = 0; s < active; ++s) {
-    const int at = col * a.splits + s;
-    const float2 x = __builtin_bit_cast(float2, (pg_u2)__builtin_amdgcn_raw_buffer_load_b64(ml, at * 8, 0, AUX));
-    const f32x4_t o = __builtin_bit_cast(f32x4_t, (pg_u4)__builtin_amdgcn_raw_buffer_load_b128(po, (at * D + d) * 4, 0, AUX));
-    const float mx = fmaxf(M, x.x), f0 = __builtin_amdgcn_exp2f(M - mx), f1 = __builtin_amdgcn_exp2f(x.x - mx);
-    L = L * f0 + x.y * f1;
-    O = O * f0 + o * f1;
-    M = mx;
+  // eight splits' loads at a time, of no bytes behind the last
+  for (int s0 = 0; s0 < active; s0 += 8) {
+    float2 x[8];
+    f32x4_t o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = col * a.splits + s0 + e;
+      const bool in = s0 + e < active;
+      x[e] = __builtin_bit_cast(float2, (pg_u2)__builtin_amdgcn_raw_buffer_load_b64(ml, in ? at * 8 : PG_SPAN, 0, AUX));
+      o[e] = __builtin_bit_cast(f32x4_t, (pg_u4)__builtin_amdgcn_raw_buffer_load_b128(po, in ? (at * D + d) * 4 : PG_SPAN, 0, AUX));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float ref = s0 + e < active ? x[e].x : -INFINITY;
+      const float mx = fmaxf(M, ref), f0 = __builtin_amdgcn_exp2f(M - mx), f1 = __builtin_amdgcn_exp2f(ref - mx);
+      L = L * f0 + x[e].y * f1;
+      O = O * f0 + o[e] * f1;
+      M = mx;
+    }
   }
   pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
 }
@@ -945,6 +956,8 @@ template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, i
     // Up to a workgroup a CU, two groups of waves share its keys
     if ((long)x * tiles * a.splits <= 256) hipLaunchKernelGGL((paged_wide_kernel<DT, D, 2>), grid, dim3(512), 0, st, c, a);
     else hipLaunchKernelGGL((paged_wide_kernel<DT, D, 1>), grid, dim3(256), 0, st, c, a);
+  } else if (cols == 48) {
+    if constexpr (D == 64) hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 3, false>), grid, dim3(256), 0, st, c, a);
   } else if (cols == 32) {
     hipLaunchKernelGGL((paged_narrow_kernel<DT, D, 2, false>), grid, dim3(256), 0, st, c, a);
   } else if (single) {
@@ -957,10 +970,10 @@ template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, i
                        a, cols);
 }
 // workgroups a split: tiles x kv heads x blocks of the columns; 0: out of range
-long paged_items(long tiles, int kv_heads, int heads, int tile_rows, int cols) {
+long paged_items(long tiles, int kv_heads, int heads, int tile_rows, int cols, int head_dim) {
   if (tiles < 0 || tiles > 65535 || kv_heads <= 0 || heads <= 0 || tile_rows <= 0 || heads % kv_heads) return 0;
   if ((long)tile_rows * (heads / kv_heads) >= 65536 - cols) return 0;  // columns are counted in 16 bits
-  if (cols != 16 && cols != 32 && cols != 128) return 0;
+  if (cols != 16 && cols != 32 && cols != 128 && !(cols == 48 && head_dim == 64)) return 0;
   const long per_tile = kv_heads * (((long)tile_rows * (heads / kv_heads) + cols - 1) / cols);
   return tiles * per_tile < 1L << 24 ? tiles * per_tile : 0;
 }
@@ -968,7 +981,7 @@ long paged_items(long tiles, int kv_heads, int heads, int tile_rows, int cols) {
 
 M3X_API size_t m3x_paged_attn_workspace(int tiles, int kv_heads, int heads, int tile_rows, int cols, int head_dim, int splits) {
   if (splits <= 1 || head_dim <= 0) return 0;
-  return (size_t)paged_items(tiles, kv_heads, heads, tile_rows, cols) * cols * splits * (head_dim + 2) * sizeof(float);
+  return (size_t)paged_items(tiles, kv_heads, heads, tile_rows, cols, head_dim) * cols * splits * (head_dim + 2) * sizeof(float);
 }
 
 M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
@@ -985,7 +998,7 @@ M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, lo
   if (!q || !out || !slots || !pos) return M3X_ENULL;
   if (((sq_b | sq_h | so_b | so_h) & 7) || !m3x_aligned16(q) || !m3x_aligned16(out) || ((uintptr_t)tiles & 3u)) return M3X_EINVAL;
   if (!tiles && (ntiles > rows || tile_rows != 1)) return M3X_EINVAL;
-  const long items = paged_items(ntiles, c.kv_heads, heads, tile_rows, cols);
+  const long items = paged_items(ntiles, c.kv_heads, heads, tile_rows, cols, cache->head_dim);
   if (items == 0) return M3X_EINVAL;
   if (splits > 1) {
     if (!workspace || (cols != 128 && !arrived)) return M3X_ENULL;

@@ -1101,26 +1101,40 @@ def paged_read(cache, slots, pos, k, v):
 NARROW_COLS, WIDE_COLS = 32, 128  # columns (rows x query heads of a kv head) that a workgroup of either kernel takes
 
 
-def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, apart=False):
+def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, apart=False, cut=0):
     """The tiles of paged_attn for rows laid out as runs, (first row, rows, first position) each, of one slot at
     consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to narrow_cols columns is one narrow
-    tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first. Rows that
-    see nothing go with the wide tiles, where there are some (apart: not)."""
+    tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first; with cut > 0
+    narrow tiles of up to `cut` columns instead, a run's one behind the other (32 runs of 32 rows onto 500 keys 19.7 us, dealt
+    by their keys alone 22.8). Rows that see nothing go with the wide tiles, where there are some (apart:
+    not)."""
     G = heads // kv_heads
     r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
     r = r[r[:, 1] > 0]
     few = (r[:, 1] * G <= narrow_cols) | (r[:, 1] == 1)
-    most = max(1, WIDE_COLS // G)
-    if not few.all() and not apart:  # rows that see nothing go along with the prompts, for their zeros, instead of a launch of their own
+    most = max(1, (cut or WIDE_COLS) // G)
+    if not few.all() and not apart and not cut:  # for their zeros, instead of a launch of their own
         few &= r[:, 2] + r[:, 1] > 0
     long = r[~few]
     n = -(-long[:, 1] // most)
     of = np.repeat(np.arange(len(long)), n)
     at = np.arange(len(of)) - np.repeat(np.cumsum(n) - n, n)
     a, b = at * long[of, 1] // n[of], (at + 1) * long[of, 1] // n[of]
-    order = np.argsort(-(long[of, 2] + b), kind="stable")
-    wide = np.stack([long[of, 0] + a, b - a], 1)[order]
-    return r[few, :2].astype(np.int32), wide.astype(np.int32)
+    # a cut run's tiles one behind the other: they read the same keys at about the same time
+    if cut:
+        order = np.lexsort((-at, of, -(long[:, 2] + long[:, 1])[of]))
+    else:
+        order = np.argsort(-(long[of, 2] + b), kind="stable")
+    tiles = np.stack([long[of, 0] + a, b - a], 1)[order]
+    if cut:
+        return np.concatenate([r[few, :2], tiles]).astype(np.int32), np.empty((0, 2), dtype=np.int32)
+    return r[few, :2].astype(np.int32), tiles.astype(np.int32)
+
+
+def _narrow_cols(head_dim):
+    """Columns of the largest narrow tile: three 16 x 16 blocks fit two workgroups a CU with heads of 64 (measured on
+    MI355X, 40 columns, us against 32 and 128: 30 tiles of up to 3001 keys 22 / 25 / 28, 100 of 2048 40 / 72 / 50)."""
+    return 48 if head_dim == 64 else NARROW_COLS
 
 
 class PagedPlan:
@@ -1129,7 +1143,7 @@ class PagedPlan:
     input, no limit), window and sinks (see paged_attn). `workspace`: bytes that a call needs. The plan holds counters that
     a call leaves as it found them: calls that may run at the same time need a plan and a workspace each."""
     __slots__ = ("rows", "heads", "kv_heads", "head_dim", "window", "sinks", "launches", "workspace", "_index", "_calls",
-                 "_arrived")
+                 "_arrived", "_cut")
 
     def __init__(self, runs, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
         r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
@@ -1140,39 +1154,69 @@ class PagedPlan:
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError(f"PagedPlan: window {window}, sinks {sinks}")
         self._begin(int((r[:, 0] + r[:, 1]).max()) if len(r) else 0, heads, kv_heads, head_dim, window, sinks)
-        narrow, wide = paged_tiles(r, heads, kv_heads)
+        # the runs' own contexts, where they are what the plan is made for and not placeholders
+        ends = r[r[:, 1] > 0, 2] + r[r[:, 1] > 0, 1]
+        known = len(ends) and 2 * ends.max() >= max_ctx
+        mean = int(ends.clip(0).mean()) if known else None
+        ends = ends[ends > 0]
+        narrow, wide = paged_tiles(r, heads, kv_heads, _narrow_cols(head_dim))
+        if len(wide):
+            cut, none = paged_tiles(r, heads, kv_heads, NARROW_COLS, cut=NARROW_COLS)
+            if self._few(len(cut) * self._blocks(cut, NARROW_COLS), max_ctx if mean is None else mean):
+                narrow, wide = cut, none
         every = len(narrow) == self.rows and (narrow[:, 1] == 1).all() and (narrow[:, 0] == np.arange(self.rows)).all()
         if len(narrow):
             tiles = None if every else torch.from_numpy(np.ascontiguousarray(narrow)).to(device)
-            self._add(tiles, len(narrow), int(narrow[:, 1].max()), max_ctx)
+            self._add(tiles, len(narrow), int(narrow[:, 1].max()), max_ctx, mean_ctx=mean)
         if len(wide):
-            ends = r[r[:, 1] > 0, 2] + r[r[:, 1] > 0, 1]
             self._add(torch.from_numpy(np.ascontiguousarray(wide)).to(device), len(wide), int(wide[:, 1].max()), max_ctx,
-                      True, int(ends[ends > 0].mean()) if (ends > 0).any() else 0)
+                      True, int(ends.mean()) if len(ends) else 0)
         self._finish(torch.device(device))
+
+    def _blocks(self, tiles, cols):
+        """Workgroups a tile (and split)."""
+        return self.kv_heads * -(-int(tiles[:, 1].max()) * (self.heads // self.kv_heads) // cols)
+
+    def _few(self, blocks, keys):
+        """Whether prompts go through narrow tiles, cut to 32 columns: `blocks` workgroups of about `keys` keys each.
+
+        Each reads its keys by itself, where the wide kernel's 128 columns share them, and starts sooner. Measured on
+        MI355X (16/8 heads of 128; blocks, us cut / wide): 32 rows onto 300 keys (16) 9.8 / 15.3, 64 onto 4000 (32) 17.3 /
+        22.2, 200 onto 2000 (104) 21.1 / 23.0, 512 onto 2048 (256) 25.8 / 28.8, 32 x 32 onto 500 (512) 19.5 / 22.6, 16 x 64
+        onto 1000 (512) 27.7 / 30.5; on the other side 256 rows onto 6000 (128) 39.5 / 34.1, 64 onto 32000 (32) 48 / 41, 512
+        onto 6000 (256) 59 / 47, 5 x 200 onto 1000 (520) 34.8 / 28.7, 40 x 32 onto 500 (640) 26.0 / 25.0."""
+        keys = min(keys, self.window + self.sinks + NARROW_COLS) if self.window else keys
+        return blocks <= 512 and blocks * keys <= 600_000
 
     @classmethod
     def reserve(cls, rows, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
         """A plan for any layout of up to `rows` rows, what a captured graph launches: before a call, `tiles` of its runs go
-        into the tensors of its two `launches` (narrow, wide)."""
+        into the tensors of its `launches` (narrow and, for more rows than _few takes if all are prompts, wide)."""
         if kv_heads < 1 or heads < 1 or heads % kv_heads or rows < 1:
             raise ValueError(f"PagedPlan: {rows} rows, {heads} query heads over {kv_heads} kv heads")
         self = cls([], heads, kv_heads, head_dim, max_ctx, window, sinks, device)
         G = heads // kv_heads
-        self.rows, few, most = rows, max(1, 16 // G), max(1, WIDE_COLS // G)
+        self.rows, most = rows, max(1, WIDE_COLS // G)
         narrow = torch.zeros(rows, 2, dtype=torch.int32, device=device)
-        # a long run has few + 1 rows at least, and one tile more than whole ones; rows that see nothing are tiles too
-        wide = torch.zeros(rows // (few + 1) + rows // most + 1 if rows > few else 1, 2, dtype=torch.int32, device=device)
-        self._add(narrow, rows, min(few, rows), max_ctx)
-        self._add(wide, len(wide), min(most, rows), max_ctx, True)
+        blocks = rows * kv_heads * -(-max(G, min(rows, max(1, NARROW_COLS // G)) * G) // NARROW_COLS)
+        if blocks <= 512 and self._few(-(-rows * G // NARROW_COLS) * kv_heads, max_ctx):
+            self._cut = NARROW_COLS
+            self._add(narrow, rows, min(max(1, NARROW_COLS // G), rows), max_ctx)
+        else:
+            few = max(1, 16 // G)
+            # a long run has few + 1 rows at least, and one tile more than whole ones
+            wide = torch.zeros(rows // (few + 1) + rows // most + 1 if rows > few else 1, 2, dtype=torch.int32, device=device)
+            self._add(narrow, rows, min(few, rows), max_ctx)
+            self._add(wide, len(wide), min(most, rows), max_ctx, True)
         self._finish(torch.device(device))
         return self
 
     def tiles(self, runs):
         """paged_tiles for a reserved plan: (narrow, wide) of its tensors' sizes, (0, 0) behind the tiles."""
         out = []
-        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
-        for x, (t, n, _, _, _) in zip(paged_tiles(r, self.heads, self.kv_heads, 16, True), self.launches):
+        narrow_cols = self._cut or 16
+        sizes = [x[1] for x in self.launches] + [0]
+        for x, n in zip(paged_tiles(runs, self.heads, self.kv_heads, narrow_cols, True, self._cut), sizes):
             if len(x) > n:
                 raise ValueError(f"PagedPlan: {len(x)} tiles, reserved for {n}")
             full = np.zeros((n, 2), dtype=np.int32)
@@ -1182,13 +1226,15 @@ class PagedPlan:
 
     def _begin(self, rows, heads, kv_heads, head_dim, window, sinks):
         self.rows, self.heads, self.kv_heads, self.head_dim = rows, heads, kv_heads, head_dim
-        self.window, self.sinks, self.launches = int(window), int(sinks), []
+        self.window, self.sinks, self.launches, self._cut = int(window), int(sinks), [], 0
 
     def _add(self, tiles, n, tile_rows, max_ctx, wide=False, mean_ctx=None):
         if n > 65535:
             raise ValueError(f"PagedPlan: {n} tiles, a call holds 65535")
         G = self.heads // self.kv_heads
         cols = WIDE_COLS if wide else 16 if tile_rows * G <= 16 else NARROW_COLS
+        if cols == NARROW_COLS < tile_rows * G <= _narrow_cols(self.head_dim):
+            cols = _narrow_cols(self.head_dim)
         blocks = n * self.kv_heads * -(-tile_rows * G // cols)
         seen = self.window + self.sinks + tile_rows if self.window else max_ctx
         keys, mean = min(max_ctx, seen), min(max_ctx if mean_ctx is None else mean_ctx, seen)
@@ -1215,23 +1261,23 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     """Workgroups that share a tile's keys, for `blocks` (tiles x kv heads x blocks of `cols` columns) of up to `keys` keys
     each.
 
-    Few columns: a workgroup a CU; two where there are one to two and a half without; at least 256 keys each. Measured on
-    MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3 whole, 14.5 / 11.0 / 8.6 / 8.5 / 8.4 at 2 / 4 / 8
-    / 16 / 32 splits; 16 rows 34.4, 24.2, 25.9, 28.9, 35.3 (16 splits); 48 of a 1024-key window 43.8, 40.3, 42.9 (3), 45.3
-    (4); 224 rows 275, 290. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at 16 / 32 / 64 / 128.
+    Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) two where there are one to two and a
+    half without; at least 256 keys each. Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3
+    whole, 14.5 / 10.3 / 8.6 / 8.5 / 8.5 at 2 / 4 / 8 / 16 / 32 splits; 16 rows 34.2, 24.4, 28.8 (3), 24.9 (4); 48 of a
+    1024-key window 39.4, 37.5, 41.1 (3), 42.4 (4); 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 /
+    17.3 / 21.5 at 1 / 2 / 4 / 8 / 16; 512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at
+    16 / 32 / 64 / 128; 30 x 5 rows over up to 3001 29.2 / 26.8 / 23.7 / 22.2 / 26.8 at 1 / 2 / 3 / 4 / 6.
 
     Prompts: the least of what the tiles' turns of 32 keys take (1.05 us for one of two groups of waves that share a
     workgroup's keys, which they do up to a workgroup a CU; 0.52 for each of more workgroups that share a CU; the longest
     tile alone 0.75) and, from two on, the join's launch and partial results (3 us, 3 TB/s). Measured: 512 rows over 2048
     keys 43.9 / 33.5 / 27.1 / 32.5 at 1 / 2 / 4 / 8; 64 rows over 4000 22.5 / 20.3 / 23.8 at 8 / 16 / 32; 8 x 200 rows over
-    500 22.9 / 31.9 at 1 / 2; 30 x 5 rows over up to 3001, 32/4 heads of 64, 47.6 / 36.9 / 30.6 / 28.1 / 31.8 at 1 / 2 / 4
-    / 6 / 8."""
-    blocks = max(blocks, 1)
+    500 22.9 / 31.9 at 1 / 2."""
+    blocks, mean_keys = max(blocks, 1), keys if mean_keys is None else max(mean_keys, 1)
     if cols != WIDE_COLS:
-        if blocks > 256:
+        if blocks > 256 and cols == 16:
             return 2 if blocks <= 640 and keys >= 1024 else 1
-        return max(1, min(256 // blocks, -(-keys // 256), 64))
-    mean_keys = keys if mean_keys is None else mean_keys
+        return max(1, min(256 * keys // max(1, blocks * mean_keys), keys // 256, 64))
 
     def time(s):
         work = blocks * s

@@ -35,10 +35,15 @@ def _case(runs, H, KV, D, page, dtype, window=0, sinks=0, seed=0, gap=0):
     return q, k, v, table, torch.tensor(slots), torch.tensor(pos, dtype=torch.int32), laid
 
 
-def _run(gpu, q, k, v, table, slots, pos, laid, scale, window=0, sinks=0, splits=None, ctx=None):
+def _run(gpu, q, k, v, table, slots, pos, laid, scale, window=0, sinks=0, splits=None, ctx=None, cut=None):
+    """cut: prompts in narrow tiles, or wide ones (None: as the plan decides)."""
     from m3x import ops
+
+    class Plan(ops.PagedPlan):
+        def _few(self, *a):
+            return super()._few(*a) if cut is None else cut
     cache = ops.PagedKv(k.to(gpu), v.to(gpu), table.to(gpu))
-    plan = ops.PagedPlan(laid, q.shape[1], k.shape[1], k.shape[3], ctx or cache.cap, window=window, sinks=sinks, device=gpu)
+    plan = Plan(laid, q.shape[1], k.shape[1], k.shape[3], ctx or cache.cap, window=window, sinks=sinks, device=gpu)
     if splits:
         plan.launches = [(*x[:4], splits) for x in plan.launches]
         plan._finish(torch.device(gpu))
@@ -50,14 +55,15 @@ def _run(gpu, q, k, v, table, slots, pos, laid, scale, window=0, sinks=0, splits
 
 def _check(gpu, case, scale, window=0, sinks=0, **kw):
     q, k, v, table, slots, pos, laid = case
-    got = _run(gpu, *case, scale, window, sinks, **kw)
     want, bound = R.attention(q, k, v, table, slots, pos, scale, window, sinks, laid)
     inside = torch.zeros(len(q), dtype=torch.bool)
     for a, n, _ in laid:
         inside[a:a + n] = True
-    assert (got[~inside] == 7).all()
-    worst = R.within(got[inside], want[inside], bound[inside])
-    assert worst <= 1, worst
+    for cut in (True, False):
+        got = _run(gpu, *case, scale, window, sinks, cut=cut, **kw)
+        assert (got[~inside] == 7).all()
+        worst = R.within(got[inside], want[inside], bound[inside])
+        assert worst <= 1, (cut, worst)
     return got
 
 
@@ -123,7 +129,8 @@ def test_outside(gpu):
 
 @pytest.mark.parametrize("n,p0,window,sinks", [(4, 60, 0, 0), (100, 10, 0, 0), (4, 60, 20, 5), (100, 40, 30, 5), (1, 90, 20, 5)])
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64), (FP, 128), (BF, 64)])
-def test_wild_values(gpu, n, p0, window, sinks, dtype, D):
+@pytest.mark.parametrize("cut", [False, True])
+def test_wild_values(gpu, n, p0, window, sinks, dtype, D, cut):
     """An infinite or NaN value reaches the rows that see its position and no other."""
     q, k, v, table, slots, pos, laid = _case([(n, p0)], 4, 2, D, 16, dtype)
     bad = {p0 + n // 2: float("inf"), p0 + 3 * n // 4: float("nan"), 25: float("-inf"), 3: float("nan")}
@@ -133,7 +140,7 @@ def test_wild_values(gpu, n, p0, window, sinks, dtype, D):
     for j, x in bad.items():
         v[table[1, j // 16].long(), 1, j % 16, 5] = x
         clean[table[1, j // 16].long(), 1, j % 16, 5] = 0.5
-    got = _run(gpu, q, k, v, table, slots, pos, laid, 0.1, window, sinks)
+    got = _run(gpu, q, k, v, table, slots, pos, laid, 0.1, window, sinks, cut=cut)
     want, bound = R.attention(q, k, clean, table, slots, pos, 0.1, window, sinks, laid)
     hit = torch.zeros(got.shape, dtype=torch.bool)
     for r in range(n):
@@ -150,9 +157,9 @@ def test_scores(gpu, n, dtype):
     big = (q * 30, k * 30, v)
     for scale in (-0.1, 0.0, 0.5, 1e-30):
         _check(gpu, (q, k, v, table, slots, pos, laid), scale)
-    got = _run(gpu, *big, table, slots, pos, laid, 3.0)  # one key has all the weight unless two are near
-    want, bound = R.attention(*big, table, slots, pos, 3.0, runs=laid)
-    assert R.within(got, want, bound) <= 1
+    want, bound = R.attention(*big, table, slots, pos, 3.0, runs=laid)  # one key has all the weight unless two are near
+    for cut in (True, False):
+        assert R.within(_run(gpu, *big, table, slots, pos, laid, 3.0, cut=cut), want, bound) <= 1
     if n == 1:
         table2 = table.clone()
         k2 = k.clone()
@@ -167,9 +174,10 @@ def test_large_values(gpu, dtype):
         q, k, v, table, slots, pos, laid = _case([(n, 999)], 2, 1, 128, 64, dtype)
         v = torch.where(torch.isfinite(v), torch.sign(v) * torch.finfo(dtype).max, v)
         v = v.abs()
-        got = _run(gpu, q, k, v, table, slots, pos, laid, 0.1, splits=2)
         u = R.unit(dtype)
-        assert torch.isfinite(got).all() and (got.double() >= torch.finfo(dtype).max * (1 - 4 * u)).all()
+        for cut in (True, False):
+            got = _run(gpu, q, k, v, table, slots, pos, laid, 0.1, splits=2, cut=cut)
+            assert torch.isfinite(got).all() and (got.double() >= torch.finfo(dtype).max * (1 - 4 * u)).all()
 
 
 def test_strides(gpu):
@@ -186,6 +194,15 @@ def test_strides(gpu):
                    torch.empty(plan.workspace, dtype=torch.uint8, device=gpu) if plan.workspace else None)
     want, bound = R.attention(q, k, v, table, slots, pos, 0.125, runs=laid)
     assert R.within(out.transpose(0, 1), want, bound) <= 1
+
+
+@pytest.mark.parametrize("H,KV,D,rows", [(32, 4, 64, 5), (32, 4, 64, 6), (24, 1, 64, 2), (40, 1, 64, 1), (48, 1, 64, 1),
+                                         (33, 1, 128, 1), (40, 1, 128, 1)])
+@pytest.mark.parametrize("splits", [1, 2, 7, 11])
+def test_middling_columns(gpu, H, KV, D, rows, splits):
+    """33 to 48 columns a tile, splits that fill no batch of eight."""
+    case = _case([(rows, 1500), (rows, 31), (1, 0), (rows, 640), (rows, -rows)], H, KV, D, 32, FP, seed=5)
+    _check(gpu, case, D ** -0.5, splits=splits)
 
 
 def test_shared_pages(gpu):

@@ -146,9 +146,11 @@ def test_two_graphs_one_workspace(gpu):
                 st.laid = [(a, n, max(0, p - 1)) for a, n, p in st.laid]
 
 
-def test_reserved_plan(gpu):
+@pytest.mark.parametrize("few", [True, False])
+def test_reserved_plan(gpu, few, monkeypatch):
     """One captured call over a reserved plan: layouts of its rows change from replay to replay."""
     from m3x import ops
+    monkeypatch.setattr(ops.PagedPlan, "_few", lambda *a: few)
     cap, rows = 640, 230
     held = {s: [(0, cap)] for s in range(6)}
     table, pages = R.table_for(held, 6, PAGE, cap // PAGE, 1)
@@ -157,6 +159,7 @@ def test_reserved_plan(gpu):
     cache = ops.PagedKv(k.to(gpu), v.to(gpu), table.to(gpu))
     for window, sinks in ((0, 0), (70, 3)):
         plan = ops.PagedPlan.reserve(rows, H, KV, D, cap, window=window, sinks=sinks, device=gpu)
+        assert len(plan.launches) == 2 - few
         slots, pos = torch.zeros(rows, dtype=torch.long, device=gpu), torch.zeros(rows, dtype=torch.int32, device=gpu)
         out, x = torch.empty(rows, H, D, dtype=BF, device=gpu), q.to(gpu)
         ws = torch.empty(max(plan.workspace, 16), dtype=torch.uint8, device=gpu)

@@ -127,7 +127,8 @@ def test_tiles(H, KV):
             n = int(rng.choice([0, 1, 1, 1, 2, 5, 16, 17, 33, 64, 65, 129, 400]))
             runs.append((at, n, int(rng.integers(-1, 3000))))
             at += n + int(rng.integers(0, 2))
-        for narrow, wide in (ops.paged_tiles(runs, H, KV), ops.PagedPlan.reserve(at, H, KV, 128, 4096, device="cpu").tiles(runs)):
+        for narrow, wide in (ops.paged_tiles(runs, H, KV), ops.paged_tiles(runs, H, KV, cut=32),
+                             ops.PagedPlan.reserve(at, H, KV, 128, 4096, device="cpu").tiles(runs)):
             seen = []
             ends = []
             for t, most in ((narrow, 32), (wide, 128)):
@@ -152,6 +153,7 @@ def test_splits():
             for cols in (16, 32, 128):
                 s = ops.paged_attn_splits(blocks, keys, cols, keys // 2, blocks * cols)
                 assert 1 <= s <= 256 and (s == 1 or s * 128 <= keys)
+    assert ops.paged_attn_splits(30, 3000, 48, 1) <= 11 and ops.paged_attn_splits(160, 3000, 48, 1500) == 3
     assert ops.paged_attn_splits(1792, 2048, 16) == 1 and ops.paged_attn_splits(8, 2048, 16) == 8
 
 
@@ -226,7 +228,7 @@ def test_status_codes():
                                 sinks, splits, ws, wb, arrived, None)
     assert attn(rows=0) == 0 and attn(n=0) == 0 and attn(q=None) == -2 and attn(heads=3) == -5 and attn(heads=0) == -1
     for kw in (dict(rows=-1), dict(n=-1), dict(scale=float("nan")), dict(scale=2.0 ** 127), dict(window=-1), dict(sinks=-1),
-               dict(splits=0), dict(splits=257), dict(s=4), dict(n=4), dict(tr=2), dict(cols=64), dict(heads=1 << 20),
+               dict(splits=0), dict(splits=257), dict(s=4), dict(n=4), dict(tr=2), dict(cols=64), dict(cols=48), dict(heads=1 << 20),
                dict(tiles=ctypes.c_void_p(4098)), dict(tiles=P, n=65536, rows=1 << 20),
                dict(tiles=P, tr=1 << 15, cols=128, rows=1 << 20), dict(q=ctypes.c_void_p(4104))):
         assert attn(**kw) == -1, kw
@@ -345,3 +347,21 @@ def test_pool_random():
         except RuntimeError:
             pass
         _sound(p)
+
+
+def test_reserved_sizes():
+    """A reserved plan holds the tiles of any layout of its rows, in one launch or two."""
+    from m3x import ops
+    rng = np.random.default_rng(2)
+    for H, KV, rows in ((16, 8, 32), (16, 8, 64), (16, 8, 300), (32, 4, 40), (64, 1, 90), (8, 8, 64), (40, 1, 7)):
+        plan = ops.PagedPlan.reserve(rows, H, KV, 64, 1500, device="cpu")
+        assert len(plan.launches) == (1 if rows * KV <= 512 else 2) or H // KV > 32
+        for _ in range(200):
+            runs, at = [], 0
+            while at < rows:
+                n = min(rows - at, int(rng.choice([1, 1, 2, 5, 9, 17, 33, 100])))
+                runs.append((at, n, int(rng.integers(-50, 1000))))
+                at += n
+            narrow, wide = plan.tiles(runs)
+            assert narrow[:, 1].sum() + wide[:, 1].sum() == rows
+            assert narrow[:, 1].max() <= plan.launches[0][2] and (len(plan.launches) == 1 or wide[:, 1].max() <= plan.launches[1][2])
