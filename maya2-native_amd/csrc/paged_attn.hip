@@ -273,11 +273,9 @@ template <int D> struct NarrowLds {
 // waves takes every fourth step of 32 keys, straight from memory to registers: K as the score product's operand, V as
 // rows whose numbers byte permutes pair over keys. The waves' results are merged through LDS.
 template <int DT, int D, int QT, bool NT>
-__global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_kernel(Paged c, PagedAttn a) {
+__global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narrow_kernel(Paged c, PagedAttn a) {
   constexpr int KT = 32, NW = NARROW_NW, KS = D / 32, NV = D / 32, COLS = 16 * QT;
-  // NV: words of V a lane holds of a key (2 NV dims); AHEAD: steps that a wave's loads run ahead (two fill the registers
-  // with 16 columns of 128 dims)
-  constexpr int AHEAD = D == 128 && QT == 2 ? 1 : 2;
+  // NV: words of V a lane holds of a key (2 NV dims)
   const int wave = pg_uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const Where w = pg_where(c, a, blockIdx.x, blockIdx.y);
   if (w.n == 0 || w.block * COLS >= w.n * a.G) return;
@@ -318,9 +316,11 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
   };
   const int inside = (1 << c.shift) - 1;
   const uint32_t k_at = li * (2 * D) + lg * 16, v_at = lg * (8 * D) + li * (D / 8);
-  // AHEAD steps' numbers in turn: a step's keys are loaded behind the score products of the keys that they replace, its
-  // values behind the output products. Loads are never conditional (one whose registers are merged behind a
-  // branch is waited for there): past the wave's last step they are of no bytes.
+  // A step's keys are loaded behind the score products of the keys that they replace, its values behind the output
+  // products. Loads are never conditional (one whose registers are merged behind a branch is waited for there): past the
+  // wave's last step they are of no bytes. Two steps ahead, in two sets of registers, were no faster over long contexts (224
+  // rows of 2048 keys 275 us either way) and slower over short ones, by their fewer waves and longer code: one row 8.6 us
+  // against 8.0, 224 rows of 300 keys 47 against 43.6.
   struct Buf {
     PgWords<4> kw[2][KS];
     PgWords<NV> vw[8];
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
       }
     __builtin_amdgcn_sched_barrier(0);
     const long off[2] = {b.off[0], b.off[1]};
-    load_k(b, i + AHEAD * NW);
+    load_k(b, i + NW);
     __builtin_amdgcn_sched_barrier(0);
     if (edge) {
 #pragma unroll
@@ -468,24 +468,12 @@ __global__ __launch_bounds__(256, D == 64 && QT == 1 ? 3 : 2) void paged_narrow_
     load_v(b);
     __builtin_amdgcn_sched_barrier(0);
   };
-  Buf b0, b1;
-  load_k(b0, i);
+  Buf b;
+  load_k(b, i);
   __builtin_amdgcn_sched_barrier(0);
-  load_v(b0);
+  load_v(b);
   __builtin_amdgcn_sched_barrier(0);
-  if constexpr (AHEAD == 2) {
-    load_k(b1, i + NW);
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(b1);
-    __builtin_amdgcn_sched_barrier(0);
-    for (; i + NW < i1; i += 2 * NW) {
-      step(b0, i);
-      step(b1, i + NW);
-    }
-    if (i < i1) step(b0, i);
-  } else {
-    for (; i < i1; i += NW) step(b0, i);
-  }
+  for (; i < i1; i += NW) step(b, i);
 
   // merge the waves, 16 columns at a time: lane (column, lg) holds dims 2 NV (4 lg + r) + T
   __shared__ NarrowLds<D> lds;
