@@ -1261,10 +1261,10 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     """Workgroups that share a tile's keys, for `blocks` (tiles x kv heads x blocks of `cols` columns) of up to `keys` keys
     each.
 
-    Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) two where there are one to two and a
-    half without; at least 256 keys each. Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3
+    Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) and one to two and a half workgroups
+    a CU without, two where that evens out what the CUs get; at least 256 keys each. Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3
     whole, 14.5 / 10.3 / 8.6 / 8.5 / 8.5 at 2 / 4 / 8 / 16 / 32 splits; 16 rows 34.2, 24.4, 28.8 (3), 24.9 (4); 48 of a
-    1024-key window 39.4, 37.5, 41.1 (3), 42.4 (4); 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 /
+    1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys 116, 102; 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 /
     17.3 / 21.5 at 1 / 2 / 4 / 8 / 16; 512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at
     16 / 32 / 64 / 128; 30 x 5 rows over up to 3001 29.2 / 26.8 / 23.7 / 22.2 / 26.8 at 1 / 2 / 3 / 4 / 6.
 
@@ -1276,7 +1276,10 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     blocks, mean_keys = max(blocks, 1), keys if mean_keys is None else max(mean_keys, 1)
     if cols != WIDE_COLS:
         if blocks > 256 and cols == 16:
-            return 2 if blocks <= 640 and keys >= 1024 else 1
+            def spare(s):  # of the CU with the most workgroups to their mean
+                return -(-blocks * s // 256) * 256 / (blocks * s)
+            uneven = 4 * mean_keys < 3 * keys or spare(1) > 1.1 * spare(2)
+            return 2 if uneven and blocks <= 640 and keys >= 1024 else 1
         return max(1, min(256 * keys // max(1, blocks * mean_keys), keys // 256, 64))
 
     def time(s):
