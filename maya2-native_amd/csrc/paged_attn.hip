@@ -45,6 +45,7 @@ struct PagedAttn {
 // a workgroup's place: a tile, a kv head, a block of the tile's columns; all uniform
 struct Where {
   int tile, kh, block, first, n, p0;  // rows first .. first + n - 1 at positions p0 ..; n == 0: nothing to do
+  int splits;  // that may share the tile's keys
   long slot;
 };
 // x, the same in every lane, in a scalar register. The empty statement hides where x comes from: a value known to be
@@ -69,9 +70,12 @@ __device__ __forceinline__ Where pg_where(const Paged& c, const PagedAttn& a, in
   }
   w.first = tile;
   w.n = 1;
+  w.splits = a.splits;
   if (a.tiles) {
     w.first = pg_uniform(a.tiles[2 * tile]);
-    w.n = pg_uniform(a.tiles[2 * tile + 1]);
+    const int rows = pg_uniform(a.tiles[2 * tile + 1]);
+    w.n = rows < 0 ? 0 : rows & 0xFFFF;
+    if (rows >> 16) w.splits = min(w.splits, rows >> 16);
   }
   w.slot = -1;
   w.p0 = -1;
@@ -103,7 +107,7 @@ template <int KT> struct Keys {
     per = nt;
     active = nt > 0;
     if (a.splits > 1) {
-      per = pg_uniform(max(least, (nt + a.splits - 1) / a.splits));
+      per = pg_uniform(max(least, (nt + w.splits - 1) / w.splits));
       active = pg_uniform((nt + per - 1) / per);
     }
   }

@@ -1101,20 +1101,17 @@ def paged_read(cache, slots, pos, k, v):
 NARROW_COLS, WIDE_COLS = 32, 128  # columns (rows x query heads of a kv head) that a workgroup of either kernel takes
 
 
-def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, apart=False, cut=0):
+def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, cut=0):
     """The tiles of paged_attn for rows laid out as runs, (first row, rows, first position) each, of one slot at
     consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to narrow_cols columns is one narrow
     tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first; with cut > 0
-    narrow tiles of up to `cut` columns instead, a run's one behind the other (32 runs of 32 rows onto 500 keys 19.7 us, dealt
-    by their keys alone 22.8). Rows that see nothing go with the wide tiles, where there are some (apart:
-    not)."""
+narrow tiles of up to `cut` columns instead, a run's one behind the other (32 runs of 32 rows onto 500 keys 19.7 us, dealt
+    by their keys alone 22.8)."""
     G = heads // kv_heads
     r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
     r = r[r[:, 1] > 0]
     few = (r[:, 1] * G <= narrow_cols) | (r[:, 1] == 1)
     most = max(1, (cut or WIDE_COLS) // G)
-    if not few.all() and not apart and not cut:  # for their zeros, instead of a launch of their own
-        few &= r[:, 2] + r[:, 1] > 0
     long = r[~few]
     n = -(-long[:, 1] // most)
     of = np.repeat(np.arange(len(long)), n)
@@ -1143,7 +1140,7 @@ class PagedPlan:
     input, no limit), window and sinks (see paged_attn). `workspace`: bytes that a call needs. The plan holds counters that
     a call leaves as it found them: calls that may run at the same time need a plan and a workspace each."""
     __slots__ = ("rows", "heads", "kv_heads", "head_dim", "window", "sinks", "launches", "workspace", "_index", "_calls",
-                 "_arrived", "_cut")
+                 "_arrived", "_apart")
 
     def __init__(self, runs, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
         r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
@@ -1154,28 +1151,48 @@ class PagedPlan:
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError(f"PagedPlan: window {window}, sinks {sinks}")
         self._begin(int((r[:, 0] + r[:, 1]).max()) if len(r) else 0, heads, kv_heads, head_dim, window, sinks)
-        # the runs' own contexts, where they are what the plan is made for and not placeholders
-        ends = r[r[:, 1] > 0, 2] + r[r[:, 1] > 0, 1]
-        known = len(ends) and 2 * ends.max() >= max_ctx
-        mean = int(ends.clip(0).mean()) if known else None
-        ends = ends[ends > 0]
-        narrow, wide = paged_tiles(r, heads, kv_heads, _narrow_cols(head_dim))
-        if len(wide):
-            cut, none = paged_tiles(r, heads, kv_heads, NARROW_COLS, cut=NARROW_COLS)
-            if self._few(len(cut) * self._blocks(cut, NARROW_COLS), max_ctx if mean is None else mean):
-                narrow, wide = cut, none
-        every = len(narrow) == self.rows and (narrow[:, 1] == 1).all() and (narrow[:, 0] == np.arange(self.rows)).all()
-        if len(narrow):
-            tiles = None if every else torch.from_numpy(np.ascontiguousarray(narrow)).to(device)
-            self._add(tiles, len(narrow), int(narrow[:, 1].max()), max_ctx, mean_ctx=mean)
-        if len(wide):
-            self._add(torch.from_numpy(np.ascontiguousarray(wide)).to(device), len(wide), int(wide[:, 1].max()), max_ctx,
-                      True, int(ends.mean()) if len(ends) else 0)
+        for x, of, wide in self._deal(r[r[:, 1] > 0], _narrow_cols(head_dim)):
+            if not len(x):
+                continue
+            # the runs' own contexts, where they are what the plan is made for and not placeholders
+            ends = (of[:, 2] + of[:, 1]).clip(0)
+            mean = int(ends.mean()) if wide or 2 * ends.max() >= max_ctx else None
+            every = len(x) == self.rows and (x[:, 1] == 1).all() and (x[:, 0] == np.arange(self.rows)).all()
+            tiles = None if every else torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).to(device)
+            self._add(tiles, len(x), int(x[:, 1].max()), max_ctx, wide, mean)
         self._finish(torch.device(device))
+
+    def _deal(self, r, narrow_cols, room=65535, long_cols=0, together=False):
+        """What each launch gets of the runs: (tiles, the runs that they are of, whether wide) of the single rows, of the
+        narrow tiles and of the wide ones. Runs of up to narrow_cols columns are one narrow tile; longer ones are cut into
+        narrow tiles where _few says so or they have no more than long_cols columns. Single rows go along with up to `room`
+        narrow tiles where they are up to a workgroup a CU, or if together (measured on MI355X, 16/8 heads of 128, us: 8 rows of 2048 keys beside
+        a prompt of 56 20 together, 33 apart; 24 beside one of 488 onto 1000 keys 40, 50, beside one of 1000 42, 64; 64
+        beside one of 192 97, 90; 224 beside one of 288 317, 286: a kernel for more columns reads many single rows' keys
+        more slowly, 64 rows of 2048 95 us against 80)."""
+        G = self.heads // self.kv_heads
+        single, rest = r[r[:, 1] == 1], r[r[:, 1] > 1]
+        none = np.empty((0, 2), dtype=np.int32)
+        cut = paged_tiles(rest, self.heads, self.kv_heads, narrow_cols, cut=NARROW_COLS)[0]
+        short, wide = rest, none
+        if len(rest) and (rest[:, 1] * G > narrow_cols).any():
+            ends = (rest[:, 2] + rest[:, 1]).clip(0)
+            if not self._few(len(cut) * self._blocks(cut, NARROW_COLS), int(ends.mean())):
+                long = rest[:, 1] * G > max(narrow_cols, long_cols)
+                short = rest[~long]
+                cut = paged_tiles(short, self.heads, self.kv_heads, narrow_cols, cut=NARROW_COLS)[0]
+                wide = paged_tiles(rest[long], self.heads, self.kv_heads, narrow_cols)[1]
+        live = int((single[:, 2] >= 0).sum())
+        if together or (len(single) and len(cut) and len(single) + len(cut) <= room and
+                        live * self._blocks(single, NARROW_COLS) <= 256):
+            cut, short, single = np.concatenate([single[:, :2], cut]), np.concatenate([single, short]), single[:0]
+        elif live == 0 and len(wide) and room == 65535:  # for their zeros, instead of a launch of their own
+            wide, single = np.concatenate([wide, single[:, :2]]), single[:0]
+        return (single[:, :2], single, False), (cut, short, False), (wide, rest, True)
 
     def _blocks(self, tiles, cols):
         """Workgroups a tile (and split)."""
-        return self.kv_heads * -(-int(tiles[:, 1].max()) * (self.heads // self.kv_heads) // cols)
+        return self.kv_heads * -(-int(tiles[:, 1].max(initial=0)) * (self.heads // self.kv_heads) // cols)
 
     def _few(self, blocks, keys):
         """Whether prompts go through narrow tiles, cut to 32 columns: `blocks` workgroups of about `keys` keys each.
@@ -1191,42 +1208,60 @@ class PagedPlan:
     @classmethod
     def reserve(cls, rows, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
         """A plan for any layout of up to `rows` rows, what a captured graph launches: before a call, `tiles` of its runs go
-        into the tensors of its `launches` (narrow and, for more rows than _few takes if all are prompts, wide)."""
+        into the tensors of its `launches`: single rows (up to two workgroups a CU together with the next), narrow tiles and,
+        for more rows than _few takes if all are one prompt, wide ones. A launch that gets no tile costs 1 to 3 us."""
         if kv_heads < 1 or heads < 1 or heads % kv_heads or rows < 1:
             raise ValueError(f"PagedPlan: {rows} rows, {heads} query heads over {kv_heads} kv heads")
         self = cls([], heads, kv_heads, head_dim, max_ctx, window, sinks, device)
         G = heads // kv_heads
-        self.rows, most = rows, max(1, WIDE_COLS // G)
-        narrow = torch.zeros(rows, 2, dtype=torch.int32, device=device)
-        blocks = rows * kv_heads * -(-max(G, min(rows, max(1, NARROW_COLS // G)) * G) // NARROW_COLS)
-        if blocks <= 512 and self._few(-(-rows * G // NARROW_COLS) * kv_heads, max_ctx):
-            self._cut = NARROW_COLS
-            self._add(narrow, rows, min(max(1, NARROW_COLS // G), rows), max_ctx)
-        else:
-            few = max(1, 16 // G)
-            # a long run has few + 1 rows at least, and one tile more than whole ones
-            wide = torch.zeros(rows // (few + 1) + rows // most + 1 if rows > few else 1, 2, dtype=torch.int32, device=device)
-            self._add(narrow, rows, min(few, rows), max_ctx)
-            self._add(wide, len(wide), min(most, rows), max_ctx, True)
+        few, most = max(1, NARROW_COLS // G), max(1, WIDE_COLS // G)
+        self.rows = rows
+        self._apart = rows * self._blocks(np.array([[0, 1]]), NARROW_COLS) > 512  # single rows have a launch of their own
+        if self._apart:
+            self._reserve(rows, 1, False, device)
+        # runs of two rows and more: a tile's part of them is the largest where one row more makes two tiles
+        n = rows if not self._apart else -(-rows * 2 // (few + 1)) if few < 3 else rows // 2
+        self._reserve(n, min(few, rows), False, device)
+        if not self._few(-(-rows * G // NARROW_COLS) * kv_heads, max_ctx):
+            self._reserve(2 * rows // most + 1, min(most, rows), True, device)
         self._finish(torch.device(device))
         return self
 
+    def _reserve(self, n, tile_rows, wide, device):
+        """A launch of up to n tiles, with splits for few of them: up to 2048 workgroups, most of which have nothing to do (64
+        rows, all of a prompt onto 3900 keys 40 us unsplit, 31 so; onto 16 keys 7.9 and 8.1)."""
+        tiles = torch.zeros(n, 2, dtype=torch.int32, device=device)
+        self._add(tiles, n, tile_rows, 0, wide)
+        cols = self.launches[-1][3]
+        blocks = n * self._blocks(np.array([[0, tile_rows]]), cols)
+        self.launches[-1] = (*self.launches[-1][:4], 1 if tile_rows == 1 < self.rows else max(1, min(16, 2048 // blocks)))
+
     def tiles(self, runs):
-        """paged_tiles for a reserved plan: (narrow, wide) of its tensors' sizes, (0, 0) behind the tiles."""
+        """A reserved plan's tiles for these runs, one array of its tensor's size for each launch, rows as they come with
+        the splits that their number and keys ask for."""
+        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
+        r = r[r[:, 1] > 0]
+        wide = self.launches[-1][3] == WIDE_COLS
+        lists = self._deal(r, 0, self.launches[self._apart][1], WIDE_COLS // 2 if wide else 1 << 31, not self._apart)
+        lists = lists[not self._apart:]
         out = []
-        narrow_cols = self._cut or 16
-        sizes = [x[1] for x in self.launches] + [0]
-        for x, n in zip(paged_tiles(runs, self.heads, self.kv_heads, narrow_cols, True, self._cut), sizes):
+        for (x, of, _), (_, n, tile_rows, cols, splits) in zip(lists, self.launches):
             if len(x) > n:
                 raise ValueError(f"PagedPlan: {len(x)} tiles, reserved for {n}")
             full = np.zeros((n, 2), dtype=np.int32)
-            full[:len(x)] = x
+            full[:len(x)] = x[:, :2]
+            if splits > 1 and len(x):
+                seen = self.window + self.sinks + tile_rows if self.window else 1 << 30
+                ends = (of[:, 2] + of[:, 1]).clip(0, seen)
+                blocks = len(x) * self._blocks(x, cols)
+                s = paged_attn_splits(blocks, int(ends.max()), cols, int(ends.mean()), blocks * cols, self.head_dim)
+                full[:len(x), 1] |= min(s, splits) << 16
             out.append(full)
         return out
 
     def _begin(self, rows, heads, kv_heads, head_dim, window, sinks):
         self.rows, self.heads, self.kv_heads, self.head_dim = rows, heads, kv_heads, head_dim
-        self.window, self.sinks, self.launches, self._cut = int(window), int(sinks), [], 0
+        self.window, self.sinks, self.launches, self._apart = int(window), int(sinks), [], False
 
     def _add(self, tiles, n, tile_rows, max_ctx, wide=False, mean_ctx=None):
         if n > 65535:
@@ -1262,7 +1297,8 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     each.
 
     Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) and one to two and a half workgroups
-    a CU without, two where that evens out what the CUs get; at least 256 keys each. Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3
+    a CU without, two where that evens out what the CUs get; at least 256 keys each, three times as many to begin with (the join's 3 to 5 us:
+    64 rows onto 500 keys 12.4 whole, 13.6 to 17 split). Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3
     whole, 14.5 / 10.3 / 8.6 / 8.5 / 8.5 at 2 / 4 / 8 / 16 / 32 splits; 16 rows 34.2, 24.4, 28.8 (3), 24.9 (4); 48 of a
     1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys 116, 102; 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 /
     17.3 / 21.5 at 1 / 2 / 4 / 8 / 16; 512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at
@@ -1280,7 +1316,7 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
                 return -(-blocks * s // 256) * 256 / (blocks * s)
             uneven = 4 * mean_keys < 3 * keys or spare(1) > 1.1 * spare(2)
             return 2 if uneven and blocks <= 640 and keys >= 1024 else 1
-        return max(1, min(256 * keys // max(1, blocks * mean_keys), keys // 256, 64))
+        return max(1, min(256 * keys // max(1, blocks * mean_keys), keys // 256, 64)) if keys >= 768 else 1
 
     def time(s):
         work = blocks * s

@@ -223,6 +223,7 @@ class StaticBackbone:
             self.pages = PagePool(n, self.page_size, self.max_slots + 1, self.capacity, self.device)
             self.paged = [ops.PagedKv.empty(n, self.kv_heads, self.page_size, self.head_dim, self.pages.table, self.dtype)
                           for _ in self.layers]
+            self._attn_ws = torch.empty(4, dtype=torch.float32, device=self.device)
             rope = self.lm.rotary_emb
             if getattr(rope, 'inv_freq', None) is None:
                 raise ValueError('a paged cache needs the rotary embedding\'s inv_freq')
@@ -394,7 +395,9 @@ class StaticBackbone:
         if self.pages is not None:
             args = (H, KV, D, ctx, self.window, self.sinks, dev)
             b.plan = ops.PagedPlan.reserve(rows, *args) if mixed else ops.PagedPlan([(r, 1, 0) for r in range(rows)], *args)
-            b.attn_ws = torch.empty(max(b.plan.workspace, 16) // 4, dtype=torch.float32, device=dev)
+            if self._attn_ws.numel() * 4 < b.plan.workspace:  # one for all graphs: their steps follow each other
+                self._attn_ws = torch.empty(b.plan.workspace // 4, dtype=torch.float32, device=dev)
+            b.attn_ws = self._attn_ws
             if mixed:  # until a step stages its own: a tile a row
                 b.plan.launches[0][0].copy_(torch.from_numpy(b.plan.tiles([(r, 1, 0) for r in range(rows)])[0]))
             return b
@@ -631,8 +634,8 @@ class StaticBackbone:
         b.table.stage(dict(slot=row_slot, real=np.ones(n, dtype=np.int64), offset=row_off),
                       key=None if prefills else ('decode', tuple(slots)))
         if g.tiles:
-            pad = np.arange(n, b.rows)  # rows on the dummy slot, which has no page
-            every = np.concatenate([runs, np.stack([pad, np.ones_like(pad), np.zeros_like(pad)], 1)])
+            pad = np.arange(n, b.rows)  # rows on the dummy slot, which has no page: they see nothing
+            every = np.concatenate([runs, np.stack([pad, np.ones_like(pad), np.full_like(pad, -1)], 1)])
             for up, tiles in zip(g.tiles, b.plan.tiles(every)):
                 up.buffer()[:] = tiles
                 up.send()

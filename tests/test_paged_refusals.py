@@ -127,8 +127,7 @@ def test_tiles(H, KV):
             n = int(rng.choice([0, 1, 1, 1, 2, 5, 16, 17, 33, 64, 65, 129, 400]))
             runs.append((at, n, int(rng.integers(-1, 3000))))
             at += n + int(rng.integers(0, 2))
-        for narrow, wide in (ops.paged_tiles(runs, H, KV), ops.paged_tiles(runs, H, KV, cut=32),
-                             ops.PagedPlan.reserve(at, H, KV, 128, 4096, device="cpu").tiles(runs)):
+        for narrow, wide in (ops.paged_tiles(runs, H, KV), ops.paged_tiles(runs, H, KV, cut=32)):
             seen = []
             ends = []
             for t, most in ((narrow, 32), (wide, 128)):
@@ -153,7 +152,7 @@ def test_splits():
             for cols in (16, 32, 128):
                 s = ops.paged_attn_splits(blocks, keys, cols, keys // 2, blocks * cols)
                 assert 1 <= s <= 256 and (s == 1 or s * 128 <= keys)
-    assert ops.paged_attn_splits(30, 3000, 48, 1) <= 11 and ops.paged_attn_splits(160, 3000, 48, 1500) == 3
+    assert ops.paged_attn_splits(30, 3000, 48, 1) <= 11 and ops.paged_attn_splits(1, 700, 16) == 1 and ops.paged_attn_splits(160, 3000, 48, 1500) == 3
     assert ops.paged_attn_splits(1792, 2048, 16) == 1 and ops.paged_attn_splits(8, 2048, 16) == 8
 
 
@@ -349,19 +348,31 @@ def test_pool_random():
         _sound(p)
 
 
-def test_reserved_sizes():
-    """A reserved plan holds the tiles of any layout of its rows, in one launch or two."""
+@pytest.mark.parametrize("few", [None, True, False])
+def test_reserved(few, monkeypatch):
+    """A reserved plan holds the tiles of any layout of its rows: each row once, within a run and within its launch."""
     from m3x import ops
+    if few is not None:
+        monkeypatch.setattr(ops.PagedPlan, "_few", lambda *a: few)
     rng = np.random.default_rng(2)
-    for H, KV, rows in ((16, 8, 32), (16, 8, 64), (16, 8, 300), (32, 4, 40), (64, 1, 90), (8, 8, 64), (40, 1, 7)):
+    for H, KV, rows in ((16, 8, 1), (16, 8, 2), (16, 8, 64), (16, 8, 300), (32, 4, 40), (32, 2, 50), (64, 1, 90), (24, 2, 33),
+                        (8, 8, 64), (40, 1, 7), (150, 1, 9)):
         plan = ops.PagedPlan.reserve(rows, H, KV, 64, 1500, device="cpu")
-        assert len(plan.launches) == (1 if rows * KV <= 512 else 2) or H // KV > 32
-        for _ in range(200):
+        assert len(plan.launches) <= 3
+        for i in range(200):
             runs, at = [], 0
             while at < rows:
-                n = min(rows - at, int(rng.choice([1, 1, 2, 5, 9, 17, 33, 100])))
-                runs.append((at, n, int(rng.integers(-50, 1000))))
+                n = min(rows - at, (2, 3, 17, 33)[i] if i < 4 else int(rng.choice([1, 1, 2, 3, 5, 9, 17, 33, 100])))
+                runs.append((at, n, int(rng.integers(-50, 3000))))
                 at += n
-            narrow, wide = plan.tiles(runs)
-            assert narrow[:, 1].sum() + wide[:, 1].sum() == rows
-            assert narrow[:, 1].max() <= plan.launches[0][2] and (len(plan.launches) == 1 or wide[:, 1].max() <= plan.launches[1][2])
+            seen = []
+            for tiles, (_, room, tile_rows, _, splits) in zip(plan.tiles(runs), plan.launches):
+                assert tiles.shape == (room, 2)
+                for a, x in tiles.tolist():
+                    n, s = x & 0xFFFF, x >> 16
+                    assert n <= tile_rows and s <= splits
+                    assert n == 0 or any(f <= a and a + n <= f + m for f, m, _ in runs)
+                    seen += range(a, a + n)
+            assert sorted(seen) == list(range(rows))
+    with pytest.raises(ValueError):
+        plan.tiles([(r, 1, 0) for r in range(30)])
