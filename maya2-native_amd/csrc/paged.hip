@@ -32,6 +32,8 @@ __device__ __forceinline__ void st16_nt(uint16_t* p, const u16x8& x) {
 //   (i, i + dim / 2) or (2i, 2i + 1).
 // D / 8 threads a head, HB heads of one row one after another with the same angles. In the first layout a thread also
 // loads its partner dims (from the cache the neighbour's load fills) instead of exchanging them.
+// Bound by the launch and one memory round trip up to some hundred rows (16/8 heads of 128: 1 row 2.9 us, 224 rows 4.1, 512
+// 4.6), then by bytes: 2048 rows of 32/8 heads of 128, half of each rotated, 50 MB in 11.1 us, 4.5 TB/s (a large copy: 4.9).
 template <int DT, int D, int HB>
 __global__ __launch_bounds__(256) void qk_norm_rope_paged_kernel(
     const uint16_t* __restrict__ qkv, long s_qkv, uint16_t* __restrict__ qo, long s_qo_b, long s_qo_h, Paged c,
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_paged_kernel(
   }
 }
 
-// K and V rows into their pages, D / 8 threads per (row, kv head)
+// K and V rows into their pages, D / 8 threads per (row, kv head): a copy, bound as the kernel above
 template <int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const uint16_t* __restrict__ k, long sk_r, long sk_h,
                                                            const uint16_t* __restrict__ v, long sv_r, long sv_h, Paged c,
@@ -146,7 +148,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const uint16_t* __res
   st16(c.v + at + d0, vx);
 }
 
-// Positions as rows, zeros where there is none; stored with the non-temporal hint (read once by their taker)
+// Positions as rows, zeros where there is none; stored with the non-temporal hint (read once by their taker). Bound by the
+// launch (300 positions of 8 heads of 128 2.7 us), then bytes: 65520 positions of 8 heads of 64, 268 MB in 41 us, 6.5 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void paged_read_kernel(Paged c, const int64_t* __restrict__ slots,
                                                          const int32_t* __restrict__ pos, uint16_t* __restrict__ k,
@@ -236,7 +239,8 @@ M3X_API int m3x_qk_norm_rope_paged(const M3xPagedKv* cache, const void* qkv, lon
   const uintptr_t o0 = (uintptr_t)q_out, o1 = o0 + 2 * ((rows - 1) * s_qo_b + (heads - 1L) * s_qo_h + D);
   if (o0 < i1 && i0 < o1) return M3X_EINVAL;
   if (heads > 65535 || !paged_fits(rows * nh, D)) return M3X_EINVAL;
-  // four heads a thread share the angles once that leaves two waves a SIMD
+  // four heads a thread share the angles once that leaves two waves a SIMD (16/8 heads of 128, us with four, with one: 1
+  // row 4.4, 3.0, 1024 rows 7.6, 6.8, 2048 rows 10.5, 11.5)
   const int hb = rows * nh * (D / 8) >= 4L * 64 * 2048 ? 4 : 1;
   const dim3 grid(m3x_ceil_div(rows * ((nh + hb - 1) / hb), 2048 / D));
 #define M3X_QKN(DT, DD, HB)                                                                                        \

@@ -9,7 +9,8 @@
 //   softmax                         running maximum and sum in fp32, exp2; a lane keeps its own column's
 //   O^T += V^T . P                  S^T's accumulators of two 16-key groups are the P operand as they stand
 // A tile's keys are counted in steps of KT positions, first those of the sinks, then those from the window's begin on,
-// and divided evenly among the splits; the splits' partial results are joined by a second launch.
+// and divided evenly among the splits. The splits' partial results are joined in the splits' order: few columns' by the
+// split that is done last, prompts' by a second launch.
 #include <algorithm>
 #include <cstring>
 
@@ -273,9 +274,14 @@ template <int D> struct NarrowLds {
 };
 }  // namespace
 
-// Tiles of up to 16 QT columns: single tokens, and the few rows of drafted ones. Bound by the keys' bytes. Each of the 4
-// waves takes every fourth step of 32 keys, straight from memory to registers: K as the score product's operand, V as
-// rows whose numbers byte permutes pair over keys. The waves' results are merged through LDS.
+// Tiles of up to 16 QT columns: single tokens, the few rows of drafted ones, and short prompts cut into such tiles. Bound by
+// the keys' bytes. Each of the 4 waves takes every fourth step of 32 keys, straight from memory to registers: K as the score
+// product's operand, V as rows whose numbers byte permutes pair over keys. The waves' results are merged through LDS.
+// Measured on MI355X (bf16, 16/8 heads of 128, page_size 64, graph-timed): 224 rows of 2048 keys 276 us, 1.87 GB at 6.8
+// TB/s; 48 rows of a 1024-key window 37 us, 5.4 TB/s; one row of 2048 keys in 8 splits 7.9 us: launch 2, loads of what the
+// next load needs (tile, slot, page, keys) 3, two steps and the merge 1, join 2.
+// NT: the keys' loads carry the non-temporal hint, for single rows, whose keys one workgroup reads once (224 rows 276 us
+// against 312; 48 rows, whose keys stay in the memory-side cache from call to call, 37 against 35).
 template <int DT, int D, int QT, bool NT>
 __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narrow_kernel(Paged c, PagedAttn a) {
   constexpr int KT = 32, NW = NARROW_NW, KS = D / 32, NV = D / 32, COLS = 16 * QT;
@@ -544,6 +550,10 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
 // keys) in steps of 32, which come to LDS by loads that need no registers, two steps
 // ahead; every wave reads K there in 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads. A row's
 // chunks lie in LDS at their number XOR a number of the row, so that neither read meets a bank twice.
+// Measured on MI355X (bf16, page_size 64 or 128, graph-timed): 4096 rows onto 12288 keys, 32/8 heads of 128, 917 us, 1050
+// TFLOP/s, where an 8192^3 product of the library reaches 1290; the matrix units are busy half of the time, the vector units
+// about as long, and the clock is down to 1.9 GHz. 8 x 200 rows onto 300 to 500 keys, 16/8 heads, 22 us: eleven turns of
+// both key groups make half of it, the rest is the start, the pipeline's filling and the merge.
 namespace {
 constexpr int WIDE_KT = 32;
 // A weight's exponent is counted from a reference that the scores of a column pass by less than WIDE_SLACK: renewing it
@@ -945,7 +955,8 @@ template <int DT, int D> void paged_launch(const Paged& c, const PagedAttn& a, i
   const int x = c.kv_heads * a.blocks;
   const dim3 grid(x, tiles, a.splits);
   if (cols == 128) {
-    // Up to a workgroup a CU, two groups of waves share its keys
+    // Up to a workgroup a CU, two groups of waves share its keys (us with two groups, with one: 512 rows onto 16000 keys
+    // unsplit 254, 324, 2048 rows onto nothing 45, 50; above, 4 x 700 rows under a window 56, 34, 4096 rows 1030, 917)
     if ((long)x * tiles * a.splits <= 256) hipLaunchKernelGGL((paged_wide_kernel<DT, D, 2>), grid, dim3(512), 0, st, c, a);
     else hipLaunchKernelGGL((paged_wide_kernel<DT, D, 1>), grid, dim3(256), 0, st, c, a);
   } else if (cols == 48) {
