@@ -1143,15 +1143,13 @@ class PagedPlan:
                  "_arrived", "_apart")
 
     def __init__(self, runs, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
-        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
         if kv_heads < 1 or heads < 1 or heads % kv_heads:
             raise ValueError(f"PagedPlan: {heads} query heads over {kv_heads} kv heads")
-        if (r[:, :2] < 0).any() or (r[:, 0] + r[:, 1] >= 1 << 31).any():
-            raise ValueError("PagedPlan: runs are (first row, rows, first position)")
+        r = self._runs(runs)
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError(f"PagedPlan: window {window}, sinks {sinks}")
         self._begin(int((r[:, 0] + r[:, 1]).max()) if len(r) else 0, heads, kv_heads, head_dim, window, sinks)
-        for x, of, wide in self._deal(r[r[:, 1] > 0], _narrow_cols(head_dim)):
+        for x, of, wide in self._deal(r, _narrow_cols(head_dim)):
             if not len(x):
                 continue
             # the runs' own contexts, where they are what the plan is made for and not placeholders
@@ -1161,6 +1159,17 @@ class PagedPlan:
             tiles = None if every else torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).to(device)
             self._add(tiles, len(x), int(x[:, 1].max()), max_ctx, wide, mean)
         self._finish(torch.device(device))
+
+    @staticmethod
+    def _runs(runs):
+        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
+        r = r[r[:, 1] != 0]
+        if (r[:, :2] < 0).any() or (r[:, 0] + r[:, 1] >= 1 << 31).any():
+            raise ValueError("PagedPlan: runs are (first row, rows, first position)")
+        o = r[np.argsort(r[:, 0], kind="stable")]
+        if (o[1:, 0] < o[:-1, 0] + o[:-1, 1]).any():
+            raise ValueError("PagedPlan: a row is in two runs")
+        return r
 
     def _deal(self, r, narrow_cols, room=65535, long_cols=0, together=False):
         """What each launch gets of the runs: (tiles, the runs that they are of, whether wide) of the single rows, of the
@@ -1239,8 +1248,9 @@ class PagedPlan:
     def tiles(self, runs):
         """A reserved plan's tiles for these runs, one array of its tensor's size for each launch, rows as they come with
         the splits that their number and keys ask for."""
-        r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
-        r = r[r[:, 1] > 0]
+        r = self._runs(runs)
+        if len(r) and (r[:, 0] + r[:, 1]).max() > self.rows:
+            raise ValueError(f"PagedPlan: runs past the {self.rows} rows that the plan is for")
         wide = self.launches[-1][3] == WIDE_COLS
         lists = self._deal(r, 0, self.launches[self._apart][1], WIDE_COLS // 2 if wide else 1 << 31, not self._apart)
         lists = lists[not self._apart:]

@@ -180,6 +180,64 @@ def test_large_values(gpu, dtype):
             assert torch.isfinite(got).all() and (got.double() >= torch.finfo(dtype).max * (1 - 4 * u)).all()
 
 
+@pytest.mark.parametrize("window,sinks", [(20, 100), (1, 1), (3, 64), (50, 2 ** 31 - 1), (2 ** 31 - 1, 5)])
+def test_more_sinks_than_window(gpu, window, sinks):
+    case = _case([(1, 300), (5, 90), (150, 40), (70, 230), (1, 2)], 4, 2, 128, 16, BF, window, sinks, seed=8)
+    for splits in (1, 3):
+        _check(gpu, case, 0.1, window, sinks, splits=splits)
+
+
+@pytest.mark.parametrize("cut", [False, True])
+@pytest.mark.parametrize("n", [1, 6, 90])
+def test_wild_queries(gpu, n, cut):
+    """An infinite or NaN query spoils its own row and head alone."""
+    q, k, v, table, slots, pos, laid = _case([(n, 200), (n, 77)], 4, 2, 128, 32, BF)
+    want, bound = R.attention(q, k, v, table, slots, pos, 0.1, runs=laid)
+    bad = torch.zeros(len(q), 4, dtype=torch.bool)
+    for r, h, x in ((0, 1, float("nan")), (n // 2, 2, float("inf")), (2 * n - 1, 0, float("nan"))):
+        q[r, h, 3], bad[r, h] = x, True
+    got = _run(gpu, q, k, v, table, slots, pos, laid, 0.1, splits=2, cut=cut)
+    assert R.within(got[~bad], want[~bad], bound[~bad]) <= 1 and torch.isnan(got[bad]).any()
+
+
+def test_far_pages(gpu):
+    """Pages more than 2^32 bytes into the pools: written, read and attended as near ones."""
+    from m3x import ops
+    KV, page, D, pages = 8, 256, 128, 9000  # 4.7 GB a pool
+    if torch.cuda.mem_get_info()[0] < 16e9:
+        pytest.skip("needs 10 GB")
+    near, far = torch.tensor([3, 1, 5]), torch.tensor([8999, 8500, 8998])
+    table = torch.stack([near, far]).int()
+    k, v = (torch.empty(pages, KV, page, D, dtype=BF, device=gpu) for _ in "kv")
+    cache = ops.PagedKv(k, v, table.to(gpu))
+    n = 700
+    x = R.normal(1, 2, n, KV, D).to(BF).to(gpu)
+    pos = torch.arange(n, dtype=torch.int32, device=gpu)
+    out = []
+    for s in (0, 1):
+        slots = torch.full((n,), s, dtype=torch.long, device=gpu)
+        ops.paged_append(x[0], x[1], cache, slots, pos)
+        a, b = torch.empty_like(x[0]), torch.empty_like(x[1])
+        ops.paged_read(cache, slots, pos, a, b)
+        assert torch.equal(a, x[0]) and torch.equal(b, x[1])
+        q = R.normal(2, 230, 16, D).to(BF).to(gpu)
+        rows = slots[:230], torch.cat([pos[:100], pos[500:630]])
+        for runs in ([(r, 1, 0) for r in range(230)], [(0, 100, 0), (100, 130, 500)]):
+            for few in (True, False):
+                class Plan(ops.PagedPlan):
+                    def _few(self, *a):
+                        return few
+                plan = Plan(runs, 16, KV, D, 700, device=gpu)
+                ws = torch.empty(max(16, plan.workspace), dtype=torch.uint8, device=gpu)
+                out.append(torch.empty_like(q))
+                ops.paged_attn(q, cache, out[-1], *rows, 0.1, plan, ws)
+    for a, b in zip(out[:4], out[4:]):
+        assert torch.equal(a, b)
+    want, bound = R.attention(q.cpu(), k[:6].cpu(), v[:6].cpu(), table[:1], torch.zeros(230, dtype=torch.long), rows[1].cpu(), 0.1)
+    for a in out[:4]:
+        assert R.within(a, want, bound) <= 1
+
+
 def test_strides(gpu):
     """q and out as views of wider rows, pools as a view of joined ones, a plan's rows in any order."""
     from m3x import ops

@@ -104,7 +104,8 @@ def test_attn_refused():
 def test_plan_refused():
     from m3x import ops
     for a in (([(0, 1, 0)], 3, 2, 128, 64), ([(0, 1, 0)], 0, 1, 128, 64), ([(-1, 2, 0)], 4, 2, 128, 64),
-              ([(0, -1, 0)], 4, 2, 128, 64), ([(0, 1 << 31, 0)], 4, 2, 128, 64)):
+              ([(0, -1, 0)], 4, 2, 128, 64), ([(0, 1 << 31, 0)], 4, 2, 128, 64), ([(4, 2, 0), (0, 5, 0)], 4, 2, 128, 64),
+              ([(1, 1, 0), (1, 1, 0)], 4, 2, 128, 64)):
         with pytest.raises(ValueError):
             ops.PagedPlan(*a, device="cpu")
     for kw in (dict(window=-1), dict(sinks=-1), dict(window=1 << 31)):
@@ -376,3 +377,7 @@ def test_reserved(few, monkeypatch):
             assert sorted(seen) == list(range(rows))
     with pytest.raises(ValueError):
         plan.tiles([(r, 1, 0) for r in range(30)])
+    with pytest.raises(ValueError):
+        plan.tiles([(8, 2, 0)])
+    with pytest.raises(ValueError):
+        plan.tiles([(0, 2, 0), (1, 1, 0)])
