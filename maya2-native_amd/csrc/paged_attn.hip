@@ -253,24 +253,32 @@ __device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, cons
       x[e] = __builtin_bit_cast(float2, (pg_u2)__builtin_amdgcn_raw_buffer_load_b64(ml, in ? at * 8 : PG_SPAN, 0, AUX));
       o[e] = __builtin_bit_cast(f32x4_t, (pg_u4)__builtin_amdgcn_raw_buffer_load_b128(po, in ? (at * D + d) * 4 : PG_SPAN, 0, AUX));
     }
+    float mx = M;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float ref = s0 + e < active ? x[e].x : -INFINITY;
-      const float mx = fmaxf(M, ref), f0 = __builtin_amdgcn_exp2f(M - mx), f1 = __builtin_amdgcn_exp2f(ref - mx);
-      L = L * f0 + x[e].y * f1;
-      O = O * f0 + o[e] * f1;
-      M = mx;
+      if (s0 + e >= active) x[e].x = -INFINITY;
+      mx = fmaxf(mx, x[e].x);
     }
+    const float f0 = __builtin_amdgcn_exp2f(M - mx);
+    L *= f0;
+    O *= f0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = __builtin_amdgcn_exp2f(x[e].x - mx);
+      L += x[e].y * f;
+      O += o[e] * f;
+    }
+    M = mx;
   }
   pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
 }
 
 constexpr int NARROW_NW = 4;
 constexpr int WIDE_LEAST = 2;  // steps a split at least
-template <int D> struct NarrowLds {
+template <int D, int COLS> struct NarrowLds {
   int order;
-  __align__(16) float o[NARROW_NW][16][D + 4];
-  float ref[NARROW_NW][16], l[NARROW_NW][16];
+  __align__(16) float o[NARROW_NW][COLS][D + 4];
+  float ref[NARROW_NW][COLS], l[NARROW_NW][COLS];
 };
 }  // namespace
 
@@ -485,49 +493,49 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
   __builtin_amdgcn_sched_barrier(0);
   for (; i < i1; i += NW) step(b, i);
 
-  // merge the waves, 16 columns at a time: lane (column, lg) holds dims 2 NV (4 lg + r) + T
-  __shared__ NarrowLds<D> lds;
+  // merge the waves: lane (column, lg) holds dims 2 NV (4 lg + r) + T
+  __shared__ NarrowLds<D, COLS> lds;
   const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    if (t) __syncthreads();
     const float sum = xor32_sum(xor16_sum(l[t]));
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int T = 0; T < 2 * NV; T += 4)
-        *reinterpret_cast<f32x4_t*>(&lds.o[wave][li][2 * NV * (4 * lg + r) + T]) =
+        *reinterpret_cast<f32x4_t*>(&lds.o[wave][16 * t + li][2 * NV * (4 * lg + r) + T]) =
             f32x4_t{acc[t][T][r], acc[t][T + 1][r], acc[t][T + 2][r], acc[t][T + 3][r]};
     if (lg == 0) {
-      lds.ref[wave][li] = pg_ref(m[t], a.c);
-      lds.l[wave][li] = sum;
+      lds.ref[wave][16 * t + li] = pg_ref(m[t], a.c);
+      lds.l[wave][16 * t + li] = sum;
     }
-    __syncthreads();
-    for (int x = threadIdx.x; x < 16 * (D / 4); x += 64 * NW) {
-      const int col = x / (D / 4), d = x % (D / 4) * 4;
-      const Col cc(a, w, w.block * COLS + 16 * t + col);
-      if (!cc.live) continue;
-      float M = lds.ref[0][col];
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int x = threadIdx.x; x < COLS * (D / 4); x += 64 * NW) {
+    const int col = x / (D / 4), d = x % (D / 4) * 4;
+    const Col cc(a, w, w.block * COLS + col);
+    if (!cc.live) continue;
+    float M = lds.ref[0][col];
 #pragma unroll
-      for (int y = 1; y < NW; ++y) M = fmaxf(M, lds.ref[y][col]);
-      float L = 0.f;
-      f32x4_t O = {0.f, 0.f, 0.f, 0.f};
+    for (int y = 1; y < NW; ++y) M = fmaxf(M, lds.ref[y][col]);
+    float L = 0.f;
+    f32x4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int y = 0; y < NW; ++y) {
-        const float f = __builtin_amdgcn_exp2f(lds.ref[y][col] - M);
-        L += lds.l[y][col] * f;
-        O += *reinterpret_cast<const f32x4_t*>(&lds.o[y][col][d]) * f;
-      }
-      if (keys.active == 1) {
-        pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
-      } else {
-        const int at = (16 * t + col) * a.splits + split;
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(pg_u4, O), pg_span(a.part + place * COLS * a.splits * D),
-                                               (at * D + d) * 4, 0, PG_SC1);
-        if (d == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(pg_u2, make_float2(M, L)),
-                                                pg_span(a.part + ncols * a.splits * D + place * COLS * a.splits * 2), at * 8, 0, PG_SC1);
-      }
+    for (int y = 0; y < NW; ++y) {
+      const float f = __builtin_amdgcn_exp2f(lds.ref[y][col] - M);
+      L += lds.l[y][col] * f;
+      O += *reinterpret_cast<const f32x4_t*>(&lds.o[y][col][d]) * f;
+    }
+    if (keys.active == 1) {
+      pg_store4<DT>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + d, O, L);
+    } else {
+      const int at = col * a.splits + split;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(pg_u4, O), pg_span(a.part + place * COLS * a.splits * D),
+                                             (at * D + d) * 4, 0, PG_SC1);
+      if (d == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(pg_u2, make_float2(M, L)),
+                                              pg_span(a.part + ncols * a.splits * D + place * COLS * a.splits * 2), at * 8, 0, PG_SC1);
     }
   }
   // The split that is done last joins them, in their order whichever it is. Its place's counter is 0 again afterwards.
@@ -552,8 +560,9 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
 // chunks lie in LDS at their number XOR a number of the row, so that neither read meets a bank twice.
 // Measured on MI355X (bf16, page_size 64 or 128, graph-timed): 4096 rows onto 12288 keys, 32/8 heads of 128, 917 us, 1050
 // TFLOP/s, where an 8192^3 product of the library reaches 1290; the matrix units are busy half of the time, the vector units
-// about as long, and the clock is down to 1.9 GHz. 8 x 200 rows onto 300 to 500 keys, 16/8 heads, 22 us: eleven turns of
-// both key groups make half of it, the rest is the start, the pipeline's filling and the merge.
+// about as long, and the clock is down to 1.9 GHz. 8 x 200 rows onto 300 to 500 keys, 16/8 heads, 21 us: launch 2, tile, slot
+// and page numbers 2.5, the first keys and queries 0.6, the first turn 2 to 3 with its code's way into the instruction
+// cache, seven more of both key groups 1.3 each, the groups' sums 2.
 namespace {
 constexpr int WIDE_KT = 32;
 // A weight's exponent is counted from a reference that the scores of a column pass by less than WIDE_SLACK: renewing it
@@ -688,9 +697,9 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   // the wave's steps: those up to its last row's key (pb lies at or behind the window's begin)
   const int steps = pb < 0 ? 0 : max(0, min(i1 - i0, pb / KT - keys.skip - i0 + 1));
   // The turns whose step every row sees whole: from plain on up to edge. Before them the window hides something (or
-  // nothing: steps of the sinks), and turn 0 begins.
+  // nothing: steps of the sinks).
   const int edge = min(steps, max(0, (pa + 1) / KT - keys.skip - i0));
-  int plain = max(1, none < 0 ? 0 : none / KT + 1 - keys.skip - i0);
+  int plain = none < 0 ? 0 : none / KT + 1 - keys.skip - i0;
 
   const uint32_t get_k = li * RB + (lh ^ wide_kx<D>(li)) * 16;
   // Sixteen lanes, four keys, 16 dims: lane x brings dims 4 (x % 4) .. of key x / 4, and takes dim x of the four. The lower
@@ -771,14 +780,13 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       }
       // Infinite and NaN values of a step that not all rows see stand apart: 0 in the product, whose values the wave then
       // takes from the spare stage (every wave that does so in this turn writes the same there), and added below to the
-      // columns that see them, as in the narrow kernel. The first turn's outputs are made of weights and values of 0.
-      if (wild || j == 0) {
-        const uint32_t keep = j ? ~0u : 0u;
+      // columns that see them, as in the narrow kernel.
+      if (wild) {
 #pragma unroll 1
         for (int x = lane * 16; x < SB; x += 1024) {
           pg_u4 v = *reinterpret_cast<const pg_u4*>(lv + vs + x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = pg_tame<DT>(v[e]) & keep;
+          for (int e = 0; e < 4; ++e) v[e] = pg_tame<DT>(v[e]);
           *reinterpret_cast<pg_u4*>(lv + RING + x) = v;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -851,6 +859,8 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   bring_k(i0 + 1, SB);
   bring_v(SB);
   bring_k(i0 + 2, 2 * SB);
+  // the first turn's outputs: of weights and values of 0, in the stage that is filled last
+  for (int x = (threadIdx.x & 255) * 16; x < SB; x += 4096) *reinterpret_cast<pg_u4*>(lv + 3 * SB + x) = pg_u4{0, 0, 0, 0};
   pg_landed<4 * LI>();
   __syncthreads();
   pg_f16 s0, s1;
@@ -886,51 +896,66 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   }
   pg_landed<0>();
 
-  if constexpr (KG == 2) {  // the second group's sums by way of LDS to the first
-    __syncthreads();
-    f32x4_t* const at = reinterpret_cast<f32x4_t*>(lds) + wave * (4 * ND * 64) + lane;
-    float2* const ml = reinterpret_cast<float2*>(lds + 4 * (4 * ND * 64) * 16) + wave * 64 + lane;
-    if (group) {
+  if constexpr (KG == 1) {  // lane (column, lh) holds dims 8 n + 4 lh + r
+    const float L = xor32_sum(l);
+    if (!col.live) return;
+    if (keys.active == 1) {
+      uint16_t* op = a.out + (long)(w.first + col.j) * a.so_b + (long)(w.kh * a.G + col.h) * a.so_h + 4 * lh;
 #pragma unroll
       for (int n = 0; n < 4 * ND; ++n) {
         const pg_f16& x = acc[n / 4];
-        at[64 * n] = f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
+        pg_store4<DT>(op + 8 * n, f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]}, L);
       }
-      *ml = make_float2(add, l);
-    }
-    __syncthreads();
-    if (group) return;
-    const float2 o = *ml;
-    const float x = fminf(add, o.x), f0 = __builtin_amdgcn_exp2f(x - add), f1 = __builtin_amdgcn_exp2f(x - o.x);
-    add = x;
-    l = l * f0 + o.y * f1;
+    } else {
+      const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
+      const long at = (place * COLS + 32 * wave + li) * a.splits + split;
 #pragma unroll
-    for (int n = 0; n < 4 * ND; ++n) {
-      const f32x4_t y = at[64 * n];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[n / 4][n % 4 * 4 + r] = acc[n / 4][n % 4 * 4 + r] * f0 + y[r] * f1;
+      for (int n = 0; n < 4 * ND; ++n) {
+        const pg_f16& x = acc[n / 4];
+        *reinterpret_cast<f32x4_t*>(a.part + at * D + 8 * n + 4 * lh) =
+            f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
+      }
+      if (lh == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(wide_up<DT> - add, L);
     }
+    return;
   }
-  // lane (column, lh) holds dims 8 n + 4 lh + r
-  const float L = xor32_sum(l);
-  if (!col.live) return;
-  if (keys.active == 1) {
-    uint16_t* op = a.out + (long)(w.first + col.j) * a.so_b + (long)(w.kh * a.G + col.h) * a.so_h + 4 * lh;
+  // The key groups' sums by way of LDS, and to 16-byte stores of whole rows: few instructions, which matter in a short call,
+  // since each is fetched for one use (8 x 200 rows 23.1 us with the groups' sums in registers, 21.0 so; with one group,
+  // where the stores above are fewer bytes moved, 3200 rows 28.0 and 28.5). An n's chunks lie at their column XOR a number
+  // of n, so that neither side meets a bank twice.
+  __syncthreads();
+  constexpr int NC = 4 * ND, SW = 16 / NC;
+  f32x4_t* const out = reinterpret_cast<f32x4_t*>(lds);
+  float2* const ml = reinterpret_cast<float2*>(lds + KG * 4 * NC * 1024);
 #pragma unroll
-    for (int n = 0; n < 4 * ND; ++n) {
-      const pg_f16& x = acc[n / 4];
-      pg_store4<DT>(op + 8 * n, f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]}, L);
+  for (int n = 0; n < NC; ++n) {
+    const pg_f16& x = acc[n / 4];
+    out[((group * 4 + wave) * NC + n) * 64 + (lane ^ SW * n)] = f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
+  }
+  l = xor32_sum(l);
+  if (lh == 0) ml[(group * 4 + wave) * 32 + li] = make_float2(add, l);
+  __syncthreads();
+#pragma unroll 1
+  for (int x = threadIdx.x; x < COLS * NC; x += 256 * KG) {
+    const int n = x % NC, y = x / NC, at = ((y / 32) * NC + n) * 64 + (y % 32 ^ SW * n);
+    const Col cc(a, w, w.block * COLS + y);
+    if (!cc.live) continue;
+    const float2 m0 = ml[y], m1 = ml[128 + y];
+    const float least = fminf(m0.x, m1.x), f0 = __builtin_amdgcn_exp2f(least - m0.x), f1 = __builtin_amdgcn_exp2f(least - m1.x);
+    const f32x4_t o0 = out[at] * f0 + out[at + 4 * NC * 64] * f1, o1 = out[at + 32] * f0 + out[at + 4 * NC * 64 + 32] * f1;
+    const float2 m = make_float2(least, m0.y * f0 + m1.y * f1);
+    if (keys.active == 1) {
+      const float r = m.y == 0.f ? 0.f : 1.f / m.y;
+      *reinterpret_cast<pg_u4*>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + 8 * n) =
+          pg_u4{pg_pack<DT>(o0[0] * r, o0[1] * r), pg_pack<DT>(o0[2] * r, o0[3] * r), pg_pack<DT>(o1[0] * r, o1[1] * r),
+                pg_pack<DT>(o1[2] * r, o1[3] * r)};
+    } else {
+      const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
+      const long col = (place * COLS + y) * a.splits + split;
+      *reinterpret_cast<f32x4_t*>(a.part + col * D + 8 * n) = o0;
+      *reinterpret_cast<f32x4_t*>(a.part + col * D + 8 * n + 4) = o1;
+      if (n == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + col * 2) = make_float2(wide_up<DT> - m.x, m.y);
     }
-  } else {
-    const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
-    const long at = (place * COLS + 32 * wave + li) * a.splits + split;
-#pragma unroll
-    for (int n = 0; n < 4 * ND; ++n) {
-      const pg_f16& x = acc[n / 4];
-      *reinterpret_cast<f32x4_t*>(a.part + at * D + 8 * n + 4 * lh) =
-          f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
-    }
-    if (lh == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(wide_up<DT> - add, L);
   }
 }
 
