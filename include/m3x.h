@@ -639,9 +639,8 @@ size_t m3x_paged_attn_workspace(int tiles, int kv_heads, int heads, int tile_row
  * tiles (device): ntiles pairs (first row, rows <= tile_rows) of rows of one slot at consecutive positions, of which the
  * first row's slot and position are read; NULL: ntiles single rows 0, 1, ... (tile_rows 1). Rows in no tile are left as
  * they are; a pair with no rows (or a negative number of them) is skipped. rows + 65536 n: n splits at most for this tile.
- * cols: columns (a tile's rows x query heads of a kv head) that a workgroup
- * takes, 16, 32 or, with heads of 64, 48 (few columns, bound by the keys' bytes) or 128 (prompts); at most 65535 tiles, and
- * fewer than 2^16 - cols columns a tile. A tile's keys are divided among up to `splits` <= 256 workgroups; arrived (device,
+ * cols: columns (a tile's rows x query heads of a kv head) that a workgroup takes, 16, 32 or, with heads of 64, 48 (few
+ * columns, bound by the keys' bytes) or 128 (prompts); at most 65535 tiles, and fewer than 2^16 - cols columns a tile. A tile's keys are divided among up to `splits` <= 256 workgroups; arrived (device,
  * for splits > 1 and cols other than 128): tiles x kv_heads x ceil(tile_rows x heads / kv_heads / cols) int32, zeroed before
  * the first call and left so. Weights are rounded to the 16-bit type and summed as rounded; all else is fp32, in a fixed
  * order. Scores times |scale| log2(e) are to be finite. What a row does not see has no part in its result, whatever it

@@ -237,9 +237,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t pg_span(float* p) {
 // dims d .. d + 3 of a column's output from its splits' partial results, in their order; AUX: how they are read. The
 // addresses are a place's (uniform, 64-bit) and a column's within it (below PG_SPAN bytes: 128 columns of 256 splits).
 template <int DT, int D, int AUX>
-__device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, const Col& cc, long place, int cols, int col, long ncols, int active,
-                                        int d) {
-  const auto po = pg_span(a.part + place * cols * a.splits * D), ml = pg_span(a.part + ncols * a.splits * D + place * cols * a.splits * 2);
+__device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, const Col& cc, long place, int cols, int col,
+                                        long ncols, int active, int d) {
+  const auto po = pg_span(a.part + place * cols * a.splits * D);
+  const auto ml = pg_span(a.part + ncols * a.splits * D + place * cols * a.splits * 2);
   float M = -INFINITY, L = 0.f;
   f32x4_t O = {0.f, 0.f, 0.f, 0.f};
   // eight splits' loads at a time, of no bytes behind the last
@@ -251,7 +252,8 @@ __device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, cons
       const int at = col * a.splits + s0 + e;
       const bool in = s0 + e < active;
       x[e] = __builtin_bit_cast(float2, (pg_u2)__builtin_amdgcn_raw_buffer_load_b64(ml, in ? at * 8 : PG_SPAN, 0, AUX));
-      o[e] = __builtin_bit_cast(f32x4_t, (pg_u4)__builtin_amdgcn_raw_buffer_load_b128(po, in ? (at * D + d) * 4 : PG_SPAN, 0, AUX));
+      o[e] = __builtin_bit_cast(
+          f32x4_t, (pg_u4)__builtin_amdgcn_raw_buffer_load_b128(po, in ? (at * D + d) * 4 : PG_SPAN, 0, AUX));
     }
     float mx = M;
 #pragma unroll
@@ -534,8 +536,9 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(pg_u4, O), pg_span(a.part + place * COLS * a.splits * D),
                                              (at * D + d) * 4, 0, PG_SC1);
       if (d == 0)
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(pg_u2, make_float2(M, L)),
-                                              pg_span(a.part + ncols * a.splits * D + place * COLS * a.splits * 2), at * 8, 0, PG_SC1);
+        __builtin_amdgcn_raw_buffer_store_b64(
+            __builtin_bit_cast(pg_u2, make_float2(M, L)),
+            pg_span(a.part + ncols * a.splits * D + place * COLS * a.splits * 2), at * 8, 0, PG_SC1);
     }
   }
   // The split that is done last joins them, in their order whichever it is. Its place's counter is 0 again afterwards.

@@ -1105,8 +1105,8 @@ def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, cut=0):
     """The tiles of paged_attn for rows laid out as runs, (first row, rows, first position) each, of one slot at
     consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to narrow_cols columns is one narrow
     tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first; with cut > 0
-narrow tiles of up to `cut` columns instead, a run's one behind the other (32 runs of 32 rows onto 500 keys 19.7 us, dealt
-    by their keys alone 22.8)."""
+    narrow tiles of up to `cut` columns instead, a run's one behind the other (32 runs of 32 rows onto 500 keys 19.7 us,
+    dealt by their keys alone 22.8)."""
     G = heads // kv_heads
     r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
     r = r[r[:, 1] > 0]
@@ -1175,10 +1175,12 @@ class PagedPlan:
         """What each launch gets of the runs: (tiles, the runs that they are of, whether wide) of the single rows, of the
         narrow tiles and of the wide ones. Runs of up to narrow_cols columns are one narrow tile; longer ones are cut into
         narrow tiles where _few says so or they have no more than long_cols columns. Single rows go along with up to `room`
-        narrow tiles where they are up to a workgroup a CU, or if together (measured on MI355X, 16/8 heads of 128, us: 8 rows of 2048 keys beside
-        a prompt of 56 20 together, 33 apart; 24 beside one of 488 onto 1000 keys 40, 50, beside one of 1000 42, 64; 64
-        beside one of 192 97, 90; 224 beside one of 288 317, 286: a kernel for more columns reads many single rows' keys
-        more slowly, 64 rows of 2048 95 us against 80)."""
+        narrow tiles where they are up to a workgroup a CU, or if `together`.
+
+        Measured on MI355X (16/8 heads of 128, us): 8 rows of 2048 keys beside a prompt of 56 20 together, 33 apart; 24
+        beside one of 488 onto 1000 keys 40, 50, beside one of 1000 42, 64; 64 beside one of 192 97, 90; 224 beside one of
+        288 317, 286: a kernel for more columns reads many single rows' keys more slowly, 64 rows of 2048 95 us against
+        80."""
         G = self.heads // self.kv_heads
         single, rest = r[r[:, 1] == 1], r[r[:, 1] > 1]
         none = np.empty((0, 2), dtype=np.int32)
@@ -1239,7 +1241,7 @@ class PagedPlan:
     def _reserve(self, n, tile_rows, wide, device):
         """A launch of up to n tiles, with splits for few of them: up to 2048 workgroups, most of which have nothing to do (64
         rows, all of a prompt onto 3900 keys 40 us unsplit, 31 so; onto 16 keys 7.9 and 8.1)."""
-        tiles = torch.zeros(n, 2, dtype=torch.int32, device=device)
+        tiles = torch.zeros(n, 2, dtype=torch.int32).to(device)
         self._add(tiles, n, tile_rows, 0, wide)
         cols = self.launches[-1][3]
         blocks = n * self._blocks(np.array([[0, tile_rows]]), cols)
@@ -1297,7 +1299,8 @@ class PagedPlan:
             self._index = -1
         G, split = self.heads // self.kv_heads, [x for x in self.launches if x[4] > 1 and x[3] != WIDE_COLS]
         need = max([0] + [n * self.kv_heads * -(-tr * G // cols) for _, n, tr, cols, _ in split])
-        self._arrived = torch.zeros(need, dtype=torch.int32, device=device) if need else None
+        # (copied, not filled on the device: in place for every stream)
+        self._arrived = torch.zeros(need, dtype=torch.int32).to(device) if need else None
         at = self._arrived.data_ptr() if need else 0
         self._calls = [(0 if t is None else t.data_ptr(), n, tr, cols, s, at) for t, n, tr, cols, s in self.launches]
 
@@ -1307,18 +1310,19 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     each.
 
     Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) and one to two and a half workgroups
-    a CU without, two where that evens out what the CUs get; at least 256 keys each, three times as many to begin with (the join's 3 to 5 us:
-    64 rows onto 500 keys 12.4 whole, 13.6 to 17 split). Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3
-    whole, 14.5 / 10.3 / 8.6 / 8.5 / 8.5 at 2 / 4 / 8 / 16 / 32 splits; 16 rows 34.2, 24.4, 28.8 (3), 24.9 (4); 48 of a
-    1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys 116, 102; 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 /
-    17.3 / 21.5 at 1 / 2 / 4 / 8 / 16; 512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at
-    16 / 32 / 64 / 128; 30 x 5 rows over up to 3001 29.2 / 26.8 / 23.7 / 22.2 / 26.8 at 1 / 2 / 3 / 4 / 6.
+    a CU without, two where that evens out what the CUs get; at least 256 keys each, and three times as many to begin with
+    (the join's 3 to 5 us: 64 rows onto 500 keys 12.4 whole, 13.6 to 17 split). Measured on MI355X (graph-timed, us, 16/8
+    heads of 128): one row at 2048 keys 21.3 whole, 14.5 / 9.8 / 8.0 / 8.2 at 2 / 4 / 8 / 16 splits; 16 rows 34.2, 24.4,
+    28.8 (3), 24.9 (4); 48 of a 1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys
+    116, 102; 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 / 17.3 / 21.5 at 1 / 2 / 4 / 8 / 16;
+    512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at 16 / 32 / 64 / 128; 30 x 5 rows
+    over up to 3001 29.2 / 26.8 / 23.7 / 22.2 / 26.8 at 1 / 2 / 3 / 4 / 6.
 
     Prompts: the least of what the tiles' turns of 32 keys take (1.05 us for one of two groups of waves that share a
     workgroup's keys, which they do up to a workgroup a CU; 0.52 for each of more workgroups that share a CU; the longest
     tile alone 0.75) and, from two on, the join's launch and partial results (3 us, 3 TB/s). Measured: 512 rows over 2048
-    keys 43.9 / 33.5 / 27.1 / 32.5 at 1 / 2 / 4 / 8; 64 rows over 4000 22.5 / 20.3 / 23.8 at 8 / 16 / 32; 8 x 200 rows over
-    500 22.9 / 31.9 at 1 / 2."""
+    keys 43.9 / 33.5 / 27.1 / 32.5 at 1 / 2 / 4 / 8; 64 rows over 32000 77 / 49 / 40 at 8 / 16 / 32; 8 x 200 rows
+    over 500 21.0 / 31.0 at 1 / 2."""
     blocks, mean_keys = max(blocks, 1), keys if mean_keys is None else max(mean_keys, 1)
     if cols != WIDE_COLS:
         if blocks > 256 and cols == 16:
