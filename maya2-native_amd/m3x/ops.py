@@ -1310,10 +1310,11 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     each.
 
     Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) and one to two and a half workgroups
-    a CU without, two where that evens out what the CUs get; at least 256 keys each, and three times as many to begin with
-    (the join's 3 to 5 us: 64 rows onto 500 keys 12.4 whole, 13.6 to 17 split). Measured on MI355X (graph-timed, us, 16/8
-    heads of 128): one row at 2048 keys 21.3 whole, 14.5 / 9.8 / 8.0 / 8.2 at 2 / 4 / 8 / 16 splits; 16 rows 34.2, 24.4,
-    28.8 (3), 24.9 (4); 48 of a 1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys
+    a CU without, two where that evens out what the CUs get. At least 128 keys each for one row's heads up to 8 splits (the
+    join is 1 us of 6 to 8: one row at 250 keys 5.8 whole, 6.4 split, at 700 keys 9.8 / 8.4 / 7.1 / 6.6 at 1 / 2 / 4 / 8, at
+    1500 16.5 / 11.7 / 8.6 / 7.5), else 256, and three times as many to begin with (the join is 3 to 5: 64 rows onto 500 keys
+    12.4 whole, 13.6 to 17 split). Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3 whole,
+    14.5 / 9.8 / 8.0 / 8.2 at 2 / 4 / 8 / 16 splits; 16 rows 34.2, 24.4, 28.8 (3), 24.9 (4); 48 of a 1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys
     116, 102; 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 / 17.3 / 21.5 at 1 / 2 / 4 / 8 / 16;
     512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at 16 / 32 / 64 / 128; 30 x 5 rows
     over up to 3001 29.2 / 26.8 / 23.7 / 22.2 / 26.8 at 1 / 2 / 3 / 4 / 6.
@@ -1330,7 +1331,10 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
                 return -(-blocks * s // 256) * 256 / (blocks * s)
             uneven = 4 * mean_keys < 3 * keys or spare(1) > 1.1 * spare(2)
             return 2 if uneven and blocks <= 640 and keys >= 1024 else 1
-        return max(1, min(256 * keys // max(1, blocks * mean_keys), keys // 256, 64)) if keys >= 768 else 1
+        if keys < (384 if cols == 16 else 768):
+            return 1
+        most = min(max(8, keys // 256), keys // 128, 64) if cols == 16 else min(keys // 256, 64)
+        return max(1, min(256 * keys // max(1, blocks * mean_keys), most))
 
     def time(s):
         work = blocks * s

@@ -153,7 +153,7 @@ def test_splits():
             for cols in (16, 32, 128):
                 s = ops.paged_attn_splits(blocks, keys, cols, keys // 2, blocks * cols)
                 assert 1 <= s <= 256 and (s == 1 or s * 128 <= keys)
-    assert ops.paged_attn_splits(30, 3000, 48, 1) <= 11 and ops.paged_attn_splits(1, 700, 16) == 1 and ops.paged_attn_splits(160, 3000, 48, 1500) == 3
+    assert ops.paged_attn_splits(30, 3000, 48, 1) <= 11 and ops.paged_attn_splits(1, 383, 16) == ops.paged_attn_splits(1, 767, 32) == 1 and ops.paged_attn_splits(160, 3000, 48, 1500) == 3
     assert ops.paged_attn_splits(1792, 2048, 16) == 1 and ops.paged_attn_splits(8, 2048, 16) == 8
 
 
