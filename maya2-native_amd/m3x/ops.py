@@ -1042,16 +1042,27 @@ def _paged_heads(name, what, t, cache, shape):
     return ptr, sr, sh
 
 
+def _paged_elsewhere(cache, fn, *args):
+    """A call whose cache is not on the current device: made there."""
+    _on_gpu(fn.__name__, cache)
+    with torch.cuda.device(cache._index):
+        return fn(*args)
+
+
 def paged_append(k, v, cache, slots, pos):
     """K and V rows [rows, kv_heads, head_dim] (the cache's type, any row and head strides) to position pos[r] (int32) of
     slot slots[r] (int64). A row whose slot, position or page is outside the cache is not written; rows at one place leave
     a mixture there."""
     rows, sp, pp = _paged_rows("paged_append", cache, slots, pos)
     shape = rows, cache.kv_heads, cache.head_dim
-    ka = _paged_heads("paged_append", "k", k, cache, shape)
-    va = _paged_heads("paged_append", "v", v, cache, shape)
-    _on_gpu("paged_append", cache)
-    _launch(cache._index, lib().m3x_paged_append, cache._ref, *ka, *va, sp, pp, rows)
+    kp, kr, kh = _paged_heads("paged_append", "k", k, cache, shape)
+    vp, vr, vh = _paged_heads("paged_append", "v", v, cache, shape)
+    dev = cache._index
+    if dev < 0 or dev != _current_device():
+        return _paged_elsewhere(cache, paged_append, k, v, cache, slots, pos)
+    rc = lib().m3x_paged_append(cache._ref, kp, kr, kh, vp, vr, vh, sp, pp, rows, _raw_stream(dev))
+    if rc:
+        check(rc, "paged_append")
 
 
 def qk_norm_rope_paged(qkv, q_out, cache, slots, pos, rotary, wq, wk, eps, heads):
@@ -1066,7 +1077,7 @@ def qk_norm_rope_paged(qkv, q_out, cache, slots, pos, rotary, wq, wk, eps, heads
         raise ValueError(f"{name}: qkv must be [{rows}, {width}], got {tuple(qkv.shape)}")
     if not isinstance(rotary, Rotary) or rotary.dim > D:
         raise ValueError(f"{name}: rotary must be an ops.Rotary of at most {D} dims")
-    qa = _paged_heads(name, "q_out", q_out, cache, (rows, heads, D))
+    op, orow, oh = _paged_heads(name, "q_out", q_out, cache, (rows, heads, D))
     qp, (s_qkv, s_one) = qkv.data_ptr(), qkv.stride()
     if qkv.dtype != cache.dtype or qkv.get_device() != cache._index or rotary._index != cache._index:
         raise ValueError(f"{name}: qkv must be {cache.dtype} on {cache.device}, as the rotation, got {qkv.dtype} on "
@@ -1081,10 +1092,13 @@ def qk_norm_rope_paged(qkv, q_out, cache, slots, pos, rotary, wq, wk, eps, heads
         if (wqp | wkp) & 15 or wq.dtype != cache.dtype or wk.dtype != cache.dtype or not wq.is_contiguous() or \
                 not wk.is_contiguous() or wq.get_device() != cache._index or wk.get_device() != cache._index:
             raise ValueError(f"{name}: wq and wk must be contiguous, 16-byte aligned {cache.dtype} on {cache.device}")
-    if cache._index < 0:
-        _on_gpu(name, cache)
-    _launch(cache._index, lib().m3x_qk_norm_rope_paged, cache._ref, qp, s_qkv, *qa, sp, pp, rotary._ref, wqp, wkp, eps,
-            rows, heads)
+    dev = cache._index
+    if dev < 0 or dev != _current_device():
+        return _paged_elsewhere(cache, qk_norm_rope_paged, qkv, q_out, cache, slots, pos, rotary, wq, wk, eps, heads)
+    rc = lib().m3x_qk_norm_rope_paged(cache._ref, qp, s_qkv, op, orow, oh, sp, pp, rotary._ref, wqp, wkp, eps, rows, heads,
+                                      _raw_stream(dev))
+    if rc:
+        check(rc, name)
 
 
 def paged_read(cache, slots, pos, k, v):
@@ -1092,10 +1106,14 @@ def paged_read(cache, slots, pos, k, v):
     zeros where there is none."""
     rows, sp, pp = _paged_rows("paged_read", cache, slots, pos)
     shape = rows, cache.kv_heads, cache.head_dim
-    ka = _paged_heads("paged_read", "k", k, cache, shape)
-    va = _paged_heads("paged_read", "v", v, cache, shape)
-    _on_gpu("paged_read", cache)
-    _launch(cache._index, lib().m3x_paged_read, cache._ref, sp, pp, *ka, *va, rows)
+    kp, kr, kh = _paged_heads("paged_read", "k", k, cache, shape)
+    vp, vr, vh = _paged_heads("paged_read", "v", v, cache, shape)
+    dev = cache._index
+    if dev < 0 or dev != _current_device():
+        return _paged_elsewhere(cache, paged_read, cache, slots, pos, k, v)
+    rc = lib().m3x_paged_read(cache._ref, sp, pp, kp, kr, kh, vp, vr, vh, rows, _raw_stream(dev))
+    if rc:
+        check(rc, "paged_read")
 
 
 NARROW_COLS, WIDE_COLS = 32, 128  # columns (rows x query heads of a kv head) that a workgroup of either kernel takes
@@ -1361,8 +1379,8 @@ def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
         raise ValueError(f"paged_attn: a plan of {plan.rows} rows, {heads} / {plan.kv_heads} heads of {plan.head_dim} for "
                          f"{rows} rows over {cache.kv_heads} kv heads of {cache.head_dim} on {cache.device}")
     shape = rows, heads, plan.head_dim
-    qa = _paged_heads("paged_attn", "q", q, cache, shape)
-    oa = _paged_heads("paged_attn", "out", out, cache, shape)
+    qp, qr, qh = _paged_heads("paged_attn", "q", q, cache, shape)
+    op, orow, oh = _paged_heads("paged_attn", "out", out, cache, shape)
     if not abs(scale) <= 2.0 ** 126:
         raise ValueError(f"paged_attn: |scale| must be at most 2^126, got {scale}")
     ws, ws_bytes = 0, 0
@@ -1373,10 +1391,15 @@ def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
             raise ValueError(f"paged_attn: a workspace of {plan.workspace} bytes is needed, got {ws_bytes}")
         if not workspace.is_contiguous() or ws % 16 or workspace.get_device() != cache._index:
             raise ValueError(f"paged_attn: the workspace must be contiguous, 16-byte aligned and on {cache.device}")
-    _on_gpu("paged_attn", cache)
+    dev = cache._index
+    if dev < 0 or dev != _current_device():
+        return _paged_elsewhere(cache, paged_attn, q, cache, out, slots, pos, scale, plan, workspace)
+    fn, stream = lib().m3x_paged_attn, _raw_stream(dev)
     for tiles, n, tile_rows, cols, splits, arrived in plan._calls:
-        _launch(cache._index, lib().m3x_paged_attn, cache._ref, *qa, *oa, sp, pp, tiles, n, tile_rows, cols, scale, rows,
-                heads, plan.window, plan.sinks, splits, ws, ws_bytes, arrived)
+        rc = fn(cache._ref, qp, qr, qh, op, orow, oh, sp, pp, tiles, n, tile_rows, cols, scale, rows, heads, plan.window,
+                plan.sinks, splits, ws, ws_bytes, arrived, stream)
+        if rc:
+            check(rc, "paged_attn")
 
 
 # ---------------------------------------------------------------- Mimi decode (serve/fast_codec.py)
