@@ -34,13 +34,21 @@ class PagePool:
     def free_pages(self):
         return len(self._free)
 
+    def _check(self, *slots):
+        for slot in slots:
+            if not 0 <= slot < self.slots:
+                raise IndexError(f"slot {slot} outside 0..{self.slots - 1}")
+
     def held(self, slot):
         """Pages that the slot names."""
+        self._check(slot)
         return int((self._host[slot] >= 0).sum())
 
     def has(self, slot, length):
         """Whether the slot's first `length` positions all lie in pages."""
-        return bool((self._host[slot, :-(-length // self.page_size)] >= 0).all())
+        self._check(slot)
+        end = -(-int(length) // self.page_size)
+        return end <= self.width and bool((self._host[slot, :max(end, 0)] >= 0).all())
 
     def _set(self, slot, at, page):
         self._host[slot, at] = page
@@ -59,6 +67,7 @@ class PagePool:
         with nothing taken, when the pool has too few."""
         todo, ends = [], {}
         for slot, length in wants:
+            self._check(slot)
             end = -(-int(length) // self.page_size)
             if end > self.width:
                 raise ValueError(f"slot {slot}: {length} positions exceed the table's {self.width * self.page_size}")
@@ -74,6 +83,7 @@ class PagePool:
 
     def trim(self, slot, first, keep=0):
         """Lets go of the pages that hold only positions below `first`, but for those of the first `keep`."""
+        self._check(slot)
         end = min(int(first) // self.page_size, self._end[slot])
         begin = max(self._begin[slot], -(-int(keep) // self.page_size))
         for at in range(begin, end):
@@ -82,6 +92,7 @@ class PagePool:
 
     def release(self, slot):
         """Lets go of all of the slot's pages."""
+        self._check(slot)
         for at in range(self._end[slot]):
             self._drop(slot, at)
         self._end[slot] = self._begin[slot] = 0
@@ -90,7 +101,8 @@ class PagePool:
         """Gives the (empty) slot the whole pages of the source's first `length` positions and, for what is left of them, a
         new page. Returns (page of the source, new page) when that is something, to be copied, else None. RuntimeError
         when the pool has no page for it, ValueError when the source has let go of one."""
-        whole, rest = divmod(int(length), self.page_size)
+        self._check(slot, source)
+        whole, rest = divmod(max(int(length), 0), self.page_size)
         if self._end[slot]:
             raise ValueError(f"slot {slot} holds pages")
         if not self.has(source, length):

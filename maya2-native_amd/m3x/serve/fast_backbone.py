@@ -256,6 +256,7 @@ class StaticBackbone:
         replay a captured step do it first. RuntimeError when the pool has too few pages."""
         if self.pages is None:
             return
+        check_slots(slots, self.max_slots)
         for s in slots:
             self._trim(s)
         self.pages.grow([(s, self.lengths_cpu[s] + ahead) for s in slots])

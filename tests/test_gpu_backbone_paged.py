@@ -274,6 +274,10 @@ def test_refusals(gpu):
         sb.fork(0, 1, 2)
     with pytest.raises(IndexError):
         sb.fork(0, S)
+    with pytest.raises(IndexError):
+        sb.reserve([-1])
+    with pytest.raises(ValueError):
+        sb.reserve([0], CAP + 1)
     with pytest.raises(ValueError):
         sb.fork(1, 1)
     with pytest.raises(ValueError):

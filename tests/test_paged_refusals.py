@@ -319,6 +319,22 @@ def test_pool_share():
     _sound(p)
 
 
+def test_pool_outside():
+    """Slots and lengths outside the table are refused, with nothing changed."""
+    p = _pool()
+    p.grow([(0, 112)])
+    for s in (-1, 4):
+        for call in (lambda: p.held(s), lambda: p.has(s, 1), lambda: p.grow([(1, 5), (s, 5)]), lambda: p.trim(s, 5),
+                     lambda: p.release(s), lambda: p.share(s, 0, 5), lambda: p.share(1, s, 0)):
+            with pytest.raises(IndexError):
+                call()
+    assert p.has(0, 112) and not p.has(0, 113) and p.has(1, 0) and p.has(1, -3)
+    with pytest.raises(ValueError):
+        p.share(1, 0, 113)
+    assert p.held(1) == 0 and p.free_pages == 3
+    _sound(p)
+
+
 def test_pool_random():
     """A long run of grows, trims, shares and releases keeps the counts."""
     rng = np.random.default_rng(1)
