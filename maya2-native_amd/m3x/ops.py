@@ -1122,28 +1122,24 @@ NARROW_COLS, WIDE_COLS = 32, 128  # columns (rows x query heads of a kv head) th
 def paged_tiles(runs, heads, kv_heads, narrow_cols=NARROW_COLS, cut=0):
     """The tiles of paged_attn for rows laid out as runs, (first row, rows, first position) each, of one slot at
     consecutive positions: (narrow, wide), int32 [n, 2] of (first row, rows). A run of up to narrow_cols columns is one narrow
-    tile, a longer one wide tiles of up to 128 columns and about the same size, those with the most keys first; with cut > 0
-    narrow tiles of up to `cut` columns instead, a run's one behind the other (32 runs of 32 rows onto 500 keys 19.7 us,
-    dealt by their keys alone 22.8)."""
+    tile, a longer one wide tiles of up to 128 columns and about the same size; with cut > 0 narrow tiles of up to `cut`
+    columns instead, a run's one behind the other (they read the same keys at about the same time: 32 runs of 32 rows onto
+    500 keys 19.7 us, dealt by their keys alone 22.8). Those with the most keys come first, so that the last ones to finish
+    are short (61 rows of up to 4000 keys 93 us, in no order 102 to 112; 30 x 5 of up to 3001 20.0, 21.4)."""
     G = heads // kv_heads
     r = np.asarray(runs, dtype=np.int64).reshape(-1, 3)
     r = r[r[:, 1] > 0]
+    r = r[np.argsort(-(r[:, 2] + r[:, 1]), kind="stable")]
     few = (r[:, 1] * G <= narrow_cols) | (r[:, 1] == 1)
     most = max(1, (cut or WIDE_COLS) // G)
-    long = r[~few]
-    n = -(-long[:, 1] // most)
+    long = r if cut else r[~few]
+    n = np.where(few, 1, -(-r[:, 1] // most)) if cut else -(-long[:, 1] // most)
     of = np.repeat(np.arange(len(long)), n)
     at = np.arange(len(of)) - np.repeat(np.cumsum(n) - n, n)
     a, b = at * long[of, 1] // n[of], (at + 1) * long[of, 1] // n[of]
-    # a cut run's tiles one behind the other: they read the same keys at about the same time
-    if cut:
-        order = np.lexsort((-at, of, -(long[:, 2] + long[:, 1])[of]))
-    else:
-        order = np.argsort(-(long[of, 2] + b), kind="stable")
-    tiles = np.stack([long[of, 0] + a, b - a], 1)[order]
-    if cut:
-        return np.concatenate([r[few, :2], tiles]).astype(np.int32), np.empty((0, 2), dtype=np.int32)
-    return r[few, :2].astype(np.int32), tiles.astype(np.int32)
+    order = np.lexsort((-at, of)) if cut else np.argsort(-(long[of, 2] + b), kind="stable")
+    tiles = np.stack([long[of, 0] + a, b - a], 1)[order].astype(np.int32)
+    return (tiles, tiles[:0]) if cut else (r[few, :2].astype(np.int32), tiles)
 
 
 def _narrow_cols(head_dim):
@@ -1214,10 +1210,21 @@ class PagedPlan:
         live = int((single[:, 2] >= 0).sum())
         if together or (len(single) and len(cut) and len(single) + len(cut) <= room and
                         live * self._blocks(single, NARROW_COLS) <= 256):
-            cut, short, single = np.concatenate([single[:, :2], cut]), np.concatenate([single, short]), single[:0]
-        elif live == 0 and len(wide) and room == 65535:  # for their zeros, instead of a launch of their own
+            short, single = np.concatenate([single, short]), single[:0]
+            cut = paged_tiles(short, self.heads, self.kv_heads, narrow_cols, cut=NARROW_COLS)[0]
+        elif self._uneven(single):
+            single = single[np.argsort(-single[:, 2], kind="stable")]
+        if live == 0 and len(single) and len(wide) and room == 65535:  # for their zeros, instead of a launch of their own
             wide, single = np.concatenate([wide, single[:, :2]]), single[:0]
         return (single[:, :2], single, False), (cut, short, False), (wide, rest, True)
+
+    def _ends(self, runs):
+        """Keys that the runs' last rows see, about."""
+        return (runs[:, 2] + runs[:, 1]).clip(0, self.window + self.sinks + 1 if self.window else None)
+
+    def _uneven(self, runs):
+        ends = self._ends(runs)
+        return len(ends) > 0 and 3 * int(ends.max()) > 4 * ends.mean()
 
     def _blocks(self, tiles, cols):
         """Workgroups a tile (and split)."""
