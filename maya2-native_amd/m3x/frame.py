@@ -120,7 +120,7 @@ class FrameStep:
 
     def replay(self, g):
         self._check_room(g, g.seats)
-        self.bb.reserve(g.seats)
+        self.bb.stage_seats(g.bufs[0], g.seats)
         if g.graph is not None:
             g.graph.replay()
         else:

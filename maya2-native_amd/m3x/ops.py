@@ -1212,7 +1212,7 @@ class PagedPlan:
                         live * self._blocks(single, NARROW_COLS) <= 256):
             short, single = np.concatenate([single, short]), single[:0]
             cut = paged_tiles(short, self.heads, self.kv_heads, narrow_cols, cut=NARROW_COLS)[0]
-        elif self._uneven(single):
+        elif self.uneven(single):
             single = single[np.argsort(-single[:, 2], kind="stable")]
         if live == 0 and len(single) and len(wide) and room == 65535:  # for their zeros, instead of a launch of their own
             wide, single = np.concatenate([wide, single[:, :2]]), single[:0]
@@ -1222,8 +1222,9 @@ class PagedPlan:
         """Keys that the runs' last rows see, about."""
         return (runs[:, 2] + runs[:, 1]).clip(0, self.window + self.sinks + 1 if self.window else None)
 
-    def _uneven(self, runs):
-        ends = self._ends(runs)
+    def uneven(self, runs):
+        """Whether the longest of the runs has more than 4/3 of their mean's keys."""
+        ends = self._ends(np.asarray(runs))
         return len(ends) > 0 and 3 * int(ends.max()) > 4 * ends.mean()
 
     def _blocks(self, tiles, cols):
@@ -1242,17 +1243,25 @@ class PagedPlan:
         return blocks <= 512 and blocks * keys <= 600_000
 
     @classmethod
-    def reserve(cls, rows, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda"):
-        """A plan for any layout of up to `rows` rows, what a captured graph launches: before a call, `tiles` of its runs go
-        into the tensors of its `launches`: single rows (up to two workgroups a CU together with the next), narrow tiles and,
-        for more rows than _few takes if all are one prompt, wide ones. A launch that gets no tile costs 1 to 3 us."""
+    def reserve(cls, rows, heads, kv_heads, head_dim, max_ctx, window=0, sinks=0, device="cuda", single=False):
+        """A plan for any layout of up to `rows` rows (single: in runs of one row), what a captured graph launches: before a
+        call, `tiles` of its runs go into the tensors of its `launches`: single rows (up to two workgroups a CU together with
+        the next), narrow tiles and, for more rows than _few takes if all are one prompt, wide ones. A launch that gets no
+        tile costs 1 to 3 us."""
         if kv_heads < 1 or heads < 1 or heads % kv_heads or rows < 1:
             raise ValueError(f"PagedPlan: {rows} rows, {heads} query heads over {kv_heads} kv heads")
         self = cls([], heads, kv_heads, head_dim, max_ctx, window, sinks, device)
         G = heads // kv_heads
         few, most = max(1, NARROW_COLS // G), max(1, WIDE_COLS // G)
         self.rows = rows
-        self._apart = rows * self._blocks(np.array([[0, 1]]), NARROW_COLS) > 512  # single rows have a launch of their own
+        one = self._blocks(np.array([[0, 1]]), NARROW_COLS)
+        self._apart = single or rows * one > 512  # single rows have a launch of their own
+        if single:  # as many splits as even rows take, two at least where uneven ones may
+            self._reserve(rows, 1, False, device)
+            most = paged_attn_splits(rows * one, max_ctx, self.launches[0][3], head_dim=head_dim)
+            self.launches[0] = (*self.launches[0][:4], max(most, 2 if 256 < rows * one <= 640 else 1))
+            self._finish(torch.device(device))
+            return self
         if self._apart:
             self._reserve(rows, 1, False, device)
         # runs of two rows and more: a tile's part of them is the largest where one row more makes two tiles
@@ -1278,8 +1287,10 @@ class PagedPlan:
         r = self._runs(runs)
         if len(r) and (r[:, 0] + r[:, 1]).max() > self.rows:
             raise ValueError(f"PagedPlan: runs past the {self.rows} rows that the plan is for")
+        if len(self.launches) == self._apart and (r[:, 1] > 1).any():
+            raise ValueError(f"PagedPlan: a run of {r[:, 1].max()} rows, reserved for single ones")
         wide = self.launches[-1][3] == WIDE_COLS
-        lists = self._deal(r, 0, self.launches[self._apart][1], WIDE_COLS // 2 if wide else 1 << 31, not self._apart)
+        lists = self._deal(r, 0, self.launches[-1 - wide][1], WIDE_COLS // 2 if wide else 1 << 31, not self._apart)
         lists = lists[not self._apart:]
         out = []
         for (x, of, _), (_, n, tile_rows, cols, splits) in zip(lists, self.launches):

@@ -106,11 +106,11 @@ def _join(modules):
 
 class _StepGraph:
     """One (row bucket, context bucket[, inline prefills | item launch]) step: buffers, row table, item upload,
-    graph, the key of the decode item list last uploaded, and the uploads of a paged step's tiles."""
-    __slots__ = ("bufs", "items", "graph", "items_key", "tiles")
+    graph, and the key of the decode item list last uploaded."""
+    __slots__ = ("bufs", "items", "graph", "items_key")
 
     def __init__(self, bufs):
-        self.bufs, self.items, self.graph, self.items_key, self.tiles = bufs, None, None, None, ()
+        self.bufs, self.items, self.graph, self.items_key = bufs, None, None, None
 
 
 class StaticBackbone:
@@ -250,6 +250,7 @@ class StaticBackbone:
         if self.window:
             self.pages.trim(slot, self.lengths_cpu[slot] - self.window + 1, self.sinks)
 
+    @torch.inference_mode()
     def reserve(self, slots, ahead=1):
         """Paged cache: takes the pages that the slots' next `ahead` positions need (and lets go of those behind their
         windows) and sends the table, in stream order before what follows. Steps do it by themselves; programs that
@@ -395,12 +396,17 @@ class StaticBackbone:
         b.items = None
         if self.pages is not None:
             args = (H, KV, D, ctx, self.window, self.sinks, dev)
-            b.plan = ops.PagedPlan.reserve(rows, *args) if mixed else ops.PagedPlan([(r, 1, 0) for r in range(rows)], *args)
+            staged = mixed or rows >= ITEM_MIN_ROWS
+            one = [(r, 1, 0) for r in range(rows)]
+            b.plan = ops.PagedPlan.reserve(rows, *args, single=not mixed) if staged else ops.PagedPlan(one, *args)
             if self._attn_ws.numel() * 4 < b.plan.workspace:  # one for all graphs: their steps follow each other
                 self._attn_ws = torch.empty(b.plan.workspace // 4, dtype=torch.float32, device=dev)
             b.attn_ws = self._attn_ws
-            if mixed:  # until a step stages its own: a tile a row
-                b.plan.launches[0][0].copy_(torch.from_numpy(b.plan.tiles([(r, 1, 0) for r in range(rows)])[0]))
+            b.tiles, b.tiles_key = (), None
+            if staged:  # until a step stages its own: a tile a row
+                for (into, *_), tiles in zip(b.plan.launches, b.plan.tiles(one)):
+                    into.copy_(torch.from_numpy(tiles))
+                b.tiles = tuple(Upload(x[0], ring=2) for x in b.plan.launches)
             return b
         if self.kv_bits == 4:
             b.chunk = ops.kv4_attn_chunk(rows, H, KV, ctx, D)
@@ -550,8 +556,6 @@ class StaticBackbone:
         g = _StepGraph(self.make_buffers(rows, ctx, mixed, items))
         if g.bufs.items is not None:
             g.items = Upload(g.bufs.items, ring=2)
-        if self.pages is not None and mixed:
-            g.tiles = tuple(Upload(x[0], ring=2) for x in g.bufs.plan.launches)
         if self.use_graphs:
             if self.pool is None:
                 self.pool = torch.cuda.graph_pool_handle()
@@ -582,6 +586,37 @@ class StaticBackbone:
             return False
         ctxs = np.asarray(runs, dtype=np.int64).reshape(-1, 3)[:, 2] + 1
         return int(ctxs.max()) > ITEM_SKEW * (int(ctxs.sum()) / len(ctxs))
+
+    def _stage_tiles(self, b, runs, n, decode):
+        """A paged step's tiles into the buffers' plan: of a mixed step's runs, or of a decode step's rows, the longest first
+        where their contexts are uneven. Sent when they differ from the last step's."""
+        if not b.tiles:
+            return
+        key = ('even', n) if decode and not b.plan.uneven(runs) else None
+        if key is not None and key == b.tiles_key:
+            return
+        pad = np.arange(n, b.rows)  # rows on the dummy slot, which has no page: they see nothing
+        every = np.concatenate([runs, np.stack([pad, np.ones_like(pad), np.full_like(pad, -1)], 1)])
+        if key is not None:
+            every[:n, 2] = b.ctx - 1
+        tiles = b.plan.tiles(every)
+        key = key or tuple(t.tobytes() for t in tiles)
+        if key != b.tiles_key:
+            for up, t in zip(b.tiles, tiles):
+                up.buffer()[:] = t
+                up.send()
+            b.tiles_key = key
+
+    @torch.inference_mode()
+    def stage_seats(self, b, seats):
+        """Paged cache: what a captured step of these seats over the buffers b (make_buffers) needs on the host before each
+        replay: their next positions' pages, and the order in which their rows are attended."""
+        if self.pages is None:
+            return
+        self.reserve(seats)
+        n = len(seats)
+        runs = np.stack([np.arange(n), np.ones(n, dtype=np.int64), [self.lengths_cpu[s] for s in seats]], 1)
+        self._stage_tiles(b, runs.reshape(-1, 3), n, True)
 
     def _rows_of(self, slots, prefills):
         """The step's rows: one per decoding seat, then T per prefill (same slot, offsets 0..T-1). Validates the
@@ -634,12 +669,8 @@ class StaticBackbone:
         # a decode step keyed by its seats restages nothing when they repeat
         b.table.stage(dict(slot=row_slot, real=np.ones(n, dtype=np.int64), offset=row_off),
                       key=None if prefills else ('decode', tuple(slots)))
-        if g.tiles:
-            pad = np.arange(n, b.rows)  # rows on the dummy slot, which has no page: they see nothing
-            every = np.concatenate([runs, np.stack([pad, np.ones_like(pad), np.full_like(pad, -1)], 1)])
-            for up, tiles in zip(g.tiles, b.plan.tiles(every)):
-                up.buffer()[:] = tiles
-                up.send()
+        if self.pages is not None:
+            self._stage_tiles(b, runs, n, not prefills)
         elif (prefills or spread) and self.kv_bits == 16:
             # a decode step's list stays valid while every row keeps its number of splits (the kernels take each
             # split's keys and a row's split count from the positions at run time): it is rebuilt only when a row

@@ -204,6 +204,40 @@ def test_window_stream(gpu):
     assert len(sb.export_prefix(1, sinks)) == 2 and full[0][0][0].shape[2] == cap
 
 
+@pytest.mark.parametrize("window", [0, 60])
+def test_many_seats(gpu, window):
+    """Decode steps of many seats whose contexts are uneven, even, and uneven in another order, in one graph: against the
+    oracle (without a window) and the same steps without graphs."""
+    from m3x.serve.fast_backbone import StaticBackbone
+    seats, cap = 30, 200
+    geo = dict(layers=2, hidden=512, heads=8, kv_heads=2, head_dim=64, inter=768, seed=31, affine=synth.AFFINE)
+    bbs = [StaticBackbone(synth.qwen3_backbone(device=gpu, **geo), seats + 1, capacity=cap, batch_buckets=(32,),
+                          ctx_buckets=(cap,), page_size=PAGE, window=window, use_graphs=graphs) for graphs in (True, False)]
+    g = torch.Generator().manual_seed(40)
+    both = _oracle(synth.qwen3_backbone(device="cpu", **geo), seats + 1, 2, cap, 64)
+    orders = set()
+    for lengths in ([180 - 6 * s for s in range(seats)], [77] * seats, [0] * 20 + [150 + s for s in range(10)]):
+        for s, n in enumerate(lengths):
+            kv = [tuple(torch.randn(1, 2, n, 64, generator=g).to(torch.bfloat16) for _ in "kv") for _ in range(2)]
+            for i, (k, v) in enumerate(kv):
+                for o in both:
+                    o[1][i][s, :, :n], o[2][i][s, :, :n] = k[0], v[0]
+            for o in both:
+                o[3][s] = n
+            for sb in bbs:
+                sb.load_prefix(s, [(k.to(gpu), v.to(gpu)) for k, v in kv], n)
+        for n in (seats, seats, 26):
+            x = torch.randn(n, 512, generator=g).to(torch.bfloat16)
+            a, b = (sb.step(list(range(n)), x.to(gpu)) for sb in bbs)
+            assert torch.equal(a, b)
+            torch.cuda.synchronize()
+            orders.add(bytes(bbs[0].graphs[(32, cap)].bufs.plan.launches[0][0].cpu().numpy()))
+            if not window:
+                ok, info = floor_check(a, *_step(both, list(range(n)), x))
+                assert ok, (lengths, info)
+    assert len(orders) >= (2 if window else 3)
+
+
 def test_pool_exhausted(gpu):
     """A step that finds no page raises before it changes anything, and goes through once there is one."""
     sb, _ = _setup(gpu, prefix=[0, 16, 0, 0, 0, 0], pages=2)
@@ -251,6 +285,40 @@ def test_frame_step(gpu):
             torch.cuda.synchronize()
         assert sb.pages.held(2) == 3
         seen.append((fs.codes(gr)[:3].clone(), gr["bufs"][0].out[:3].clone(), sb.lengths.clone()))
+    for a, b in zip(*seen):
+        assert torch.equal(a, b)
+
+
+def test_frame_step_many_seats(gpu):
+    """A captured frame step of seats of all ages, whose rows are attended longest first."""
+    from m3x.cb0 import Cb0Sampler
+    from m3x.frame import FrameStep
+    from m3x.serve.fast_backbone import StaticBackbone
+    from m3x.serve.fast_depth import FastDepth
+    seats, lengths = 26, [(53 * s) % 220 for s in range(30)]
+    seen = []
+    for use_graph in (True, False):
+        bb = synth.qwen3_backbone(layers=2, seed=21, device=gpu, affine=synth.AFFINE)
+        sb = StaticBackbone(bb, 30, capacity=256, batch_buckets=(28,), ctx_buckets=(256,), page_size=PAGE)
+        g = torch.Generator().manual_seed(50)
+        for s, n in enumerate(lengths):
+            sb.load_prefix(s, [tuple(torch.randn(1, 8, n, 128, generator=g).to(torch.bfloat16).to(gpu) for _ in "kv")
+                               for _ in range(2)], n)
+        cb = Cb0Sampler(bb.cb0_head.weight, 30, temp=0.9, top_k=50, rep=0.0)
+        for s in range(30):
+            cb.bind(s, seed=11 + s)
+        fd = FastDepth(synth.swiglu_depth(seed=9, device=gpu, affine=synth.AFFINE), 30, dtype=torch.bfloat16, temp=0.9,
+                       top_k=50, batch_buckets=(28,), fused=True)
+        fs = FrameStep(sb, cb, fd, ring_depth=4)
+        fs.feedback.copy_(torch.randn(31, 1024, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16))
+        gr = fs.capture(28, 256, use_graph=use_graph)
+        fs.set_slots(gr, list(range(3, 3 + seats)))
+        for _ in range(3):
+            fs.replay(gr)
+            torch.cuda.synchronize()
+        order = gr["bufs"][0].plan.launches[0][0][:seats, 0].tolist()
+        assert order == sorted(range(seats), key=lambda r: -lengths[3 + r])
+        seen.append((fs.codes(gr)[:seats].clone(), gr["bufs"][0].out[:seats].clone(), sb.lengths.clone()))
     for a, b in zip(*seen):
         assert torch.equal(a, b)
 
