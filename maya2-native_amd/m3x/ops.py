@@ -1163,15 +1163,20 @@ class PagedPlan:
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError(f"PagedPlan: window {window}, sinks {sinks}")
         self._begin(int((r[:, 0] + r[:, 1]).max()) if len(r) else 0, heads, kv_heads, head_dim, window, sinks)
-        for x, of, wide in self._deal(r, _narrow_cols(head_dim)):
+        for i, (x, of, wide) in enumerate(self._deal(r, _narrow_cols(head_dim))):
             if not len(x):
                 continue
             # the runs' own contexts, where they are what the plan is made for and not placeholders
             ends = (of[:, 2] + of[:, 1]).clip(0)
             mean = int(ends.mean()) if wide or 2 * ends.max() >= max_ctx else None
             every = len(x) == self.rows and (x[:, 1] == 1).all() and (x[:, 0] == np.arange(self.rows)).all()
+            most, caps = int(x[:, 1].max()), None if i else self._caps(of)
+            if caps is not None:
+                x, every = np.stack([x[:, 0], x[:, 1] | caps << 16], 1), False
             tiles = None if every else torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).to(device)
-            self._add(tiles, len(x), int(x[:, 1].max()), max_ctx, wide, mean)
+            self._add(tiles, len(x), most, max_ctx, wide, mean)
+            if caps is not None:
+                self.launches[-1] = (*self.launches[-1][:4], int(caps.max()))
         self._finish(torch.device(device))
 
     @staticmethod
@@ -1222,6 +1227,17 @@ class PagedPlan:
         """Keys that the runs' last rows see, about."""
         return (runs[:, 2] + runs[:, 1]).clip(0, self.window + self.sinks + 1 if self.window else None)
 
+    def _caps(self, runs):
+        """Splits a tile for single rows of uneven contexts: chunks of 256 to 800 keys that come to two to three workgroups a
+        CU; none beyond two a CU without. Measured on MI355X (16/8 heads of 128, rows of up to 4000 keys, us: none, chunks of
+        400 / 600 / 800 / 1000 / 1600 keys): 32 rows 67, 56.5 / 56.0 / 53.8 / 55.1 / 65.6; 64 rows 93.8, 97 / 97 / 91.8 / 97 /
+        95; 128 rows 168, 177 to 194."""
+        ends = self._ends(runs)
+        one = self._blocks(runs, 16)
+        if not self.uneven(runs) or len(runs) * one > 512:
+            return None
+        return (-(-ends // min(800, max(256, int(ends.sum()) * one // 640)))).clip(1, 16)
+
     def uneven(self, runs):
         """Whether the longest of the runs has more than 4/3 of their mean's keys."""
         ends = self._ends(np.asarray(runs))
@@ -1256,10 +1272,10 @@ class PagedPlan:
         self.rows = rows
         one = self._blocks(np.array([[0, 1]]), NARROW_COLS)
         self._apart = single or rows * one > 512  # single rows have a launch of their own
-        if single:  # as many splits as even rows take, two at least where uneven ones may
+        if single:  # as many splits as even rows take, and room for uneven ones'
             self._reserve(rows, 1, False, device)
             most = paged_attn_splits(rows * one, max_ctx, self.launches[0][3], head_dim=head_dim)
-            self.launches[0] = (*self.launches[0][:4], max(most, 2 if 256 < rows * one <= 640 else 1))
+            self.launches[0] = (*self.launches[0][:4], max(most, min(8, 1536 // (rows * one), -(-max_ctx // 800))))
             self._finish(torch.device(device))
             return self
         if self._apart:
@@ -1293,12 +1309,15 @@ class PagedPlan:
         lists = self._deal(r, 0, self.launches[-1 - wide][1], WIDE_COLS // 2 if wide else 1 << 31, not self._apart)
         lists = lists[not self._apart:]
         out = []
-        for (x, of, _), (_, n, tile_rows, cols, splits) in zip(lists, self.launches):
+        for i, ((x, of, _), (_, n, tile_rows, cols, splits)) in enumerate(zip(lists, self.launches)):
             if len(x) > n:
                 raise ValueError(f"PagedPlan: {len(x)} tiles, reserved for {n}")
             full = np.zeros((n, 2), dtype=np.int32)
             full[:len(x)] = x[:, :2]
-            if splits > 1 and len(x):
+            caps = self._caps(of) if self._apart and i == 0 else None
+            if caps is not None:
+                full[:len(x), 1] |= np.minimum(caps, splits).astype(np.int32) << 16
+            elif splits > 1 and len(x):
                 seen = self.window + self.sinks + tile_rows if self.window else 1 << 30
                 ends = (of[:, 2] + of[:, 1]).clip(0, seen)
                 blocks = len(x) * self._blocks(x, cols)
@@ -1345,15 +1364,17 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     """Workgroups that share a tile's keys, for `blocks` (tiles x kv heads x blocks of `cols` columns) of up to `keys` keys
     each.
 
-    Few columns: a workgroup a CU, of the mean's keys; with one row's heads (16 columns) and one to two and a half workgroups
-    a CU without, two where that evens out what the CUs get. At least 128 keys each for one row's heads up to 8 splits (the
-    join is 1 us of 6 to 8: one row at 250 keys 5.8 whole, 6.4 split, at 700 keys 9.8 / 8.4 / 7.1 / 6.6 at 1 / 2 / 4 / 8, at
-    1500 16.5 / 11.7 / 8.6 / 7.5), else 256, and three times as many to begin with (the join is 3 to 5: 64 rows onto 500 keys
-    12.4 whole, 13.6 to 17 split). Measured on MI355X (graph-timed, us, 16/8 heads of 128): one row at 2048 keys 21.3 whole,
-    14.5 / 9.8 / 8.0 / 8.2 at 2 / 4 / 8 / 16 splits; 16 rows 34.2, 24.4, 28.8 (3), 24.9 (4); 48 of a 1024-key window 40.0, 37.1, 39.4 (3), 42.4 (4); 64 rows 85.5, 90.1; 61 of up to 4000 keys
-    116, 102; 224 rows 277, 293. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 / 17.3 / 21.5 at 1 / 2 / 4 / 8 / 16;
-    512 onto 2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at 16 / 32 / 64 / 128; 30 x 5 rows
-    over up to 3001 29.2 / 26.8 / 23.7 / 22.2 / 26.8 at 1 / 2 / 3 / 4 / 6.
+    Few columns: up to half a workgroup a CU without splits, as many as make one a CU of the mean's keys. At least 128 keys each
+    for one row's heads (16 columns) up to 8 splits (the join is 1 us of 6 to 8: one row at 250 keys 5.8 whole, 6.4 split, at
+    700 keys 9.8 / 8.4 / 7.1 / 6.6 at 1 / 2 / 4 / 8, at 1500 16.5 / 11.7 / 8.6 / 7.5), else 256, and three times as many to
+    begin with (the join is 3 to 5: 64 rows onto 500 keys 12.4 whole, 13.6 to 17 split). More single rows: as many of up to
+    four as even out what the CUs get. Measured on MI355X (graph-timed, us, 16/8 heads of 128, 1 / 2 / 3 / 4 splits): 20 rows
+    of 2048 keys 40.4 / 38.5 / 30.8 / 32.9, 28 38.1 / 41.6 / 43.0 / 43.0, 34 67.5 / 57.2 / 53.8 / 52.2, 48 71.8 / 64.5 / 69.3
+    / 66.5, 64 80 / 85 / - / 87, 100 144.5 / 137.4 / 136.7 / 136.3, 224 277 / 293; 40 of 1000 35.7 / 32.4 / 31.1 / 30.7; 48
+    of a 1024-key window 40.0 / 37.1 / 39.4 / 42.4. One row of 2048 21.3 / 14.5 / - / 9.8, 8.0 at 8, 8.2 at 16; 16 rows 34.2 /
+    24.4 / 28.8 / 24.9. 32 columns: 64 rows onto 4000 keys 40.7 / 28.8 / 20.5 / 17.3 / 21.5 at 1 / 2 / 4 / 8 / 16; 512 onto
+    2048 25.8 / 32.1. 32/4 heads of 64: 2 rows at 120000 keys 73 / 44 / 48 / 56 at 16 / 32 / 64 / 128; 30 x 5 rows over up to
+    3001 29.8 / 25.2 / 22.5 / 21.1 / 25.0 at 1 / 2 / 3 / 4 / 5.
 
     Prompts: the least of what the tiles' turns of 32 keys take (1.05 us for one of two groups of waves that share a
     workgroup's keys, which they do up to a workgroup a CU; 0.52 for each of more workgroups that share a CU; the longest
@@ -1362,11 +1383,11 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     over 500 21.0 / 31.0 at 1 / 2."""
     blocks, mean_keys = max(blocks, 1), keys if mean_keys is None else max(mean_keys, 1)
     if cols != WIDE_COLS:
-        if blocks > 256 and cols == 16:
-            def spare(s):  # of the CU with the most workgroups to their mean
-                return -(-blocks * s // 256) * 256 / (blocks * s)
-            uneven = 4 * mean_keys < 3 * keys or spare(1) > 1.1 * spare(2)
-            return 2 if uneven and blocks <= 640 and keys >= 1024 else 1
+        if blocks > 128 and cols == 16:
+            def cost(s):  # the CU with the most workgroups sets the time; from two on the join
+                return 0.0195 * head_dim / 128 * -(-blocks * s // 256) * mean_keys / s + (2.5 + 0.5 * s if s > 1 else 0)
+            best = min((s for s in (1, 2, 3, 4) if s == 1 or s * 256 <= keys), key=cost)
+            return best if cost(best) < 0.97 * cost(1) else 1
         if keys < (384 if cols == 16 else 768):
             return 1
         most = min(max(8, keys // 256), keys // 128, 64) if cols == 16 else min(keys // 256, 64)

@@ -392,7 +392,7 @@ def test_reserved(few, monkeypatch):
                     seen += range(a, a + n)
             assert sorted(seen) == list(range(rows))
     one = ops.PagedPlan.reserve(40, 16, 8, 128, 2048, device="cpu", single=True)
-    assert len(one.launches) == 1 and one.launches[0][1:4] == (40, 1, 16) and one.launches[0][4] == 2
+    assert len(one.launches) == 1 and one.launches[0][1:4] == (40, 1, 16) and one.launches[0][4] > 1
     even, uneven = (one.tiles([(r, 1, p) for r, p in enumerate(at)])[0] for at in ([2000] * 40, range(100, 2060, 49)))
     assert even[:, 0].tolist() == list(range(40)) and uneven[:, 0].tolist() == list(range(39, -1, -1))
     with pytest.raises(ValueError):
