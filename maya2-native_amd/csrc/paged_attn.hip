@@ -773,7 +773,8 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
     const bool was_wild = wild;
     if (j < plain || j >= edge || holes) {
       const int key = keys.key(i0 + j);
-      pg_mask<16, 8>(s, key + 4 * lh, min(cp, j == steps ? -1 : keys.last), pg_low(a, cp), a.sinks, a.window != 0, holes ? gaps(key) : 0u);
+      pg_mask<16, 8>(s, key + 4 * lh, min(cp, j == steps ? -1 : keys.last), pg_low(a, cp), a.sinks,
+                     key <= none && key + KT > a.sinks, holes ? gaps(key) : 0u);
       float any = 0.f;
 #pragma unroll
       for (int x = 0; x < SB / 1024; ++x) {
