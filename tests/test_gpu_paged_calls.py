@@ -182,6 +182,27 @@ def test_reserved_plan(gpu, few, monkeypatch):
             assert (out[at:] == 7).all() and R.within(out[:at], want[:at], bound[:at]) <= 1
 
 
+@pytest.mark.parametrize("rows", [20, 40])
+def test_plan_of_other_positions(gpu, rows):
+    """A plan's positions are a rule's input: rows elsewhere (shorter, longer, past the largest context, none) get theirs."""
+    from m3x import ops
+    held = {s: [(0, 1280)] for s in range(rows)}
+    table, pages = R.table_for(held, rows, PAGE, 1280 // PAGE, 1)
+    k, v = R.pools(table, pages, held, KV, PAGE, D, BF, 2)
+    q, slots = R.normal(3, rows, H, D).to(BF), torch.arange(rows)
+    cache = ops.PagedKv(k.to(gpu), v.to(gpu), table.to(gpu))
+    plan = ops.PagedPlan([(r, 1, 20 * (r + 1)) for r in range(rows)], H, KV, D, 20 * rows, device=gpu)
+    assert plan.launches[0][0] is not None and plan.launches[0][4] > 1
+    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=gpu)
+    out = torch.empty(rows, H, D, dtype=BF, device=gpu)
+    for at in (lambda r: 20 * (r + 1), lambda r: 1279 - 30 * r, lambda r: r - 3, lambda r: 1279):
+        pos = torch.tensor([at(r) for r in range(rows)], dtype=torch.int32)
+        out.fill_(7.0)
+        ops.paged_attn(q.to(gpu), cache, out, slots.to(gpu), pos.to(gpu), SCALE, plan, ws)
+        want, bound = R.attention(q, k, v, table, slots, pos, SCALE)
+        assert R.within(out, want, bound) <= 1
+
+
 def test_no_rows(gpu):
     """Calls without rows, and a plan without runs, do nothing."""
     from m3x import ops

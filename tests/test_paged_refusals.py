@@ -145,6 +145,31 @@ def test_tiles(H, KV):
             assert ends == sorted(ends, reverse=True)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_plans(D):
+    """Every row of a plan's runs is in one tile of one launch, whatever its layout, window and largest context."""
+    from m3x import ops
+    rng = np.random.default_rng(D)
+    for H, KV in ((16, 8), (8, 8), (32, 4), (24, 1), (71, 1), (300, 2)):
+        for _ in range(60):
+            runs, at = [], int(rng.integers(0, 3))
+            sizes = rng.choice([1, 1, 1, 2, 5, 6, 17, 33, 65, 300], int(rng.integers(1, 50))) if rng.integers(3) else [1] * 40
+            for n in sizes:
+                runs.append((at, int(n), int(rng.integers(-n - 1, rng.choice([2, 500, 4000])))))
+                at += n + int(rng.integers(0, 2))
+            window = int(rng.choice([0, 0, 1, 100, 5000]))
+            plan = ops.PagedPlan([runs[i] for i in rng.permutation(len(runs))], H, KV, D, int(rng.choice([0, 50, 4000])),
+                                 window=window, sinks=int(rng.choice([0, 4, 900])) if window else 0, device="cpu")
+            seen = []
+            for tiles, n, tile_rows, cols, splits in plan.launches:
+                assert cols in ((16, 32, 48, 128) if D == 64 else (16, 32, 128)) and 1 <= splits <= 256 and n <= 65535
+                for a, x in [(r, 1) for r in range(n)] if tiles is None else tiles.tolist():
+                    m, s = x & 0xFFFF, x >> 16
+                    assert 1 <= m <= tile_rows and 0 <= s <= splits and any(f <= a and a + m <= f + k for f, k, _ in runs)
+                    seen += range(a, a + m)
+            assert sorted(seen) == [r for f, k, _ in runs for r in range(f, f + k)] and plan.rows == runs[-1][0] + runs[-1][1]
+
+
 def test_splits():
     """At least one workgroup, none with fewer keys than the kernels' least, within the ABI's limit."""
     from m3x import ops
