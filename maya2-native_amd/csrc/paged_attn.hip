@@ -561,7 +561,7 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
 // keys) in steps of 32, which come to LDS by loads that need no registers, two steps
 // ahead; every wave reads K there in 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads. A row's
 // chunks lie in LDS at their number XOR a number of the row, so that neither read meets a bank twice.
-// Measured on MI355X (bf16, page_size 64 or 128, graph-timed): 4096 rows onto 12288 keys, 32/8 heads of 128, 917 us, 1050
+// Measured on MI355X (bf16, page_size 64 or 128, graph-timed): 4096 rows onto 12288 keys, 32/8 heads of 128, 902 us, 1067
 // TFLOP/s, where an 8192^3 product of the library reaches 1290; the matrix units are busy half of the time, the vector units
 // about as long, and the clock is down to 1.9 GHz. 8 x 200 rows onto 300 to 500 keys, 16/8 heads, 21 us: launch 2, tile, slot
 // and page numbers 2.5, the first keys and queries 0.6, the first turn 2 to 3 with its code's way into the instruction
@@ -815,7 +815,7 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       add = x;
     }
     const uint32_t gv = get_v + vs;
-    constexpr int SLOTS = KS + 2 * ND, LEAD = 4;  // LEAD: slots that a value's read is ahead of its product
+    constexpr int SLOTS = KS + 2 * ND, LEAD = 2;  // LEAD: slots that a value's read is ahead of its product (1: 4 % slower, 4: 1 %)
 #pragma unroll
     for (int e = 0; e < 16; ++e) next[e] = 0.f;
 #pragma unroll
