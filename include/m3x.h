@@ -643,7 +643,7 @@ size_t m3x_paged_attn_workspace(int tiles, int kv_heads, int heads, int tile_row
  * columns, bound by the keys' bytes) or 128 (prompts); at most 65535 tiles, and fewer than 2^16 - cols columns a tile. A tile's keys are divided among up to `splits` <= 256 workgroups; arrived (device,
  * for splits > 1 and cols other than 128): tiles x kv_heads x ceil(tile_rows x heads / kv_heads / cols) int32, zeroed before
  * the first call and left so. Weights are rounded to the 16-bit type and summed as rounded; all else is fp32, in a fixed
- * order. Scores times |scale| log2(e) are to be finite. What a row does not see has no part in its result, whatever it
+ * order. Scores q . k are fp32 sums, to be below 2^127 in size. What a row does not see has no part in its result, whatever it
  * holds. Two calls that may run at the same time need a workspace and counters each. */
 int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, long sq_h, void* out, long so_b, long so_h,
                    const int64_t* slots, const int32_t* pos, const int32_t* tiles, int ntiles, int tile_rows, int cols,

@@ -39,7 +39,7 @@ struct PagedAttn {
   uint32_t q_flip;       // the sign bits of two query elements where scale < 0
   int rows, heads, G, tile_rows, blocks, window, sinks, splits;
   uint32_t over_G;  // ceil(2^32 / G): x / G = x * over_G >> 32 for x, G < 2^16 (0 for G = 1)
-  float* part;   // [columns][splits][D], then [columns][splits][2]: (reference, sum)
+  float* part;   // [columns][splits][D], then [columns][splits][2]: (maximum, sum)
   int* arrived;  // narrow: a counter for each (tile, kv head, block), 0 between calls
 };
 
@@ -185,10 +185,12 @@ template <int DT> __device__ __forceinline__ float pg_wild_number(uint16_t x) {
   return pg_wild<DT>(x) & 0x8000u ? E<DT>::to_f(x) : 0.f;
 }
 
-// A column's running maximum (raw score) and its reference ref = maximum * c, what weights' exponents are counted from:
-// exp2(s c - ref). Any reference serves as long as all of a column's weights and its sum go by the same one, so its
-// rounding is no error; kept finite (no row sees a key below -FLT_MAX).
-__device__ __forceinline__ float pg_ref(float m, float c) { return fmaxf(m * c, -3.402823466e38f); }
+// A weight's exponent is (s - m) c + up, m the column's running maximum: the difference of the raw scores, exact near the
+// maximum, is taken first, so that the largest weight is 2^up whatever the scores' size (s c - m c, each rounded, would be
+// off by half a unit of m c, which from 2^24 on is more than the weights' whole range). Waves, key groups and splits hand
+// their raw maximum on with their sums, which are then joined by the same differences. A column that has seen nothing
+// stands at PG_LEAST, below every score.
+constexpr float PG_LEAST = -3.402823466e38f;
 
 // 4 outputs O / L (zeros for a column that saw nothing)
 template <int DT> __device__ __forceinline__ void pg_store4(uint16_t* p, const f32x4_t& O, float L) {
@@ -261,12 +263,12 @@ __device__ __forceinline__ void pg_join(const PagedAttn& a, const Where& w, cons
       if (s0 + e >= active) x[e].x = -INFINITY;
       mx = fmaxf(mx, x[e].x);
     }
-    const float f0 = __builtin_amdgcn_exp2f(M - mx);
+    const float f0 = __builtin_amdgcn_exp2f((M - mx) * a.c);
     L *= f0;
     O *= f0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float f = __builtin_amdgcn_exp2f(x[e].x - mx);
+      const float f = __builtin_amdgcn_exp2f((x[e].x - mx) * a.c);
       L += x[e].y * f;
       O += o[e] * f;
     }
@@ -280,7 +282,7 @@ constexpr int WIDE_LEAST = 2;  // steps a split at least
 template <int D, int COLS> struct NarrowLds {
   int order;
   __align__(16) float o[NARROW_NW][COLS][D + 4];
-  float ref[NARROW_NW][COLS], l[NARROW_NW][COLS];
+  float m[NARROW_NW][COLS], l[NARROW_NW][COLS];
 };
 }  // namespace
 
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
   f32x4_t acc[QT][2 * NV];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    m[t] = -3.402823466e38f;
+    m[t] = PG_LEAST;
     l[t] = 0.f;
 #pragma unroll
     for (int T = 0; T < 2 * NV; ++T) acc[t][T] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -418,17 +420,16 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
       for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[t][e]);
       mx = fmaxf(m[t], xor32_max(xor16_max(mx)));
       if (__ballot(mx > m[t])) {
-        const float f = __builtin_amdgcn_exp2f(pg_ref(m[t], a.c) - pg_ref(mx, a.c));
+        const float f = __builtin_amdgcn_exp2f((m[t] - mx) * a.c);
         l[t] *= f;
 #pragma unroll
         for (int T = 0; T < 2 * NV; ++T) acc[t][T] *= f;
         m[t] = mx;
       }
-      const float sub = pg_up<DT> - pg_ref(m[t], a.c);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const uint32_t x = pg_pack<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], a.c, sub)),
-                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1], a.c, sub)));
+        const uint32_t x = pg_pack<DT>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e] - m[t], a.c, pg_up<DT>)),
+                                       __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1] - m[t], a.c, pg_up<DT>)));
         pop[t][e / 2] = x;
         l[t] = pg_add2<DT>(x, l[t]);
       }
@@ -508,7 +509,7 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
         *reinterpret_cast<f32x4_t*>(&lds.o[wave][16 * t + li][2 * NV * (4 * lg + r) + T]) =
             f32x4_t{acc[t][T][r], acc[t][T + 1][r], acc[t][T + 2][r], acc[t][T + 3][r]};
     if (lg == 0) {
-      lds.ref[wave][16 * t + li] = pg_ref(m[t], a.c);
+      lds.m[wave][16 * t + li] = m[t];
       lds.l[wave][16 * t + li] = sum;
     }
   }
@@ -518,14 +519,14 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
     const int col = x / (D / 4), d = x % (D / 4) * 4;
     const Col cc(a, w, w.block * COLS + col);
     if (!cc.live) continue;
-    float M = lds.ref[0][col];
+    float M = lds.m[0][col];
 #pragma unroll
-    for (int y = 1; y < NW; ++y) M = fmaxf(M, lds.ref[y][col]);
+    for (int y = 1; y < NW; ++y) M = fmaxf(M, lds.m[y][col]);
     float L = 0.f;
     f32x4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int y = 0; y < NW; ++y) {
-      const float f = __builtin_amdgcn_exp2f(lds.ref[y][col] - M);
+      const float f = __builtin_amdgcn_exp2f((lds.m[y][col] - M) * a.c);
       L += lds.l[y][col] * f;
       O += *reinterpret_cast<const f32x4_t*>(&lds.o[y][col][d]) * f;
     }
@@ -568,10 +569,13 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
 // cache, seven more of both key groups 1.3 each, the groups' sums 2.
 namespace {
 constexpr int WIDE_KT = 32;
-// A weight's exponent is counted from a reference that the scores of a column pass by less than WIDE_SLACK: renewing it
-// whenever a maximum grows would mean scaling the outputs in most turns of a wave's 32 columns. Weights stand at 2^wide_up
-// of their size, as in the narrow kernel.
-constexpr float WIDE_SLACK = 8.f;
+// A weight's exponent is counted from a reference m (a raw score) that the scores of a column pass by less than WIDE_SLACK:
+// renewing it whenever a maximum grows would mean scaling the outputs in most turns of a wave's 32 columns. Weights stand at
+// 2^wide_up of their size, as in the narrow kernel. While m c is up to WIDE_NEAR, exponents are s c + add, one multiply-add,
+// add = wide_up - m c rounded to 2^-7 at worst: all of the column's weights are in the same proportion as with m c itself,
+// and what it is off by is made good where sums are handed on. A wave that meets a larger score takes the differences
+// (s - m) c from then on, in every turn.
+constexpr float WIDE_SLACK = 8.f, WIDE_NEAR = 65536.f;
 template <int DT> constexpr float wide_up = pg_up<DT> - WIDE_SLACK;
 
 // chunk x of a row lies at chunk x ^ wide_kx (wide_vx) of its row in LDS
@@ -710,7 +714,9 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   const int rv = 4 * lh + (lane >> 2 & 3);
   const uint32_t get_v = rv * RB + ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ wide_vx<D>(rv)) * 16 + (lane & 1) * 8;
 
-  float add = wide_up<DT> - pg_ref(-3.402823466e38f, a.c), l = 0.f;  // wide_up less the column's reference, its sum
+  // the column's reference, what is added to a weight's exponent, the score that a higher one renews them for (-inf: the
+  // wave takes differences, whose reference is the running maximum), the sum of the weights
+  float m = PG_LEAST, add = wide_up<DT> - fmaxf(m * a.c, PG_LEAST), most = m, l = 0.f;
   pg_f16 acc[ND];
 #pragma unroll
   for (int T = 0; T < ND; ++T)
@@ -805,15 +811,28 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
     // A reference is renewed once a score passes it by WIDE_SLACK: the column's sum so far goes by the new one, and behind
     // this turn its outputs
-    constexpr float most = wide_up<DT> + WIDE_SLACK;
-    const bool grew = __ballot(__builtin_fmaf(mx, a.c, add) > most) != 0;
+    const bool grew = __ballot(mx > most) != 0;
     float f;
     if (grew) {
-      const float x = fminf(add, wide_up<DT> - pg_ref(xor32_max(mx), a.c));
-      f = __builtin_amdgcn_exp2f(x - add);
+      const float x = fmaxf(m, xor32_max(mx));
+      const bool far = most == -INFINITY;
+      const float to = wide_up<DT> - fmaxf(x * a.c, PG_LEAST);
+      most = x + WIDE_SLACK * __builtin_amdgcn_rcpf(a.c);
+      f = __builtin_amdgcn_exp2f(to - add);
+      if (__builtin_expect(__ballot(far || (x > m && !(fabsf(to) <= WIDE_NEAR))) != 0, 0)) {
+        f = __builtin_amdgcn_exp2f(far ? (m - x) * a.c : fminf(__builtin_fmaf(-x, a.c, -add) + wide_up<DT>, 1.f));
+        add = wide_up<DT>;
+        most = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] -= x;
+      } else {
+        add = to;
+      }
+      m = x;
       l *= f;
-      add = x;
     }
+    // one place for the scores behind the branch, or copies of them are made in every turn (8 x 200 rows 21.0 us, 21.6 without)
+    asm volatile("" : "+v"(s));
     const uint32_t gv = get_v + vs;
     constexpr int SLOTS = KS + 2 * ND, LEAD = 2;  // LEAD: slots that a value's read is ahead of its product (1: 4 % slower, 4: 1 %)
 #pragma unroll
@@ -904,6 +923,9 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   }
   pg_landed<0>();
 
+  // by what power of two the sums are to be taken up to stand at 2^wide_up at m (what add's rounding left; a column that saw
+  // nothing has sums of 0)
+  const float due = most == -INFINITY ? 0.f : __builtin_amdgcn_fmed3f(wide_up<DT> - __builtin_fmaf(m, a.c, add), -1.f, 1.f);
   if constexpr (KG == 1) {  // lane (column, lh) holds dims 8 n + 4 lh + r
     const float L = xor32_sum(l);
     if (!col.live) return;
@@ -917,13 +939,14 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
     } else {
       const long place = (long)blockIdx.y * gridDim.x + blockIdx.x, ncols = (long)gridDim.y * gridDim.x * COLS;
       const long at = (place * COLS + 32 * wave + li) * a.splits + split;
+      const float g = __builtin_amdgcn_exp2f(due);
 #pragma unroll
       for (int n = 0; n < 4 * ND; ++n) {
         const pg_f16& x = acc[n / 4];
         *reinterpret_cast<f32x4_t*>(a.part + at * D + 8 * n + 4 * lh) =
-            f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
+            f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]} * g;
       }
-      if (lh == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(wide_up<DT> - add, L);
+      if (lh == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + at * 2) = make_float2(m, L * g);
     }
     return;
   }
@@ -934,26 +957,28 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   __syncthreads();
   constexpr int NC = 4 * ND, SW = 16 / NC;
   f32x4_t* const out = reinterpret_cast<f32x4_t*>(lds);
-  float2* const ml = reinterpret_cast<float2*>(lds + KG * 4 * NC * 1024);
+  float4* const ml = reinterpret_cast<float4*>(lds + KG * 4 * NC * 1024);
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const pg_f16& x = acc[n / 4];
     out[((group * 4 + wave) * NC + n) * 64 + (lane ^ SW * n)] = f32x4_t{x[n % 4 * 4], x[n % 4 * 4 + 1], x[n % 4 * 4 + 2], x[n % 4 * 4 + 3]};
   }
   l = xor32_sum(l);
-  if (lh == 0) ml[(group * 4 + wave) * 32 + li] = make_float2(add, l);
+  if (lh == 0) ml[(group * 4 + wave) * 32 + li] = make_float4(m, l, due, 0.f);
   __syncthreads();
 #pragma unroll 1
   for (int x = threadIdx.x; x < COLS * NC; x += 256 * KG) {
     const int n = x % NC, y = x / NC, at = ((y / 32) * NC + n) * 64 + (y % 32 ^ SW * n);
     const Col cc(a, w, w.block * COLS + y);
     if (!cc.live) continue;
-    const float2 m0 = ml[y], m1 = ml[128 + y];
-    const float least = fminf(m0.x, m1.x), f0 = __builtin_amdgcn_exp2f(least - m0.x), f1 = __builtin_amdgcn_exp2f(least - m1.x);
+    const float4 m0 = ml[y], m1 = ml[128 + y];
+    const float M = fmaxf(m0.x, m1.x);
+    const float f0 = __builtin_amdgcn_exp2f(__builtin_fmaf(m0.x - M, a.c, m0.z));
+    const float f1 = __builtin_amdgcn_exp2f(__builtin_fmaf(m1.x - M, a.c, m1.z));
     const f32x4_t o0 = out[at] * f0 + out[at + 4 * NC * 64] * f1, o1 = out[at + 32] * f0 + out[at + 4 * NC * 64 + 32] * f1;
-    const float2 m = make_float2(least, m0.y * f0 + m1.y * f1);
+    const float L = m0.y * f0 + m1.y * f1;
     if (keys.active == 1) {
-      const float r = m.y == 0.f ? 0.f : 1.f / m.y;
+      const float r = L == 0.f ? 0.f : 1.f / L;
       *reinterpret_cast<pg_u4*>(a.out + (long)(w.first + cc.j) * a.so_b + (long)(w.kh * a.G + cc.h) * a.so_h + 8 * n) =
           pg_u4{pg_pack<DT>(o0[0] * r, o0[1] * r), pg_pack<DT>(o0[2] * r, o0[3] * r), pg_pack<DT>(o1[0] * r, o1[1] * r),
                 pg_pack<DT>(o1[2] * r, o1[3] * r)};
@@ -962,7 +987,7 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
       const long col = (place * COLS + y) * a.splits + split;
       *reinterpret_cast<f32x4_t*>(a.part + col * D + 8 * n) = o0;
       *reinterpret_cast<f32x4_t*>(a.part + col * D + 8 * n + 4) = o1;
-      if (n == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + col * 2) = make_float2(wide_up<DT> - m.x, m.y);
+      if (n == 0) *reinterpret_cast<float2*>(a.part + ncols * a.splits * D + col * 2) = make_float2(M, L);
     }
   }
 }
@@ -1043,9 +1068,9 @@ M3X_API int m3x_paged_attn(const M3xPagedKv* cache, const void* q, long sq_b, lo
       return M3X_EWORKSPACE;
     if (!m3x_aligned16(workspace)) return M3X_EINVAL;
   }
-  // The factor of the scores' exponents, never 0 (0 * -inf of a hidden key). fp32's smallest normal number stands for all
-  // below it: scores up to 2^100 weigh alike under either.
-  const float factor = std::max(fabsf(scale) * 1.44269504088896341f, 0x1p-126f);
+  // The factor of the scores' exponents, never 0 (0 * -inf of a hidden key). fp32's smallest number stands for all below it:
+  // scores up to 2^127 weigh alike under either, within 2^-21.
+  const float factor = std::max(fabsf(scale) * 1.44269504088896341f, 0x1p-149f);
   const int G = heads / c.kv_heads;
   const PagedAttn a = {(const uint16_t*)q, sq_b, sq_h, (uint16_t*)out, so_b, so_h, slots, pos, tiles, factor,
                        scale < 0.f ? 0x80008000u : 0u, rows, heads, G, tile_rows, (tile_rows * G + cols - 1) / cols,

@@ -1409,7 +1409,7 @@ def paged_attn(q, cache, out, slots, pos, scale, plan, workspace=None):
     (the cache's type, any row and head strides). A row that sees nothing gets zeros (pos[r] < 0, a slot outside the
     cache, positions in no page); a row in none of the plan's runs is left as it is. The rows of a run are of one slot at
     consecutive positions: its first row's are read. workspace: a tensor of plan.workspace bytes, or None when that is 0.
-    Scores times |scale| are finite numbers below 2^127, |scale| at most 2^126."""
+    Scores q . k are below 2^127 in size, |scale| is at most 2^126."""
     rows, sp, pp = _paged_rows("paged_attn", cache, slots, pos)
     if not isinstance(plan, PagedPlan):
         raise TypeError("paged_attn: the plan must be an ops.PagedPlan")
