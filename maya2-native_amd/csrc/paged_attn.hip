@@ -701,8 +701,9 @@ __global__ __launch_bounds__(256 * KG, 2) void paged_wide_kernel(Paged c, PagedA
   const int jl = w.n - 1, ja = min(pg_row(a, c0), jl), jb = min(pg_row(a, c0 + 31), jl);
   const int pa = min(pg_uniform(w.p0 + ja), keys.last), pb = min(pg_uniform(c0 < w.n * a.G ? w.p0 + jb : -1), keys.last);
   const int none = a.window ? pg_uniform(w.p0 + jb) - a.window : -1;
-  // the wave's steps: those up to its last row's key (pb lies at or behind the window's begin)
-  const int steps = pb < 0 ? 0 : max(0, min(i1 - i0, pb / KT - keys.skip - i0 + 1));
+  // the wave's steps: those up to its last row's key, the sinks' in any case: a window that begins past the table's end lies
+  // behind pb, and leaves them alone
+  const int steps = pb < 0 ? 0 : max(0, min(i1 - i0, max(pb / KT - keys.skip, keys.sink - 1) - i0 + 1));
   // The turns whose step every row sees whole: from plain on up to edge. Before them the window hides something (or
   // nothing: steps of the sinks).
   const int edge = min(steps, max(0, (pa + 1) / KT - keys.skip - i0));
