@@ -7,6 +7,8 @@ the one slot that took them new, so shared ones never change. Changes to the tab
 by `flush`, in stream order before the step that needs them."""
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 import numpy as np
 import torch
 
@@ -29,6 +31,7 @@ class PagePool:
         self._begin = [0] * self.slots  # first entry behind those that were released
         self._changed = {}              # flat table index -> page, not yet sent
         self._index = self._value = None
+        self._log = None                # within an attempt: (slot, entry, page before) of each change
 
     @property
     def free_pages(self):
@@ -50,7 +53,37 @@ class PagePool:
         end = -(-int(length) // self.page_size)
         return end <= self.width and bool((self._host[slot, :max(end, 0)] >= 0).all())
 
+    @contextmanager
+    def attempt(self):
+        """Changes that belong together (none of them sent in between): where one of them raises, all are taken back."""
+        kept = list(self._end), list(self._begin), dict(self._changed)
+        log = self._log = []
+        try:
+            yield
+        except BaseException:
+            self._undo(log, *kept)
+            raise
+        finally:
+            self._log = None
+
+    def _undo(self, log, end, begin, changed):
+        """The log's changes backwards: pages go back to the free ones' top, and come from there, in the opposite order."""
+        for slot, at, page in reversed(log):
+            taken = int(self._host[slot, at])
+            if taken >= 0:
+                self._uses[taken] -= 1
+                if self._uses[taken] == 0:
+                    self._free.append(taken)
+            if page >= 0:
+                if self._uses[page] == 0:
+                    self._free.pop()
+                self._uses[page] += 1
+            self._host[slot, at] = page
+        self._end, self._begin, self._changed = end, begin, changed
+
     def _set(self, slot, at, page):
+        if self._log is not None:
+            self._log.append((slot, at, int(self._host[slot, at])))
         self._host[slot, at] = page
         self._changed[slot * self.width + at] = page
 

@@ -250,6 +250,15 @@ class StaticBackbone:
         if self.window:
             self.pages.trim(slot, self.lengths_cpu[slot] - self.window + 1, self.sinks)
 
+    def _take(self, wants):
+        """Lets go of what lies behind the windows of the slots in wants ((slot, length) pairs), takes the pages of their first
+        `length` positions and sends the table; all of it, or nothing when the pool has too few pages."""
+        with self.pages.attempt():
+            for s, _ in wants:
+                self._trim(s)
+            self.pages.grow(wants)
+        self.pages.flush()
+
     @torch.inference_mode()
     def reserve(self, slots, ahead=1):
         """Paged cache: takes the pages that the slots' next `ahead` positions need (and lets go of those behind their
@@ -258,10 +267,7 @@ class StaticBackbone:
         if self.pages is None:
             return
         check_slots(slots, self.max_slots)
-        for s in slots:
-            self._trim(s)
-        self.pages.grow([(s, self.lengths_cpu[s] + ahead) for s in slots])
-        self.pages.flush()
+        self._take([(s, self.lengths_cpu[s] + ahead) for s in slots])
 
     def _positions_of(self, slot, length):
         """(slots, positions) of a slot's first `length` positions, as the 4-bit cache's rows."""
@@ -275,9 +281,11 @@ class StaticBackbone:
             raise ValueError(f'length {length} exceeds capacity {self.capacity}')
         if self.kv_bits == 4 or self.pages is not None:
             if self.pages is not None:
-                self.pages.release(slot)
+                with self.pages.attempt():
+                    self.pages.release(slot)
+                    self.pages.grow([(slot, length)])
+                self.pages.flush()
                 self._set_length(slot, 0)
-                self.reserve([slot], length)
             if length:
                 at = self._positions_of(slot, length)
                 for c, (keys, values) in zip(self.paged or self.kv4, pairs):
@@ -316,9 +324,10 @@ class StaticBackbone:
             raise ValueError(f'length {n} outside the slot\'s {self.lengths_cpu[source]} cached positions')
         if not self.pages.has(source, n):
             raise ValueError(f'slot {source} has let go of positions behind its window')
-        self.pages.release(slot)
+        with self.pages.attempt():
+            self.pages.release(slot)
+            rest = self.pages.share(slot, source, n)
         self._set_length(slot, 0)
-        rest = self.pages.share(slot, source, n)
         if rest is not None:
             for c in self.paged:
                 c.k[rest[1]].copy_(c.k[rest[0]])
@@ -658,11 +667,8 @@ class StaticBackbone:
         n = len(row_slot)
         rows = self._rows.pick(n, 'batch')
         if self.pages is not None:
-            grown = [(s, self.lengths_cpu[s] + 1) for s in slots] + [(s, self.lengths_cpu[s] + t.shape[0]) for s, t in prefills]
-            for s, _ in grown:
-                self._trim(s)
-            self.pages.grow(grown)
-            self.pages.flush()
+            self._take([(s, self.lengths_cpu[s] + 1) for s in slots]
+                       + [(s, self.lengths_cpu[s] + t.shape[0]) for s, t in prefills])
         spread = not prefills and self._spread(rows, runs)
         g = self._graph(rows, self._ctx.pick(need, 'context'), bool(prefills), spread)
         b = g.bufs
