@@ -54,17 +54,20 @@ class PagePool:
         return end <= self.width and bool((self._host[slot, :max(end, 0)] >= 0).all())
 
     @contextmanager
-    def attempt(self):
-        """Changes that belong together (none of them sent in between): where one of them raises, all are taken back."""
+    def attempt(self, keep=True):
+        """Changes that belong together (none of them sent in between): where one of them raises, all are taken back; without
+        keep in any case, to see whether one does."""
         kept = list(self._end), list(self._begin), dict(self._changed)
         log = self._log = []
         try:
             yield
         except BaseException:
-            self._undo(log, *kept)
+            keep = False
             raise
         finally:
             self._log = None
+            if not keep:
+                self._undo(log, *kept)
 
     def _undo(self, log, end, begin, changed):
         """The log's changes backwards: pages go back to the free ones' top, and come from there, in the opposite order."""

@@ -245,10 +245,12 @@ class StaticBackbone:
         self.lengths[slot] = n
         self.lengths_cpu[slot] = n
 
-    def _trim(self, slot):
-        """Pages that no later row of the slot sees go back to the pool (a row at position p sees p - window + 1 on)."""
+    def _trim(self, slot, length=None):
+        """Pages that no row of the slot from position `length` (default: its length) on sees go back to the pool (a row at
+        position p sees p - window + 1 on)."""
         if self.window:
-            self.pages.trim(slot, self.lengths_cpu[slot] - self.window + 1, self.sinks)
+            length = self.lengths_cpu[slot] if length is None else length
+            self.pages.trim(slot, length - self.window + 1, self.sinks)
 
     def _take(self, wants):
         """Lets go of what lies behind the windows of the slots in wants ((slot, length) pairs), takes the pages of their first
@@ -374,9 +376,13 @@ class StaticBackbone:
             raise ValueError(f'x must be [T>0, {self.hidden}], got {tuple(x.shape)}')
         if self.lengths_cpu[slot] + x.shape[0] > self.capacity:
             raise ValueError(f'context {self.lengths_cpu[slot] + x.shape[0]} exceeds capacity {self.capacity}')
-        if not self.window:
-            self.reserve([slot], x.shape[0])  # all or nothing
         piece = self.batch_buckets[-1]
+        if self.pages is not None:  # all or nothing: the pieces' pages one after the other before the first of them
+            with self.pages.attempt(keep=False):
+                for t0 in range(0, x.shape[0], piece):
+                    begin = self.lengths_cpu[slot] + t0
+                    self._trim(slot, begin)
+                    self.pages.grow([(slot, min(begin + piece, self.lengths_cpu[slot] + x.shape[0]))])
         last = None
         for t0 in range(0, x.shape[0], piece):
             last = self.step_mixed([], None, [(slot, x[t0:t0 + piece])])[1][0]

@@ -64,3 +64,22 @@ def test_random_attempts():
         except RuntimeError:
             assert _state(p) == before
         _sound(p)
+
+
+def test_rehearsal():
+    """Without keep nothing stays, and what the pool has no pages for is found."""
+    p = _pool()
+    p.grow([(0, 40), (1, 16)])
+    before = _state(p)
+    with p.attempt(keep=False):
+        p.grow([(0, 100)])
+        p.trim(0, 60)
+        p.grow([(2, 80)])
+        assert p.held(0) == 4 and p.held(2) == 5
+    assert _state(p) == before
+    with pytest.raises(RuntimeError, match="exhausted"):
+        with p.attempt(keep=False):
+            p.grow([(0, 100)])
+            p.grow([(2, 80)])
+    assert _state(p) == before
+    _sound(p)
