@@ -215,7 +215,7 @@ class StaticBackbone:
         self._extent = -(-self.capacity // TILE) * TILE
         full = (self.max_slots + 1, self.kv_heads, self._extent, self.head_dim)
         self.kv4 = [ops.Kv4Cache.empty(*full, self.device) for _ in self.layers] if self.kv_bits == 4 else []
-        self.pages, self.paged = None, []
+        self.pages, self.paged, self._stream = None, [], None
         if self.page_size is not None:
             n = self._wanted_pages
             if n is None:
@@ -252,6 +252,15 @@ class StaticBackbone:
             length = self.lengths_cpu[slot] if length is None else length
             self.pages.trim(slot, length - self.window + 1, self.sinks)
 
+    def _follow(self):
+        """Paged cache: this call's work goes behind that of the last one. Calls share the table, a workspace and pages that
+        change hands, so one on another stream than the last waits for it, also where their slots differ."""
+        if self.pages is not None:
+            now = torch.cuda.current_stream(self.device)
+            if self._stream is not None and now.cuda_stream != self._stream.cuda_stream:
+                now.wait_stream(self._stream)
+            self._stream = now
+
     def _take(self, wants):
         """Lets go of what lies behind the windows of the slots in wants ((slot, length) pairs), takes the pages of their first
         `length` positions and sends the table; all of it, or nothing when the pool has too few pages."""
@@ -259,6 +268,7 @@ class StaticBackbone:
             for s, _ in wants:
                 self._trim(s)
             self.pages.grow(wants)
+        self._follow()
         self.pages.flush()
 
     @torch.inference_mode()
@@ -286,6 +296,7 @@ class StaticBackbone:
                 with self.pages.attempt():
                     self.pages.release(slot)
                     self.pages.grow([(slot, length)])
+                self._follow()
                 self.pages.flush()
                 self._set_length(slot, 0)
             if length:
@@ -312,6 +323,7 @@ class StaticBackbone:
     def free(self, slot):
         if self.pages is not None:
             self.pages.release(slot)
+            self._follow()
         self._set_length(slot, 0)
 
     @torch.inference_mode()
@@ -329,6 +341,7 @@ class StaticBackbone:
         with self.pages.attempt():
             self.pages.release(slot)
             rest = self.pages.share(slot, source, n)
+        self._follow()
         self._set_length(slot, 0)
         if rest is not None:
             for c in self.paged:
@@ -353,6 +366,7 @@ class StaticBackbone:
             raise ValueError(f'length {n} outside the slot\'s {self.lengths_cpu[slot]} cached positions')
         if self.pages is not None and not self.pages.has(slot, n):
             raise ValueError(f'slot {slot} has let go of positions behind its window')
+        self._follow()
         if self.kv_bits == 4 or self.pages is not None:
             at, out = self._positions_of(slot, n), []
             for c in self.paged or self.kv4:
@@ -410,11 +424,12 @@ class StaticBackbone:
         b.q = torch.empty(rows, H, D, dtype=dt, device=dev)
         b.items = None
         if self.pages is not None:
+            self._follow()
             args = (H, KV, D, ctx, self.window, self.sinks, dev)
             staged = mixed or rows >= ITEM_MIN_ROWS
             one = [(r, 1, 0) for r in range(rows)]
             b.plan = ops.PagedPlan.reserve(rows, *args, single=not mixed) if staged else ops.PagedPlan(one, *args)
-            if self._attn_ws.numel() * 4 < b.plan.workspace:  # one for all graphs: their steps follow each other
+            if self._attn_ws.numel() * 4 < b.plan.workspace:  # one for all graphs: their steps follow each other (_follow)
                 self._attn_ws = torch.empty(b.plan.workspace // 4, dtype=torch.float32, device=dev)
             b.attn_ws = self._attn_ws
             b.tiles, b.tiles_key = (), None
