@@ -236,9 +236,11 @@ class StaticBackbone:
         self.v = [t[:, :, :self.capacity] for t in self._vfull]
         self.lengths = torch.zeros(self.max_slots + 1, dtype=torch.long, device=self.device)
         self.lengths_cpu = [0] * (self.max_slots + 1)
-        cos, sin = self.lm.rotary_emb(torch.zeros(1, 1, self.hidden, dtype=self.dtype, device=self.device),
-                                      torch.arange(self._extent, device=self.device)[None])
-        self.cos, self.sin = cos[0].contiguous(), sin[0].contiguous()  # [extent, head_dim], model dtype (as HF)
+        self.cos = self.sin = None
+        if self.page_size is None:
+            cos, sin = self.lm.rotary_emb(torch.zeros(1, 1, self.hidden, dtype=self.dtype, device=self.device),
+                                          torch.arange(self._extent, device=self.device)[None])
+            self.cos, self.sin = cos[0].contiguous(), sin[0].contiguous()  # [extent, head_dim], model dtype (as HF)
 
     # ---------------------------------------------------------------- slots
     def _set_length(self, slot, n):
