@@ -90,3 +90,27 @@ def test_small_scales(gpu, scale, n):
     for cut in (True, False):
         worst = R.within(_run(gpu, q, k, v, table, slots, pos, laid, scale, splits=2, cut=cut), want, bound)
         assert worst <= 1, (cut, worst)
+
+
+@pytest.mark.parametrize("dtype,D", [(FP, 128), (BF, 64)])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_many_workgroups(gpu, dtype, D, splits):
+    """The same in a prompt of more workgroups than there are CUs, whose keys one group of waves has to itself: sums whose
+    references differ from split to split, by more and less than what one multiply-add a weight bears."""
+    page, n, p0 = 64, 320, 400
+    q0, k0 = (60000.0, 50000.0) if dtype == FP else (3e6, 1e9)
+    q, k, v, table, slots, pos, laid = _case([(n, p0)], 32, 8, D, page, dtype, seed=15)
+    q[:, :, 0] = 0
+    q[:, 1::3] = 0
+    q[:, 1::3, 0] = q0
+    q[:, 2::3] *= 40  # scores of some hundreds
+    for best in ([7], [395], [7, 200, 395]):
+        k1 = k.clone()
+        for j in best:
+            k1[table[1, j // page].long(), :, j % page, 0] = k0
+        want, bound = R.attention(q, k1, v, table, slots, pos, 0.1, runs=laid)
+        size = R.rows_of(v.abs(), table, 1, torch.tensor(best), page).mean(0).repeat_interleave(4, 0)
+        bound[:, 1::3] = _one_hot(size, dtype)[None, 1::3].expand(n, -1, -1)
+        got = _run(gpu, q, k1, v, table, slots, pos, laid, 0.1, splits=splits, cut=False)
+        worst = R.within(got, want, bound)
+        assert worst <= 1, (best, worst)
