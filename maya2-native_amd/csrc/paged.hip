@@ -128,7 +128,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_paged_kernel(
   }
 }
 
-// K and V rows into their pages, D / 8 threads per (row, kv head): a copy, bound as the kernel above
+// K and V rows into their pages, D / 8 threads per (row, kv head): a copy, bound by the launch (8 heads of 128: 1 row 2.3
+// us, 300 rows 2.9), then by bytes: 16384 rows, 134 MB in 22 us, 6.0 TB/s (what it writes stays in the memory-side cache).
 template <int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const uint16_t* __restrict__ k, long sk_r, long sk_h,
                                                            const uint16_t* __restrict__ v, long sv_r, long sv_h, Paged c,

@@ -289,7 +289,7 @@ template <int D, int COLS> struct NarrowLds {
 // Tiles of up to 16 QT columns: single tokens, the few rows of drafted ones, and short prompts cut into such tiles. Bound by
 // the keys' bytes. Each of the 4 waves takes every fourth step of 32 keys, straight from memory to registers: K as the score
 // product's operand, V as rows whose numbers byte permutes pair over keys. The waves' results are merged through LDS.
-// Measured on MI355X (bf16, 16/8 heads of 128, page_size 64, graph-timed): 224 rows of 2048 keys 276 us, 1.87 GB at 6.8
+// Measured on MI355X (bf16, 16/8 heads of 128, page_size 64, graph-timed): 224 rows of 2048 keys 275 us, 1.87 GB at 6.8
 // TB/s; 48 rows of a 1024-key window 37 us, 5.4 TB/s; one row of 2048 keys in 8 splits 7.9 us: launch 2, loads of what the
 // next load needs (tile, slot, page, keys) 3, two steps and the merge 1, join 2.
 // NT: the keys' loads carry the non-temporal hint, for single rows, whose keys one workgroup reads once (224 rows 276 us
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(256, QT > 1 ? 2 : D == 64 ? 4 : 3) void paged_narro
 // keys) in steps of 32, which come to LDS by loads that need no registers, two steps
 // ahead; every wave reads K there in 16-byte chunks and V transposed by the LDS's own 16-bit transposing reads. A row's
 // chunks lie in LDS at their number XOR a number of the row, so that neither read meets a bank twice.
-// Measured on MI355X (bf16, page_size 64 or 128, graph-timed): 4096 rows onto 12288 keys, 32/8 heads of 128, 902 us, 1067
+// Measured on MI355X (bf16, page_size 64 or 128, graph-timed): 4096 rows onto 12288 keys, 32/8 heads of 128, 895 us, 1075
 // TFLOP/s, where an 8192^3 product of the library reaches 1290; the matrix units are busy half of the time, the vector units
 // about as long, and the clock is down to 1.9 GHz. 8 x 200 rows onto 300 to 500 keys, 16/8 heads, 21 us: launch 2, tile, slot
 // and page numbers 2.5, the first keys and queries 0.6, the first turn 2 to 3 with its code's way into the instruction

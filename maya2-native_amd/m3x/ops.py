@@ -1231,7 +1231,9 @@ class PagedPlan:
         """Splits a tile for single rows of uneven contexts: chunks of 256 to 800 keys that come to two to three workgroups a
         CU; none beyond two a CU without. Measured on MI355X (16/8 heads of 128, rows of up to 4000 keys, us: none, chunks of
         400 / 600 / 800 / 1000 / 1600 keys): 32 rows 67, 56.5 / 56.0 / 53.8 / 55.1 / 65.6; 64 rows 93.8, 97 / 97 / 91.8 / 97 /
-        95; 128 rows 168, 177 to 194."""
+        95; 128 rows 168, 177 to 194. The rule was made at heads of 128; at heads of 64 (16/8): 32 rows 32.7, 31.6 / 32.1 /
+        37.4 / 36.9 / 36.0, the rule 37.9; 64 rows 54.3, 54.5 / 52.4 / 51.3 / 52.0 / 57.4, the rule 51.2; 128 rows 96.7, 97 to
+        106."""
         ends = self._ends(runs)
         one = self._blocks(runs, 16)
         if not self.uneven(runs) or len(runs) * one > 512:
@@ -1254,7 +1256,9 @@ class PagedPlan:
         MI355X (16/8 heads of 128; blocks, us cut / wide): 32 rows onto 300 keys (16) 9.8 / 15.3, 64 onto 4000 (32) 17.3 /
         22.2, 200 onto 2000 (104) 21.1 / 23.0, 512 onto 2048 (256) 25.8 / 28.8, 32 x 32 onto 500 (512) 19.5 / 22.6, 16 x 64
         onto 1000 (512) 27.7 / 30.5; on the other side 256 rows onto 6000 (128) 39.5 / 34.1, 64 onto 32000 (32) 48 / 41, 512
-        onto 6000 (256) 59 / 47, 5 x 200 onto 1000 (520) 34.8 / 28.7, 40 x 32 onto 500 (640) 26.0 / 25.0."""
+        onto 6000 (256) 59 / 47, 5 x 200 onto 1000 (520) 34.8 / 28.7, 40 x 32 onto 500 (640) 26.0 / 25.0. Heads of 64 take
+        the same side (16/8 heads): 7.7 / 12.4, 13.1 / 15.6, 16.1 / 16.2, 21.3 / 21.2, 13.8 / 16.8, 19.7 / 24.4; 28.1 / 23.4,
+        35.3 / 31.8, 44.2 / 35.1, 24.8 / 23.6, and, where cut would be faster, 17.7 / 19.2."""
         keys = min(keys, self.window + self.sinks + NARROW_COLS) if self.window else keys
         return blocks <= 512 and blocks * keys <= 600_000
 
@@ -1380,7 +1384,9 @@ def paged_attn_splits(blocks, keys, cols, mean_keys=None, columns=0, head_dim=12
     workgroup's keys, which they do up to a workgroup a CU; 0.52 for each of more workgroups that share a CU; the longest
     tile alone 0.75) and, from two on, the join's launch and partial results (3 us, 3 TB/s). Measured: 512 rows over 2048
     keys 43.9 / 33.5 / 27.1 / 32.5 at 1 / 2 / 4 / 8; 64 rows over 32000 77 / 49 / 40 at 8 / 16 / 32; 8 x 200 rows
-    over 500 21.0 / 31.0 at 1 / 2."""
+    over 500 21.0 / 31.0 at 1 / 2. Heads of 64, whose turns are shorter, go by the same figures (16/8 heads, chosen first):
+    512 rows over 2048 20.5 at 4, 34.2 / 25.3 / 19.4 at 1 / 2 / 8; 64 over 32000 31.9 at 32, 64 / 41 at 8 / 16; 8 x 200 over
+    500 15.1 at 1, 21.6 at 2; 1024 onto 8000 73 at 2, 64 at 4; 4096 onto 4000 161 to 170 at 1, 150 / 146 at 2 / 4."""
     blocks, mean_keys = max(blocks, 1), keys if mean_keys is None else max(mean_keys, 1)
     if cols != WIDE_COLS:
         if blocks > 128 and cols == 16:

@@ -37,8 +37,10 @@ exported prefix installs as exactly itself.
 `page_size` (no counterpart in the reference) keeps the cache in pages (ops.PagedKv, one per layer in `paged`; `k` and `v`
 are then empty): a slot takes memory as it grows, from a pool of `pages` pages, `fork` gives a slot another one's prefix
 without copying its whole pages, and with a `window` a row sees the last `window` positions and the first `sinks`, and
-pages that no row will see again go back to the pool, so that a stream's memory stays the same however long it gets. A
-step writes the cache with qk_norm_rope_paged (the model's frequencies, angles exact at any position) and attends with
+pages that no row will see again go back to the pool, so that a stream's memory stays the same up to `capacity`, where
+it ends; a position of capacity costs a table entry a page and slot and nothing else. A call that finds the pool too small
+raises RuntimeError and changes nothing; calls on several streams wait for each other, whichever slots they are of. A step
+writes the cache with qk_norm_rope_paged (the model's frequencies, angles exact at any position) and attends with
 paged_attn; one-row steps take the same launches.
 """
 from __future__ import annotations
